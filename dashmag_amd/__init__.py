@@ -8,14 +8,16 @@ The operations run as hand-written HIP kernels in ``libdashmi.so`` behind the C 
 from .contract import (Activation, AttentionMask, AttentionOptions, CausalConv1dOptions,
                        CrossEntropyOptions, Reduction,
                        CausalConv1dStepOptions, ChunkGatedDeltaOptions, DType,
-                       GatedDeltaStepOptions, LogprobOptions, UNBOUNDED, Unsupported, Window)
+                       GatedDeltaStepOptions, LogprobOptions, QkNormRopeOptions, UNBOUNDED,
+                       Unsupported, Window)
 from .ops import (attention, attention_backward, attention_decode, attention_decode_packed,
                   attention_decode_paged, attention_with_lse,
                   causal_conv1d, causal_conv1d_backward, causal_conv1d_update, chosen_logprob,
                   chosen_logprob_with_grad, linear_cross_entropy,
                   linear_cross_entropy_backward,
                   chunk_gated_delta_rule, chunk_gated_delta_rule_backward, gated_delta_step,
-                  gated_delta_step_backward)
+                  gated_delta_step_backward, qk_norm_rope, qk_norm_rope_backward,
+                  qk_norm_rope_paged)
 
 __all__ = [
     "Activation", "AttentionMask", "AttentionOptions", "CausalConv1dOptions",
@@ -28,4 +30,5 @@ __all__ = [
     "CrossEntropyOptions", "Reduction",
     "chunk_gated_delta_rule", "chunk_gated_delta_rule_backward", "gated_delta_step",
     "gated_delta_step_backward",
+    "QkNormRopeOptions", "qk_norm_rope", "qk_norm_rope_backward", "qk_norm_rope_paged",
 ]

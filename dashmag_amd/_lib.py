@@ -17,7 +17,8 @@ DM_UNBOUNDED = (1 << 64) - 1
 PROBES = ["attn_fwd_mfma", "attn_fwd_generic", "attn_bwd_mfma", "attn_bwd_generic",
           "decode_split", "decode_merge", "gdr_chunk_fwd", "gdr_chunk_bwd", "gdr_step",
           "conv1d_fwd", "conv1d_bwd", "conv1d_update", "logprob", "lce_fwd", "lce_bwd",
-          "gdr_chunk_fwd_mfma", "gdr_chunk_bwd_mfma", "gdr_step_bwd"]
+          "gdr_chunk_fwd_mfma", "gdr_chunk_bwd_mfma", "gdr_step_bwd", "qk_norm_rope",
+          "qk_norm_rope_bwd"]
 DM_ACT_NONE, DM_ACT_SILU = 0, 1
 
 
@@ -75,12 +76,31 @@ class LceDesc(ctypes.Structure):
                 ("entropy", ctypes.c_int32)]
 
 
+class QkNormRopeDesc(ctypes.Structure):
+    _fields_ = [("b", ctypes.c_int64), ("t", ctypes.c_int64), ("hq", ctypes.c_int64),
+                ("hkv", ctypes.c_int64), ("d", ctypes.c_int64), ("n", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32), ("unit_offset", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("positions", ctypes.c_void_p),
+                ("positions_i64", ctypes.c_int32), ("positions_b", ctypes.c_int64),
+                ("strided", ctypes.c_int32), ("sq", Strides), ("sk", Strides), ("sv", Strides),
+                ("sgq", Strides), ("sgk", Strides)]
+
+
+class KvPages(ctypes.Structure):
+    _fields_ = [("num_pages", ctypes.c_int64), ("page_size", ctypes.c_int64),
+                ("max_pages", ctypes.c_int64), ("nseq", ctypes.c_int64),
+                ("block_table", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("cu_seqlens", ctypes.c_void_p), ("sk", Strides), ("sv", Strides)]
+
+
 #: Every symbol include/dashmi.h declares, with (restype, argtypes).
 _VP, _SZ, _I64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int64
 _AD, _GD = ctypes.POINTER(AttentionDesc), ctypes.POINTER(GdrDesc)
 _CD = ctypes.POINTER(Conv1dDesc)
 _LD = ctypes.POINTER(LogprobDesc)
 _XD = ctypes.POINTER(LceDesc)
+_QD, _PD = ctypes.POINTER(QkNormRopeDesc), ctypes.POINTER(KvPages)
 SIGNATURES = {
     "dm_last_error": (ctypes.c_char_p, []),
     "dm_describe": (ctypes.c_int, [ctypes.c_char_p, _SZ]),
@@ -129,6 +149,10 @@ SIGNATURES = {
     "dm_causal_conv1d_bwd": (ctypes.c_int, [_CD] + [_VP] * 5 + [ctypes.c_int] + [_VP] * 6
                              + [_SZ, _VP]),
     "dm_causal_conv1d_update": (ctypes.c_int, [_CD] + [_VP] * 7),
+    "dm_qk_norm_rope": (ctypes.c_int, [_QD] + [_VP] * 8),
+    "dm_qk_norm_rope_bwd_workspace": (_SZ, [_QD]),
+    "dm_qk_norm_rope_bwd": (ctypes.c_int, [_QD] + [_VP] * 12 + [_SZ, _VP]),
+    "dm_qk_norm_rope_paged": (ctypes.c_int, [_QD, _PD] + [_VP] * 10),
 }
 
 _lib = None

@@ -213,6 +213,26 @@ class CrossEntropyOptions:
     chunks: LogprobOptions = LogprobOptions()
 
 
+@dataclasses.dataclass(frozen=True)
+class QkNormRopeOptions:
+    """The norms and the rotation of queries and keys: ``eps`` under the root, pairs ``(j, n + j)``
+    unless ``interleaved`` (then ``(2 j, 2 j + 1)``), weights as they are unless ``unit_offset``
+    (then ``1 + weight``)."""
+
+    eps: float = 1e-6
+    interleaved: bool = False
+    unit_offset: bool = False
+
+    def with_eps(self, eps: float):
+        return dataclasses.replace(self, eps=float(eps))
+
+    def with_interleaved(self, v: bool):
+        return dataclasses.replace(self, interleaved=v)
+
+    def with_unit_offset(self, v: bool):
+        return dataclasses.replace(self, unit_offset=v)
+
+
 def query_scale(scale: Optional[float], dk: int) -> float:
     """The gated delta rule's query scale: ``1/sqrt(Dk)`` unless given
     (crates/dash-ops/src/gated_delta.rs:17)."""

@@ -19,7 +19,8 @@ import torch
 from . import _lib
 from .contract import (Activation, AttentionMask, AttentionOptions, CausalConv1dOptions,
                        CausalConv1dStepOptions, ChunkGatedDeltaOptions, GatedDeltaStepOptions,
-                       CrossEntropyOptions, LogprobOptions, Reduction, UNBOUNDED, Unsupported)
+                       CrossEntropyOptions, LogprobOptions, QkNormRopeOptions, Reduction,
+                       UNBOUNDED, Unsupported)
 
 _DT = {torch.float32: _lib.DM_F32, torch.bfloat16: _lib.DM_BF16, torch.float16: _lib.DM_F16}
 
@@ -435,6 +436,228 @@ def attention_decode_paged(query, key_pages, value_pages, block_table, lengths=N
             _ptr(v), npages, page_size, _ptr(bt), max_pages, _ptr(ln), _ptr(out), _ptr(ws), nbytes,
             _stream())
     return out
+
+
+# ------------------------------------------------------------------------------------------
+# Norms and rotation of queries and keys
+# ------------------------------------------------------------------------------------------
+
+def _run(op, device, fn, *args):
+    """The library call ``fn(*args, stream)`` on ``device`` (which need not be torch's current one) and
+    its current stream."""
+    with torch.cuda.device(device):
+        rc = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+    if rc == _lib.DM_OK:
+        return
+    msg = _lib.last_error()
+    if rc == _lib.DM_ERR_REFUSED:
+        raise Unsupported(msg if msg.startswith(op) else f"{op}: {msg}")
+    raise RuntimeError(msg)
+
+
+def _one_device(op, first, *ts):
+    _device(op, first, *ts)
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise Unsupported(f"{op}: the tensors must be on one GPU (got {first.device} and {t.device})")
+
+
+_INTS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
+def _device_i32(op, t, device, what):
+    """``t`` as the int32 device array that kernels read which take any values in it: an int32 array on
+    the GPU in place and unread (no wait for the GPU, so such a call can be captured), any other
+    converted, values outside int32 refused."""
+    if isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device:
+        return t.detach() if t.is_contiguous() else t.detach().contiguous()
+    t = torch.as_tensor(t)
+    if t.numel() and t.dtype not in _INTS:
+        raise Unsupported(f"{op}: {what} must be whole numbers, got {t.dtype}")
+    return _offsets(t.detach(), device, op, what)
+
+
+def _qk_norm_rope_desc(op, query, key, q_weight, k_weight, inv_freq, options, paged):
+    dims, form = (3, "[N, H, D]") if paged else (4, "[B, T, H, D]")
+    if query.dim() != dims or key.dim() != dims:
+        raise Unsupported(f"{op}: query and key are {form}")
+    if tuple(query.shape[:-2]) != tuple(key.shape[:-2]):
+        raise Unsupported(f"{op}: query and key must have the same tokens")
+    if query.shape[-1] != key.shape[-1]:
+        raise Unsupported(f"{op}: query and key must have one head dimension")
+    if query.dtype != key.dtype:
+        raise Unsupported(f"{op}: query and key must share one dtype")
+    d = query.shape[-1]
+    desc = _lib.QkNormRopeDesc(b=1 if paged else query.shape[0], t=query.shape[-3],
+                               hq=query.shape[-2], hkv=key.shape[-2], d=d, dtype=_dtype(op, query),
+                               interleaved=int(bool(options.interleaved)),
+                               unit_offset=int(bool(options.unit_offset)), eps=float(options.eps))
+    desc.weight_dtype = desc.dtype
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            continue
+        if tuple(w.shape) != (d,):
+            raise Unsupported(f"{op}: {name} is [D] = [{d}]")
+        if w.dtype not in (torch.float32, query.dtype):
+            raise Unsupported(f"{op}: {name} must be f32 or the queries' dtype")
+        desc.weight_dtype = _DT[w.dtype]
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise Unsupported(f"{op}: q_weight and k_weight must share one dtype")
+    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
+        raise Unsupported(f"{op}: inv_freq is [n] f32")
+    desc.n = inv_freq.shape[0]
+    if 2 * desc.n > d:
+        raise Unsupported(f"{op}: the frequencies are [n] with 2 n at most the head dimension ({d}), "
+                          f"got n = {desc.n}")
+    desc.strided = 1
+    return desc
+
+
+def _positions(op, desc, positions, device):
+    """Fills in the positions ``[B, T]`` or ``[T]``, read where they are if int32 or int64 on the GPU."""
+    if positions is None:
+        return None
+    p = torch.as_tensor(positions)
+    if p.dtype not in _INTS:
+        raise Unsupported(f"{op}: the positions must be whole numbers, got {p.dtype}")
+    if tuple(p.shape) not in ((desc.b, desc.t), (desc.t,)):
+        raise Unsupported(f"{op}: the positions are [B, T] or [T], [{desc.b}, {desc.t}]")
+    p = p.detach().to(device=device, dtype=p.dtype if p.dtype in (torch.int32, torch.int64) else torch.int32)
+    if p.shape[-1] > 1 and p.stride(-1) != 1:
+        p = p.contiguous()
+    desc.positions, desc.positions_i64 = p.data_ptr(), int(p.dtype == torch.int64)
+    desc.positions_b = p.stride(0) if p.dim() == 2 and p.shape[0] > 1 else 0
+    return p
+
+
+def _flat(w):
+    return None if w is None else w.contiguous()
+
+
+def qk_norm_rope(query, key, q_weight, k_weight, inv_freq, positions=None,
+                 options: Optional[QkNormRopeOptions] = None):
+    """Each head of ``query [B, T, Hq, D]`` and ``key [B, T, Hkv, D]`` normalised over its D values,
+    scaled by its weight ``[D]`` (f32 or the queries' dtype; None: no weight) and its first ``2 n``
+    values rotated by the token's position with the frequencies ``inv_freq [n]`` f32:
+    ``(query, key)`` in the inputs' dtype. ``positions`` is ``[B, T]`` or ``[T]`` of whole numbers
+    (None: 0 .. T - 1); int32 and int64 on the GPU are read in place."""
+    op = "qk_norm_rope"
+    options = options or QkNormRopeOptions()
+    _one_device(op, query, key, q_weight, k_weight, inv_freq)
+    desc = _qk_norm_rope_desc(op, query, key, q_weight, k_weight, inv_freq, options, False)
+    dev = query.device
+    at = _positions(op, desc, positions, dev)
+    q, k, wq, wk, freq = _readable(query), _readable(key), _flat(q_weight), _flat(k_weight), _flat(inv_freq)
+    _set_strides(desc.sq, q, (0, 1, 2))
+    _set_strides(desc.sk, k, (0, 1, 2))
+    qo, ko = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k))
+    _run(op, dev, _lib.lib().dm_qk_norm_rope, ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(wq), _ptr(wk),
+         _ptr(freq), _ptr(qo), _ptr(ko))
+    return qo, ko
+
+
+def qk_norm_rope_backward(query, key, q_weight, k_weight, inv_freq, grad_query, grad_key, positions=None,
+                          options: Optional[QkNormRopeOptions] = None):
+    """The gradients of :func:`qk_norm_rope` from its inputs and the gradients of its outputs (read in
+    the inputs' dtype): ``(dquery, dkey, dq_weight, dk_weight)``, each in its input's dtype and shape
+    (None for a weight that is None). The weights' are summed in a fixed order."""
+    op = "qk_norm_rope_backward"
+    options = options or QkNormRopeOptions()
+    _one_device(op, query, key, q_weight, k_weight, inv_freq, grad_query, grad_key)
+    desc = _qk_norm_rope_desc(op, query, key, q_weight, k_weight, inv_freq, options, False)
+    if tuple(grad_query.shape) != tuple(query.shape) or tuple(grad_key.shape) != tuple(key.shape):
+        raise Unsupported(f"{op}: the gradients have the outputs' shapes")
+    dev = query.device
+    at = _positions(op, desc, positions, dev)
+    q, k, wq, wk, freq = _readable(query), _readable(key), _flat(q_weight), _flat(k_weight), _flat(inv_freq)
+    gq, gk = _readable(grad_query.to(q.dtype)), _readable(grad_key.to(q.dtype))
+    for f, t in ((desc.sq, q), (desc.sk, k), (desc.sgq, gq), (desc.sgk, gk)):
+        _set_strides(f, t, (0, 1, 2))
+    dq, dk = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k))
+    dwq, dwk = (None if w is None else torch.empty(w.shape, dtype=w.dtype, device=dev) for w in (wq, wk))
+    nbytes = _lib.lib().dm_qk_norm_rope_bwd_workspace(ctypes.byref(desc))
+    ws = _workspace(nbytes, dev)
+    _run(op, dev, _lib.lib().dm_qk_norm_rope_bwd, ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(wq), _ptr(wk),
+         _ptr(freq), _ptr(gq), _ptr(gk), _ptr(dq), _ptr(dk), _ptr(dwq), _ptr(dwk), _ptr(ws), nbytes)
+    return dq, dk, dwq, dwk
+
+
+def _in_pages(op, pages, what):
+    """Pages that a call writes: a view is written in place, so its rows must be whole and apart."""
+    st, shape = pages.stride(), pages.shape
+    if pages.numel() and ((shape[-1] > 1 and st[-1] != 1)
+                          or any(n > 1 and x == 0 for n, x in zip(shape, st))):
+        raise Unsupported(f"{op}: {what} must be a view whose last dimension is contiguous and whose "
+                          "elements are apart")
+
+
+def _block_table(op, block_table, rows, device, keep):
+    bt = block_table if isinstance(block_table, torch.Tensor) else torch.as_tensor(block_table)
+    if bt.dim() != 2 or (rows is not None and bt.shape[0] != rows):
+        raise Unsupported(f"{op}: the block table is [{'R' if rows is None else rows}, max_pages]")
+    bt = _device_i32(op, bt, device, "the block table")
+    keep.append(bt)
+    return bt
+
+
+def qk_norm_rope_paged(query, key, value, q_weight, k_weight, inv_freq, key_pages, value_pages, block_table,
+                       lengths, cu_seqlens=None, options: Optional[QkNormRopeOptions] = None):
+    """:func:`qk_norm_rope` of the tokens that join a paged cache, prompts or one token a sequence:
+    returns ``query [N, Hq, D]`` normalised and rotated, and writes ``key [N, Hkv, D]``, normalised and
+    rotated, and ``value`` as it is to their rows of ``key_pages, value_pages [P, page_size, Hkv, D]``
+    in place. ``lengths [S]`` are the sequences' lengths with these tokens, as the decode that follows
+    takes them; the rows ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1`` are sequence ``s``'s last tokens
+    (without ``cu_seqlens [S + 1]`` each sequence has one, N = S), each at its place in the sequence,
+    which is its position too; ``block_table [S, max_pages]`` holds the sequences' pages.
+
+    int32 arrays on the GPU are not read back: what they hold is checked on the GPU. A token of no
+    sequence, or with a position below zero (the padding of a batch: length 0), gets a query of zeros
+    and writes nothing; one whose page lies outside the pages or past the table writes nothing. No two
+    tokens may go to one row of a page."""
+    op = "qk_norm_rope_paged"
+    options = options or QkNormRopeOptions()
+    _one_device(op, query, key, value, q_weight, k_weight, inv_freq, key_pages, value_pages)
+    desc = _qk_norm_rope_desc(op, query, key, q_weight, k_weight, inv_freq, options, True)
+    if tuple(value.shape) != tuple(key.shape):
+        raise Unsupported(f"{op}: key and value must have one shape")
+    if key_pages.dim() != 4 or tuple(key_pages.shape) != tuple(value_pages.shape):
+        raise Unsupported(f"{op}: the key and value pages are [P, page_size, Hkv, D], one shape")
+    if tuple(key_pages.shape[2:]) != tuple(key.shape[1:]):
+        raise Unsupported(f"{op}: the pages' rows are the keys' [Hkv, D] = {list(key.shape[1:])}")
+    if not (query.dtype == value.dtype == key_pages.dtype == value_pages.dtype):
+        raise Unsupported(f"{op}: query, key, value and the pages must share one dtype")
+    if key_pages.shape[1] < 1:
+        raise Unsupported(f"{op}: pages hold at least one key")
+    _in_pages(op, key_pages, "key_pages")
+    _in_pages(op, value_pages, "value_pages")
+    dev, n = query.device, query.shape[0]
+    keep = []
+    ln = _device_i32(op, lengths, dev, "the cache lengths")
+    if ln.dim() != 1:
+        raise Unsupported(f"{op}: the cache lengths are [S]")
+    nseq = ln.shape[0]
+    bt = _block_table(op, block_table, nseq, dev, keep)
+    cu = None
+    if cu_seqlens is not None:
+        cu = _device_i32(op, cu_seqlens, dev, "cu_seqlens")
+        if tuple(cu.shape) != (nseq + 1,):
+            raise Unsupported(f"{op}: cu_seqlens is [S + 1] = [{nseq + 1}]")
+    elif nseq != n:
+        raise Unsupported(f"{op}: without cu_seqlens there is one token a sequence, got {n} tokens and "
+                          f"{nseq} sequences")
+    q, k, v = _readable(query), _readable(key), _readable(value)
+    wq, wk, freq = _flat(q_weight), _flat(k_weight), _flat(inv_freq)
+    for f, t in ((desc.sq, q), (desc.sk, k), (desc.sv, v)):
+        _set_strides(f, t, (None, 0, 1))
+    pages = _lib.KvPages(num_pages=key_pages.shape[0], page_size=key_pages.shape[1], max_pages=bt.shape[1],
+                         nseq=nseq, block_table=bt.data_ptr(), lengths=ln.data_ptr(),
+                         cu_seqlens=None if cu is None else cu.data_ptr())
+    _set_strides(pages.sk, key_pages, (0, 1, 2))
+    _set_strides(pages.sv, value_pages, (0, 1, 2))
+    qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    _run(op, dev, _lib.lib().dm_qk_norm_rope_paged, ctypes.byref(desc), ctypes.byref(pages), _ptr(q), _ptr(k),
+         _ptr(v), _ptr(wq), _ptr(wk), _ptr(freq), _ptr(qo), _ptr(key_pages), _ptr(value_pages))
+    return qo
 
 
 # ------------------------------------------------------------------------------------------

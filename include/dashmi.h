@@ -8,6 +8,8 @@
  *   dm_attention_bwd     AttentionBackend::attention_backward   crates/dash-ops/src/attention.rs:689
  *   dm_attention_decode  AttentionBackend::attention_decode     crates/dash-ops/src/attention.rs:732
  *   dm_attention_decode_paged  (none: the decode over a paged cache)
+ *   dm_qk_norm_rope{,_bwd,_paged}  (none: the norms and the rotation of queries and keys that
+ *                        precede the attention; the reference's callers bring them rotated)
  *   dm_gdr_chunk_fwd     ChunkGatedDeltaBackend::chunk_gated_delta_forward
  *                                                               crates/dash-ops/src/gated_delta/chunk.rs:340-425, :856
  *   dm_gdr_chunk_bwd     ChunkGatedDeltaBackend::chunk_gated_delta_backward (the Autodiff node's
@@ -169,6 +171,42 @@ typedef struct {
     int32_t entropy;
 } dm_lce_desc;
 
+/* One call of the queries' and keys' norms and rotation: q [B, T, Hq, D], k [B, T, Hkv, D]. Each
+ * head x of each token is normalised over its D values and scaled, y = x (mean(x^2) + eps)^-1/2 w
+ * (w the weight [D]; 1 + weight with unit_offset; 1 without a weight), and the first 2 n of y's
+ * values rotate by the token's position p: pair j turns by p * inv_freq[j], pairs being (j, n + j),
+ * or (2 j, 2 j + 1) with interleaved. The angles are taken in 64 bits, all else in 32, and an
+ * output is rounded once. D is at most 256, 2 n at most D. The paged form reads q [N, Hq, D] and k,
+ * v [N, Hkv, D] with b = 1, t = N. */
+typedef struct {
+    int64_t b, t, hq, hkv, d;
+    int64_t n;            /* rotated pairs: inv_freq is [n] f32 */
+    int32_t dtype;        /* q, k, v, the outputs, the pages and the gradients of q and k */
+    int32_t weight_dtype; /* the weights and their gradients: DM_F32 or dtype */
+    int32_t interleaved, unit_offset;
+    float eps;
+    const void *positions;   /* [B, T] int32 or int64 on the device; NULL: 0 .. T - 1 in each row */
+    int32_t positions_i64;   /* 1: int64 */
+    int64_t positions_b;     /* the elements between two batch rows' positions (0: one row for all) */
+    int32_t strided;         /* 1: the strides below (each >= 0); sv is the paged form's v, sgq and
+                              * sgk the backward's gradients of the outputs */
+    dm_strides sq, sk, sv, sgq, sgk;
+} dm_qk_norm_rope_desc;
+
+/* The pages that the paged form writes: k and v pages [num_pages, page_size, Hkv, D] (b = page, t =
+ * row, h = head strides in elements, the last dimension contiguous), the sequences' pages
+ * block_table [nseq, max_pages] and their lengths [nseq] after the call. cu_seqlens [nseq + 1]
+ * cuts the N tokens into the sequences' (NULL: one token a sequence, N = nseq): a sequence's
+ * tokens are its last ones, so that the token in front of i others has position
+ * lengths[s] - 1 - i. All three are int32 on the device and are read there only: a token that
+ * belongs to no sequence or whose position would be negative writes no page and its query output
+ * is 0; one whose page is outside [0, num_pages) or past the table writes no page. */
+typedef struct {
+    int64_t num_pages, page_size, max_pages, nseq;
+    const int32_t *block_table, *lengths, *cu_seqlens;
+    dm_strides sk, sv;
+} dm_kv_pages;
+
 /* The message of this thread's last refusal or error. */
 const char *dm_last_error(void);
 
@@ -211,6 +249,8 @@ typedef enum {
     DM_PROBE_GDR_CHUNK_FWD_MFMA, /* the MFMA kernels of the chunked forward (a subset of the above) */
     DM_PROBE_GDR_CHUNK_BWD_MFMA, /* the MFMA kernels of the chunked backward */
     DM_PROBE_GDR_STEP_BWD,       /* the recurrent step's backward */
+    DM_PROBE_QK_NORM_ROPE,       /* the queries' and keys' norms and rotation, the paged form too */
+    DM_PROBE_QK_NORM_ROPE_BWD,
     DM_PROBE_COUNT
 } dm_probe;
 uint64_t dm_probe_count(int probe);
@@ -310,6 +350,29 @@ int dm_attention_decode_paged(const dm_attention_desc *desc, const void *q, cons
                               const int32_t *block_table, int64_t max_pages,
                               const int32_t *lengths, void *o, void *workspace,
                               size_t workspace_bytes, void *stream);
+
+/* The queries' and keys' norms and rotation: q_out [B, T, Hq, D] and k_out [B, T, Hkv, D],
+ * contiguous. q_weight and k_weight [D] may be NULL (no weight). */
+int dm_qk_norm_rope(const dm_qk_norm_rope_desc *desc, const void *q, const void *k,
+                    const void *q_weight, const void *k_weight, const float *inv_freq, void *q_out,
+                    void *k_out, void *stream);
+/* Its backward from the inputs and the gradients of the outputs: dq, dk contiguous in dtype and the
+ * weights' gradients dq_weight, dk_weight [D] in weight_dtype (NULL: not wanted), summed over
+ * tokens and heads in a fixed order (deterministic). */
+size_t dm_qk_norm_rope_bwd_workspace(const dm_qk_norm_rope_desc *desc);
+int dm_qk_norm_rope_bwd(const dm_qk_norm_rope_desc *desc, const void *q, const void *k,
+                        const void *q_weight, const void *k_weight, const float *inv_freq,
+                        const void *grad_q, const void *grad_k, void *dq, void *dk,
+                        void *dq_weight, void *dk_weight, void *workspace, size_t workspace_bytes,
+                        void *stream);
+/* The same into a paged cache: q_out [N, Hq, D] contiguous; the keys, normalised and rotated, and
+ * the values as they are go to their rows of k_pages and v_pages. No two tokens of a call may have
+ * one page row (sequences that share the page that they append to, a page twice in a row's table):
+ * which of them it then holds is not said. */
+int dm_qk_norm_rope_paged(const dm_qk_norm_rope_desc *desc, const dm_kv_pages *pages, const void *q,
+                          const void *k, const void *v, const void *q_weight, const void *k_weight,
+                          const float *inv_freq, void *q_out, void *k_pages, void *v_pages,
+                          void *stream);
 
 /* The chunked gated delta rule forward: out [B, T, H, Dv] in dtype and, if final_state is not
  * NULL, each sequence's final state [S, H, Dk, Dv] f32; h0 [S, H, Dk, Dv] f32 or NULL (zeros).
