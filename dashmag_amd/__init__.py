@@ -11,7 +11,7 @@ from .contract import (Activation, AttentionMask, AttentionOptions, CausalConv1d
                        GatedDeltaStepOptions, LogprobOptions, QkNormRopeOptions, UNBOUNDED,
                        Unsupported, Window)
 from .ops import (attention, attention_backward, attention_decode, attention_decode_packed,
-                  attention_decode_paged, attention_with_lse,
+                  attention_decode_paged, attention_decode_shared, attention_with_lse,
                   causal_conv1d, causal_conv1d_backward, causal_conv1d_update, chosen_logprob,
                   chosen_logprob_with_grad, linear_cross_entropy,
                   linear_cross_entropy_backward,
@@ -24,7 +24,7 @@ __all__ = [
     "CausalConv1dStepOptions", "ChunkGatedDeltaOptions", "DType",
     "GatedDeltaStepOptions", "LogprobOptions", "UNBOUNDED", "Unsupported", "Window",
     "attention", "attention_backward", "attention_decode", "attention_decode_packed",
-    "attention_decode_paged", "attention_with_lse",
+    "attention_decode_paged", "attention_decode_shared", "attention_with_lse",
     "causal_conv1d", "causal_conv1d_backward", "causal_conv1d_update", "chosen_logprob",
     "chosen_logprob_with_grad", "linear_cross_entropy", "linear_cross_entropy_backward",
     "CrossEntropyOptions", "Reduction",

@@ -18,7 +18,7 @@ PROBES = ["attn_fwd_mfma", "attn_fwd_generic", "attn_bwd_mfma", "attn_bwd_generi
           "decode_split", "decode_merge", "gdr_chunk_fwd", "gdr_chunk_bwd", "gdr_step",
           "conv1d_fwd", "conv1d_bwd", "conv1d_update", "logprob", "lce_fwd", "lce_bwd",
           "gdr_chunk_fwd_mfma", "gdr_chunk_bwd_mfma", "gdr_step_bwd", "qk_norm_rope",
-          "qk_norm_rope_bwd"]
+          "qk_norm_rope_bwd", "decode_shared"]
 DM_ACT_NONE, DM_ACT_SILU = 0, 1
 
 
@@ -149,6 +149,10 @@ SIGNATURES = {
     "dm_causal_conv1d_bwd": (ctypes.c_int, [_CD] + [_VP] * 5 + [ctypes.c_int] + [_VP] * 6
                              + [_SZ, _VP]),
     "dm_causal_conv1d_update": (ctypes.c_int, [_CD] + [_VP] * 7),
+    "dm_attention_decode_shared_workspace": (_SZ, [_AD, ctypes.c_int64, ctypes.c_int64]),
+    "dm_attention_decode_shared": (ctypes.c_int, [_AD, _VP, _VP, _VP, ctypes.c_int64, ctypes.c_int64,
+                                                  _VP, ctypes.c_int64, _VP, _VP, ctypes.c_int64, _VP,
+                                                  _VP, _VP, _SZ, _VP]),
     "dm_qk_norm_rope": (ctypes.c_int, [_QD] + [_VP] * 8),
     "dm_qk_norm_rope_bwd_workspace": (_SZ, [_QD]),
     "dm_qk_norm_rope_bwd": (ctypes.c_int, [_QD] + [_VP] * 12 + [_SZ, _VP]),

@@ -12,6 +12,9 @@ void fill_f32(float *p, float value, int64_t n, hipStream_t st);
 void fill_zero(void *p, size_t bytes, hipStream_t st);
 
 int check_attention(const dm_attention_desc *d, const char *op);
+// A decode's checks, and its window's left side (-1: open) (decode.hip).
+int check_decode(const char *op, const dm_attention_desc *d);
+int64_t left_of(const dm_attention_desc *d);
 // f32 arithmetic, any dtype and head width up to 256 (attention_f32.hip).
 int launch_attn_fwd_f32(const MaskInfo &m, const dm_attention_desc *d, float scale, const void *q,
                         const void *k, const void *v, void *o, float *lse, hipStream_t st);

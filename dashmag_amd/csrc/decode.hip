@@ -506,7 +506,7 @@ static bool paged_split_takes(const dm_attention_desc *d, int64_t page_size) {
     return split_takes(d, page_size) && page_size % 16 == 0;
 }
 
-static int64_t left_of(const dm_attention_desc *d) {
+int64_t left_of(const dm_attention_desc *d) {
     const uint64_t span = (uint64_t)d->tk + 1;  // `bound(left, s + 1)`, reference.rs:449
     const uint64_t left = d->options.has_window ? d->options.window_left : DM_UNBOUNDED;
     return left < span ? (int64_t)left : -1;
@@ -534,8 +534,8 @@ static int nsplit_of(const dm_attention_desc *d) {
     return (int)((keys + span - 1) / span);
 }
 
-// The checks both entry points share; returns DM_OK or the refusal.
-static int check_decode(const char *op, const dm_attention_desc *d) {
+// The checks the entry points share; returns DM_OK or the refusal.
+int check_decode(const char *op, const dm_attention_desc *d) {
     const std::string o(op);
     if (!d) return refuse(o + ": null descriptor");
     if (d->b < 0 || d->tk < 0 || d->hq < 0 || d->hkv <= 0 || d->d < 0)

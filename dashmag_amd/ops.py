@@ -660,6 +660,63 @@ def qk_norm_rope_paged(query, key, value, q_weight, k_weight, inv_freq, key_page
     return qo
 
 
+def attention_decode_shared(query, key_pages, value_pages, block_table, lengths, groups, prefix_lengths,
+                            options=None):
+    """:func:`attention_decode_paged` for a batch whose sequences share prefixes (many answers to one
+    prompt, one system prompt in front of many conversations): the rows
+    ``groups[g] .. groups[g + 1] - 1`` hold the same first ``prefix_lengths[g]`` keys, and those are read
+    once for the group, each row's own keys behind them for itself. ``groups [G + 1]`` goes up from 0
+    at least to B at most; a row outside it shares nothing. ``[B, Hq, D]`` in the queries' dtype.
+
+    A group's prefix is read through the block table of its longest row (the first of them), which has
+    to hold all of the prefix that any row of the group sees, a window's too; that the others' tables
+    hold the same keys is the caller's to see to (``cache_fork`` makes such tables). int32 arrays on
+    the GPU are not read back: a negative length counts as 0, and groups that do not go up as none."""
+    op = "attention_decode_shared"
+    options = options or AttentionOptions()
+    _one_device(op, query, key_pages, value_pages)
+    if key_pages.dim() != 4:
+        raise Unsupported(f"{op}: the key pages are [P, page_size, Hkv, D]")
+    npages, page_size = key_pages.shape[0], key_pages.shape[1]
+    if page_size < 1:
+        raise Unsupported(f"{op}: pages hold at least one key")
+    dev, b = query.device, query.shape[0] if query.dim() == 3 else -1
+    keep = []
+    bt = _block_table(op, block_table, b, dev, keep)
+    max_pages = bt.shape[1]
+    desc = _decode_desc(op, query, key_pages, value_pages, max_pages * page_size, options)
+    ln, cu, pl = _shared_arrays(op, lengths, groups, prefix_lengths, b, dev)
+    q, k, v = _readable(query), _readable(key_pages), _readable(value_pages)
+    _decode_strides(desc, q, k, v, (0, 1, 2))
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    ng = cu.shape[0] - 1
+    nbytes = _lib.lib().dm_attention_decode_shared_workspace(ctypes.byref(desc), page_size, ng)
+    ws = _workspace(nbytes, dev)
+    _run(op, dev, _lib.lib().dm_attention_decode_shared, ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), npages,
+         page_size, _ptr(bt), max_pages, _ptr(ln), _ptr(cu), ng, _ptr(pl), _ptr(out), _ptr(ws), nbytes)
+    return out
+
+
+def _shared_arrays(op, lengths, groups, prefix_lengths, b, device):
+    """The lengths (None: every key), groups and prefix lengths as int32 device arrays; groups that lie
+    on the host are checked there."""
+    ln = None if lengths is None else _device_i32(op, lengths, device, "the cache lengths")
+    if ln is not None and tuple(ln.shape) != (b,):
+        raise Unsupported(f"{op}: the cache lengths are [B] = [{b}]")
+    cu = _device_i32(op, groups, device, "groups")
+    if cu.dim() != 1 or cu.shape[0] < 1:
+        raise Unsupported(f"{op}: groups is [G + 1], got {list(cu.shape)}")
+    if not (isinstance(groups, torch.Tensor) and groups.is_cuda):
+        at = torch.as_tensor(groups).tolist()
+        if min(at) < 0 or max(at) > b or any(x > y for x, y in zip(at, at[1:])):
+            raise Unsupported(f"{op}: groups must go from 0 or more to at most B = {b} without decreasing, "
+                              f"got {at}")
+    pl = _device_i32(op, prefix_lengths, device, "the prefix lengths")
+    if tuple(pl.shape) != (cu.shape[0] - 1,):
+        raise Unsupported(f"{op}: the prefix lengths are [G] = [{cu.shape[0] - 1}]")
+    return ln, cu, pl
+
+
 # ------------------------------------------------------------------------------------------
 # Gated delta rule
 # ------------------------------------------------------------------------------------------

@@ -8,6 +8,7 @@
  *   dm_attention_bwd     AttentionBackend::attention_backward   crates/dash-ops/src/attention.rs:689
  *   dm_attention_decode  AttentionBackend::attention_decode     crates/dash-ops/src/attention.rs:732
  *   dm_attention_decode_paged  (none: the decode over a paged cache)
+ *   dm_attention_decode_shared  (none: the paged decode of sequences that share prefixes)
  *   dm_qk_norm_rope{,_bwd,_paged}  (none: the norms and the rotation of queries and keys that
  *                        precede the attention; the reference's callers bring them rotated)
  *   dm_gdr_chunk_fwd     ChunkGatedDeltaBackend::chunk_gated_delta_forward
@@ -251,6 +252,7 @@ typedef enum {
     DM_PROBE_GDR_STEP_BWD,       /* the recurrent step's backward */
     DM_PROBE_QK_NORM_ROPE,       /* the queries' and keys' norms and rotation, the paged form too */
     DM_PROBE_QK_NORM_ROPE_BWD,
+    DM_PROBE_DECODE_SHARED,
     DM_PROBE_COUNT
 } dm_probe;
 uint64_t dm_probe_count(int probe);
@@ -350,6 +352,23 @@ int dm_attention_decode_paged(const dm_attention_desc *desc, const void *q, cons
                               const int32_t *block_table, int64_t max_pages,
                               const int32_t *lengths, void *o, void *workspace,
                               size_t workspace_bytes, void *stream);
+
+/* dm_attention_decode_paged for sequences that share prefixes: rows groups[g] .. groups[g + 1] - 1
+ * of the batch hold the same first prefix_lengths[g] keys, which are read once for the group, through
+ * the block table of its longest row (the first of them), which has to hold all of the prefix that
+ * any row of the group sees; each row's own keys behind them through its own. Results are the paged decode's of the same arguments wherever that holds. groups
+ * [ngroups + 1] and prefix_lengths [ngroups] are int32 on the device, as block_table and lengths,
+ * and are read there only. Rows in front of the first group or behind the last share nothing, and
+ * no row does if groups does not go up from 0 at least to B at most; a prefix length is taken
+ * between 0 and desc->tk. */
+size_t dm_attention_decode_shared_workspace(const dm_attention_desc *desc, int64_t page_size,
+                                            int64_t ngroups);
+int dm_attention_decode_shared(const dm_attention_desc *desc, const void *q, const void *k_pages,
+                               const void *v_pages, int64_t num_pages, int64_t page_size,
+                               const int32_t *block_table, int64_t max_pages,
+                               const int32_t *lengths, const int32_t *groups, int64_t ngroups,
+                               const int32_t *prefix_lengths, void *o, void *workspace,
+                               size_t workspace_bytes, void *stream);
 
 /* The queries' and keys' norms and rotation: q_out [B, T, Hq, D] and k_out [B, T, Hkv, D],
  * contiguous. q_weight and k_weight [D] may be NULL (no weight). */
