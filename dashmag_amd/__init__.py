@@ -12,6 +12,7 @@ from .contract import (Activation, AttentionMask, AttentionOptions, CausalConv1d
                        Unsupported, Window)
 from .ops import (attention, attention_backward, attention_decode, attention_decode_packed,
                   attention_decode_paged, attention_decode_shared, attention_with_lse,
+                  cache_compact, cache_fork, cache_free, cache_reserve,
                   causal_conv1d, causal_conv1d_backward, causal_conv1d_update, chosen_logprob,
                   chosen_logprob_with_grad, linear_cross_entropy,
                   linear_cross_entropy_backward,
@@ -31,4 +32,5 @@ __all__ = [
     "chunk_gated_delta_rule", "chunk_gated_delta_rule_backward", "gated_delta_step",
     "gated_delta_step_backward",
     "QkNormRopeOptions", "qk_norm_rope", "qk_norm_rope_backward", "qk_norm_rope_paged",
+    "cache_compact", "cache_fork", "cache_free", "cache_reserve",
 ]

@@ -18,7 +18,8 @@ PROBES = ["attn_fwd_mfma", "attn_fwd_generic", "attn_bwd_mfma", "attn_bwd_generi
           "decode_split", "decode_merge", "gdr_chunk_fwd", "gdr_chunk_bwd", "gdr_step",
           "conv1d_fwd", "conv1d_bwd", "conv1d_update", "logprob", "lce_fwd", "lce_bwd",
           "gdr_chunk_fwd_mfma", "gdr_chunk_bwd_mfma", "gdr_step_bwd", "qk_norm_rope",
-          "qk_norm_rope_bwd", "decode_shared"]
+          "qk_norm_rope_bwd", "decode_shared", "cache_reserve", "cache_fork", "cache_free",
+          "cache_compact"]
 DM_ACT_NONE, DM_ACT_SILU = 0, 1
 
 
@@ -94,6 +95,18 @@ class KvPages(ctypes.Structure):
                 ("cu_seqlens", ctypes.c_void_p), ("sk", Strides), ("sv", Strides)]
 
 
+class CacheTable(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("max_pages", ctypes.c_int64),
+                ("num_pages", ctypes.c_int64), ("page_size", ctypes.c_int64),
+                ("block_table", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("refcounts", ctypes.c_void_p)]
+
+
+class CachePool(ctypes.Structure):
+    _fields_ = [("pages", ctypes.c_void_p), ("page_bytes", ctypes.c_int64),
+                ("page_stride", ctypes.c_int64)]
+
+
 #: Every symbol include/dashmi.h declares, with (restype, argtypes).
 _VP, _SZ, _I64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int64
 _AD, _GD = ctypes.POINTER(AttentionDesc), ctypes.POINTER(GdrDesc)
@@ -101,6 +114,7 @@ _CD = ctypes.POINTER(Conv1dDesc)
 _LD = ctypes.POINTER(LogprobDesc)
 _XD = ctypes.POINTER(LceDesc)
 _QD, _PD = ctypes.POINTER(QkNormRopeDesc), ctypes.POINTER(KvPages)
+_TD, _LP = ctypes.POINTER(CacheTable), ctypes.POINTER(CachePool)
 SIGNATURES = {
     "dm_last_error": (ctypes.c_char_p, []),
     "dm_describe": (ctypes.c_int, [ctypes.c_char_p, _SZ]),
@@ -153,6 +167,13 @@ SIGNATURES = {
     "dm_attention_decode_shared": (ctypes.c_int, [_AD, _VP, _VP, _VP, ctypes.c_int64, ctypes.c_int64,
                                                   _VP, ctypes.c_int64, _VP, _VP, ctypes.c_int64, _VP,
                                                   _VP, _VP, _SZ, _VP]),
+    "dm_cache_reserve_workspace": (_SZ, [_TD]),
+    "dm_cache_reserve": (ctypes.c_int, [_TD, _VP, _VP, _VP, _SZ, _VP]),
+    "dm_cache_fork_workspace": (_SZ, [_TD, _I64]),
+    "dm_cache_fork": (ctypes.c_int, [_TD, _LP, _I64, _VP, _VP, _I64, _VP, _VP, _SZ, _VP]),
+    "dm_cache_free": (ctypes.c_int, [_TD, _VP, _I64, _VP]),
+    "dm_cache_compact_workspace": (_SZ, [_TD]),
+    "dm_cache_compact": (ctypes.c_int, [_TD, _LP, _I64, _VP, _VP, _SZ, _VP]),
     "dm_qk_norm_rope": (ctypes.c_int, [_QD] + [_VP] * 8),
     "dm_qk_norm_rope_bwd_workspace": (_SZ, [_QD]),
     "dm_qk_norm_rope_bwd": (ctypes.c_int, [_QD] + [_VP] * 12 + [_SZ, _VP]),

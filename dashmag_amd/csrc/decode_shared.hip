@@ -343,12 +343,12 @@ static SharedPlan shared_plan(const dm_attention_desc *d, int64_t ngroups) {
     return p;
 }
 
-// sizes whose products below fit 64 bits, and a grid 31
+// sizes whose products below fit 64 bits, and grids of fewer than 2^32 threads
 static bool shared_sizes(const dm_attention_desc *d, int64_t ngroups) {
     const int64_t big = (int64_t)1 << 31;
     return d && d->hkv > 0 && d->b >= 0 && d->b < big && d->hq >= 0 && d->hq < 65536 && d->tk >= 0 &&
            d->tk < big && d->d >= 0 && d->d <= 256 && ngroups >= 0 && ngroups < big &&
-           (d->b + ngroups) * std::max<int64_t>(d->hq, d->hkv) < ((int64_t)1 << 28);
+           (d->b + ngroups) * std::max<int64_t>(d->hq, d->hkv) < ((int64_t)1 << 23);
 }
 
 }  // namespace dm

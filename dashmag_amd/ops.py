@@ -718,6 +718,133 @@ def _shared_arrays(op, lengths, groups, prefix_lengths, b, device):
 
 
 # ------------------------------------------------------------------------------------------
+# The pages of a cache
+# ------------------------------------------------------------------------------------------
+
+def _cache_table(op, block_table, lengths, refcounts, page_size):
+    """The table that a call changes in place: int32 arrays of one GPU, contiguous."""
+    _one_device(op, block_table, lengths, refcounts)
+    return _cache_desc(op, block_table, lengths, refcounts, page_size)
+
+
+def _cache_desc(op, block_table, lengths, refcounts, page_size):
+    for t, name, dims in ((block_table, "the block table is [R, max_pages]", 2),
+                          (lengths, "the cache lengths are [R]", 1), (refcounts, "the page counts are [P]", 1)):
+        if t.dim() != dims or t.dtype != torch.int32 or not t.is_contiguous():
+            raise Unsupported(f"{op}: {name}, contiguous int32, changed in place")
+    rows, max_pages = block_table.shape
+    if lengths.shape[0] != rows:
+        raise Unsupported(f"{op}: the cache lengths are [R] = [{rows}]")
+    if page_size < 1:
+        raise Unsupported(f"{op}: pages hold at least one key")
+    return _lib.CacheTable(rows=rows, max_pages=max_pages, num_pages=refcounts.shape[0], page_size=page_size,
+                           block_table=block_table.data_ptr(), lengths=lengths.data_ptr(),
+                           refcounts=refcounts.data_ptr())
+
+
+def _cache_pools(op, pools, num_pages, device):
+    """The pools as the C array, and their page size: tensors ``[P, page_size, ...]`` whose pages are
+    each contiguous."""
+    if isinstance(pools, torch.Tensor) or len(pools) == 0:
+        raise Unsupported(f"{op}: the pools are a list of at least one tensor [P, page_size, ...]")
+    page_size = pools[0].shape[1] if pools[0].dim() >= 2 else 0
+    arr = (_lib.CachePool * len(pools))()
+    for x, t in zip(arr, pools):
+        if t.dim() < 2 or t.shape[0] != num_pages or t.shape[1] != page_size or t.device != device:
+            raise Unsupported(f"{op}: the pools are [P, page_size, ...] with P = {num_pages} and one page_size, "
+                              f"on {device}")
+        if page_size < 1:
+            raise Unsupported(f"{op}: pages hold at least one key")
+        if not t.is_contiguous():  # (a slice of a wider pool, say: whole pages, apart)
+            if num_pages and t.numel() and not (t[0].is_contiguous() and
+                                                (num_pages == 1 or t.stride(0) >= t[0].numel())):
+                raise Unsupported(f"{op}: the pools' pages must each be contiguous and apart")
+        size = t.element_size()
+        each = t.numel() // num_pages if num_pages else 0
+        x.pages, x.page_bytes, x.page_stride = t.data_ptr(), each * size, (t.stride(0) if num_pages > 1 else each) * size
+    return arr, page_size
+
+
+def _rows_i32(op, rows, device, what):
+    r = _device_i32(op, rows, device, what)
+    if r.dim() != 1:
+        raise Unsupported(f"{op}: {what} are [N]")
+    return r
+
+
+def cache_reserve(block_table, lengths, refcounts, new_lengths, page_size):
+    """Pages for the keys that rows are about to hold: row ``r`` grows to ``new_lengths[r]`` keys
+    (no change where it holds as many), taking the free pages (``refcounts[p] == 0``) of the lowest
+    indices, the rows in order. ``block_table [R, max_pages]``, ``lengths [R]`` and ``refcounts [P]``
+    (contiguous int32 on the GPU) change in place. Returns ``granted [R]`` bool: False where the row
+    was left as it was, because the table is too narrow or the free pages fell short; once they do,
+    no later row that needs a page gets one. Nothing is read back."""
+    op = "cache_reserve"
+    desc = _cache_table(op, block_table, lengths, refcounts, page_size)
+    dev = block_table.device
+    new = _rows_i32(op, new_lengths, dev, "the new lengths")
+    if new.shape[0] != desc.rows:
+        raise Unsupported(f"{op}: the new lengths are [R] = [{desc.rows}]")
+    granted = torch.empty(desc.rows, dtype=torch.bool, device=dev)
+    nbytes = _lib.lib().dm_cache_reserve_workspace(ctypes.byref(desc))
+    ws = _workspace(nbytes, dev)
+    _run(op, dev, _lib.lib().dm_cache_reserve, ctypes.byref(desc), _ptr(new), _ptr(granted), _ptr(ws), nbytes)
+    return granted
+
+
+def cache_fork(pools, block_table, lengths, refcounts, parents, children):
+    """Row ``children[i]`` of the table becomes a second holder of row ``parents[i]``'s keys: it shares
+    the whole pages and gets a page of its own for a last one that is partly filled, whose filled rows
+    are copied in every tensor of ``pools`` (``[P, page_size, ...]``: each layer's keys and values). So
+    what either row appends goes to pages that the other does not hold. All rows are taken as they were
+    before the call; the arrays change in place, as in :func:`cache_reserve`.
+
+    Returns ``fresh [N]`` int32: the copied page, -1 where none was needed, -2 where nothing was done (a
+    row outside the table, a child that holds keys, a child named before, free pages that fell short)."""
+    op = "cache_fork"
+    dev = block_table.device
+    arr, page_size = _cache_pools(op, pools, refcounts.shape[0], dev)
+    desc = _cache_table(op, block_table, lengths, refcounts, page_size)
+    pa, ch = (_rows_i32(op, x, dev, w) for x, w in ((parents, "the parents"), (children, "the children")))
+    n = pa.shape[0]
+    if ch.shape[0] != n:
+        raise Unsupported(f"{op}: the parents and children are [N], one N")
+    fresh = torch.empty(n, dtype=torch.int32, device=dev)
+    nbytes = _lib.lib().dm_cache_fork_workspace(ctypes.byref(desc), n)
+    ws = _workspace(nbytes, dev)
+    _run(op, dev, _lib.lib().dm_cache_fork, ctypes.byref(desc), arr, len(arr), _ptr(pa), _ptr(ch), n,
+         _ptr(fresh), _ptr(ws), nbytes)
+    return fresh
+
+
+def cache_free(block_table, lengths, refcounts, rows, page_size):
+    """The ``rows`` of the table give up their pages: each is counted once less, their entries become -1
+    and their lengths 0, in place. A row outside the table, one that holds no key and one that is named
+    twice (the second time) are passed over."""
+    op = "cache_free"
+    desc = _cache_table(op, block_table, lengths, refcounts, page_size)
+    dev = block_table.device
+    r = _rows_i32(op, rows, dev, "the rows")
+    _run(op, dev, _lib.lib().dm_cache_free, ctypes.byref(desc), _ptr(r), r.shape[0])
+
+
+def cache_compact(pools, block_table, lengths, refcounts):
+    """The c pages in use moved to the indices below c, so that what lies behind is free: the k-th of the
+    pages at c or above goes to the k-th free index below it, in every tensor of ``pools``, in
+    ``refcounts`` and in the rows of ``block_table``, in place. Returns ``moved [P]`` int32: each page's
+    new index, -1 for a free one."""
+    op = "cache_compact"
+    dev = block_table.device
+    arr, page_size = _cache_pools(op, pools, refcounts.shape[0], dev)
+    desc = _cache_table(op, block_table, lengths, refcounts, page_size)
+    moved = torch.empty(desc.num_pages, dtype=torch.int32, device=dev)
+    nbytes = _lib.lib().dm_cache_compact_workspace(ctypes.byref(desc))
+    ws = _workspace(nbytes, dev)
+    _run(op, dev, _lib.lib().dm_cache_compact, ctypes.byref(desc), arr, len(arr), _ptr(moved), _ptr(ws), nbytes)
+    return moved
+
+
+# ------------------------------------------------------------------------------------------
 # Gated delta rule
 # ------------------------------------------------------------------------------------------
 

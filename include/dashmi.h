@@ -9,6 +9,7 @@
  *   dm_attention_decode  AttentionBackend::attention_decode     crates/dash-ops/src/attention.rs:732
  *   dm_attention_decode_paged  (none: the decode over a paged cache)
  *   dm_attention_decode_shared  (none: the paged decode of sequences that share prefixes)
+ *   dm_cache_reserve, _fork, _free, _compact  (none: the pages of a paged cache)
  *   dm_qk_norm_rope{,_bwd,_paged}  (none: the norms and the rotation of queries and keys that
  *                        precede the attention; the reference's callers bring them rotated)
  *   dm_gdr_chunk_fwd     ChunkGatedDeltaBackend::chunk_gated_delta_forward
@@ -208,6 +209,23 @@ typedef struct {
     dm_strides sk, sv;
 } dm_kv_pages;
 
+/* The pages of a cache: rows' pages block_table [rows, max_pages] (-1 where a row has none), the keys
+ * that a row holds lengths [rows], and how many rows hold a page, refcounts [num_pages] (a page of 0
+ * is free), int32 on the device, changed in place. A row of n keys holds its first
+ * ceil(n / page_size) entries. Only whole pages are ever shared, so what a row appends to its last,
+ * partly filled page no other row holds. Whatever the arrays hold, no page outside the pools and no
+ * entry outside the table is touched. */
+typedef struct {
+    int64_t rows, max_pages, num_pages, page_size;
+    int32_t *block_table, *lengths, *refcounts;
+} dm_cache_table;
+/* One tensor of pages (a layer's keys, its values): page p is the page_bytes from
+ * pages + p * page_stride on, its page_size rows one after another (page_bytes / page_size each). */
+typedef struct {
+    void *pages;
+    int64_t page_bytes, page_stride; /* bytes */
+} dm_cache_pool;
+
 /* The message of this thread's last refusal or error. */
 const char *dm_last_error(void);
 
@@ -253,6 +271,10 @@ typedef enum {
     DM_PROBE_QK_NORM_ROPE,       /* the queries' and keys' norms and rotation, the paged form too */
     DM_PROBE_QK_NORM_ROPE_BWD,
     DM_PROBE_DECODE_SHARED,
+    DM_PROBE_CACHE_RESERVE,
+    DM_PROBE_CACHE_FORK,
+    DM_PROBE_CACHE_FREE,
+    DM_PROBE_CACHE_COMPACT,
     DM_PROBE_COUNT
 } dm_probe;
 uint64_t dm_probe_count(int probe);
@@ -369,6 +391,35 @@ int dm_attention_decode_shared(const dm_attention_desc *desc, const void *q, con
                                const int32_t *lengths, const int32_t *groups, int64_t ngroups,
                                const int32_t *prefix_lengths, void *o, void *workspace,
                                size_t workspace_bytes, void *stream);
+
+/* Pages for what rows are about to hold: row r grows to new_lengths[r] keys (unchanged where that is
+ * no more than it holds), taking the free pages of the lowest indices, the rows in order, each page
+ * counted 1. granted [rows] (bytes): 0 where the row was left as it was, because the table has no
+ * room for so many or the free pages did not reach it: once they fall short for a row, no later row
+ * that needs a page gets one. */
+size_t dm_cache_reserve_workspace(const dm_cache_table *table);
+int dm_cache_reserve(const dm_cache_table *table, const int32_t *new_lengths, uint8_t *granted,
+                     void *workspace, size_t workspace_bytes, void *stream);
+/* Row children[i] becomes a second holder of row parents[i]'s keys, i < n: it shares the parent's
+ * whole pages, each counted once more, and gets a page of its own for a last one that is partly
+ * filled (the free pages of the lowest indices, in the order of i), whose filled rows are copied in
+ * every pool (npools of them, on the host). All rows are taken as they were before the call.
+ * fresh [n]: that page, -1 where none was needed, -2 where nothing was done: a row outside the
+ * table, a child that holds keys already, a child that an earlier fork of the call names, or free
+ * pages that fell short (for no later fork that needs one either). */
+size_t dm_cache_fork_workspace(const dm_cache_table *table, int64_t n);
+int dm_cache_fork(const dm_cache_table *table, const dm_cache_pool *pools, int64_t npools,
+                  const int32_t *parents, const int32_t *children, int64_t n, int32_t *fresh,
+                  void *workspace, size_t workspace_bytes, void *stream);
+/* The rows[0 .. n - 1] of the table give up their pages (each counted once less), hold no key and
+ * their entries are -1; a row outside the table and one that holds none are passed over. */
+int dm_cache_free(const dm_cache_table *table, const int32_t *rows, int64_t n, void *stream);
+/* The pages in use, of which there are c, moved to the indices below c: the k-th of those at c or
+ * above goes to the k-th free index below it, in every pool, in the counts and in the rows' entries.
+ * moved [num_pages]: each page's new index, -1 for a free one. */
+size_t dm_cache_compact_workspace(const dm_cache_table *table);
+int dm_cache_compact(const dm_cache_table *table, const dm_cache_pool *pools, int64_t npools,
+                     int32_t *moved, void *workspace, size_t workspace_bytes, void *stream);
 
 /* The queries' and keys' norms and rotation: q_out [B, T, Hq, D] and k_out [B, T, Hkv, D],
  * contiguous. q_weight and k_weight [D] may be NULL (no weight). */
