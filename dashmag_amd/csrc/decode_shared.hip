@@ -20,7 +20,7 @@
 namespace dm {
 
 struct SharedArgs {
-    int64_t B, S, left;
+    int32_t B, S, left;   // left: the window's, -1 for none
     int32_t hq, hkv, d, rep;
     float scale;
     const int32_t *lengths, *groups, *prefix, *block_table;
@@ -28,7 +28,7 @@ struct SharedArgs {
     int64_t page_size, max_pages, num_pages;
     int64_t qb, qh, kb, kt, kh, vb, vt, vh;
     int32_t nsp, nso;     // ranges of a prefix, and of a row's own keys
-    int64_t ptiles;       // prefix tiles of a key-value head (an upper bound, see tile_of)
+    int32_t ptiles;       // prefix tiles of a key-value head (an upper bound, see first_tile)
     int32_t otiles;       // tiles of a row's own heads
     float *part_o;        // [B, Hq, nsp + nso, D], each range's output normalised
     float *part_lse;      // [B, Hq, nsp + nso] natural log, -inf for a range without keys (its output unwritten)
@@ -36,15 +36,13 @@ struct SharedArgs {
 
 constexpr int kOwnRows = 32;  // rows of a tile of own keys
 
-__device__ __forceinline__ int64_t clamp_len(const SharedArgs &a, int64_t x) {
-    return x < 0 ? 0 : (x > a.S ? a.S : x);
-}
-__device__ __forceinline__ int64_t len_of(const SharedArgs &a, int64_t m) {
+__device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int32_t clamp_len(const SharedArgs &a, int32_t x) { return min(max(x, 0), a.S); }
+__device__ __forceinline__ int32_t len_of(const SharedArgs &a, int32_t m) {
     return a.lengths ? clamp_len(a, a.lengths[m]) : a.S;
 }
-__device__ __forceinline__ int64_t low_of(const SharedArgs &a, int64_t len) {
-    const int64_t lo = a.left >= 0 ? len - 1 - a.left : 0;
-    return lo < 0 ? 0 : lo;
+__device__ __forceinline__ int32_t low_of(const SharedArgs &a, int32_t len) {
+    return a.left >= 0 ? max(len - 1 - a.left, 0) : 0;
 }
 // The page of key j of sequence m, or -1.
 __device__ __forceinline__ int64_t shared_page(const SharedArgs &a, int64_t m, int64_t j) {
@@ -52,138 +50,137 @@ __device__ __forceinline__ int64_t shared_page(const SharedArgs &a, int64_t m, i
     return pg >= 0 && pg < a.num_pages ? pg : -1;
 }
 
-// Whether the groups go up from 0 at least to B at most. For the whole workgroup.
-__device__ __forceinline__ bool groups_ok(const SharedArgs &a) {
-    if (a.ngroups == 0) return false;
-    bool ok = true;
-    for (int i = threadIdx.x; i < a.ngroups; i += blockDim.x) {
-        const int x = a.groups[i], y = a.groups[i + 1];
-        ok = ok && x >= 0 && x <= y && y <= a.B;
-    }
-    return __syncthreads_and(ok);
-}
-
-// What a workgroup does: range `slot` of the rows r0 .. r0 + nrow - 1 (row r: member m0 + r / rep, query
-// head kh rep + r % rep) over the keys [s0, s1), which lie on `table`'s pages; a member sees those of
-// its own range that lie within [base, cap).
+// What a team of wavefronts does: range `slot` of the rows r0 .. r0 + nrow - 1 (row r: member
+// m0 + r / rep, query head kh rep + r % rep) over the keys [s0, s1), which lie on `table`'s pages; a
+// member sees those of its own range that lie in front of `cap`. Every field is the wavefront's.
 struct SharedItem {
-    int64_t m0, table, s0, s1, base, cap;
-    int32_t r0, nrow, kh, slot;
+    int32_t m0, table, s0, s1, cap, r0, nrow, kh, slot;
     bool prefix;
 };
 
-struct SharedScratch {
-    unsigned long long best[16];
-    int32_t least[16];
-};
-
-// Fills in the workgroup's item; false: there is nothing to do (its rows' part is another's, or
-// none's). unit: the ranges are multiples of this many keys (a multiple of 16). RT: rows of a prefix tile.
+// The first tile of group g, whose rows start at row s (of all rows of a key-value head): behind every
+// tile of the groups in front, since ceil(r / RT) <= floor((x + r - 1) / RT) - floor(x / RT) + 1.
 template <int RT>
-__device__ __forceinline__ bool item_of(const SharedArgs &a, int unit, SharedScratch &sc, SharedItem &it) {
-    const bool ok = groups_ok(a);
-    int64_t x = blockIdx.x;
-    it.kh = (int32_t)(x % a.hkv);
-    x /= a.hkv;
-    const int64_t np = a.ptiles * a.nsp;
-    int64_t lo, hi;
-    it.prefix = x < np;
+__device__ __forceinline__ int32_t first_tile(int32_t s, int32_t g) {
+    constexpr int shift = RT == 32 ? 5 : (RT == 128 ? 7 : 8);
+    static_assert(RT == 1 << shift, "a tile's rows");
+    return ((s - g) >> shift) + g;
+}
+
+// The item of `index`; false: it has no keys (where it is a row's to say so, that is written down). A
+// whole wavefront; with several in a team each does the same, and the first (`writes`) writes.
+// unit: ranges are multiples of this many keys (a multiple of 16). RT: rows of a prefix tile.
+template <int RT>
+__device__ __forceinline__ bool item_of(const SharedArgs &a, int32_t index, int unit, bool writes, SharedItem &it) {
+    const int lane = threadIdx.x & 63;
+    const int32_t np = a.ptiles * a.nsp;
+    uint32_t x = (uint32_t)index;
+    it.kh = (int32_t)(x % (uint32_t)a.hkv);
+    x /= (uint32_t)a.hkv;
+    it.prefix = x < (uint32_t)np;
+    int32_t b = 0, tile = 0, split, ot = 0, len = 0;
     if (it.prefix) {
-        if (!ok) return false;
-        const int64_t tile = x % a.ptiles;
-        it.slot = (int32_t)(x / a.ptiles);
-        // Group g's tiles begin at groups[g] rep / RT + g (rounded down): far enough apart for its
-        // rows, whatever the groups' sizes.
-        int32_t g0 = 0, g1 = a.ngroups - 1;
-        while (g0 < g1) {
-            const int32_t mid = (g0 + g1 + 1) >> 1;
-            if ((int64_t)a.groups[mid] * a.rep / RT + mid <= tile)
-                g0 = mid;
-            else
-                g1 = mid - 1;
+        tile = (int32_t)(x % (uint32_t)a.ptiles), split = (int32_t)(x / (uint32_t)a.ptiles);
+        it.slot = split;
+    } else {
+        x -= np;
+        b = (int32_t)(x % (uint32_t)a.B);
+        x /= (uint32_t)a.B;
+        ot = (int32_t)(x % (uint32_t)a.otiles), split = (int32_t)(x / (uint32_t)a.otiles);
+        it.slot = a.nsp + split;
+        len = len_of(a, b);
+    }
+    // the group (the first of those that hold the tile or the row), if the groups go up from 0 at least
+    // to B at most: 64 of them at a time, a lane each
+    bool ok = true;
+    int32_t g = -1, m0 = 0, m1 = 0, plen = 0;
+    for (int32_t g0 = 0; g0 < a.ngroups; g0 += 64) {
+        const int32_t i = g0 + lane;
+        const bool on = i < a.ngroups;
+        const int32_t s = on ? a.groups[i] : 0, e = on ? a.groups[i + 1] : 0, pl = on ? a.prefix[i] : 0;
+        ok = ok && s >= 0 && s <= e && e <= a.B;
+        const bool here = it.prefix ? on && first_tile<RT>(s * a.rep, i) <= tile : on && s <= b && b < e;
+        const unsigned long long v = __ballot(here);
+        if (v) {
+            const int at = it.prefix ? 63 - __builtin_clzll(v) : __builtin_ctzll(v);
+            g = g0 + at;
+            m0 = __builtin_amdgcn_readlane(s, at), m1 = __builtin_amdgcn_readlane(e, at);
+            plen = clamp_len(a, __builtin_amdgcn_readlane(pl, at));
         }
-        const int64_t m0 = a.groups[g0], m1 = a.groups[g0 + 1];
-        const int64_t first = (tile - (m0 * a.rep / RT + g0)) * RT;
-        const int64_t rows = (m1 - m0) * a.rep;
-        if (first < 0 || first >= rows) return false;
-        it.m0 = m0, it.r0 = (int32_t)first, it.nrow = (int32_t)min((int64_t)RT, rows - first);
-        it.base = 0, it.cap = clamp_len(a, a.prefix[g0]);
+    }
+    ok = __all(ok);
+    int32_t lo, hi;
+    if (it.prefix) {
+        if (!ok || g < 0) return false;
+        const int32_t first = (tile - first_tile<RT>(m0 * a.rep, g)) * RT, rows = (m1 - m0) * a.rep;
+        if (first >= rows) return false;
+        it.m0 = m0, it.r0 = first, it.nrow = min(RT, rows - first), it.cap = plen;
         // the longest member (the first of them), and the shortest that sees any key
         unsigned long long best = 0;
         int32_t least = INT32_MAX;
-        for (int64_t m = m0 + threadIdx.x; m < m1; m += blockDim.x) {
-            const int64_t len = len_of(a, m);
-            best = max(best, ((unsigned long long)len << 32) | (uint32_t)(0xffffffffu - (uint32_t)m));
-            if (len > 0) least = min(least, (int32_t)min(len, (int64_t)INT32_MAX));
+        for (int32_t m = m0 + lane; m < m1; m += 64) {
+            const int32_t l = len_of(a, m);
+            const unsigned long long k = ((unsigned long long)l << 32) | (0xffffffffu - (uint32_t)m);
+            best = best > k ? best : k;
+            if (l > 0) least = min(least, l);
         }
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) {
-            best = max(best, __shfl_xor(best, o, 64));
+            const unsigned long long k = __shfl_xor(best, o, 64);
+            best = best > k ? best : k;
             least = min(least, __shfl_xor(least, o, 64));
         }
-        const int wave = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) sc.best[wave] = best, sc.least[wave] = least;
-        __syncthreads();
-        for (int w = 0; w < (int)blockDim.x / 64; w++) best = max(best, sc.best[w]), least = min(least, sc.least[w]);
-        __syncthreads();
-        it.table = (int64_t)(0xffffffffu - (uint32_t)best);
-        const int64_t longest = (int64_t)(best >> 32);
-        hi = min(it.cap, longest);
-        lo = longest > 0 ? low_of(a, least) : 0;
+        it.table = uniform((int32_t)(0xffffffffu - (uint32_t)best));
+        const int32_t longest = uniform((int32_t)(best >> 32));
+        hi = min(plen, longest);
+        lo = longest > 0 ? low_of(a, uniform(least)) : 0;
     } else {
-        x -= np;
-        const int64_t b = x % a.B;
-        x /= a.B;
-        const int32_t ot = (int32_t)(x % a.otiles), split = (int32_t)(x / a.otiles);
+        const bool grouped = ok && g >= 0;
         it.m0 = it.table = b;
         it.r0 = ot * kOwnRows, it.nrow = min(kOwnRows, a.rep - it.r0);
-        it.slot = a.nsp + split;
-        it.base = 0, it.cap = a.S;
-        bool grouped = false;
-        if (ok) {
-            const int32_t g = sequence_of(a.groups, a.ngroups, b);
-            grouped = b >= a.groups[g] && b < a.groups[g + 1];
-            if (grouped) it.base = clamp_len(a, a.prefix[g]);
-        }
-        if (!grouped && split == 0)  // the prefix's ranges, which no other workgroup writes
-            for (int i = threadIdx.x; i < it.nrow * a.nsp; i += blockDim.x)
-                a.part_lse[(b * a.hq + it.kh * a.rep + it.r0 + i / a.nsp) * (a.nsp + a.nso) + i % a.nsp] = -INFINITY;
-        hi = len_of(a, b);
-        lo = max(it.base, low_of(a, hi));
+        it.cap = a.S;
+        if (!grouped && split == 0 && writes)  // the prefix's ranges, which no other team writes
+            for (int i = lane; i < it.nrow * a.nsp; i += 64)
+                a.part_lse[((int64_t)b * a.hq + it.kh * a.rep + it.r0 + i / a.nsp) * (a.nsp + a.nso) + i % a.nsp] =
+                    -INFINITY;
+        hi = uniform(len);
+        lo = max(grouped ? plen : 0, low_of(a, hi));
     }
-    const int64_t from = lo & ~(int64_t)15, n = it.prefix ? a.nsp : a.nso;
-    const int64_t split = it.prefix ? it.slot : it.slot - a.nsp;
-    const int64_t each = hi > from ? ((hi - from + n - 1) / n + unit - 1) / unit * unit : 0;
-    it.s0 = max(lo, from + split * each);
-    it.s1 = min(hi, from + (split + 1) * each);
-    if (it.s0 >= it.s1) {
-        for (int r = threadIdx.x; r < it.nrow; r += blockDim.x) {
+    const int32_t from = lo & ~15, n = it.prefix ? a.nsp : a.nso;
+    const int32_t each = hi > from ? (int32_t)(((uint32_t)(hi - from) + n - 1) / (uint32_t)n + unit - 1) / unit * unit : 0;
+    const int64_t start = from + (int64_t)split * each;
+    it.s0 = (int32_t)max((int64_t)lo, min(start, (int64_t)hi));
+    it.s1 = (int32_t)min((int64_t)hi, start + each);
+    if (it.s0 < it.s1) return true;
+    if (writes)
+        for (int r = lane; r < it.nrow; r += 64) {
             const int rr = it.r0 + r;
-            const int64_t row = (it.m0 + rr / a.rep) * a.hq + it.kh * a.rep + rr % a.rep;
+            const int64_t row = (int64_t)(it.m0 + rr / a.rep) * a.hq + it.kh * a.rep + rr % a.rep;
             a.part_lse[row * (a.nsp + a.nso) + it.slot] = -INFINITY;
         }
-        return false;
-    }
-    return true;
+    return false;
 }
 
 // Row r of an item (it may be past its rows): its place among the partial results, and the keys of
 // the item that it sees.
 struct SharedRow {
-    int64_t member, part;
-    int32_t head;
-    int64_t lo, hi;
+    int32_t member, head, lo, hi;
+    int64_t part;
 };
 __device__ __forceinline__ SharedRow row_of(const SharedArgs &a, const SharedItem &it, int r) {
     SharedRow w;
     const bool on = r < it.nrow;
-    const int rr = it.r0 + (on ? r : 0);
-    w.member = it.m0 + rr / a.rep;
-    w.head = it.kh * a.rep + rr % a.rep;
-    w.part = ((w.member * a.hq + w.head) * (a.nsp + a.nso)) + it.slot;
-    const int64_t len = len_of(a, w.member);
-    w.lo = max(max(low_of(a, len), it.base), it.s0);
-    w.hi = on ? min(min(len, it.cap), it.s1) : 0;
+    const uint32_t rr = it.r0 + (on ? r : 0);
+    w.member = it.m0 + (it.prefix ? (int32_t)(rr / (uint32_t)a.rep) : 0);
+    w.head = it.kh * a.rep + (int32_t)(it.prefix ? rr % (uint32_t)a.rep : rr);
+    w.part = ((int64_t)w.member * a.hq + w.head) * (a.nsp + a.nso) + it.slot;
+    w.lo = it.s0, w.hi = it.s1;
+    if (it.prefix) {
+        const int32_t len = len_of(a, w.member);
+        w.lo = max(low_of(a, len), it.s0);
+        w.hi = min(min(len, it.cap), it.s1);
+    }
+    if (!on) w.hi = 0;
     return w;
 }
 
@@ -195,15 +192,14 @@ __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const
                                                              const void *__restrict__ k,
                                                              const void *__restrict__ v) {
     __shared__ float qs[32][257], kv[kGenKeys][257], ps[32][kGenKeys + 1];
-    __shared__ SharedScratch sc;
     SharedItem it;
-    if (!item_of<32>(a, kGenKeys, sc, it)) return;
+    if (!item_of<32>(a, blockIdx.x, kGenKeys, threadIdx.x < 64, it)) return;
     const int tid = threadIdx.x, r = tid >> 3, c = tid & 7;
     const SharedRow row = row_of(a, it, r);
     for (int i = tid; i < 32 * a.d; i += 256) {
         const int x = i / a.d, e = i - x * a.d;
         const int rr = it.r0 + (x < it.nrow ? x : 0);
-        qs[x][e] = ld<DT>(q, (it.m0 + rr / a.rep) * a.qb + (it.kh * a.rep + rr % a.rep) * a.qh + e) * a.scale;
+        qs[x][e] = ld<DT>(q, (int64_t)(it.m0 + rr / a.rep) * a.qb + (it.kh * a.rep + rr % a.rep) * a.qh + e) * a.scale;
     }
     float acc[32], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -293,32 +289,46 @@ __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const
 // item's end reads zeros behind it, and a page outside the pages, or in front of the item's start,
 // reads as zeros too.
 
-template <int D>
-constexpr int shared_waves() { return D == 256 ? 4 : 8; }
+template <int D, bool WIDE>
+constexpr int shared_waves() { return D == 256 || !WIDE ? 4 : 8; }
+constexpr int kTeam = 4;  // wavefronts that take a narrow item
 
-// The pages' geometry in 32 bits: byte strides of a row, shifts where the page size is a power of two.
+// Where the keys of an item lie: byte strides of a page and of a row (keys' and values' alike).
 struct PageMap {
     const char *k, *v;  // at the item's key-value head
     const int32_t *table;
-    uint32_t kt, vt;    // bytes
-    int32_t shift;      // log2 page_size, -1 otherwise
+    uint32_t page, row;
+    uint32_t size;      // rows of a page
 };
 
-// The page of the 16-key block at key j, -1 for none or a block behind `end`.
-__device__ __forceinline__ int32_t block_page(const SharedArgs &a, const PageMap &m, int32_t j, int32_t end) {
-    if (j >= end) return -1;
-    const uint32_t at = m.shift >= 0 ? (uint32_t)j >> m.shift : (uint32_t)j / (uint32_t)a.page_size;
-    const int32_t pg = m.table[at];
-    return pg >= 0 && pg < a.num_pages ? pg : -1;
+// Walks 16-key blocks: which entry of the table a block's page is, and its first row there.
+struct Walker {
+    int32_t entry;
+    uint32_t row;
+};
+__device__ __forceinline__ Walker walk_from(const PageMap &m, int32_t j) {
+    const int32_t e = (int32_t)((uint32_t)j / m.size);
+    return Walker{uniform(e), (uint32_t)uniform((int32_t)((uint32_t)j - e * m.size))};
 }
-__device__ __forceinline__ uint32_t row_in_page(const SharedArgs &a, const PageMap &m, int32_t j) {
-    return m.shift >= 0 ? (uint32_t)j & ((1u << m.shift) - 1u) : (uint32_t)j % (uint32_t)a.page_size;
+__device__ __forceinline__ void walk(const PageMap &m, Walker &w, uint32_t keys) {
+    w.row += keys;
+    while (w.row >= m.size) w.row -= m.size, w.entry++;
 }
-// The resource of the 16-key block at key j on page pg: its rows in front of `end`.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const char *base, int64_t page_bytes, uint32_t row_bytes,
-                                                             uint32_t row, int32_t pg, int32_t j, int32_t end) {
-    const uint32_t n = (uint32_t)max(0, min(16, end - j));
-    return make_rsrc(base + (pg >= 0 ? pg * page_bytes + (int64_t)row * row_bytes : 0), pg >= 0 ? n * row_bytes : 0u);
+// A block as its loads take it: its offset, and the bytes of its rows in front of the item's end (0: a
+// page outside the pages, or nothing in front of the end). The entry comes from `peek`, called so far
+// ahead that its wait (all of the wavefront's earlier loads) costs nothing.
+struct Block {
+    uint64_t at;
+    uint32_t bytes;
+};
+__device__ __forceinline__ int32_t peek(const PageMap &m, const Walker &w, int32_t j, int32_t end) {
+    return j < end ? m.table[w.entry] : -1;
+}
+__device__ __forceinline__ Block block_of(const SharedArgs &a, const PageMap &m, int32_t entry, uint32_t row, int32_t j,
+                                          int32_t end) {
+    const int32_t pg = uniform(entry), n = min(16, end - j);
+    if (pg < 0 || pg >= a.num_pages || n <= 0) return Block{0, 0};
+    return Block{(uint64_t)(uint32_t)pg * m.page + row * m.row, (uint32_t)n * m.row};
 }
 
 template <int DT>
@@ -341,9 +351,9 @@ __device__ __forceinline__ bool take_out(uint4 &x) {
     return any;
 }
 
-template <int D>
+template <int D, bool WIDE>
 struct SharedSmem {
-    static constexpr int NW = shared_waves<D>(), KS = D + 8, VS = D + 32;
+    static constexpr int NW = shared_waves<D, WIDE>(), KS = D + 8, VS = D + 32;
     struct Narrow {
         uint16_t k[32 * KS], v[32 * VS];
     };
@@ -352,10 +362,9 @@ struct SharedSmem {
     };
     union {
         Narrow narrow[NW];
-        Wide wide;
-        float join[NW * 32 * (D + 2)];
+        Wide wide[WIDE];
+        float join[NW / kTeam][kTeam * 32 * (D + 2)];
     };
-    SharedScratch sc;
     int32_t lo[NW], hi[NW], bad;
 };
 
@@ -374,8 +383,8 @@ __device__ __forceinline__ void load_rows(const SharedArgs &a, const SharedItem 
     const int half = (threadIdx.x >> 5) & 1;
     const SharedRow row = row_of(a, it, r);
     w.on = r < it.nrow;
-    w.lo = (int32_t)row.lo, w.hi = (int32_t)max(row.hi, (int64_t)0);
-    const uint16_t *qp = (const uint16_t *)q + row.member * a.qb + (int64_t)row.head * a.qh;
+    w.lo = row.lo, w.hi = row.hi;
+    const uint16_t *qp = (const uint16_t *)q + row.member * a.qb + row.head * a.qh;
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // (the softmax below takes a scale above 0)
 #pragma unroll
     for (int s = 0; s < D / 16; s++) {
@@ -406,10 +415,11 @@ template <int DT, int D>
 __device__ __forceinline__ void add_back(const SharedArgs &a, const PageMap &m, int32_t j0, int32_t j1, int32_t lo,
                                          int32_t hi, f32x16_t (&acc)[D / 32]) {
     const int lane = threadIdx.x & 63;
-    for (int32_t j = j0; j < j1; j++) {
-        const int32_t pg = block_page(a, m, j & ~15, j1);
-        if (pg < 0 || j < lo || j >= hi) continue;
-        const uint16_t *row = (const uint16_t *)(m.v + pg * a.vb * 2 + (int64_t)row_in_page(a, m, j) * m.vt);
+    Walker w = walk_from(m, j0);
+    for (int32_t j = j0; j < j1; j++, walk(m, w, 1)) {
+        const int32_t pg = uniform(m.table[w.entry]);
+        if (pg < 0 || pg >= a.num_pages || j < lo || j >= hi) continue;
+        const uint16_t *row = (const uint16_t *)(m.v + (uint64_t)(uint32_t)pg * m.page + w.row * m.row);
 #pragma unroll
         for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
@@ -428,53 +438,61 @@ struct Partial {
     float m, l;
 };
 
-template <int DT, int D>
-__device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedItem &it, const PageMap &map,
-                                              const void *q, SharedSmem<D> &sm) {
-    constexpr int NW = shared_waves<D>(), KS = SharedSmem<D>::KS, VS = SharedSmem<D>::VS;
+// (`has`: the team has an item. Teams of a workgroup meet at its barriers, so one without passes them too.)
+template <int DT, int D, bool WIDE>
+__device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedItem &it, bool has, const PageMap &map,
+                                              const void *q, SharedSmem<D, WIDE> &sm) {
+    constexpr int NW = kTeam, KS = SharedSmem<D, WIDE>::KS, VS = SharedSmem<D, WIDE>::VS;
     constexpr int LPR = D / 8, RPL = 64 / LPR, NLD = 32 / RPL;  // lanes a row, rows a load, loads
     constexpr int KST = D / 16, DTN = D / 32;
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = uniform(threadIdx.x >> 6) % kTeam, team = uniform(threadIdx.x >> 6) / kTeam;
     RowState<D> rs;
-    load_rows<DT, D>(a, it, q, col, true, rs);
     const float qscale = fabsf(a.scale) * 1.4426950408889634f;
-    const int32_t s0 = (int32_t)it.s0, s1 = (int32_t)it.s1, a0 = s0 & ~15;
-    const int32_t per = ((s1 - a0 + NW - 1) / NW + 31) & ~31;
-    const int32_t w0 = max(s0, a0 + wave * per), w1 = min(s1, a0 + (wave + 1) * per), b0 = w0 & ~15;
-    typename SharedSmem<D>::Narrow &t = sm.narrow[wave];
-    uint4 sk[NLD], sv[NLD];
-    int32_t pg[2];
-    auto pages = [&](int32_t j) __attribute__((always_inline)) {
-        pg[0] = block_page(a, map, j, w1);
-        pg[1] = block_page(a, map, j + 16, w1);
-    };
-    auto load = [&](int32_t j0) __attribute__((always_inline)) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int32_t j = j0 + 16 * h;
-            const uint32_t row = pg[h] >= 0 ? row_in_page(a, map, j) : 0u;
-            const __amdgpu_buffer_rsrc_t kr = block_rsrc(map.k, a.kb * 2, map.kt, row, pg[h], j, w1);
-            const __amdgpu_buffer_rsrc_t vr = block_rsrc(map.v, a.vb * 2, map.vt, row, pg[h], j, w1);
-#pragma unroll
-            for (int u = h * NLD / 2; u < (h + 1) * NLD / 2; u++) {
-                const uint32_t r = RPL * u - 16 * h + lane / LPR, c = (lane % LPR) * 16;
-                const bool in = j + (int32_t)r >= w0;
-                sk[u] = buf_load16_nt(kr, in ? r * map.kt + c : 0xffffffffu);
-                sv[u] = buf_load16_nt(vr, in ? r * map.vt + c : 0xffffffffu);
-            }
-        }
-    };
     Partial<D> p;
     p.m = -INFINITY, p.l = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DTN; dt++) p.acc[dt] = zero16();
+    const int32_t s0 = it.s0, s1 = it.s1, a0 = s0 & ~15;
+    const int32_t per = ((s1 - a0 + NW - 1) / NW + 31) & ~31;
+    const int32_t w0 = max(s0, a0 + wave * per), w1 = has ? min(s1, a0 + (wave + 1) * per) : 0, b0 = w0 & ~15;
+    typename SharedSmem<D, WIDE>::Narrow &t = sm.narrow[team * kTeam + wave];
+    uint4 sk[NLD], sv[NLD];
+    Walker at[2];
+    int32_t entry[2];
+    auto load = [&](int32_t j0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int32_t j = j0 + 16 * h;
+            const Block blk = block_of(a, map, entry[h], at[h].row, j, w1);
+            const __amdgpu_buffer_rsrc_t kr = make_rsrc(map.k + blk.at, blk.bytes), vr = make_rsrc(map.v + blk.at, blk.bytes);
+#pragma unroll
+            for (int u = h * NLD / 2; u < (h + 1) * NLD / 2; u++) {
+                const uint32_t r = RPL * u - 16 * h + lane / LPR;
+                const uint32_t off = j + (int32_t)r >= w0 ? r * map.row + (lane % LPR) * 16 : 0xffffffffu;
+                sk[u] = buf_load16_nt(kr, off);
+                sv[u] = buf_load16_nt(vr, off);
+            }
+        }
+    };
+    auto ahead = [&](int32_t j0) __attribute__((always_inline)) {  // the entries of the block at j0, the next one
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            walk(map, at[h], 32);
+            entry[h] = peek(map, at[h], j0 + 16 * h, w1);
+        }
+    };
     bool bad = false;
     if (w0 < w1) {
         const int nblk = (w1 - b0 + 31) / 32;
-        pages(b0);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            at[h] = walk_from(map, b0 + 16 * h);
+            entry[h] = peek(map, at[h], b0 + 16 * h, w1);
+        }
         load(b0);
-        pages(b0 + 32);
+        ahead(b0 + 32);
+        load_rows<DT, D>(a, it, q, col, true, rs);
         for (int n = 0; n < nblk; n++) {
             const int32_t j0 = b0 + n * 32;
             const bool cut = j0 < rs.flo || j0 + 32 > rs.fhi;
@@ -489,7 +507,7 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
                 *(uint4 *)(t.v + r * VS + c) = sv[u];
             }
             load(j0 + 32);
-            pages(j0 + 64);
+            ahead(j0 + 64);
             f32x16_t sc = zero16();
 #pragma unroll
             for (int st = 0; st < KST; st++) sc = mfma32<DT>(row_frag(t.k, KS, 0, st * 16, lane), rs.qf[st], sc);
@@ -536,8 +554,8 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
     const float l = p.l + __shfl_xor(p.l, 32, 64);
     // the wavefronts' results joined through LDS: [wave][row][D], their references and sums behind
     __syncthreads();
-    float *sa = sm.join, *sm_m = sa + NW * 32 * D, *sm_l = sm_m + NW * 32;
-    if (col < it.nrow) {
+    float *sa = sm.join[team], *sm_m = sa + NW * 32 * D, *sm_l = sm_m + NW * 32;
+    if (has && col < it.nrow) {
 #pragma unroll
         for (int dt = 0; dt < DTN; dt++)
 #pragma unroll
@@ -547,7 +565,8 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
         if (half == 0) sm_m[wave * 32 + col] = p.m, sm_l[wave * 32 + col] = l;
     }
     __syncthreads();
-    for (int x = threadIdx.x; x < it.nrow * (D / 4); x += NW * 64) {
+    if (!has) return;
+    for (int x = wave * 64 + lane; x < it.nrow * (D / 4); x += NW * 64) {
         const int r = x / (D / 4), d = x % (D / 4) * 4;
         float M = -INFINITY;
         for (int w = 0; w < NW; w++) M = fmaxf(M, sm_m[w * 32 + r]);
@@ -572,8 +591,8 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
 
 template <int DT, int D>
 __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedItem &it, const PageMap &map,
-                                            const void *q, SharedSmem<D> &sm) {
-    constexpr int NW = shared_waves<D>(), NT = NW * 64, KS = SharedSmem<D>::KS, VS = SharedSmem<D>::VS;
+                                            const void *q, SharedSmem<D, true> &sm) {
+    constexpr int NW = shared_waves<D, true>(), NT = NW * 64, KS = SharedSmem<D, true>::KS, VS = SharedSmem<D, true>::VS;
     constexpr int CPR = D / 8, RPW = 64 / CPR, RSTEP = NT / CPR, NCH = 64 / RSTEP;  // pieces a row, rows a wavefront
     constexpr int KST = D / 16, DTN = D / 32;
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
@@ -592,41 +611,45 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
 #pragma unroll
     for (int w = 0; w < NW; w++) tlo = max(tlo, sm.lo[w]), thi = min(thi, sm.hi[w]);
     tlo = __builtin_amdgcn_readfirstlane(tlo), thi = __builtin_amdgcn_readfirstlane(thi);
-    const int32_t s0 = (int32_t)it.s0, s1 = (int32_t)it.s1, k0 = s0 & ~15;
+    const int32_t s0 = it.s0, s1 = it.s1, k0 = s0 & ~15;
     const int32_t nt = (s1 - k0 + 63) / 64;
     const float c2 = fabsf(a.scale) * 1.4426950408889634f;
 
     // staging: NCH pieces of a tile's K and of its V a thread; a wavefront's rows of a piece lie in one
-    // 16-key block, whose page is looked up a step before its keys are loaded, and two before its values
+    // 16-key block, of which it has NB a tile. A block's entry in the table is read a step before its
+    // keys are loaded, and its place kept for its values another step later.
+    constexpr int NB = NCH < 4 ? NCH : 4, PB = NCH / NB;
     const int wr = wave * RPW, lr = lane / CPR, lc = lane % CPR;
     uint4 rk[NCH], rv[NCH];
-    int32_t pk[NCH], pn[NCH];
-    auto tile_key = [&](int32_t j) { return k0 + min(j, nt - 1) * 64; };
-    auto look_up = [&](int32_t j) __attribute__((always_inline)) {
+    Walker at[NB];
+    int32_t entry[NB];
+    Block vb[NB];  // the tile whose values are loaded next
+    auto block_key = [&](int32_t j, int n) { return k0 + j * 64 + ((wr + n * PB * RSTEP) & ~15); };
+    auto peek_at = [&](int32_t j) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < NCH; u++) pn[u] = block_page(a, map, tile_key(j) + ((wr + u * RSTEP) & ~15), s1);
+        for (int n = 0; n < NB; n++) entry[n] = peek(map, at[n], block_key(j, n), s1);
     };
-    auto load = [&](int32_t j, const char *base, int64_t page_bytes, uint32_t row_bytes, const int32_t (&pg)[NCH],
-                    uint4 (&x)[NCH]) __attribute__((always_inline)) {
+    auto load = [&](int32_t j, const char *base, const Block (&b)[NB], uint4 (&x)[NCH]) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < NCH; u++) {
-            const int32_t b = tile_key(j) + ((wr + u * RSTEP) & ~15);
             const uint32_t r = ((wr + u * RSTEP) & 15) + lr;
-            const __amdgpu_buffer_rsrc_t rs_ = block_rsrc(base, page_bytes, row_bytes,
-                                                          pg[u] >= 0 ? row_in_page(a, map, b) : 0u, pg[u], b, s1);
-            x[u] = buf_load16(rs_, b + (int32_t)r >= s0 ? r * row_bytes + lc * 16 : 0xffffffffu);
+            x[u] = buf_load16(make_rsrc(base + b[u / PB].at, b[u / PB].bytes),
+                              block_key(j, u / PB) + (int32_t)r >= s0 ? r * map.row + lc * 16 : 0xffffffffu);
         }
     };
-    auto load_k = [&](int32_t j) __attribute__((always_inline)) { load(j, map.k, a.kb * 2, map.kt, pn, rk); };
-    auto load_v = [&](int32_t j) __attribute__((always_inline)) { load(j, map.v, a.vb * 2, map.vt, pk, rv); };
-    auto next_pages = [&](int32_t j) __attribute__((always_inline)) {
+    auto load_v = [&](int32_t j) __attribute__((always_inline)) { load(j, map.v, vb, rv); };
+    // the keys of tile j, whose entries were read; then the entries of the tile behind it
+    auto load_k = [&](int32_t j) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < NCH; u++) pk[u] = pn[u];
-        look_up(j);
+        for (int n = 0; n < NB; n++) vb[n] = block_of(a, map, entry[n], at[n].row, block_key(j, n), s1);
+        load(j, map.k, vb, rk);
+#pragma unroll
+        for (int n = 0; n < NB; n++) walk(map, at[n], 64);
+        peek_at(j + 1);
     };
     auto store_k = [&](int32_t j) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < NCH; u++) *(uint4 *)(sm.wide.k[j & 1] + (wr + u * RSTEP + lr) * KS + lc * 8) = rk[u];
+        for (int u = 0; u < NCH; u++) *(uint4 *)(sm.wide[0].k[j & 1] + (wr + u * RSTEP + lr) * KS + lc * 8) = rk[u];
     };
     auto store_v = [&](int32_t j) __attribute__((always_inline)) {
         const int32_t t = k0 + j * 64;
@@ -637,7 +660,7 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
             if (__any(bad) && lane == 0) sm.bad = 1;
         }
 #pragma unroll
-        for (int u = 0; u < NCH; u++) *(uint4 *)(sm.wide.v[j & 1] + (wr + u * RSTEP + lr) * VS + lc * 8) = rv[u];
+        for (int u = 0; u < NCH; u++) *(uint4 *)(sm.wide[0].v[j & 1] + (wr + u * RSTEP + lr) * VS + lc * 8) = rv[u];
     };
     Partial<D> p;
     p.m = -INFINITY, p.l = 0.f;
@@ -648,7 +671,7 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
     auto products = [&](int32_t j) __attribute__((always_inline)) {
         __builtin_amdgcn_s_setprio(1);
         if (rows && j < nt) {
-            const uint16_t *sk = sm.wide.k[j & 1];
+            const uint16_t *sk = sm.wide[0].k[j & 1];
 #pragma unroll
             for (int t = 0; t < 2; t++) s[t] = zero16();
 #pragma unroll
@@ -662,7 +685,7 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
         }
         __builtin_amdgcn_sched_barrier(0);
         if (rows && j > 0) {
-            const uint16_t *v = sm.wide.v[(j - 1) & 1];
+            const uint16_t *v = sm.wide[0].v[(j - 1) & 1];
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -681,7 +704,7 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int32_t j = j0 + t * 32 + crow(i, lane);
-                    s[t][i] = (j >= rs.lo) & (j < rs.hi) ? s[t][i] : -INFINITY;
+                    s[t][i] = ((j >= rs.lo) & (j < rs.hi)) ? s[t][i] : -INFINITY;
                 }
         }
         float tmax = -INFINITY;
@@ -725,15 +748,14 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
         store_v(j + ahead);
         load_v(j + 1 + ahead);
         load_k(j + 2 + ahead);
-        next_pages(j + 3 + ahead);
     };
-    look_up(0);
+#pragma unroll
+    for (int n = 0; n < NB; n++) at[n] = walk_from(map, block_key(0, n));
+    peek_at(0);
     load_k(0);
     store_k(0);
-    next_pages(1);
     load_v(0);
     load_k(1);
-    next_pages(2);
     __syncthreads();
     if (!first) {
         stage(-1);
@@ -769,23 +791,32 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
 }
 
 template <int DT, int D, bool WIDE>
-__global__ __launch_bounds__(64 * shared_waves<D>(), 1) void decode_shared_mfma(SharedArgs a,
-                                                                                  const void *__restrict__ q,
-                                                                                  const void *__restrict__ k,
-                                                                                  const void *__restrict__ v) {
-    __shared__ SharedSmem<D> sm;
-    SharedItem it;
-    if (!item_of<WIDE ? 32 * shared_waves<D>() : 32>(a, WIDE ? 64 : 32, sm.sc, it)) return;
+__global__ __launch_bounds__((64 * shared_waves<D, WIDE>()), (D == 256 ? 1 : 2)) void decode_shared_mfma(SharedArgs a, int32_t items,
+                                                                                        const void *__restrict__ q,
+                                                                                        const void *__restrict__ k,
+                                                                                        const void *__restrict__ v) {
+    constexpr int TEAMS = shared_waves<D, WIDE>() / kTeam, RT = WIDE ? 32 * shared_waves<D, WIDE>() : 32;
+    __shared__ SharedSmem<D, WIDE> sm;
+    // the wide items first, a workgroup each, then the others, a team each
+    const int32_t np = WIDE ? a.ptiles * a.nsp * a.hkv : 0;
+    const int wave = uniform(threadIdx.x >> 6);
+    const bool wide = WIDE && (int32_t)blockIdx.x < np;
+    const int32_t index = wide ? (int32_t)blockIdx.x : np + ((int32_t)blockIdx.x - np) * TEAMS + wave / kTeam;
+    SharedItem it{};
+    const bool has = index < items && item_of<RT>(a, index, wide ? 64 : 32, wave % (wide ? 8 : kTeam) == 0, it);
+    if (wide && !has) return;
     PageMap map;
     map.k = (const char *)k + (int64_t)it.kh * a.kh * 2;
     map.v = (const char *)v + (int64_t)it.kh * a.vh * 2;
     map.table = a.block_table + it.table * a.max_pages;
-    map.kt = (uint32_t)(a.kt * 2), map.vt = (uint32_t)(a.vt * 2);
-    map.shift = (a.page_size & (a.page_size - 1)) ? -1 : __builtin_ctzll(a.page_size);
-    if (WIDE && it.prefix)
-        shared_wide<DT, D>(a, it, map, q, sm);
-    else
-        shared_narrow<DT, D>(a, it, map, q, sm);
+    map.page = (uint32_t)(a.kb * 2), map.row = (uint32_t)(a.kt * 2), map.size = (uint32_t)a.page_size;
+    if constexpr (WIDE) {
+        if (wide) {
+            shared_wide<DT, D>(a, it, map, q, sm);
+            return;
+        }
+    }
+    shared_narrow<DT, D, WIDE>(a, it, has, map, q, sm);
 }
 
 // The ranges of a row joined, a workgroup a row: its four wavefronts take every fourth range each, a
@@ -835,16 +866,16 @@ __global__ __launch_bounds__(256) void decode_shared_merge(SharedArgs a, void *_
     }
 }
 
-// The 16-bit kernel's calls: rows in 16-byte pieces, a block's bytes in 32 bits.
+// The 16-bit kernel's calls: 16-byte pieces, keys' and values' pages laid out alike, a page under 2 GB.
 static bool shared_mfma_takes(const dm_attention_desc *d, int64_t page_size) {
     if ((d->dtype != DM_BF16 && d->dtype != DM_F16) || (d->d != 64 && d->d != 128 && d->d != 256) ||
         page_size % 16 != 0)
         return false;
-    if (!d->strided) return true;
-    auto ok = [&](const dm_strides &x) {
-        return x.b % 8 == 0 && x.t % 8 == 0 && x.h % 8 == 0 && x.t >= d->d && x.t < ((int64_t)1 << 24);
-    };
-    return d->sq.b % 8 == 0 && d->sq.h % 8 == 0 && ok(d->sk) && ok(d->sv);
+    const int64_t most = (int64_t)1 << 30;
+    if (!d->strided) return d->hkv * d->d < most / page_size;
+    const dm_strides &k = d->sk, &v = d->sv;
+    return d->sq.b % 8 == 0 && d->sq.h % 8 == 0 && k.b % 8 == 0 && k.t % 8 == 0 && k.h % 8 == 0 && v.h % 8 == 0 &&
+           k.b == v.b && k.t == v.t && k.t >= d->d && k.b < most && k.t < most / page_size;
 }
 
 // The split of a call: ranges of the prefixes and of the rows' own keys, so that there are about
@@ -855,13 +886,15 @@ struct SharedPlan {
     int32_t rows;  // rows of a prefix tile
     int64_t ptiles;
     int32_t otiles, nsp, nso;
+    int64_t items;
 };
 static SharedPlan shared_plan(const dm_attention_desc *d, bool mfma, int64_t ngroups) {
     SharedPlan p{};
     const int64_t rep = d->hq / d->hkv;
     p.wide = mfma && ngroups > 0 && d->b * rep > 32 * ngroups;
     p.rows = p.wide ? (d->d == 256 ? 128 : 256) : 32;
-    p.ptiles = ngroups > 0 ? d->b * rep / p.rows + ngroups : 0;
+    // (first_tile of the group behind the last)
+    p.ptiles = ngroups > 0 && d->b * rep > 0 ? std::max<int64_t>(0, (d->b * rep - ngroups) / p.rows) + ngroups : 0;
     p.otiles = (int32_t)((rep + kOwnRows - 1) / kOwnRows);
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kSharedSplits / 2, (d->tk + 127) / 128));
     auto split = [&](int64_t tiles) {
@@ -869,6 +902,7 @@ static SharedPlan shared_plan(const dm_attention_desc *d, bool mfma, int64_t ngr
     };
     p.nsp = split(p.ptiles * d->hkv);
     p.nso = split(d->b * p.otiles * d->hkv);
+    p.items = (p.ptiles * p.nsp + d->b * p.otiles * p.nso) * d->hkv;
     return p;
 }
 
@@ -923,7 +957,7 @@ int dm_attention_decode_shared(const dm_attention_desc *d, const void *q, const 
     const bool mfma = shared_mfma_takes(d, page_size) && aligned_16b(q) && aligned_16b(k_pages) && aligned_16b(v_pages);
     const SharedPlan p = shared_plan(d, mfma, ngroups);
     SharedArgs a{};
-    a.B = d->b, a.S = d->tk, a.left = left_of(d);
+    a.B = (int32_t)d->b, a.S = (int32_t)d->tk, a.left = (int32_t)left_of(d);
     a.hq = (int32_t)d->hq, a.hkv = (int32_t)d->hkv, a.d = (int32_t)d->d, a.rep = (int32_t)(d->hq / d->hkv);
     a.scale = scale_of(d);
     a.lengths = lengths, a.groups = groups, a.prefix = prefix_lengths, a.block_table = block_table;
@@ -938,17 +972,19 @@ int dm_attention_decode_shared(const dm_attention_desc *d, const void *q, const 
         a.qb = d->hq * d->d, a.qh = d->d;
         a.kb = a.vb = page_size * row, a.kt = a.vt = row, a.kh = a.vh = d->d;
     }
-    a.nsp = p.nsp, a.nso = p.nso, a.ptiles = p.ptiles, a.otiles = p.otiles;
+    a.nsp = p.nsp, a.nso = p.nso, a.ptiles = (int32_t)p.ptiles, a.otiles = p.otiles;
     const size_t parts = (size_t)rows * (p.nsp + p.nso);
     a.part_o = (float *)workspace;
     a.part_lse = (float *)((char *)workspace + align_up(parts * d->d * sizeof(float)));
-    const int64_t grid = (p.ptiles * p.nsp + d->b * p.otiles * p.nso) * d->hkv;
-    const unsigned g = (unsigned)grid;
+    const int32_t items = (int32_t)p.items;
+    // (a workgroup of two teams takes two narrow items, see decode_shared_mfma)
+    const int64_t np = p.wide ? p.ptiles * p.nsp * d->hkv : 0, teams = p.wide && d->d != 256 ? 2 : 1;
+    const unsigned g = (unsigned)(np + (p.items - np + teams - 1) / teams);
 #define SHARED_W(DT, D)                                                                            \
     if (p.wide)                                                                                    \
-        decode_shared_mfma<DT, D, true><<<g, 64 * shared_waves<D>(), 0, st>>>(a, q, k_pages, v_pages); \
+        decode_shared_mfma<DT, D, true><<<g, 64 * shared_waves<D, true>(), 0, st>>>(a, items, q, k_pages, v_pages); \
     else                                                                                           \
-        decode_shared_mfma<DT, D, false><<<g, 64 * shared_waves<D>(), 0, st>>>(a, q, k_pages, v_pages)
+        decode_shared_mfma<DT, D, false><<<g, 64 * shared_waves<D, false>(), 0, st>>>(a, items, q, k_pages, v_pages)
 #define SHARED(DT)                                                             \
     if (!mfma) {                                                               \
         decode_shared_generic<DT><<<g, 256, 0, st>>>(a, q, k_pages, v_pages);  \
