@@ -115,25 +115,25 @@ __device__ __forceinline__ bool item_of(const SharedArgs &a, int32_t index, int 
         const int32_t first = (tile - first_tile<RT>(m0 * a.rep, g)) * RT, rows = (m1 - m0) * a.rep;
         if (first >= rows) return false;
         it.m0 = m0, it.r0 = first, it.nrow = min(RT, rows - first), it.cap = plen;
-        // the longest member (the first of them), and the shortest that sees any key
-        unsigned long long best = 0;
-        int32_t least = INT32_MAX;
+        // the longest member, and the shortest that sees any key
+        int32_t most = -1, least = INT32_MAX, at = 0;
         for (int32_t m = m0 + lane; m < m1; m += 64) {
             const int32_t l = len_of(a, m);
-            const unsigned long long k = ((unsigned long long)l << 32) | (0xffffffffu - (uint32_t)m);
-            best = best > k ? best : k;
+            if (l > most) most = l, at = m;
             if (l > 0) least = min(least, l);
         }
+        int32_t longest = most;
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
-            const unsigned long long k = __shfl_xor(best, o, 64);
-            best = best > k ? best : k;
-            least = min(least, __shfl_xor(least, o, 64));
-        }
-        it.table = uniform((int32_t)(0xffffffffu - (uint32_t)best));
-        const int32_t longest = uniform((int32_t)(best >> 32));
+        for (int o = 32; o >= 1; o >>= 1) longest = max(longest, __shfl_xor(longest, o, 64));
+        longest = uniform(longest);
+        it.table = __builtin_amdgcn_readlane(at, __builtin_ctzll(__ballot(most == longest)));
         hi = min(plen, longest);
-        lo = longest > 0 ? low_of(a, uniform(least)) : 0;
+        lo = 0;
+        if (a.left >= 0 && longest > 0) {
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) least = min(least, __shfl_xor(least, o, 64));
+            lo = low_of(a, uniform(least));
+        }
     } else {
         const bool grouped = ok && g >= 0;
         it.m0 = it.table = b;
@@ -301,53 +301,33 @@ struct PageMap {
     uint32_t size;      // rows of a page
 };
 
-// Walks 16-key blocks: which entry of the table a block's page is, and its first row there.
-struct Walker {
-    int32_t entry;
-    uint32_t row;
-};
-__device__ __forceinline__ Walker walk_from(const PageMap &m, int32_t j) {
-    const int32_t e = (int32_t)((uint32_t)j / m.size);
-    return Walker{uniform(e), (uint32_t)uniform((int32_t)((uint32_t)j - e * m.size))};
-}
-__device__ __forceinline__ void walk(const PageMap &m, Walker &w, uint32_t keys) {
-    w.row += keys;
-    while (w.row >= m.size) w.row -= m.size, w.entry++;
-}
-// A block as its loads take it: its offset, and the bytes of its rows in front of the item's end (0: a
-// page outside the pages, or nothing in front of the end). The entry comes from `peek`, called so far
-// ahead that its wait (all of the wavefront's earlier loads) costs nothing.
-struct Block {
-    uint64_t at;
-    uint32_t bytes;
-};
-__device__ __forceinline__ int32_t peek(const PageMap &m, const Walker &w, int32_t j, int32_t end) {
-    return j < end ? m.table[w.entry] : -1;
-}
-__device__ __forceinline__ Block block_of(const SharedArgs &a, const PageMap &m, int32_t entry, uint32_t row, int32_t j,
-                                          int32_t end) {
-    const int32_t pg = uniform(entry), n = min(16, end - j);
-    if (pg < 0 || pg >= a.num_pages || n <= 0) return Block{0, 0};
-    return Block{(uint64_t)(uint32_t)pg * m.page + row * m.row, (uint32_t)n * m.row};
+// The offset of the 16-key block at key j, kNoBlock for a page outside the pages or a block behind `end`.
+constexpr uint64_t kNoBlock = ~(uint64_t)0;
+__device__ __forceinline__ uint64_t block_at(const SharedArgs &a, const PageMap &m, int32_t j, int32_t end) {
+    if (j >= end) return kNoBlock;
+    const uint32_t e = (uint32_t)j / m.size;
+    const int32_t pg = m.table[e];
+    return pg >= 0 && pg < a.num_pages ? (uint64_t)(uint32_t)pg * m.page + ((uint32_t)j - e * m.size) * m.row : kNoBlock;
 }
 
+// All ones in each 16-bit half of w that is not finite: its exponent plus one carries into the sign's
+// place. (Arithmetic alone: a comparison an element would hold a mask of lanes for each.)
 template <int DT>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-    constexpr uint32_t e = DT == DM_BF16 ? 0x7f80u : 0x7c00u;
-    return (w & e) == e || ((w >> 16) & e) == e;
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    constexpr uint32_t e = DT == DM_BF16 ? 0x7f807f80u : 0x7c007c00u, one = DT == DM_BF16 ? 0x00800080u : 0x04000400u;
+    const uint32_t m = ((w & e) + one) & 0x80008000u;
+    return (m - (m >> 15)) | m;
 }
 // Values that are not finite taken out of a piece of V (whoever sees them adds them at the end).
 template <int DT>
-__device__ __forceinline__ bool take_out(uint4 &x) {
-    constexpr uint32_t e = DT == DM_BF16 ? 0x7f80u : 0x7c00u;
-    bool any = false;
-    uint32_t *w = (uint32_t *)&x;
+__device__ __forceinline__ uint32_t take_out(uint4 &x) {
+    uint32_t *w = (uint32_t *)&x, any = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (not_finite<DT>(w[i])) {
-            any = true;
-            w[i] &= ((w[i] & e) == e ? 0u : 0xffffu) | ((((w[i] >> 16) & e) == e) ? 0u : 0xffff0000u);
-        }
+    for (int i = 0; i < 4; i++) {
+        const uint32_t m = not_finite<DT>(w[i]);
+        w[i] &= ~m;
+        any |= m;
+    }
     return any;
 }
 
@@ -355,17 +335,18 @@ template <int D, bool WIDE>
 struct SharedSmem {
     static constexpr int NW = shared_waves<D, WIDE>(), KS = D + 8, VS = D + 32;
     struct Narrow {
-        uint16_t k[32 * KS], v[32 * VS];
+        alignas(16) uint16_t k[32 * KS], v[32 * VS];
     };
     struct Wide {
-        uint16_t k[2][64 * KS], v[2][64 * VS];
+        alignas(16) uint16_t k[2][64 * KS], v[2][64 * VS];
     };
     union {
         Narrow narrow[NW];
         Wide wide[WIDE];
-        float join[NW / kTeam][kTeam * 32 * (D + 2)];
+        alignas(16) float join[NW / kTeam][kTeam * 32 * (D + 2)];
     };
     int32_t lo[NW], hi[NW], bad;
+    uint64_t blocks[WIDE ? 512 : 1];  // wide: the offsets of 128 tiles' blocks, see fill
 };
 
 // What the lanes of a wavefront know of their rows: the queries as the second operand, and the keys seen.
@@ -415,18 +396,21 @@ template <int DT, int D>
 __device__ __forceinline__ void add_back(const SharedArgs &a, const PageMap &m, int32_t j0, int32_t j1, int32_t lo,
                                          int32_t hi, f32x16_t (&acc)[D / 32]) {
     const int lane = threadIdx.x & 63;
-    Walker w = walk_from(m, j0);
-    for (int32_t j = j0; j < j1; j++, walk(m, w, 1)) {
-        const int32_t pg = uniform(m.table[w.entry]);
-        if (pg < 0 || pg >= a.num_pages || j < lo || j >= hi) continue;
-        const uint16_t *row = (const uint16_t *)(m.v + (uint64_t)(uint32_t)pg * m.page + w.row * m.row);
+    for (int32_t j = j0; j < j1; j++) {
+        const uint64_t at = block_at(a, m, j, j1);
+        if (at == kNoBlock || j < lo || j >= hi) continue;
+        const uint16_t *row = (const uint16_t *)(m.v + at);
 #pragma unroll
-        for (int dt = 0; dt < D / 32; dt++)
+        for (int dt = 0; dt < D / 32; dt++) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const uint32_t x = row[dt * 32 + crow(i, lane)];
-                if (not_finite<DT>(x)) acc[dt][i] += unpack_lo<DT>(x);
+            for (int i = 0; i < 16; i += 2) {
+                uint32_t x = *(const uint32_t *)(row + dt * 32 + crow(i, lane));  // elements i and i + 1
+                x &= not_finite<DT>(x);
+                acc[dt][i] += unpack_lo<DT>(x);
+                acc[dt][i + 1] += unpack_hi<DT>(x);
             }
+            __builtin_amdgcn_sched_barrier(0);  // (with every load of a row up front the registers run out)
+        }
     }
 }
 
@@ -458,14 +442,19 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
     const int32_t w0 = max(s0, a0 + wave * per), w1 = has ? min(s1, a0 + (wave + 1) * per) : 0, b0 = w0 & ~15;
     typename SharedSmem<D, WIDE>::Narrow &t = sm.narrow[team * kTeam + wave];
     uint4 sk[NLD], sv[NLD];
-    Walker at[2];
-    int32_t entry[2];
-    auto load = [&](int32_t j0) __attribute__((always_inline)) {
+    // the offsets of 64 blocks of 16 keys from block `from` on, a lane each
+    uint64_t at;
+    auto look_up = [&](int32_t from) __attribute__((always_inline)) { at = block_at(a, map, b0 + 16 * (from + lane), w1); };
+    auto load = [&](int32_t n) __attribute__((always_inline)) {  // the n-th 32 keys
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int32_t j = j0 + 16 * h;
-            const Block blk = block_of(a, map, entry[h], at[h].row, j, w1);
-            const __amdgpu_buffer_rsrc_t kr = make_rsrc(map.k + blk.at, blk.bytes), vr = make_rsrc(map.v + blk.at, blk.bytes);
+            const int32_t j = b0 + 32 * n + 16 * h, i = (2 * n + h) & 63;
+            const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at, i);
+            const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(at >> 32), i);
+            const bool none = hi == 0xffffffffu;
+            const uint64_t from = none ? 0 : ((uint64_t)hi << 32) | lo;
+            const uint32_t bytes = uniform(none ? 0 : max(0, min(16, w1 - j))) * map.row;
+            const __amdgpu_buffer_rsrc_t kr = make_rsrc(map.k + from, bytes), vr = make_rsrc(map.v + from, bytes);
 #pragma unroll
             for (int u = h * NLD / 2; u < (h + 1) * NLD / 2; u++) {
                 const uint32_t r = RPL * u - 16 * h + lane / LPR;
@@ -475,23 +464,11 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
             }
         }
     };
-    auto ahead = [&](int32_t j0) __attribute__((always_inline)) {  // the entries of the block at j0, the next one
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            walk(map, at[h], 32);
-            entry[h] = peek(map, at[h], j0 + 16 * h, w1);
-        }
-    };
-    bool bad = false;
+    uint32_t bad = 0;
     if (w0 < w1) {
         const int nblk = (w1 - b0 + 31) / 32;
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            at[h] = walk_from(map, b0 + 16 * h);
-            entry[h] = peek(map, at[h], b0 + 16 * h, w1);
-        }
-        load(b0);
-        ahead(b0 + 32);
+        look_up(0);
+        load(0);
         load_rows<DT, D>(a, it, q, col, true, rs);
         for (int n = 0; n < nblk; n++) {
             const int32_t j0 = b0 + n * 32;
@@ -506,8 +483,8 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
                 *(uint4 *)(t.k + r * KS + c) = sk[u];
                 *(uint4 *)(t.v + r * VS + c) = sv[u];
             }
-            load(j0 + 32);
-            ahead(j0 + 64);
+            if ((n & 31) == 31) look_up(2 * n + 2);
+            load(n + 1);
             f32x16_t sc = zero16();
 #pragma unroll
             for (int st = 0; st < KST; st++) sc = mfma32<DT>(row_frag(t.k, KS, 0, st * 16, lane), rs.qf[st], sc);
@@ -593,11 +570,15 @@ template <int DT, int D>
 __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedItem &it, const PageMap &map,
                                             const void *q, SharedSmem<D, true> &sm) {
     constexpr int NW = shared_waves<D, true>(), NT = NW * 64, KS = SharedSmem<D, true>::KS, VS = SharedSmem<D, true>::VS;
-    constexpr int CPR = D / 8, RPW = 64 / CPR, RSTEP = NT / CPR, NCH = 64 / RSTEP;  // pieces a row, rows a wavefront
+    constexpr int CPR = D / 8, RSTEP = NT / CPR, NCH = 64 / RSTEP;  // pieces a row, rows at a time, pieces a thread
     constexpr int KST = D / 16, DTN = D / 32;
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool first = NW == 4 || wave < 4;  // products first in each step
+    const int32_t s0 = it.s0, s1 = it.s1, k0 = s0 & ~15;
+    auto fill = [&](int32_t block) __attribute__((always_inline)) {
+        sm.blocks[block & 511] = block_at(a, map, k0 + 16 * block, s1);
+    };
     RowState<D> rs;
     load_rows<DT, D>(a, it, q, wave * 32 + col, false, rs);
     // (the queries are waited for here: behind the tiles' loads they would leave a wait for all of
@@ -606,61 +587,65 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
     const bool rows = wave * 32 < it.nrow;  // this wavefront has rows
     if (lane == 0) sm.lo[wave] = rs.flo, sm.hi[wave] = rs.fhi;
     if (threadIdx.x == 0) sm.bad = 0;
+    fill(threadIdx.x);
+    if (NT < 512) fill(threadIdx.x + 256);
     __syncthreads();
     int32_t tlo = INT32_MIN, thi = INT32_MAX;  // the keys that every row of the tile sees
 #pragma unroll
     for (int w = 0; w < NW; w++) tlo = max(tlo, sm.lo[w]), thi = min(thi, sm.hi[w]);
     tlo = __builtin_amdgcn_readfirstlane(tlo), thi = __builtin_amdgcn_readfirstlane(thi);
-    const int32_t s0 = it.s0, s1 = it.s1, k0 = s0 & ~15;
     const int32_t nt = (s1 - k0 + 63) / 64;
     const float c2 = fabsf(a.scale) * 1.4426950408889634f;
 
-    // staging: NCH pieces of a tile's K and of its V a thread; a wavefront's rows of a piece lie in one
-    // 16-key block, of which it has NB a tile. A block's entry in the table is read a step before its
-    // keys are loaded, and its place kept for its values another step later.
-    constexpr int NB = NCH < 4 ? NCH : 4, PB = NCH / NB;
-    const int wr = wave * RPW, lr = lane / CPR, lc = lane % CPR;
+    // staging: NCH pieces of a tile's K and of its V a thread. The offsets of the tiles' blocks lie in
+    // LDS, a ring of 128 tiles: 64 of them are looked up 64 steps before they are read.
+    const int row0 = threadIdx.x / CPR, lc = threadIdx.x % CPR;
     uint4 rk[NCH], rv[NCH];
-    Walker at[NB];
-    int32_t entry[NB];
-    Block vb[NB];  // the tile whose values are loaded next
-    auto block_key = [&](int32_t j, int n) { return k0 + j * 64 + ((wr + n * PB * RSTEP) & ~15); };
-    auto peek_at = [&](int32_t j) __attribute__((always_inline)) {
+    // A tile's offsets are read from LDS a step before its keys are loaded, and kept for its values.
+    uint64_t ak[NCH], av[NCH];
+    auto offsets = [&](int32_t j) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < NB; n++) entry[n] = peek(map, at[n], block_key(j, n), s1);
+        for (int u = 0; u < NCH; u++) ak[u] = sm.blocks[(j * 4 + ((row0 + u * RSTEP) >> 4)) & 511];
     };
-    auto load = [&](int32_t j, const char *base, const Block (&b)[NB], uint4 (&x)[NCH]) __attribute__((always_inline)) {
+    // (a piece of no key is read from the first page and zeroed when it is stored: with its load left out
+    // the compiler waits for the others' at once)
+    bool okk[NCH], okv[NCH];
+    auto load = [&](int32_t j, const char *base, const uint64_t (&at)[NCH], uint4 (&x)[NCH],
+                    bool (&ok)[NCH]) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < NCH; u++) {
-            const uint32_t r = ((wr + u * RSTEP) & 15) + lr;
-            x[u] = buf_load16(make_rsrc(base + b[u / PB].at, b[u / PB].bytes),
-                              block_key(j, u / PB) + (int32_t)r >= s0 ? r * map.row + lc * 16 : 0xffffffffu);
+            const int r = row0 + u * RSTEP;
+            ok[u] = at[u] != kNoBlock && (uint32_t)(k0 + j * 64 + r - s0) < (uint32_t)(s1 - s0);
+            x[u] = *(const uint4 *)(base + (ok[u] ? at[u] : 0) + ((uint32_t)(r & 15) * map.row + lc * 16));
         }
     };
-    auto load_v = [&](int32_t j) __attribute__((always_inline)) { load(j, map.v, vb, rv); };
-    // the keys of tile j, whose entries were read; then the entries of the tile behind it
+    auto zeroed = [](const uint4 &x, bool ok) {
+        return make_uint4(ok ? x.x : 0u, ok ? x.y : 0u, ok ? x.z : 0u, ok ? x.w : 0u);
+    };
+    auto load_v = [&](int32_t j) __attribute__((always_inline)) { load(j, map.v, av, rv, okv); };
+    // the keys of tile j, then the offsets of the tile behind it
     auto load_k = [&](int32_t j) __attribute__((always_inline)) {
+        load(j, map.k, ak, rk, okk);
 #pragma unroll
-        for (int n = 0; n < NB; n++) vb[n] = block_of(a, map, entry[n], at[n].row, block_key(j, n), s1);
-        load(j, map.k, vb, rk);
-#pragma unroll
-        for (int n = 0; n < NB; n++) walk(map, at[n], 64);
-        peek_at(j + 1);
+        for (int u = 0; u < NCH; u++) av[u] = ak[u];
+        offsets(j + 1);
     };
     auto store_k = [&](int32_t j) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < NCH; u++) *(uint4 *)(sm.wide[0].k[j & 1] + (wr + u * RSTEP + lr) * KS + lc * 8) = rk[u];
+        for (int u = 0; u < NCH; u++) *(uint4 *)(sm.wide[0].k[j & 1] + (row0 + u * RSTEP) * KS + lc * 8) = zeroed(rk[u], okk[u]);
     };
     auto store_v = [&](int32_t j) __attribute__((always_inline)) {
         const int32_t t = k0 + j * 64;
+#pragma unroll
+        for (int u = 0; u < NCH; u++) rv[u] = zeroed(rv[u], okv[u]);
         if (t < tlo || t + 64 > thi) {  // (a tile that some row does not see all of)
-            bool bad = false;
+            uint32_t bad = 0;
 #pragma unroll
             for (int u = 0; u < NCH; u++) bad |= take_out<DT>(rv[u]);
             if (__any(bad) && lane == 0) sm.bad = 1;
         }
 #pragma unroll
-        for (int u = 0; u < NCH; u++) *(uint4 *)(sm.wide[0].v[j & 1] + (wr + u * RSTEP + lr) * VS + lc * 8) = rv[u];
+        for (int u = 0; u < NCH; u++) *(uint4 *)(sm.wide[0].v[j & 1] + (row0 + u * RSTEP) * VS + lc * 8) = rv[u];
     };
     Partial<D> p;
     p.m = -INFINITY, p.l = 0.f;
@@ -748,13 +733,13 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
         store_v(j + ahead);
         load_v(j + 1 + ahead);
         load_k(j + 2 + ahead);
+        // (the ring's half that it goes to held tiles j - 64 .. j - 1, read by all; only wavefronts 0-3)
+        if (first && (j & 63) == 0 && j > 0) fill(4 * (j + 64) + threadIdx.x);
     };
-#pragma unroll
-    for (int n = 0; n < NB; n++) at[n] = walk_from(map, block_key(0, n));
-    peek_at(0);
+    offsets(0);
     load_k(0);
-    store_k(0);
     load_v(0);
+    store_k(0);
     load_k(1);
     __syncthreads();
     if (!first) {
@@ -803,8 +788,12 @@ __global__ __launch_bounds__((64 * shared_waves<D, WIDE>()), (D == 256 ? 1 : 2))
     const bool wide = WIDE && (int32_t)blockIdx.x < np;
     const int32_t index = wide ? (int32_t)blockIdx.x : np + ((int32_t)blockIdx.x - np) * TEAMS + wave / kTeam;
     SharedItem it{};
-    const bool has = index < items && item_of<RT>(a, index, wide ? 64 : 32, wave % (wide ? 8 : kTeam) == 0, it);
+    const bool has = uniform(index < items && item_of<RT>(a, index, wide ? 64 : 32, wave % (wide ? 8 : kTeam) == 0, it));
     if (wide && !has) return;
+    // (the wavefront's, which the compiler does not see of every one: the loads below take scalar bases)
+    it.m0 = uniform(it.m0), it.table = uniform(it.table), it.s0 = uniform(it.s0), it.s1 = uniform(it.s1);
+    it.cap = uniform(it.cap), it.r0 = uniform(it.r0), it.nrow = uniform(it.nrow), it.kh = uniform(it.kh);
+    it.slot = uniform(it.slot);
     PageMap map;
     map.k = (const char *)k + (int64_t)it.kh * a.kh * 2;
     map.v = (const char *)v + (int64_t)it.kh * a.vh * 2;
@@ -819,50 +808,77 @@ __global__ __launch_bounds__((64 * shared_waves<D, WIDE>()), (D == 256 ? 1 : 2))
     shared_narrow<DT, D, WIDE>(a, it, has, map, q, sm);
 }
 
-// The ranges of a row joined, a workgroup a row: its four wavefronts take every fourth range each, a
-// lane the columns lane, lane + 64, ...; a range of no key is not read.
+// The ranges of a row joined, a workgroup a row: the ranges that hold keys are listed with their
+// weights, and thread t sums, for the columns of its piece t % pieces (four of them where D is a multiple of
+// 4, one otherwise), every groups-th of the list, eight loads in flight; the groups are added in order.
 constexpr int kSharedSplits = 512;  // most ranges of a row
-template <int DT>
+template <int DT, int V>
 __global__ __launch_bounds__(256) void decode_shared_merge(SharedArgs a, void *__restrict__ o) {
-    __shared__ float w[kSharedSplits], red[4][256], tops[4], sums[4];
+    __shared__ float w[kSharedSplits], red[256 * V], tops[4], sums[4];
+    __shared__ int32_t list[kSharedSplits], counts[4];
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.nsp + a.nso;
-    float mx = -INFINITY;
-    bool nan = false;
-    for (int s = tid; s < n; s += 256) {
-        const float x = a.part_lse[row * n + s];
-        w[s] = x;
-        nan |= x != x;
-        mx = fmaxf(mx, x);
-    }
-    mx = wave_max(mx);
+    const float x0 = tid < n ? a.part_lse[row * n + tid] : -INFINITY;
+    const float x1 = tid + 256 < n ? a.part_lse[row * n + tid + 256] : -INFINITY;
+    const float mx = wave_max(fmaxf(x0, x1));
     if (lane == 0) tops[wave] = mx;
-    nan = __syncthreads_or(nan);
+    const bool nan = __syncthreads_or(x0 != x0 || x1 != x1);
     const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    float sum = 0.f;
-    for (int s = tid; s < n; s += 256) {
-        const float x = w[s] == -INFINITY ? 0.f : (w[s] == top ? 1.f : expf(w[s] - top));
-        w[s] = x;
-        sum += x;
-    }
-    sum = wave_sum(sum);
-    if (lane == 0) sums[wave] = sum;
+    auto weight = [&](float x) { return x == -INFINITY ? 0.f : (x == top ? 1.f : expf(x - top)); };
+    const float w0 = weight(x0), w1 = weight(x1);
+    const float part = wave_sum(w0 + w1);
+    const unsigned long long b0 = __ballot(w0 != 0.f), b1 = __ballot(w1 != 0.f);
+    if (lane == 0) sums[wave] = part, counts[wave] = __popcll(b0) + __popcll(b1);
     __syncthreads();
-    sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-    float acc[4] = {};
-    for (int s = wave; s < n; s += 4) {
-        if (w[s] == 0.f) continue;
-        const float *po = a.part_o + (row * n + s) * a.d;
+    const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    int at = 0, m = 0;
+    for (int i = 0; i < 4; i++) {
+        if (i < wave) at += counts[i];
+        m += counts[i];
+    }
+    const unsigned long long below = ((unsigned long long)1 << lane) - 1;
+    if (w0 != 0.f) {
+        const int i = at + __popcll(b0 & below);
+        list[i] = tid, w[i] = w0;
+    }
+    if (w1 != 0.f) {
+        const int i = at + __popcll(b0) + __popcll(b1 & below);
+        list[i] = tid + 256, w[i] = w1;
+    }
+    __syncthreads();
+    const int pieces = a.d / V, groups = 256 / pieces, p = tid % pieces, g = tid / pieces;
+    float acc[V] = {};
+    if (g < groups) {
+        const float *po = a.part_o + row * n * a.d + p * V;
+        for (int i = g; i < m; i += 8 * groups) {
+            float x[8][V], f[8];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (lane + 64 * i < a.d) acc[i] += w[s] * po[lane + 64 * i];
+            for (int u = 0; u < 8; u++) {
+                const int k = i + u * groups;
+                f[u] = k < m ? w[k] : 0.f;
+                const float *at = po + (int64_t)list[k < m ? k : i] * a.d;
+                if constexpr (V == 4)
+                    *(float4 *)x[u] = *(const float4 *)at;
+                else
+                    x[u][0] = *at;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+#pragma unroll
+                for (int c = 0; c < V; c++) acc[c] += f[u] != 0.f ? f[u] * x[u][c] : 0.f;
+        }
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) red[wave][lane + 64 * i] = acc[i];
+    for (int c = 0; c < V; c++) red[tid * V + c] = acc[c];
     __syncthreads();
-    if (tid < a.d) {
-        const float t = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
-        st<DT>(o, row * a.d + tid, nan ? NAN : (sum > 0.f ? t / sum : 0.f));
+    if (tid < pieces) {
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+        for (int c = 0; c < V; c++) {
+            float t = red[tid * V + c];
+            for (int i = 1; i < groups; i++) t += red[(i * pieces + tid) * V + c];
+            st<DT>(o, row * a.d + tid * V + c, nan ? NAN : t * inv);
+        }
     }
 }
 
@@ -956,6 +972,11 @@ int dm_attention_decode_shared(const dm_attention_desc *d, const void *q, const 
     }
     const bool mfma = shared_mfma_takes(d, page_size) && aligned_16b(q) && aligned_16b(k_pages) && aligned_16b(v_pages);
     const SharedPlan p = shared_plan(d, mfma, ngroups);
+    if (p.wide && num_pages == 0) {  // (its kernel reads the first page in the place of one that is not there)
+        fill_zero(o, rows * d->d * dtype_bytes(d->dtype), st);
+        DM_LAUNCH_CHECK("attention_decode_shared: fill");
+        return DM_OK;
+    }
     SharedArgs a{};
     a.B = (int32_t)d->b, a.S = (int32_t)d->tk, a.left = (int32_t)left_of(d);
     a.hq = (int32_t)d->hq, a.hkv = (int32_t)d->hkv, a.d = (int32_t)d->d, a.rep = (int32_t)(d->hq / d->hkv);
@@ -997,7 +1018,10 @@ int dm_attention_decode_shared(const dm_attention_desc *d, const void *q, const 
             SHARED_W(DT, 256);                                                 \
         }                                                                      \
     }                                                                          \
-    decode_shared_merge<DT><<<(unsigned)rows, 256, 0, st>>>(a, o)
+    if (d->d % 4 == 0)                                                         \
+        decode_shared_merge<DT, 4><<<(unsigned)rows, 256, 0, st>>>(a, o);      \
+    else                                                                       \
+        decode_shared_merge<DT, 1><<<(unsigned)rows, 256, 0, st>>>(a, o)
     if (d->dtype == DM_F32) {
         SHARED(DM_F32);
     } else if (d->dtype == DM_BF16) {

@@ -668,7 +668,7 @@ def attention_decode_shared(query, key_pages, value_pages, block_table, lengths,
     once for the group, each row's own keys behind them for itself. ``groups [G + 1]`` goes up from 0
     at least to B at most; a row outside it shares nothing. ``[B, Hq, D]`` in the queries' dtype.
 
-    A group's prefix is read through the block table of its longest row (the first of them), which has
+    A group's prefix is read through the block table of its longest row (one of them), which has
     to hold all of the prefix that any row of the group sees, a window's too; that the others' tables
     hold the same keys is the caller's to see to (``cache_fork`` makes such tables). int32 arrays on
     the GPU are not read back: a negative length counts as 0, and groups that do not go up as none."""

@@ -377,7 +377,7 @@ int dm_attention_decode_paged(const dm_attention_desc *desc, const void *q, cons
 
 /* dm_attention_decode_paged for sequences that share prefixes: rows groups[g] .. groups[g + 1] - 1
  * of the batch hold the same first prefix_lengths[g] keys, which are read once for the group, through
- * the block table of its longest row (the first of them), which has to hold all of the prefix that
+ * the block table of its longest row (one of them), which has to hold all of the prefix that
  * any row of the group sees; each row's own keys behind them through its own. Results are the paged decode's of the same arguments wherever that holds. groups
  * [ngroups + 1] and prefix_lengths [ngroups] are int32 on the device, as block_table and lengths,
  * and are read there only. Rows in front of the first group or behind the last share nothing, and
