@@ -253,21 +253,320 @@ __global__ __launch_bounds__(256) void rope_bwd_generic(RopeArgs a, const void *
     }
 }
 
-// The workgroups' weight gradients added in order: a workgroup takes 16 columns, its 16 groups of
-// threads every sixteenth part each.
-__global__ __launch_bounds__(256) void rope_weights(const float *__restrict__ parts, int64_t nparts, int d,
-                                                    int weight_dtype, void *dwq, void *dwk) {
-    __shared__ float sums[16][17];
+// The kernels for heads of 64, 128 and 256 in 16-byte pieces of V values: D / (2 V) lanes take a head,
+// each the pieces at V li and n + V li, the first and the second elements of its pairs (half style), or
+// of adjacent ones (interleaved); past the rotated 2 n the rest of the head in the same manner. So a
+// pair never leaves its lane, and a head's sums are moves within 16 lanes (32 in f32).
+//
+// A workgroup takes `tile` tokens: the angles of all of them go to LDS first, one a thread, since every
+// head of a token turns by the same ones, then its lanes go through the tokens' heads.
+template <int DT>
+constexpr int rope_v() { return DT == DM_F32 ? 4 : 8; }
+
+template <int DT, int V>
+__device__ __forceinline__ void piece(const void *p, int64_t at, float (&x)[V]) {
+    if constexpr (DT == DM_F32) {
+        const float4 a = *(const float4 *)((const float *)p + at);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+    } else {
+        const uint4 a = *(const uint4 *)((const uint16_t *)p + at);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[2 * i] = unpack_lo<DT>(w[i]), x[2 * i + 1] = unpack_hi<DT>(w[i]);
+    }
+}
+template <int DT, int V>
+__device__ __forceinline__ void put_piece(void *p, int64_t at, const float (&x)[V]) {
+    if constexpr (DT == DM_F32)
+        *(float4 *)((float *)p + at) = make_float4(x[0], x[1], x[2], x[3]);
+    else
+        *(uint4 *)((uint16_t *)p + at) =
+            make_uint4(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]), pack2<DT>(x[4], x[5]), pack2<DT>(x[6], x[7]));
+}
+
+// Sum over aligned groups of N lanes (4, 8, 16 or 32).
+template <int N>
+__device__ __forceinline__ float head_sum(float t) {
+    if constexpr (N == 4) {
+        t += __shfl_xor(t, 1, 64);
+        return t + __shfl_xor(t, 2, 64);
+    } else {
+        return group_sum<N>(t);
+    }
+}
+
+// What a lane holds of a head of D: its two pieces' places, and where its angles begin.
+template <int D, int V, bool INTER>
+struct HeadLane {
+    int a, b;      // the pieces' first elements
+    bool turns;    // they rotate
+    int ja, jb;    // the first angle of each (half style: of both)
+    __device__ __forceinline__ HeadLane(int li, int n) {
+        turns = li * V < n;
+        a = turns ? li * V : 2 * n + (li * V - n);
+        b = turns ? n + li * V : 2 * n + (D - 2 * n) / 2 + (li * V - n);
+        ja = INTER ? a / 2 : a;
+        jb = INTER ? b / 2 : a;
+    }
+};
+
+// The pieces turned by the angles c, s [n] of their token; BACK: back.
+template <int V, bool INTER, bool BACK>
+__device__ __forceinline__ void turn_pieces(float (&a)[V], float (&b)[V], const float *c, const float *s, int ja, int jb) {
+    if constexpr (INTER) {
+#pragma unroll
+        for (int i = 0; i < V / 2; i++) {
+            const float ca = c[ja + i], sa = BACK ? -s[ja + i] : s[ja + i];
+            const float cb = c[jb + i], sb = BACK ? -s[jb + i] : s[jb + i];
+            const float a0 = a[2 * i], a1 = a[2 * i + 1], b0 = b[2 * i], b1 = b[2 * i + 1];
+            a[2 * i] = a0 * ca - a1 * sa, a[2 * i + 1] = a0 * sa + a1 * ca;
+            b[2 * i] = b0 * cb - b1 * sb, b[2 * i + 1] = b0 * sb + b1 * cb;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const float ci = c[ja + i], si = BACK ? -s[ja + i] : s[ja + i];
+            const float x = a[i], y = b[i];
+            a[i] = x * ci - y * si, b[i] = x * si + y * ci;
+        }
+    }
+}
+
+// Goes through rows = tile x heads, `by` at a time, as (token of the tile, head).
+struct RowWalk {
+    int t, h, dt, dh, heads;
+    __device__ __forceinline__ RowWalk(int from, int by, int heads_)
+        : t(from / heads_), h(from % heads_), dt(by / heads_), dh(by % heads_), heads(heads_) {}
+    __device__ __forceinline__ void next() {
+        t += dt, h += dh;
+        if (h >= heads) h -= heads, t++;
+    }
+};
+
+template <int V>
+__device__ __forceinline__ void load_weight(int dtype, const void *w, float unit, int at, float (&x)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) x[i] = w ? ld_any(dtype, w, at + i) + unit : 1.f;
+}
+
+constexpr int kRopeTile = 16;  // most tokens of a tile
+
+template <int DT, int D, int MODE, bool INTER>
+__global__ __launch_bounds__(256) void rope_fast(RopeArgs a, RopePages pg, int tile, const void *__restrict__ q,
+                                                 const void *__restrict__ k, const void *__restrict__ v,
+                                                 void *__restrict__ qo, void *__restrict__ ko, void *__restrict__ vo) {
+    constexpr int V = rope_v<DT>(), LPH = D / (2 * V), BY = 256 / LPH, U = 4;
+    extern __shared__ float angles[];  // cos [tile, n], sin [tile, n]
+    __shared__ int64_t at[kRopeTile], krow[kRopeTile], vrow[kRopeTile];
+    __shared__ int is[kRopeTile];
+    const int tid = threadIdx.x, li = tid % LPH, r0 = tid / LPH, n = a.n;
+    const int64_t first = (int64_t)blockIdx.x * tile;
+    const int here = (int)min((int64_t)tile, a.tokens - first);
+    float *cs = angles, *sn = angles + tile * n;
+    if constexpr (MODE == kRopePaged) {
+        if (tid < here) {
+            int64_t p, kr, vr;
+            is[tid] = place_paged(pg, first + tid, &p, &kr, &vr);
+            at[tid] = p, krow[tid] = kr, vrow[tid] = vr;
+        }
+        __syncthreads();
+    }
+    for (int i = tid; i < here * n; i += 256) {
+        const int t = i / n, j = i - t * n;
+        int64_t p;
+        if constexpr (MODE == kRopePaged) {
+            p = at[t];
+        } else {
+            const int64_t b = (first + t) / a.T;
+            p = place_plain(a, b, first + t - b * a.T);
+        }
+        const float2 x = turn_of(p, a.inv_freq[j]);
+        cs[i] = x.x, sn[i] = x.y;
+    }
+    __syncthreads();
+    const HeadLane<D, V, INTER> hl(li, n);
+#pragma unroll 1
+    for (int x = 0; x < 2; x++) {
+        const bool isq = x == 0;
+        const int heads = isq ? a.hq : a.hkv, rows = here * heads;
+        if (heads == 0) continue;
+        const void *src = isq ? q : k;
+        void *dst = isq ? qo : ko;
+        const Strd sd = isq ? a.q : a.k;
+        float wa[V], wb[V];
+        load_weight<V>(a.weight_dtype, isq ? a.wq : a.wk, a.unit, hl.a, wa);
+        load_weight<V>(a.weight_dtype, isq ? a.wq : a.wk, a.unit, hl.b, wb);
+        RowWalk w(r0, BY, heads), put(r0, BY, heads);
+        for (int r = r0; r < rows; r += BY * U) {
+            float pa[U][V], pb[U][V];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (r + u * BY < rows) {
+                    const int64_t token = first + w.t, b = token / a.T;
+                    const int64_t from = b * sd.b + (token - b * a.T) * sd.t + w.h * sd.h;
+                    piece<DT, V>(src, from + hl.a, pa[u]);
+                    piece<DT, V>(src, from + hl.b, pb[u]);
+                }
+                w.next();
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (r + u * BY < rows) {  // (a head's lanes agree)
+                    float ss = 0.f;
+#pragma unroll
+                    for (int i = 0; i < V; i++) ss += pa[u][i] * pa[u][i] + pb[u][i] * pb[u][i];
+                    const float rs = rsqrtf(head_sum<LPH>(ss) * (1.f / D) + a.eps);
+#pragma unroll
+                    for (int i = 0; i < V; i++) pa[u][i] *= rs * wa[i], pb[u][i] *= rs * wb[i];
+                    if (hl.turns) turn_pieces<V, INTER, false>(pa[u], pb[u], cs + put.t * n, sn + put.t * n, hl.ja, hl.jb);
+                    int64_t to;
+                    bool on = true;
+                    if (MODE == kRopePaged && !isq) {
+                        to = krow[put.t] + put.h * pg.k.h;
+                        on = krow[put.t] >= 0;
+                    } else {
+                        to = ((first + put.t) * heads + put.h) * D;
+                        if (MODE == kRopePaged && !is[put.t]) {
+#pragma unroll
+                            for (int i = 0; i < V; i++) pa[u][i] = pb[u][i] = 0.f;
+                        }
+                    }
+                    if (on) {
+                        put_piece<DT, V>(dst, to + hl.a, pa[u]);
+                        put_piece<DT, V>(dst, to + hl.b, pb[u]);
+                    }
+                }
+                put.next();
+            }
+        }
+    }
+    if constexpr (MODE == kRopePaged) {
+        constexpr int E = DT == DM_F32 ? 4 : 2;
+        const int rows = here * a.hkv;
+        if (rows == 0) return;
+        RowWalk w(r0, BY, a.hkv);
+        for (int r = r0; r < rows; r += BY, w.next()) {
+            if (vrow[w.t] < 0) continue;
+            const uint4 *from = (const uint4 *)((const char *)v + ((first + w.t) * a.v.t + w.h * a.v.h) * E);
+            uint4 *to = (uint4 *)((char *)vo + (vrow[w.t] + w.h * pg.v.h) * E);
+            const uint4 x = from[li], y = from[li + LPH];
+            to[li] = x, to[li + LPH] = y;
+        }
+    }
+}
+
+// The gradients, the same split. A lane's weight gradients are of its own two pieces for every head that
+// it takes, so they stay in registers over the workgroup's tiles and meet in LDS at the end.
+template <int DT, int D, bool INTER>
+__global__ __launch_bounds__(256) void rope_bwd_fast(RopeArgs a, int tile, const void *__restrict__ q,
+                                                     const void *__restrict__ k, const void *__restrict__ gq,
+                                                     const void *__restrict__ gk, void *__restrict__ dq,
+                                                     void *__restrict__ dk, float *__restrict__ parts) {
+    constexpr int V = rope_v<DT>(), LPH = D / (2 * V), BY = 256 / LPH, U = 2;
+    extern __shared__ float angles[];  // cos [tile, n], sin [tile, n]; at the end the lanes' sums [BY, D]
+    const int tid = threadIdx.x, li = tid % LPH, r0 = tid / LPH, n = a.n;
+    float *cs = angles, *sn = angles + tile * n;
+    const HeadLane<D, V, INTER> hl(li, n);
+    float wa[2][V], wb[2][V], da[2][V] = {}, db[2][V] = {};
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        load_weight<V>(a.weight_dtype, x ? a.wk : a.wq, a.unit, hl.a, wa[x]);
+        load_weight<V>(a.weight_dtype, x ? a.wk : a.wq, a.unit, hl.b, wb[x]);
+    }
+    for (int64_t first = (int64_t)blockIdx.x * tile; first < a.tokens; first += (int64_t)gridDim.x * tile) {
+        const int here = (int)min((int64_t)tile, a.tokens - first);
+        __syncthreads();
+        for (int i = tid; i < here * n; i += 256) {
+            const int t = i / n, j = i - t * n;
+            const int64_t b = (first + t) / a.T;
+            const float2 x = turn_of(place_plain(a, b, first + t - b * a.T), a.inv_freq[j]);
+            cs[i] = x.x, sn[i] = x.y;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int heads = x ? a.hkv : a.hq, rows = here * heads;
+            if (heads == 0) continue;
+            const void *src = x ? k : q, *grad = x ? gk : gq;
+            void *dst = x ? dk : dq;
+            const Strd sd = x ? a.k : a.q, sg = x ? a.gk : a.gq;
+            RowWalk w(r0, BY, heads), put(r0, BY, heads);
+            for (int r = r0; r < rows; r += BY * U) {
+                float xa[U][V], xb[U][V], za[U][V], zb[U][V];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (r + u * BY < rows) {
+                        const int64_t token = first + w.t, b = token / a.T, t = token - b * a.T;
+                        const int64_t from = b * sd.b + t * sd.t + w.h * sd.h, g = b * sg.b + t * sg.t + w.h * sg.h;
+                        piece<DT, V>(src, from + hl.a, xa[u]);
+                        piece<DT, V>(src, from + hl.b, xb[u]);
+                        piece<DT, V>(grad, g + hl.a, za[u]);
+                        piece<DT, V>(grad, g + hl.b, zb[u]);
+                    }
+                    w.next();
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (r + u * BY < rows) {
+                        float ss = 0.f, gh = 0.f;
+#pragma unroll
+                        for (int i = 0; i < V; i++) ss += xa[u][i] * xa[u][i] + xb[u][i] * xb[u][i];
+                        const float rs = rsqrtf(head_sum<LPH>(ss) * (1.f / D) + a.eps);
+                        if (hl.turns) turn_pieces<V, INTER, true>(za[u], zb[u], cs + put.t * n, sn + put.t * n, hl.ja, hl.jb);
+#pragma unroll
+                        for (int i = 0; i < V; i++) {
+                            xa[u][i] *= rs, xb[u][i] *= rs;
+                            da[x][i] += za[u][i] * xa[u][i], db[x][i] += zb[u][i] * xb[u][i];
+                            za[u][i] *= wa[x][i], zb[u][i] *= wb[x][i];
+                            gh += za[u][i] * xa[u][i] + zb[u][i] * xb[u][i];
+                        }
+                        const float mean = head_sum<LPH>(gh) * (1.f / D);
+#pragma unroll
+                        for (int i = 0; i < V; i++) {
+                            za[u][i] = rs * (za[u][i] - xa[u][i] * mean);
+                            zb[u][i] = rs * (zb[u][i] - xb[u][i] * mean);
+                        }
+                        const int64_t to = ((first + put.t) * heads + put.h) * D;
+                        put_piece<DT, V>(dst, to + hl.a, za[u]);
+                        put_piece<DT, V>(dst, to + hl.b, zb[u]);
+                    }
+                    put.next();
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; i++) angles[r0 * D + hl.a + i] = da[x][i], angles[r0 * D + hl.b + i] = db[x][i];
+        __syncthreads();
+        for (int e = tid; e < D; e += 256) {
+            float t = 0.f;
+            for (int i = 0; i < BY; i++) t += angles[i * D + e];
+            parts[((int64_t)blockIdx.x * 2 + x) * D + e] = t;
+        }
+    }
+}
+
+// The workgroups' weight gradients added in order: a workgroup takes 16 columns, its 64 groups of
+// threads every 64th part each.
+__global__ __launch_bounds__(1024) void rope_weights(const float *__restrict__ parts, int64_t nparts, int d,
+                                                     int weight_dtype, void *dwq, void *dwk) {
+    __shared__ float sums[64][17];
     const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
     const int64_t col = (int64_t)blockIdx.x * 16 + c;
     float s = 0.f;
-    if (col < 2 * d)
-        for (int64_t i = g; i < nparts; i += 16) s += parts[i * 2 * d + col];
+    if (col < 2 * d) {
+#pragma unroll 8
+        for (int64_t i = g; i < nparts; i += 64) s += parts[i * 2 * d + col];
+    }
     sums[g][c] = s;
     __syncthreads();
     if (g == 0 && col < 2 * d) {
         float t = 0.f;
-        for (int i = 0; i < 16; i++) t += sums[i][c];
+#pragma unroll 8
+        for (int i = 0; i < 64; i++) t += sums[i][c];
         void *to = col < d ? dwq : dwk;
         if (to) st_any(weight_dtype, to, col < d ? col : col - d, t);
     }
@@ -321,18 +620,69 @@ static RopeArgs rope_args(const dm_qk_norm_rope_desc *d, const void *wq, const v
     return a;
 }
 
+// The fast kernels' calls: 16-byte pieces that no pair leaves.
+static bool fast_takes(const dm_qk_norm_rope_desc *d, const RopeArgs &a, const void *const *ptrs, int n,
+                       const Strd *strides, int ns) {
+    const int v = d->dtype == DM_F32 ? 4 : 8;
+    if ((d->d != 64 && d->d != 128 && d->d != 256) || d->n % v != 0) return false;
+    for (int i = 0; i < n; i++)
+        if (!aligned_16b(ptrs[i])) return false;
+    for (int i = 0; i < ns; i++)
+        if (strides[i].b % v || strides[i].t % v || strides[i].h % v) return false;
+    return true;
+}
+
+// Tokens of a tile: enough heads for every lane of the workgroup to take a few, while there are tiles
+// for the compute units to share (at least 1024 workgroups), at most kRopeTile.
+static int rope_tile(const RopeArgs &a, int by) {
+    const int64_t heads = std::max(1, a.hq + a.hkv);
+    int64_t tile = 1;
+    while (tile < kRopeTile && tile * heads < 4 * by && a.tokens >= 2048 * tile) tile *= 2;
+    return (int)tile;
+}
+
+#define ROPE_D(KERNEL, DT, MODE_, GRID, LDS, ...)                                                           \
+    do {                                                                                                    \
+        if (d->d == 64) {                                                                                   \
+            if (a.interleaved) KERNEL<DT, 64 MODE_, true><<<GRID, 256, LDS, st>>>(__VA_ARGS__);             \
+            else KERNEL<DT, 64 MODE_, false><<<GRID, 256, LDS, st>>>(__VA_ARGS__);                          \
+        } else if (d->d == 128) {                                                                           \
+            if (a.interleaved) KERNEL<DT, 128 MODE_, true><<<GRID, 256, LDS, st>>>(__VA_ARGS__);            \
+            else KERNEL<DT, 128 MODE_, false><<<GRID, 256, LDS, st>>>(__VA_ARGS__);                         \
+        } else {                                                                                            \
+            if (a.interleaved) KERNEL<DT, 256 MODE_, true><<<GRID, 256, LDS, st>>>(__VA_ARGS__);            \
+            else KERNEL<DT, 256 MODE_, false><<<GRID, 256, LDS, st>>>(__VA_ARGS__);                         \
+        }                                                                                                   \
+    } while (0)
+#define ROPE_COMMA ,
+
 template <int MODE>
 static int run_rope(const char *op, const dm_qk_norm_rope_desc *d, const RopeArgs &a, const RopePages &pg,
                     const void *q, const void *k, const void *v, void *qo, void *ko, void *vo,
                     hipStream_t st) {
-    const int64_t rows = a.tokens * (a.hq + a.hkv * (MODE == kRopePaged ? 2 : 1));
-    const unsigned grid = (unsigned)std::min<int64_t>((rows + 3) / 4, 16384);
-    if (d->dtype == DM_F32)
-        rope_generic<DM_F32, MODE><<<grid, 256, 0, st>>>(a, pg, q, k, v, qo, ko, vo);
-    else if (d->dtype == DM_BF16)
-        rope_generic<DM_BF16, MODE><<<grid, 256, 0, st>>>(a, pg, q, k, v, qo, ko, vo);
-    else
-        rope_generic<DM_F16, MODE><<<grid, 256, 0, st>>>(a, pg, q, k, v, qo, ko, vo);
+    const void *ptrs[] = {q, k, qo, ko, v, vo};
+    const Strd strides[] = {a.q, a.k, a.v, pg.k, pg.v};
+    constexpr bool paged = MODE == kRopePaged;
+    if (fast_takes(d, a, ptrs, paged ? 6 : 4, strides, paged ? 5 : 2)) {
+        const int by = 256 / (int)(d->d / (d->dtype == DM_F32 ? 8 : 16)), tile = rope_tile(a, by);
+        const unsigned grid = (unsigned)((a.tokens + tile - 1) / tile);
+        const size_t lds = (size_t)tile * d->n * 2 * sizeof(float);
+        if (d->dtype == DM_F32)
+            ROPE_D(rope_fast, DM_F32, ROPE_COMMA MODE, grid, lds, a, pg, tile, q, k, v, qo, ko, vo);
+        else if (d->dtype == DM_BF16)
+            ROPE_D(rope_fast, DM_BF16, ROPE_COMMA MODE, grid, lds, a, pg, tile, q, k, v, qo, ko, vo);
+        else
+            ROPE_D(rope_fast, DM_F16, ROPE_COMMA MODE, grid, lds, a, pg, tile, q, k, v, qo, ko, vo);
+    } else {
+        const int64_t rows = a.tokens * (a.hq + a.hkv * (paged ? 2 : 1));
+        const unsigned grid = (unsigned)std::min<int64_t>((rows + 3) / 4, 16384);
+        if (d->dtype == DM_F32)
+            rope_generic<DM_F32, MODE><<<grid, 256, 0, st>>>(a, pg, q, k, v, qo, ko, vo);
+        else if (d->dtype == DM_BF16)
+            rope_generic<DM_BF16, MODE><<<grid, 256, 0, st>>>(a, pg, q, k, v, qo, ko, vo);
+        else
+            rope_generic<DM_F16, MODE><<<grid, 256, 0, st>>>(a, pg, q, k, v, qo, ko, vo);
+    }
     probe_add(DM_PROBE_QK_NORM_ROPE);
     DM_LAUNCH_CHECK((std::string(op) + ": launch").c_str());
     return DM_OK;
@@ -370,17 +720,34 @@ int dm_qk_norm_rope_bwd(const dm_qk_norm_rope_desc *d, const void *q, const void
     hipStream_t st = (hipStream_t)stream;
     const RopeArgs a = rope_args(d, q_weight, k_weight, inv_freq);
     float *parts = (float *)workspace;
-    const int64_t nparts = a.tokens * (a.hq + a.hkv) > 0 ? bwd_workgroups(d) : 0;
-    if (nparts > 0) {
-        if (d->dtype == DM_F32)
-            rope_bwd_generic<DM_F32><<<(unsigned)nparts, 256, 0, st>>>(a, q, k, grad_q, grad_k, dq, dk, parts);
-        else if (d->dtype == DM_BF16)
-            rope_bwd_generic<DM_BF16><<<(unsigned)nparts, 256, 0, st>>>(a, q, k, grad_q, grad_k, dq, dk, parts);
-        else
-            rope_bwd_generic<DM_F16><<<(unsigned)nparts, 256, 0, st>>>(a, q, k, grad_q, grad_k, dq, dk, parts);
+    int64_t nparts = 0;
+    if (a.tokens * (a.hq + a.hkv) > 0) {
+        const void *ptrs[] = {q, k, grad_q, grad_k, dq, dk};
+        const Strd strides[] = {a.q, a.k, a.gq, a.gk};
+        if (fast_takes(d, a, ptrs, 6, strides, 4)) {
+            const int by = 256 / (int)(d->d / (d->dtype == DM_F32 ? 8 : 16)), tile = rope_tile(a, by);
+            nparts = std::min<int64_t>((a.tokens + tile - 1) / tile, kRopeParts);
+            const unsigned grid = (unsigned)nparts;
+            const size_t lds = std::max((size_t)tile * d->n * 2, (size_t)by * d->d) * sizeof(float);
+            if (d->dtype == DM_F32)
+                ROPE_D(rope_bwd_fast, DM_F32, , grid, lds, a, tile, q, k, grad_q, grad_k, dq, dk, parts);
+            else if (d->dtype == DM_BF16)
+                ROPE_D(rope_bwd_fast, DM_BF16, , grid, lds, a, tile, q, k, grad_q, grad_k, dq, dk, parts);
+            else
+                ROPE_D(rope_bwd_fast, DM_F16, , grid, lds, a, tile, q, k, grad_q, grad_k, dq, dk, parts);
+        } else {
+            nparts = bwd_workgroups(d);
+            const unsigned grid = (unsigned)nparts;
+            if (d->dtype == DM_F32)
+                rope_bwd_generic<DM_F32><<<grid, 256, 0, st>>>(a, q, k, grad_q, grad_k, dq, dk, parts);
+            else if (d->dtype == DM_BF16)
+                rope_bwd_generic<DM_BF16><<<grid, 256, 0, st>>>(a, q, k, grad_q, grad_k, dq, dk, parts);
+            else
+                rope_bwd_generic<DM_F16><<<grid, 256, 0, st>>>(a, q, k, grad_q, grad_k, dq, dk, parts);
+        }
     }
     if (dq_weight || dk_weight)
-        rope_weights<<<(unsigned)((2 * a.d + 15) / 16), 256, 0, st>>>(parts, nparts, a.d, a.weight_dtype,
+        rope_weights<<<(unsigned)((2 * a.d + 15) / 16), 1024, 0, st>>>(parts, nparts, a.d, a.weight_dtype,
                                                                       dq_weight, dk_weight);
     probe_add(DM_PROBE_QK_NORM_ROPE_BWD);
     DM_LAUNCH_CHECK((op + ": launch").c_str());
