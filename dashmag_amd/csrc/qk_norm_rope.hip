@@ -263,14 +263,17 @@ __global__ __launch_bounds__(256) void rope_bwd_generic(RopeArgs a, const void *
 template <int DT>
 constexpr int rope_v() { return DT == DM_F32 ? 4 : 8; }
 
+template <int DT>
+__device__ __forceinline__ uint4 raw_piece(const void *p, int64_t at) {
+    return *(const uint4 *)((const char *)p + at * (DT == DM_F32 ? 4 : 2));
+}
 template <int DT, int V>
-__device__ __forceinline__ void piece(const void *p, int64_t at, float (&x)[V]) {
+__device__ __forceinline__ void unpack_piece(const uint4 &a, float (&x)[V]) {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
     if constexpr (DT == DM_F32) {
-        const float4 a = *(const float4 *)((const float *)p + at);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = __uint_as_float(w[i]);
     } else {
-        const uint4 a = *(const uint4 *)((const uint16_t *)p + at);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) x[2 * i] = unpack_lo<DT>(w[i]), x[2 * i + 1] = unpack_hi<DT>(w[i]);
     }
@@ -343,207 +346,239 @@ struct RowWalk {
     }
 };
 
-template <int V>
-__device__ __forceinline__ void load_weight(int dtype, const void *w, float unit, int at, float (&x)[V]) {
-#pragma unroll
-    for (int i = 0; i < V; i++) x[i] = w ? ld_any(dtype, w, at + i) + unit : 1.f;
-}
-
 constexpr int kRopeTile = 16;  // most tokens of a tile
 
-template <int DT, int D, int MODE, bool INTER>
-__global__ __launch_bounds__(256) void rope_fast(RopeArgs a, RopePages pg, int tile, const void *__restrict__ q,
-                                                 const void *__restrict__ k, const void *__restrict__ v,
-                                                 void *__restrict__ qo, void *__restrict__ ko, void *__restrict__ vo) {
-    constexpr int V = rope_v<DT>(), LPH = D / (2 * V), BY = 256 / LPH, U = 4;
-    extern __shared__ float angles[];  // cos [tile, n], sin [tile, n]
-    __shared__ int64_t at[kRopeTile], krow[kRopeTile], vrow[kRopeTile];
-    __shared__ int is[kRopeTile];
-    const int tid = threadIdx.x, li = tid % LPH, r0 = tid / LPH, n = a.n;
-    const int64_t first = (int64_t)blockIdx.x * tile;
-    const int here = (int)min((int64_t)tile, a.tokens - first);
-    float *cs = angles, *sn = angles + tile * n;
-    if constexpr (MODE == kRopePaged) {
-        if (tid < here) {
-            int64_t p, kr, vr;
-            is[tid] = place_paged(pg, first + tid, &p, &kr, &vr);
-            at[tid] = p, krow[tid] = kr, vrow[tid] = vr;
-        }
-        __syncthreads();
+// The weights, as they multiply, into LDS [2, D]: queries' and keys'.
+template <int D>
+__device__ __forceinline__ void fill_weights(const RopeArgs &a, float *w) {
+    for (int e = threadIdx.x; e < 2 * D; e += 256) {
+        const void *p = e < D ? a.wq : a.wk;
+        w[e] = p ? ld_any(a.weight_dtype, p, e % D) + a.unit : 1.f;
     }
-    for (int i = tid; i < here * n; i += 256) {
-        const int t = i / n, j = i - t * n;
+}
+// The tile's positions in the pages (paged), and its angles: cos [tile, n] and sin [tile, n].
+struct RopePlaces {
+    int64_t at[kRopeTile], krow[kRopeTile], vrow[kRopeTile];
+    int is[kRopeTile];
+};
+__device__ __forceinline__ void fill_places(const RopeArgs &a, const RopePages &pg, int64_t first, int tile, RopePlaces &o) {
+    const int t = threadIdx.x;
+    if (t < tile && first + t < a.tokens) {
+        int64_t p, kr, vr;
+        o.is[t] = place_paged(pg, first + t, &p, &kr, &vr);
+        o.at[t] = p, o.krow[t] = kr, o.vrow[t] = vr;
+    }
+}
+template <bool PAGED>
+__device__ __forceinline__ void fill_angles(const RopeArgs &a, int64_t first, int tile, const RopePlaces *places,
+                                            float *cs) {
+    const int here = (int)max((int64_t)0, min((int64_t)tile, a.tokens - first));
+    for (int i = threadIdx.x; i < here * a.n; i += 256) {
+        const int t = i / a.n, j = i - t * a.n;
         int64_t p;
-        if constexpr (MODE == kRopePaged) {
-            p = at[t];
+        if constexpr (PAGED) {
+            p = places->at[t];
         } else {
             const int64_t b = (first + t) / a.T;
             p = place_plain(a, b, first + t - b * a.T);
         }
         const float2 x = turn_of(p, a.inv_freq[j]);
-        cs[i] = x.x, sn[i] = x.y;
-    }
-    __syncthreads();
-    const HeadLane<D, V, INTER> hl(li, n);
-#pragma unroll 1
-    for (int x = 0; x < 2; x++) {
-        const bool isq = x == 0;
-        const int heads = isq ? a.hq : a.hkv, rows = here * heads;
-        if (heads == 0) continue;
-        const void *src = isq ? q : k;
-        void *dst = isq ? qo : ko;
-        const Strd sd = isq ? a.q : a.k;
-        float wa[V], wb[V];
-        load_weight<V>(a.weight_dtype, isq ? a.wq : a.wk, a.unit, hl.a, wa);
-        load_weight<V>(a.weight_dtype, isq ? a.wq : a.wk, a.unit, hl.b, wb);
-        RowWalk w(r0, BY, heads), put(r0, BY, heads);
-        for (int r = r0; r < rows; r += BY * U) {
-            float pa[U][V], pb[U][V];
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (r + u * BY < rows) {
-                    const int64_t token = first + w.t, b = token / a.T;
-                    const int64_t from = b * sd.b + (token - b * a.T) * sd.t + w.h * sd.h;
-                    piece<DT, V>(src, from + hl.a, pa[u]);
-                    piece<DT, V>(src, from + hl.b, pb[u]);
-                }
-                w.next();
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (r + u * BY < rows) {  // (a head's lanes agree)
-                    float ss = 0.f;
-#pragma unroll
-                    for (int i = 0; i < V; i++) ss += pa[u][i] * pa[u][i] + pb[u][i] * pb[u][i];
-                    const float rs = rsqrtf(head_sum<LPH>(ss) * (1.f / D) + a.eps);
-#pragma unroll
-                    for (int i = 0; i < V; i++) pa[u][i] *= rs * wa[i], pb[u][i] *= rs * wb[i];
-                    if (hl.turns) turn_pieces<V, INTER, false>(pa[u], pb[u], cs + put.t * n, sn + put.t * n, hl.ja, hl.jb);
-                    int64_t to;
-                    bool on = true;
-                    if (MODE == kRopePaged && !isq) {
-                        to = krow[put.t] + put.h * pg.k.h;
-                        on = krow[put.t] >= 0;
-                    } else {
-                        to = ((first + put.t) * heads + put.h) * D;
-                        if (MODE == kRopePaged && !is[put.t]) {
-#pragma unroll
-                            for (int i = 0; i < V; i++) pa[u][i] = pb[u][i] = 0.f;
-                        }
-                    }
-                    if (on) {
-                        put_piece<DT, V>(dst, to + hl.a, pa[u]);
-                        put_piece<DT, V>(dst, to + hl.b, pb[u]);
-                    }
-                }
-                put.next();
-            }
-        }
-    }
-    if constexpr (MODE == kRopePaged) {
-        constexpr int E = DT == DM_F32 ? 4 : 2;
-        const int rows = here * a.hkv;
-        if (rows == 0) return;
-        RowWalk w(r0, BY, a.hkv);
-        for (int r = r0; r < rows; r += BY, w.next()) {
-            if (vrow[w.t] < 0) continue;
-            const uint4 *from = (const uint4 *)((const char *)v + ((first + w.t) * a.v.t + w.h * a.v.h) * E);
-            uint4 *to = (uint4 *)((char *)vo + (vrow[w.t] + w.h * pg.v.h) * E);
-            const uint4 x = from[li], y = from[li + LPH];
-            to[li] = x, to[li + LPH] = y;
-        }
+        cs[i] = x.x, cs[tile * a.n + i] = x.y;
     }
 }
 
-// The gradients, the same split. A lane's weight gradients are of its own two pieces for every head that
-// it takes, so they stay in registers over the workgroup's tiles and meet in LDS at the end.
-template <int DT, int D, bool INTER>
-__global__ __launch_bounds__(256) void rope_bwd_fast(RopeArgs a, int tile, const void *__restrict__ q,
-                                                     const void *__restrict__ k, const void *__restrict__ gq,
-                                                     const void *__restrict__ gk, void *__restrict__ dq,
-                                                     void *__restrict__ dk, float *__restrict__ parts) {
+// A workgroup goes through tiles of tokens. Each round fills in the next tile's angles (paged: and the
+// places of the one behind that) and begins the loads of its first heads, so that a tile costs one barrier and
+// every part of the code stands once: the first rounds have a tile before the first token, which is empty.
+template <int DT, int D, int MODE, bool INTER>
+__global__ __launch_bounds__(256) void rope_fast(RopeArgs a, RopePages pg, int tile, const void *__restrict__ q,
+                                                 const void *__restrict__ k, const void *__restrict__ v,
+                                                 void *__restrict__ qo, void *__restrict__ ko, void *__restrict__ vo) {
     constexpr int V = rope_v<DT>(), LPH = D / (2 * V), BY = 256 / LPH, U = 2;
-    extern __shared__ float angles[];  // cos [tile, n], sin [tile, n]; at the end the lanes' sums [BY, D]
+    constexpr bool PAGED = MODE == kRopePaged;
+    extern __shared__ __align__(16) float lds[];  // the weights [2, D], two tiles' angles
+    __shared__ RopePlaces places[PAGED ? 3 : 1];
     const int tid = threadIdx.x, li = tid % LPH, r0 = tid / LPH, n = a.n;
-    float *cs = angles, *sn = angles + tile * n;
+    float *angles = lds + 2 * D;
+    const int64_t step = (int64_t)gridDim.x * tile, start = (int64_t)blockIdx.x * tile;
     const HeadLane<D, V, INTER> hl(li, n);
-    float wa[2][V], wb[2][V], da[2][V] = {}, db[2][V] = {};
+    uint4 ra[U], rb[U];
+    auto load = [&](int64_t first, int r, RowWalk &w, int rows, const void *src, const Strd &sd) __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
-        load_weight<V>(a.weight_dtype, x ? a.wk : a.wq, a.unit, hl.a, wa[x]);
-        load_weight<V>(a.weight_dtype, x ? a.wk : a.wq, a.unit, hl.b, wb[x]);
-    }
-    for (int64_t first = (int64_t)blockIdx.x * tile; first < a.tokens; first += (int64_t)gridDim.x * tile) {
-        const int here = (int)min((int64_t)tile, a.tokens - first);
-        __syncthreads();
-        for (int i = tid; i < here * n; i += 256) {
-            const int t = i / n, j = i - t * n;
-            const int64_t b = (first + t) / a.T;
-            const float2 x = turn_of(place_plain(a, b, first + t - b * a.T), a.inv_freq[j]);
-            cs[i] = x.x, sn[i] = x.y;
+        for (int u = 0; u < U; u++) {
+            if (r + u * BY < rows) {
+                const int64_t token = first + w.t, b = token / a.T;
+                const int64_t from = b * sd.b + (token - b * a.T) * sd.t + w.h * sd.h;
+                ra[u] = raw_piece<DT>(src, from + hl.a);
+                rb[u] = raw_piece<DT>(src, from + hl.b);
+            }
+            w.next();
         }
-        __syncthreads();
-#pragma unroll
+    };
+    // the heads whose first batch is loaded ahead: the queries', or the keys' where there are none
+    const bool ahead_k = a.hq == 0;
+    const int heads0 = max(ahead_k ? a.hkv : a.hq, 1);
+    int buf = 0, pl = 0;
+    for (int64_t first = start - (PAGED ? 2 : 1) * step; first < a.tokens; first += step) {
+        const int64_t next = first + step;
+        if constexpr (PAGED) {
+            if (next + step >= start) fill_places(a, pg, next + step, tile, places[(pl + 2) % 3]);
+        }
+        if (next >= start)
+            fill_angles<PAGED>(a, next, tile, &places[PAGED ? (pl + 1) % 3 : 0], angles + (buf ^ 1) * 2 * tile * n);
+        if (first < start && next >= start) fill_weights<D>(a, lds);
+        const int here = first < start ? 0 : (int)min((int64_t)tile, a.tokens - first);
+        const float *cs = angles + buf * 2 * tile * n, *sn = cs + tile * n;
+        const RopePlaces &place = places[PAGED ? pl : 0];
+#pragma unroll 1
         for (int x = 0; x < 2; x++) {
             const int heads = x ? a.hkv : a.hq, rows = here * heads;
-            if (heads == 0) continue;
-            const void *src = x ? k : q, *grad = x ? gk : gq;
-            void *dst = x ? dk : dq;
-            const Strd sd = x ? a.k : a.q, sg = x ? a.gk : a.gq;
+            if (rows == 0) continue;
+            const void *src = x ? k : q;
+            void *dst = x ? ko : qo;
+            const Strd sd = x ? a.k : a.q;
+            const float *wa = lds + x * D + hl.a, *wb = lds + x * D + hl.b;
             RowWalk w(r0, BY, heads), put(r0, BY, heads);
             for (int r = r0; r < rows; r += BY * U) {
-                float xa[U][V], xb[U][V], za[U][V], zb[U][V];
+                if (x == ahead_k && r == r0) {
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    if (r + u * BY < rows) {
-                        const int64_t token = first + w.t, b = token / a.T, t = token - b * a.T;
-                        const int64_t from = b * sd.b + t * sd.t + w.h * sd.h, g = b * sg.b + t * sg.t + w.h * sg.h;
-                        piece<DT, V>(src, from + hl.a, xa[u]);
-                        piece<DT, V>(src, from + hl.b, xb[u]);
-                        piece<DT, V>(grad, g + hl.a, za[u]);
-                        piece<DT, V>(grad, g + hl.b, zb[u]);
-                    }
-                    w.next();
+                    for (int u = 0; u < U; u++) w.next();
+                } else {
+                    load(first, r, w, rows, src, sd);
                 }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    if (r + u * BY < rows) {
-                        float ss = 0.f, gh = 0.f;
+                    if (r + u * BY < rows) {  // (a head's lanes agree)
+                        float pa[V], pb[V], ss = 0.f;
+                        unpack_piece<DT, V>(ra[u], pa);
+                        unpack_piece<DT, V>(rb[u], pb);
 #pragma unroll
-                        for (int i = 0; i < V; i++) ss += xa[u][i] * xa[u][i] + xb[u][i] * xb[u][i];
+                        for (int i = 0; i < V; i++) ss += pa[i] * pa[i] + pb[i] * pb[i];
                         const float rs = rsqrtf(head_sum<LPH>(ss) * (1.f / D) + a.eps);
-                        if (hl.turns) turn_pieces<V, INTER, true>(za[u], zb[u], cs + put.t * n, sn + put.t * n, hl.ja, hl.jb);
 #pragma unroll
-                        for (int i = 0; i < V; i++) {
-                            xa[u][i] *= rs, xb[u][i] *= rs;
-                            da[x][i] += za[u][i] * xa[u][i], db[x][i] += zb[u][i] * xb[u][i];
-                            za[u][i] *= wa[x][i], zb[u][i] *= wb[x][i];
-                            gh += za[u][i] * xa[u][i] + zb[u][i] * xb[u][i];
-                        }
-                        const float mean = head_sum<LPH>(gh) * (1.f / D);
+                        for (int i = 0; i < V; i++) pa[i] *= rs * wa[i], pb[i] *= rs * wb[i];
+                        if (hl.turns) turn_pieces<V, INTER, false>(pa, pb, cs + put.t * n, sn + put.t * n, hl.ja, hl.jb);
+                        int64_t to;
+                        bool on = true;
+                        if (PAGED && x) {
+                            to = place.krow[put.t] + put.h * pg.k.h;
+                            on = place.krow[put.t] >= 0;
+                        } else {
+                            to = ((first + put.t) * heads + put.h) * D;
+                            if (PAGED && !place.is[put.t]) {
 #pragma unroll
-                        for (int i = 0; i < V; i++) {
-                            za[u][i] = rs * (za[u][i] - xa[u][i] * mean);
-                            zb[u][i] = rs * (zb[u][i] - xb[u][i] * mean);
+                                for (int i = 0; i < V; i++) pa[i] = pb[i] = 0.f;
+                            }
                         }
-                        const int64_t to = ((first + put.t) * heads + put.h) * D;
-                        put_piece<DT, V>(dst, to + hl.a, za[u]);
-                        put_piece<DT, V>(dst, to + hl.b, zb[u]);
+                        if (on) {
+                            put_piece<DT, V>(dst, to + hl.a, pa);
+                            put_piece<DT, V>(dst, to + hl.b, pb);
+                        }
                     }
                     put.next();
                 }
             }
         }
+        if constexpr (PAGED) {
+            constexpr int E = DT == DM_F32 ? 4 : 2;
+            RowWalk w(r0, BY, max(a.hkv, 1));
+            for (int r = r0; r < here * a.hkv; r += BY, w.next()) {
+                if (place.vrow[w.t] < 0) continue;
+                const uint4 *from = (const uint4 *)((const char *)v + ((first + w.t) * a.v.t + w.h * a.v.h) * E);
+                uint4 *to = (uint4 *)((char *)vo + (place.vrow[w.t] + w.h * pg.v.h) * E);
+                const uint4 y = from[li], z = from[li + LPH];
+                to[li] = y, to[li + LPH] = z;
+            }
+        }
+        if (next >= start && next < a.tokens) {
+            RowWalk w(r0, BY, heads0);
+            load(next, r0, w, (int)min((int64_t)tile, a.tokens - next) * (ahead_k ? a.hkv : a.hq), ahead_k ? k : q,
+                 ahead_k ? a.k : a.q);
+        }
+        __syncthreads();
+        buf ^= 1;
+        pl = (pl + 1) % 3;
+    }
+}
+
+// The gradients, the same rounds. A lane's weight gradients are of its own two pieces for every head that
+// it takes, so they stay in registers over the workgroup's tiles (the queries' and the keys' in turn) and
+// meet in LDS at the end.
+template <int DT, int D, bool INTER>
+__global__ __launch_bounds__(256) void rope_bwd_fast(RopeArgs a, int tile, const void *__restrict__ q,
+                                                     const void *__restrict__ k, const void *__restrict__ gq,
+                                                     const void *__restrict__ gk, void *__restrict__ dq,
+                                                     void *__restrict__ dk, float *__restrict__ parts) {
+    constexpr int V = rope_v<DT>(), LPH = D / (2 * V), BY = 256 / LPH;
+    extern __shared__ __align__(16) float lds[];  // the weights [2, D], two tiles' angles; at the end the lanes' sums [BY, D]
+    const int tid = threadIdx.x, li = tid % LPH, r0 = tid / LPH, n = a.n;
+    float *angles = lds + 2 * D;
+    const HeadLane<D, V, INTER> hl(li, n);
+    float da[2][V] = {}, db[2][V] = {};  // of the heads that are gone through now, and of the others
+    const int64_t step = (int64_t)gridDim.x * tile, start = (int64_t)blockIdx.x * tile;
+    int buf = 0;
+    for (int64_t first = start - step; first < a.tokens; first += step, buf ^= 1) {
+        fill_angles<false>(a, first + step, tile, nullptr, angles + (buf ^ 1) * 2 * tile * n);
+        if (first < start) fill_weights<D>(a, lds);
+        const int here = first < start ? 0 : (int)min((int64_t)tile, a.tokens - first);
+        const float *cs = angles + buf * 2 * tile * n, *sn = cs + tile * n;
+#pragma unroll 1
+        for (int x = 0; x < 2; x++) {
+            const int heads = max(x ? a.hkv : a.hq, 1), rows = here * (x ? a.hkv : a.hq);
+            const void *src = x ? k : q, *grad = x ? gk : gq;
+            void *dst = x ? dk : dq;
+            const Strd sd = x ? a.k : a.q, sg = x ? a.gk : a.gq;
+            const float *wa = lds + x * D + hl.a, *wb = lds + x * D + hl.b;
+            RowWalk w(r0, BY, heads);
+            for (int r = r0; r < rows; r += BY, w.next()) {
+                const int64_t token = first + w.t, b = token / a.T, t = token - b * a.T;
+                const int64_t from = b * sd.b + t * sd.t + w.h * sd.h, g = b * sg.b + t * sg.t + w.h * sg.h;
+                const uint4 rxa = raw_piece<DT>(src, from + hl.a), rxb = raw_piece<DT>(src, from + hl.b);
+                const uint4 rza = raw_piece<DT>(grad, g + hl.a), rzb = raw_piece<DT>(grad, g + hl.b);
+                float xa[V], xb[V], za[V], zb[V], ss = 0.f, gh = 0.f;
+                unpack_piece<DT, V>(rxa, xa);
+                unpack_piece<DT, V>(rxb, xb);
+#pragma unroll
+                for (int i = 0; i < V; i++) ss += xa[i] * xa[i] + xb[i] * xb[i];
+                const float rs = rsqrtf(head_sum<LPH>(ss) * (1.f / D) + a.eps);
+                unpack_piece<DT, V>(rza, za);
+                unpack_piece<DT, V>(rzb, zb);
+                if (hl.turns) turn_pieces<V, INTER, true>(za, zb, cs + w.t * n, sn + w.t * n, hl.ja, hl.jb);
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    xa[i] *= rs, xb[i] *= rs;
+                    da[0][i] += za[i] * xa[i], db[0][i] += zb[i] * xb[i];
+                    za[i] *= wa[i], zb[i] *= wb[i];
+                    gh += za[i] * xa[i] + zb[i] * xb[i];
+                }
+                const float mean = head_sum<LPH>(gh) * (1.f / D);
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    za[i] = rs * (za[i] - xa[i] * mean);
+                    zb[i] = rs * (zb[i] - xb[i] * mean);
+                }
+                const int64_t to = ((first + w.t) * heads + w.h) * D;
+                put_piece<DT, V>(dst, to + hl.a, za);
+                put_piece<DT, V>(dst, to + hl.b, zb);
+            }
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const float ta = da[0][i], tb = db[0][i];
+                da[0][i] = da[1][i], db[0][i] = db[1][i];
+                da[1][i] = ta, db[1][i] = tb;
+            }
+        }
+        __syncthreads();
     }
 #pragma unroll
     for (int x = 0; x < 2; x++) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < V; i++) angles[r0 * D + hl.a + i] = da[x][i], angles[r0 * D + hl.b + i] = db[x][i];
+        for (int i = 0; i < V; i++) lds[r0 * D + hl.a + i] = da[x][i], lds[r0 * D + hl.b + i] = db[x][i];
         __syncthreads();
         for (int e = tid; e < D; e += 256) {
             float t = 0.f;
-            for (int i = 0; i < BY; i++) t += angles[i * D + e];
+            for (int i = 0; i < BY; i++) t += lds[i * D + e];
             parts[((int64_t)blockIdx.x * 2 + x) * D + e] = t;
         }
     }
@@ -572,7 +607,7 @@ __global__ __launch_bounds__(1024) void rope_weights(const float *__restrict__ p
     }
 }
 
-constexpr int64_t kRopeParts = 1024;  // workgroups of the backward at most
+constexpr int64_t kRopeParts = 768;  // workgroups of the backward at most
 
 static int64_t bwd_workgroups(const dm_qk_norm_rope_desc *d) {
     const int64_t tokens = d->b * d->t;
@@ -640,6 +675,8 @@ static int rope_tile(const RopeArgs &a, int by) {
     while (tile < kRopeTile && tile * heads < 4 * by && a.tokens >= 2048 * tile) tile *= 2;
     return (int)tile;
 }
+constexpr int64_t kRopeGrid = 4096;  // workgroups at most
+static size_t rope_lds(const RopeArgs &a, int tile) { return ((size_t)2 * a.d + (size_t)4 * tile * a.n) * sizeof(float); }
 
 #define ROPE_D(KERNEL, DT, MODE_, GRID, LDS, ...)                                                           \
     do {                                                                                                    \
@@ -665,8 +702,8 @@ static int run_rope(const char *op, const dm_qk_norm_rope_desc *d, const RopeArg
     constexpr bool paged = MODE == kRopePaged;
     if (fast_takes(d, a, ptrs, paged ? 6 : 4, strides, paged ? 5 : 2)) {
         const int by = 256 / (int)(d->d / (d->dtype == DM_F32 ? 8 : 16)), tile = rope_tile(a, by);
-        const unsigned grid = (unsigned)((a.tokens + tile - 1) / tile);
-        const size_t lds = (size_t)tile * d->n * 2 * sizeof(float);
+        const unsigned grid = (unsigned)std::min((a.tokens + tile - 1) / tile, kRopeGrid);
+        const size_t lds = rope_lds(a, tile);
         if (d->dtype == DM_F32)
             ROPE_D(rope_fast, DM_F32, ROPE_COMMA MODE, grid, lds, a, pg, tile, q, k, v, qo, ko, vo);
         else if (d->dtype == DM_BF16)
@@ -728,7 +765,7 @@ int dm_qk_norm_rope_bwd(const dm_qk_norm_rope_desc *d, const void *q, const void
             const int by = 256 / (int)(d->d / (d->dtype == DM_F32 ? 8 : 16)), tile = rope_tile(a, by);
             nparts = std::min<int64_t>((a.tokens + tile - 1) / tile, kRopeParts);
             const unsigned grid = (unsigned)nparts;
-            const size_t lds = std::max((size_t)tile * d->n * 2, (size_t)by * d->d) * sizeof(float);
+            const size_t lds = std::max(rope_lds(a, tile), (size_t)by * d->d * sizeof(float));
             if (d->dtype == DM_F32)
                 ROPE_D(rope_bwd_fast, DM_F32, , grid, lds, a, tile, q, k, grad_q, grad_k, dq, dk, parts);
             else if (d->dtype == DM_BF16)
