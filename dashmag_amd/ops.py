@@ -12,6 +12,7 @@ outside the contract raises :class:`~dashmag_amd.contract.Unsupported` whose mes
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -442,11 +443,21 @@ def attention_decode_paged(query, key_pages, value_pages, block_table, lengths=N
 # Norms and rotation of queries and keys
 # ------------------------------------------------------------------------------------------
 
+# (The calls of these operators take a few microseconds on the GPU, as long as the host takes for a dozen
+# attribute look-ups: pointers go to the library as numbers, strides into a descriptor by one
+# ``pack_into``, and the device is switched only where it is another.)
+_STRIDES = {n: struct.Struct(f"{n}q") for n in (3, 6, 9, 12, 15)}
+
+
 def _run(op, device, fn, *args):
     """The library call ``fn(*args, stream)`` on ``device`` (which need not be torch's current one) and
     its current stream."""
-    with torch.cuda.device(device):
-        rc = fn(*args, ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc == _lib.DM_OK:
         return
     msg = _lib.last_error()
@@ -456,10 +467,26 @@ def _run(op, device, fn, *args):
 
 
 def _one_device(op, first, *ts):
-    _device(op, first, *ts)
+    dev = first.device
+    _device(op, first)
     for t in ts:
-        if t is not None and t.device != first.device:
-            raise Unsupported(f"{op}: the tensors must be on one GPU (got {first.device} and {t.device})")
+        if t is not None and t.device != dev:
+            _device(op, t)
+            raise Unsupported(f"{op}: the tensors must be on one GPU (got {dev} and {t.device})")
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _whole(t):
+    """``_readable`` of a tensor that most often is contiguous and aligned as it is."""
+    return t if t.is_contiguous() and not t.data_ptr() % 16 else _readable(t)
+
+
+def _put_strides(desc, first, *values):
+    """The ``dm_strides`` of ``desc`` from the field ``first`` on."""
+    _STRIDES[len(values)].pack_into(desc, getattr(type(desc), first).offset, *values)
 
 
 _INTS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
@@ -470,7 +497,7 @@ def _device_i32(op, t, device, what):
     the GPU in place and unread (no wait for the GPU, so such a call can be captured), any other
     converted, values outside int32 refused."""
     if isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device:
-        return t.detach() if t.is_contiguous() else t.detach().contiguous()
+        return t if t.is_contiguous() else t.contiguous()
     t = torch.as_tensor(t)
     if t.numel() and t.dtype not in _INTS:
         raise Unsupported(f"{op}: {what} must be whole numbers, got {t.dtype}")
@@ -478,39 +505,38 @@ def _device_i32(op, t, device, what):
 
 
 def _qk_norm_rope_desc(op, query, key, q_weight, k_weight, inv_freq, options, paged):
-    dims, form = (3, "[N, H, D]") if paged else (4, "[B, T, H, D]")
-    if query.dim() != dims or key.dim() != dims:
-        raise Unsupported(f"{op}: query and key are {form}")
-    if tuple(query.shape[:-2]) != tuple(key.shape[:-2]):
+    qs, ks, dtype = query.shape, key.shape, query.dtype
+    if len(qs) != (3 if paged else 4) or len(ks) != len(qs):
+        raise Unsupported(f"{op}: query and key are {'[N, H, D]' if paged else '[B, T, H, D]'}")
+    if qs[:-2] != ks[:-2]:
         raise Unsupported(f"{op}: query and key must have the same tokens")
-    if query.shape[-1] != key.shape[-1]:
+    d = qs[-1]
+    if d != ks[-1]:
         raise Unsupported(f"{op}: query and key must have one head dimension")
-    if query.dtype != key.dtype:
+    if dtype != key.dtype:
         raise Unsupported(f"{op}: query and key must share one dtype")
-    d = query.shape[-1]
-    desc = _lib.QkNormRopeDesc(b=1 if paged else query.shape[0], t=query.shape[-3],
-                               hq=query.shape[-2], hkv=key.shape[-2], d=d, dtype=_dtype(op, query),
-                               interleaved=int(bool(options.interleaved)),
-                               unit_offset=int(bool(options.unit_offset)), eps=float(options.eps))
-    desc.weight_dtype = desc.dtype
+    dt = weight_dtype = _dtype(op, query)
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is None:
             continue
-        if tuple(w.shape) != (d,):
+        if w.shape != (d,):
             raise Unsupported(f"{op}: {name} is [D] = [{d}]")
-        if w.dtype not in (torch.float32, query.dtype):
+        if w.dtype != dtype and w.dtype != torch.float32:
             raise Unsupported(f"{op}: {name} must be f32 or the queries' dtype")
-        desc.weight_dtype = _DT[w.dtype]
+        weight_dtype = _DT[w.dtype]
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise Unsupported(f"{op}: q_weight and k_weight must share one dtype")
     if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
         raise Unsupported(f"{op}: inv_freq is [n] f32")
-    desc.n = inv_freq.shape[0]
-    if 2 * desc.n > d:
+    n = inv_freq.shape[0]
+    if 2 * n > d:
         raise Unsupported(f"{op}: the frequencies are [n] with 2 n at most the head dimension ({d}), "
-                          f"got n = {desc.n}")
-    desc.strided = 1
-    return desc
+                          f"got n = {n}")
+    # (b, t, hq, hkv, d, n, dtype, weight_dtype, interleaved, unit_offset, eps, positions, positions_i64,
+    # positions_b, strided)
+    return _lib.QkNormRopeDesc(1 if paged else qs[0], qs[-3], qs[-2], ks[-2], d, n, dt, weight_dtype,
+                               1 if options.interleaved else 0, 1 if options.unit_offset else 0,
+                               options.eps, None, 0, 0, 1)
 
 
 def _positions(op, desc, positions, device):
@@ -531,7 +557,7 @@ def _positions(op, desc, positions, device):
 
 
 def _flat(w):
-    return None if w is None else w.contiguous()
+    return w if w is None or w.is_contiguous() else w.contiguous()
 
 
 def qk_norm_rope(query, key, q_weight, k_weight, inv_freq, positions=None,
@@ -547,12 +573,11 @@ def qk_norm_rope(query, key, q_weight, k_weight, inv_freq, positions=None,
     desc = _qk_norm_rope_desc(op, query, key, q_weight, k_weight, inv_freq, options, False)
     dev = query.device
     at = _positions(op, desc, positions, dev)
-    q, k, wq, wk, freq = _readable(query), _readable(key), _flat(q_weight), _flat(k_weight), _flat(inv_freq)
-    _set_strides(desc.sq, q, (0, 1, 2))
-    _set_strides(desc.sk, k, (0, 1, 2))
+    q, k, wq, wk, freq = _whole(query), _whole(key), _flat(q_weight), _flat(k_weight), _flat(inv_freq)
+    _put_strides(desc, "sq", *q.stride()[:3], *k.stride()[:3])
     qo, ko = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k))
-    _run(op, dev, _lib.lib().dm_qk_norm_rope, ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(wq), _ptr(wk),
-         _ptr(freq), _ptr(qo), _ptr(ko))
+    _run(op, dev, _lib.lib().dm_qk_norm_rope, ctypes.byref(desc), q.data_ptr(), k.data_ptr(), _at(wq), _at(wk),
+         freq.data_ptr(), qo.data_ptr(), ko.data_ptr())
     return qo, ko
 
 
@@ -569,35 +594,35 @@ def qk_norm_rope_backward(query, key, q_weight, k_weight, inv_freq, grad_query, 
         raise Unsupported(f"{op}: the gradients have the outputs' shapes")
     dev = query.device
     at = _positions(op, desc, positions, dev)
-    q, k, wq, wk, freq = _readable(query), _readable(key), _flat(q_weight), _flat(k_weight), _flat(inv_freq)
-    gq, gk = _readable(grad_query.to(q.dtype)), _readable(grad_key.to(q.dtype))
-    for f, t in ((desc.sq, q), (desc.sk, k), (desc.sgq, gq), (desc.sgk, gk)):
-        _set_strides(f, t, (0, 1, 2))
+    q, k, wq, wk, freq = _whole(query), _whole(key), _flat(q_weight), _flat(k_weight), _flat(inv_freq)
+    gq, gk = _whole(grad_query.to(q.dtype)), _whole(grad_key.to(q.dtype))
+    _put_strides(desc, "sq", *q.stride()[:3], *k.stride()[:3])
+    _put_strides(desc, "sgq", *gq.stride()[:3], *gk.stride()[:3])
     dq, dk = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k))
     dwq, dwk = (None if w is None else torch.empty(w.shape, dtype=w.dtype, device=dev) for w in (wq, wk))
     nbytes = _lib.lib().dm_qk_norm_rope_bwd_workspace(ctypes.byref(desc))
     ws = _workspace(nbytes, dev)
-    _run(op, dev, _lib.lib().dm_qk_norm_rope_bwd, ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(wq), _ptr(wk),
-         _ptr(freq), _ptr(gq), _ptr(gk), _ptr(dq), _ptr(dk), _ptr(dwq), _ptr(dwk), _ptr(ws), nbytes)
+    _run(op, dev, _lib.lib().dm_qk_norm_rope_bwd, ctypes.byref(desc), q.data_ptr(), k.data_ptr(), _at(wq), _at(wk),
+         freq.data_ptr(), gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr(), _at(dwq), _at(dwk),
+         ws.data_ptr(), nbytes)
     return dq, dk, dwq, dwk
 
 
 def _in_pages(op, pages, what):
     """Pages that a call writes: a view is written in place, so its rows must be whole and apart."""
+    if pages.is_contiguous() or not pages.numel():
+        return
     st, shape = pages.stride(), pages.shape
-    if pages.numel() and ((shape[-1] > 1 and st[-1] != 1)
-                          or any(n > 1 and x == 0 for n, x in zip(shape, st))):
+    if (shape[-1] > 1 and st[-1] != 1) or any(n > 1 and x == 0 for n, x in zip(shape, st)):
         raise Unsupported(f"{op}: {what} must be a view whose last dimension is contiguous and whose "
                           "elements are apart")
 
 
-def _block_table(op, block_table, rows, device, keep):
+def _block_table(op, block_table, rows, device):
     bt = block_table if isinstance(block_table, torch.Tensor) else torch.as_tensor(block_table)
     if bt.dim() != 2 or (rows is not None and bt.shape[0] != rows):
         raise Unsupported(f"{op}: the block table is [{'R' if rows is None else rows}, max_pages]")
-    bt = _device_i32(op, bt, device, "the block table")
-    keep.append(bt)
-    return bt
+    return _device_i32(op, bt, device, "the block table")
 
 
 def qk_norm_rope_paged(query, key, value, q_weight, k_weight, inv_freq, key_pages, value_pages, block_table,
@@ -618,45 +643,43 @@ def qk_norm_rope_paged(query, key, value, q_weight, k_weight, inv_freq, key_page
     options = options or QkNormRopeOptions()
     _one_device(op, query, key, value, q_weight, k_weight, inv_freq, key_pages, value_pages)
     desc = _qk_norm_rope_desc(op, query, key, q_weight, k_weight, inv_freq, options, True)
-    if tuple(value.shape) != tuple(key.shape):
+    if value.shape != key.shape:
         raise Unsupported(f"{op}: key and value must have one shape")
-    if key_pages.dim() != 4 or tuple(key_pages.shape) != tuple(value_pages.shape):
+    ps = key_pages.shape
+    if len(ps) != 4 or ps != value_pages.shape:
         raise Unsupported(f"{op}: the key and value pages are [P, page_size, Hkv, D], one shape")
-    if tuple(key_pages.shape[2:]) != tuple(key.shape[1:]):
+    if ps[2:] != key.shape[1:]:
         raise Unsupported(f"{op}: the pages' rows are the keys' [Hkv, D] = {list(key.shape[1:])}")
-    if not (query.dtype == value.dtype == key_pages.dtype == value_pages.dtype):
+    dtype = query.dtype
+    if not (dtype == value.dtype == key_pages.dtype == value_pages.dtype):
         raise Unsupported(f"{op}: query, key, value and the pages must share one dtype")
-    if key_pages.shape[1] < 1:
+    if ps[1] < 1:
         raise Unsupported(f"{op}: pages hold at least one key")
     _in_pages(op, key_pages, "key_pages")
     _in_pages(op, value_pages, "value_pages")
     dev, n = query.device, query.shape[0]
-    keep = []
     ln = _device_i32(op, lengths, dev, "the cache lengths")
     if ln.dim() != 1:
         raise Unsupported(f"{op}: the cache lengths are [S]")
     nseq = ln.shape[0]
-    bt = _block_table(op, block_table, nseq, dev, keep)
+    bt = _block_table(op, block_table, nseq, dev)
     cu = None
     if cu_seqlens is not None:
         cu = _device_i32(op, cu_seqlens, dev, "cu_seqlens")
-        if tuple(cu.shape) != (nseq + 1,):
+        if cu.shape != (nseq + 1,):
             raise Unsupported(f"{op}: cu_seqlens is [S + 1] = [{nseq + 1}]")
     elif nseq != n:
         raise Unsupported(f"{op}: without cu_seqlens there is one token a sequence, got {n} tokens and "
                           f"{nseq} sequences")
-    q, k, v = _readable(query), _readable(key), _readable(value)
+    q, k, v = _whole(query), _whole(key), _whole(value)
     wq, wk, freq = _flat(q_weight), _flat(k_weight), _flat(inv_freq)
-    for f, t in ((desc.sq, q), (desc.sk, k), (desc.sv, v)):
-        _set_strides(f, t, (None, 0, 1))
-    pages = _lib.KvPages(num_pages=key_pages.shape[0], page_size=key_pages.shape[1], max_pages=bt.shape[1],
-                         nseq=nseq, block_table=bt.data_ptr(), lengths=ln.data_ptr(),
-                         cu_seqlens=None if cu is None else cu.data_ptr())
-    _set_strides(pages.sk, key_pages, (0, 1, 2))
-    _set_strides(pages.sv, value_pages, (0, 1, 2))
-    qo = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    _run(op, dev, _lib.lib().dm_qk_norm_rope_paged, ctypes.byref(desc), ctypes.byref(pages), _ptr(q), _ptr(k),
-         _ptr(v), _ptr(wq), _ptr(wk), _ptr(freq), _ptr(qo), _ptr(key_pages), _ptr(value_pages))
+    _put_strides(desc, "sq", 0, *q.stride()[:2], 0, *k.stride()[:2], 0, *v.stride()[:2])
+    pages = _lib.KvPages(ps[0], ps[1], bt.shape[1], nseq, bt.data_ptr(), ln.data_ptr(), _at(cu))
+    _put_strides(pages, "sk", *key_pages.stride()[:3], *value_pages.stride()[:3])
+    qo = torch.empty(q.shape, dtype=dtype, device=dev)
+    _run(op, dev, _lib.lib().dm_qk_norm_rope_paged, ctypes.byref(desc), ctypes.byref(pages), q.data_ptr(),
+         k.data_ptr(), v.data_ptr(), _at(wq), _at(wk), freq.data_ptr(), qo.data_ptr(), key_pages.data_ptr(),
+         value_pages.data_ptr())
     return qo
 
 
@@ -675,33 +698,56 @@ def attention_decode_shared(query, key_pages, value_pages, block_table, lengths,
     op = "attention_decode_shared"
     options = options or AttentionOptions()
     _one_device(op, query, key_pages, value_pages)
-    if key_pages.dim() != 4:
-        raise Unsupported(f"{op}: the key pages are [P, page_size, Hkv, D]")
-    npages, page_size = key_pages.shape[0], key_pages.shape[1]
+    qs, ps, dtype = query.shape, key_pages.shape, query.dtype
+    if len(qs) != 3:
+        raise Unsupported(f"{op}: query is [B, Hq, D]")
+    if len(ps) != 4 or ps != value_pages.shape:
+        raise Unsupported(f"{op}: the key and value pages are [P, page_size, Hkv, D], one shape")
+    (b, hq, d), (npages, page_size, hkv, dk) = qs, ps
     if page_size < 1:
         raise Unsupported(f"{op}: pages hold at least one key")
-    dev, b = query.device, query.shape[0] if query.dim() == 3 else -1
-    keep = []
-    bt = _block_table(op, block_table, b, dev, keep)
+    if d != dk:
+        raise Unsupported(f"{op}: query and key must have one head dimension")
+    if hkv == 0 or hq % hkv != 0:
+        raise Unsupported(f"{op}: the query heads ({hq}) must be a multiple of the key-value heads ({hkv})")
+    if not (dtype == key_pages.dtype == value_pages.dtype):
+        raise Unsupported(f"{op}: query, key and value must share one dtype")
+    dev = query.device
+    bt = _block_table(op, block_table, b, dev)
     max_pages = bt.shape[1]
-    desc = _decode_desc(op, query, key_pages, value_pages, max_pages * page_size, options)
     ln, cu, pl = _shared_arrays(op, lengths, groups, prefix_lengths, b, dev)
-    q, k, v = _readable(query), _readable(key_pages), _readable(value_pages)
-    _decode_strides(desc, q, k, v, (0, 1, 2))
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    q, k, v = _whole(query), _whole(key_pages), _whole(value_pages)
+    desc = _lib.AttentionDesc(b, 1, max_pages * page_size, hq, hkv, d, _dtype(op, query), _lib.DM_MASK_NONE)
+    if options.scale is not None or options.window is not None:
+        _decode_options(desc.options, options)
+    desc.strided = 1
+    sq = q.stride()
+    _put_strides(desc, "sq", sq[0], 0, sq[1], *k.stride()[:3], *v.stride()[:3])
+    out = torch.empty(qs, dtype=dtype, device=dev)
     ng = cu.shape[0] - 1
     nbytes = _lib.lib().dm_attention_decode_shared_workspace(ctypes.byref(desc), page_size, ng)
     ws = _workspace(nbytes, dev)
-    _run(op, dev, _lib.lib().dm_attention_decode_shared, ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), npages,
-         page_size, _ptr(bt), max_pages, _ptr(ln), _ptr(cu), ng, _ptr(pl), _ptr(out), _ptr(ws), nbytes)
+    _run(op, dev, _lib.lib().dm_attention_decode_shared, ctypes.byref(desc), q.data_ptr(), k.data_ptr(),
+         v.data_ptr(), npages, page_size, bt.data_ptr(), max_pages, _at(ln), cu.data_ptr(), ng, pl.data_ptr(),
+         out.data_ptr(), ws.data_ptr(), nbytes)
     return out
+
+
+def _decode_options(o, options):
+    """The scale and the window of a decode."""
+    o.has_scale = int(options.scale is not None)
+    o.scale = float(options.scale) if options.scale is not None else 0.0
+    o.has_window = int(options.window is not None)
+    if options.window is not None:
+        o.window_left = min(int(options.window.left), UNBOUNDED)
+        o.window_right = min(int(options.window.right), UNBOUNDED)
 
 
 def _shared_arrays(op, lengths, groups, prefix_lengths, b, device):
     """The lengths (None: every key), groups and prefix lengths as int32 device arrays; groups that lie
     on the host are checked there."""
     ln = None if lengths is None else _device_i32(op, lengths, device, "the cache lengths")
-    if ln is not None and tuple(ln.shape) != (b,):
+    if ln is not None and ln.shape != (b,):
         raise Unsupported(f"{op}: the cache lengths are [B] = [{b}]")
     cu = _device_i32(op, groups, device, "groups")
     if cu.dim() != 1 or cu.shape[0] < 1:
@@ -712,7 +758,7 @@ def _shared_arrays(op, lengths, groups, prefix_lengths, b, device):
             raise Unsupported(f"{op}: groups must go from 0 or more to at most B = {b} without decreasing, "
                               f"got {at}")
     pl = _device_i32(op, prefix_lengths, device, "the prefix lengths")
-    if tuple(pl.shape) != (cu.shape[0] - 1,):
+    if pl.shape != (cu.shape[0] - 1,):
         raise Unsupported(f"{op}: the prefix lengths are [G] = [{cu.shape[0] - 1}]")
     return ln, cu, pl
 
@@ -737,9 +783,8 @@ def _cache_desc(op, block_table, lengths, refcounts, page_size):
         raise Unsupported(f"{op}: the cache lengths are [R] = [{rows}]")
     if page_size < 1:
         raise Unsupported(f"{op}: pages hold at least one key")
-    return _lib.CacheTable(rows=rows, max_pages=max_pages, num_pages=refcounts.shape[0], page_size=page_size,
-                           block_table=block_table.data_ptr(), lengths=lengths.data_ptr(),
-                           refcounts=refcounts.data_ptr())
+    return _lib.CacheTable(rows, max_pages, refcounts.shape[0], page_size, block_table.data_ptr(),
+                           lengths.data_ptr(), refcounts.data_ptr())
 
 
 def _cache_pools(op, pools, num_pages, device):
@@ -748,20 +793,22 @@ def _cache_pools(op, pools, num_pages, device):
     if isinstance(pools, torch.Tensor) or len(pools) == 0:
         raise Unsupported(f"{op}: the pools are a list of at least one tensor [P, page_size, ...]")
     page_size = pools[0].shape[1] if pools[0].dim() >= 2 else 0
-    arr = (_lib.CachePool * len(pools))()
-    for x, t in zip(arr, pools):
+    values = []
+    for t in pools:
         if t.dim() < 2 or t.shape[0] != num_pages or t.shape[1] != page_size or t.device != device:
             raise Unsupported(f"{op}: the pools are [P, page_size, ...] with P = {num_pages} and one page_size, "
                               f"on {device}")
         if page_size < 1:
             raise Unsupported(f"{op}: pages hold at least one key")
+        each = t.numel() // num_pages if num_pages else 0
         if not t.is_contiguous():  # (a slice of a wider pool, say: whole pages, apart)
             if num_pages and t.numel() and not (t[0].is_contiguous() and
-                                                (num_pages == 1 or t.stride(0) >= t[0].numel())):
+                                                (num_pages == 1 or t.stride(0) >= each)):
                 raise Unsupported(f"{op}: the pools' pages must each be contiguous and apart")
         size = t.element_size()
-        each = t.numel() // num_pages if num_pages else 0
-        x.pages, x.page_bytes, x.page_stride = t.data_ptr(), each * size, (t.stride(0) if num_pages > 1 else each) * size
+        values += (t.data_ptr(), each * size, (t.stride(0) if num_pages > 1 else each) * size)
+    arr = (_lib.CachePool * len(pools))()
+    struct.pack_into(f"{len(values)}q", arr, 0, *values)
     return arr, page_size
 
 
@@ -788,7 +835,7 @@ def cache_reserve(block_table, lengths, refcounts, new_lengths, page_size):
     granted = torch.empty(desc.rows, dtype=torch.bool, device=dev)
     nbytes = _lib.lib().dm_cache_reserve_workspace(ctypes.byref(desc))
     ws = _workspace(nbytes, dev)
-    _run(op, dev, _lib.lib().dm_cache_reserve, ctypes.byref(desc), _ptr(new), _ptr(granted), _ptr(ws), nbytes)
+    _run(op, dev, _lib.lib().dm_cache_reserve, ctypes.byref(desc), new.data_ptr(), granted.data_ptr(), ws.data_ptr(), nbytes)
     return granted
 
 
@@ -812,8 +859,8 @@ def cache_fork(pools, block_table, lengths, refcounts, parents, children):
     fresh = torch.empty(n, dtype=torch.int32, device=dev)
     nbytes = _lib.lib().dm_cache_fork_workspace(ctypes.byref(desc), n)
     ws = _workspace(nbytes, dev)
-    _run(op, dev, _lib.lib().dm_cache_fork, ctypes.byref(desc), arr, len(arr), _ptr(pa), _ptr(ch), n,
-         _ptr(fresh), _ptr(ws), nbytes)
+    _run(op, dev, _lib.lib().dm_cache_fork, ctypes.byref(desc), arr, len(arr), pa.data_ptr(), ch.data_ptr(), n,
+         fresh.data_ptr(), ws.data_ptr(), nbytes)
     return fresh
 
 
@@ -825,7 +872,7 @@ def cache_free(block_table, lengths, refcounts, rows, page_size):
     desc = _cache_table(op, block_table, lengths, refcounts, page_size)
     dev = block_table.device
     r = _rows_i32(op, rows, dev, "the rows")
-    _run(op, dev, _lib.lib().dm_cache_free, ctypes.byref(desc), _ptr(r), r.shape[0])
+    _run(op, dev, _lib.lib().dm_cache_free, ctypes.byref(desc), r.data_ptr(), r.shape[0])
 
 
 def cache_compact(pools, block_table, lengths, refcounts):
@@ -840,7 +887,7 @@ def cache_compact(pools, block_table, lengths, refcounts):
     moved = torch.empty(desc.num_pages, dtype=torch.int32, device=dev)
     nbytes = _lib.lib().dm_cache_compact_workspace(ctypes.byref(desc))
     ws = _workspace(nbytes, dev)
-    _run(op, dev, _lib.lib().dm_cache_compact, ctypes.byref(desc), arr, len(arr), _ptr(moved), _ptr(ws), nbytes)
+    _run(op, dev, _lib.lib().dm_cache_compact, ctypes.byref(desc), arr, len(arr), moved.data_ptr(), ws.data_ptr(), nbytes)
     return moved
 
 
