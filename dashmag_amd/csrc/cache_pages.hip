@@ -38,57 +38,72 @@ __device__ __forceinline__ int64_t pages_of(const CacheArgs &a, int64_t keys) {
     return (keys + a.page_size - 1) / a.page_size;
 }
 
-// The workgroup's exclusive prefix sums of x, and its total. For every thread of kPlan; `sums` is LDS.
-__device__ __forceinline__ int64_t plan_scan(int64_t x, int64_t *sums, int64_t *total) {
+// The workgroup's exclusive prefix sums of x, and its total, in 32 bits (the host sees to it that the sums
+// fit). For every thread of kPlan; `sums` is LDS, two turns of it, so that a scan costs one barrier.
+struct PlanSums {
+    int4 of[2][kPlan / 64 / 4];
+};
+__device__ __forceinline__ int32_t plan_scan(int32_t x, PlanSums &sums, int &turn, int32_t *total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t in = x;
+    int32_t in = x;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int64_t y = __shfl_up(in, o, 64);
+        const int32_t y = __shfl_up(in, o, 64);
         if (lane >= o) in += y;
     }
+    int4 *s = sums.of[turn];
+    turn ^= 1;
+    if (lane == 63) ((int32_t *)s)[wave] = in;
     __syncthreads();
-    if (lane == 63) sums[wave] = in;
-    __syncthreads();
-    int64_t before = 0, all = 0;
-    for (int w = 0; w < kPlan / 64; w++) {
-        const int64_t s = sums[w];
-        if (w < wave) before += s;
-        all += s;
+    int32_t before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kPlan / 64 / 4; i++) {
+        const int4 v = s[i];
+        const int32_t y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            before += 4 * i + u < wave ? y[u] : 0;
+            all += y[u];
+        }
     }
     *total = all;
     return before + in - x;
 }
 
+// The counts of four pages from p on (1 past the last).
+__device__ __forceinline__ int4 four_counts(const CacheArgs &a, int64_t p) {
+    if (p + 4 <= a.num_pages && ((uintptr_t)a.counts & 15) == 0) return *(const int4 *)(a.counts + p);
+    int4 x;
+    x.x = p < a.num_pages ? a.counts[p] : 1, x.y = p + 1 < a.num_pages ? a.counts[p + 1] : 1;
+    x.z = p + 2 < a.num_pages ? a.counts[p + 2] : 1, x.w = p + 3 < a.num_pages ? a.counts[p + 3] : 1;
+    return x;
+}
+
 // Walks the counts from *cursor until `want` free pages are in `list` (lowest index first) or there
-// are no more; *found and *cursor are the workgroup's.
+// are no more; *found and *cursor are the workgroup's. (`list` is written when the workgroup next meets.)
 __device__ __forceinline__ void find_free(const CacheArgs &a, int64_t want, int32_t *list, int64_t *cursor,
-                                          int64_t *found, int64_t *sums) {
+                                          int32_t *found, PlanSums &sums, int &turn) {
     while (*found < want && *cursor < a.num_pages) {
         const int64_t i = *cursor + (int64_t)threadIdx.x * 4;
-        bool is[4];
-        int64_t mine = 0, total;
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            is[u] = i + u < a.num_pages && a.counts[i + u] <= 0;
-            mine += is[u];
-        }
-        int64_t at = *found + plan_scan(mine, sums, &total);
+        const int4 c = four_counts(a, i);
+        const bool is[4] = {c.x <= 0, c.y <= 0, c.z <= 0, c.w <= 0};
+        int32_t total, at = *found + plan_scan(is[0] + is[1] + is[2] + is[3], sums, turn, &total);
 #pragma unroll
         for (int u = 0; u < 4; u++)
             if (is[u]) list[at++] = (int32_t)(i + u);
         *found += total;
         *cursor += kPlan * 4;
     }
-    __syncthreads();  // the list is written
 }
 
 __global__ __launch_bounds__(kPlan) void cache_reserve_kernel(CacheArgs a, const int32_t *__restrict__ want,
                                                               uint8_t *__restrict__ granted, int32_t *list) {
-    __shared__ int64_t sums[kPlan / 64];
+    __shared__ PlanSums sums;
     __shared__ int32_t first[kPlan], need_of[kPlan], have_of[kPlan];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int64_t cursor = 0, found = 0, wanted = 0;
+    int turn = 0;
+    int64_t cursor = 0, wanted = 0;
+    int32_t found = 0;
     for (int64_t r0 = 0; r0 < a.rows; r0 += kPlan) {
         const int64_t r = r0 + tid;
         int64_t have = 0, need = 0, to = 0;
@@ -101,11 +116,13 @@ __global__ __launch_bounds__(kPlan) void cache_reserve_kernel(CacheArgs a, const
             have = pages_of(a, len);
             need = grows && fits ? pages_of(a, to) - have : 0;
         }
-        int64_t total;
-        const int64_t at = wanted + plan_scan(need, sums, &total);
+        // (a need of more pages than there are is one of one more than there are: its sums fit)
+        const int32_t asked = (int32_t)min(need, a.num_pages + 1);
+        int32_t total;
+        const int64_t at = wanted + plan_scan(asked, sums, turn, &total);
         wanted += total;
-        find_free(a, min(wanted, a.num_pages), list, &cursor, &found, sums);
-        const bool ok = fits && (need == 0 || at + need <= found);
+        find_free(a, min(wanted, a.num_pages), list, &cursor, &found, sums, turn);
+        const bool ok = fits && (need == 0 || at + asked <= found);
         if (r < a.rows) {
             granted[r] = ok;
             if (ok && grows) a.lengths[r] = (int32_t)to;
@@ -114,53 +131,76 @@ __global__ __launch_bounds__(kPlan) void cache_reserve_kernel(CacheArgs a, const
         need_of[tid] = ok ? (int32_t)need : 0;
         have_of[tid] = (int32_t)have;
         __syncthreads();
-        for (int x = wave; x < kPlan && r0 + x < a.rows; x += kPlan / 64)
-            for (int i = lane; i < need_of[x]; i += 64) {
-                const int32_t page = list[first[x] + i];
-                a.table[(r0 + x) * a.max_pages + have_of[x] + i] = page;
-                a.counts[page] = 1;
+        // a wavefront the pages of 64 rows at a time: those of few by their lanes, long ones together
+        for (int x0 = wave * 64; x0 < kPlan && r0 + x0 < a.rows; x0 += kPlan) {
+            const int x = x0 + lane;
+            const int mine = need_of[x];
+            if (mine <= 8)
+                for (int i = 0; i < mine; i++) {
+                    const int32_t page = list[first[x] + i];
+                    a.table[(r0 + x) * a.max_pages + have_of[x] + i] = page;
+                    a.counts[page] = 1;
+                }
+            for (unsigned long long more = __ballot(mine > 8); more; more &= more - 1) {
+                const int y = x0 + __builtin_ctzll(more), n = need_of[y];
+                for (int i = lane; i < n; i += 64) {
+                    const int32_t page = list[first[y] + i];
+                    a.table[(r0 + y) * a.max_pages + have_of[y] + i] = page;
+                    a.counts[page] = 1;
+                }
             }
+        }
         __syncthreads();
     }
 }
 
 // Which forks are made, and the pages of their own: held [n] is the keys that the child takes over, -1
-// for a fork that is not made. claim [rows]: the first fork that names a child.
+// for a fork that is not made. The first fork that names a child has it: claim [rows], in LDS for tables
+// of up to kClaims rows.
+constexpr int kClaims = 4096;
+template <bool LDS>
 __global__ __launch_bounds__(kPlan) void cache_fork_plan(CacheArgs a, const int32_t *__restrict__ parents,
                                                          const int32_t *__restrict__ children, int64_t n,
                                                          int32_t *__restrict__ fresh, int32_t *__restrict__ held,
-                                                         int32_t *claim, int32_t *list) {
-    __shared__ int64_t sums[kPlan / 64];
+                                                         int32_t *claims, int32_t *list) {
+    __shared__ PlanSums sums;
+    __shared__ int32_t lds[LDS ? kClaims : 1];
     const int tid = threadIdx.x;
-    for (int64_t r = tid; r < a.rows; r += kPlan)
-        __hip_atomic_store(claim + r, INT32_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    int turn = 0;
+    for (int64_t r = tid; r < a.rows; r += kPlan) {
+        if constexpr (LDS)
+            lds[r] = INT32_MAX;
+        else
+            __hip_atomic_store(claims + r, INT32_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
     __syncthreads();
     for (int64_t i = tid; i < n; i += kPlan) {
         const int64_t c = children[i];
-        if (c >= 0 && c < a.rows) atomicMin(claim + c, (int32_t)i);
+        if (c >= 0 && c < a.rows) atomicMin(LDS ? lds + c : claims + c, (int32_t)i);
     }
     __syncthreads();
-    int64_t cursor = 0, found = 0, wanted = 0;
+    int64_t cursor = 0, wanted = 0;
+    int32_t found = 0;
     for (int64_t i0 = 0; i0 < n; i0 += kPlan) {
         const int64_t i = i0 + tid;
         int64_t keys = -1;
         if (i < n) {
             const int64_t p = parents[i], c = children[i];
             if (p >= 0 && p < a.rows && c >= 0 && c < a.rows && a.lengths[c] <= 0 &&
-                __hip_atomic_load(claim + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int32_t)i)
+                (LDS ? lds[c] : __hip_atomic_load(claims + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == (int32_t)i)
                 keys = keys_of(a, a.lengths[p]);
         }
         const bool part = keys > 0 && keys % a.page_size != 0;
-        int64_t total;
-        const int64_t at = wanted + plan_scan(part, sums, &total);
+        int32_t total;
+        const int64_t at = wanted + plan_scan(part, sums, turn, &total);
         wanted += total;
-        find_free(a, min(wanted, a.num_pages), list, &cursor, &found, sums);
+        find_free(a, min(wanted, a.num_pages), list, &cursor, &found, sums, turn);
+        __syncthreads();  // the list is written
         const bool ok = keys >= 0 && (!part || at < found);
         if (i < n) {
             held[i] = ok ? (int32_t)keys : -1;
             fresh[i] = ok ? (part ? list[at] : -1) : -2;
         }
-        __syncthreads();
     }
 }
 
@@ -168,17 +208,18 @@ __global__ __launch_bounds__(kPlan) void cache_fork_plan(CacheArgs a, const int3
 template <int VEC>
 __device__ __forceinline__ void copy_bytes(char *__restrict__ to, const char *__restrict__ from, int64_t bytes) {
     if constexpr (VEC == 16) {
-        const int64_t n = bytes / 16;
-        for (int64_t i = threadIdx.x; i < n; i += 256 * 4) {
-            uint4 x[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++)
-                if (i + 256 * u < n) x[u] = ((const uint4 *)from)[i + 256 * u];
-#pragma unroll
-            for (int u = 0; u < 4; u++)
-                if (i + 256 * u < n) ((uint4 *)to)[i + 256 * u] = x[u];
+        const int n = (int)(bytes / 16);
+        for (int i = threadIdx.x; i < n; i += 256 * 4) {
+            // (four loads without conditions, the last piece again where there are fewer)
+            const uint4 *f = (const uint4 *)from;
+            uint4 *t = (uint4 *)to;
+            const uint4 x0 = f[i], x1 = f[min(i + 256, n - 1)], x2 = f[min(i + 512, n - 1)], x3 = f[min(i + 768, n - 1)];
+            t[i] = x0;
+            if (i + 256 < n) t[i + 256] = x1;
+            if (i + 512 < n) t[i + 512] = x2;
+            if (i + 768 < n) t[i + 768] = x3;
         }
-        for (int64_t i = n * 16 + threadIdx.x; i < bytes; i += 256) to[i] = from[i];
+        for (int i = n * 16 + threadIdx.x; i < bytes; i += 256) to[i] = from[i];
     } else {
         for (int64_t i = threadIdx.x; i < bytes; i += 256) to[i] = from[i];
     }
@@ -251,49 +292,58 @@ struct CompactWork {
     int32_t *holes, *movers;
 };
 
-__device__ __forceinline__ int in_use(const CacheArgs &a, int64_t p) { return p < a.num_pages && a.counts[p] > 0; }
+__device__ __forceinline__ void uses(const CacheArgs &a, int64_t p, int32_t (&is)[4]) {
+    const int4 c = four_counts(a, p);
+    is[0] = p < a.num_pages && c.x > 0, is[1] = p + 1 < a.num_pages && c.y > 0;
+    is[2] = p + 2 < a.num_pages && c.z > 0, is[3] = p + 3 < a.num_pages && c.w > 0;
+}
 
 __global__ __launch_bounds__(kPlan) void cache_compact_count(CacheArgs a, CompactWork w) {
-    __shared__ int64_t sums[kPlan / 64];
-    const int64_t p = (int64_t)blockIdx.x * kChunk + threadIdx.x * 4;
-    int64_t total;
-    plan_scan(in_use(a, p) + in_use(a, p + 1) + in_use(a, p + 2) + in_use(a, p + 3), sums, &total);
-    if (threadIdx.x == 0) w.chunks[blockIdx.x] = (int32_t)total;
+    __shared__ PlanSums sums;
+    int turn = 0;
+    int32_t is[4], total;
+    uses(a, (int64_t)blockIdx.x * kChunk + threadIdx.x * 4, is);
+    plan_scan(is[0] + is[1] + is[2] + is[3], sums, turn, &total);
+    if (threadIdx.x == 0) w.chunks[blockIdx.x] = total;
 }
 
 __global__ __launch_bounds__(kPlan) void cache_compact_plan(CacheArgs a, CompactWork w, int32_t *__restrict__ moved) {
-    __shared__ int64_t sums[kPlan / 64];
+    __shared__ PlanSums sums;
+    int turn = 0;
     const int tid = threadIdx.x;
-    int64_t total, before = 0, all = 0;
+    const int64_t p0 = (int64_t)blockIdx.x * kChunk + tid * 4;
+    int32_t is[4], total;
+    uses(a, p0, is);
+    int32_t before = 0, all = 0;  // the pages in use in front of this chunk, and altogether
     for (int64_t c0 = 0; c0 < w.nchunks; c0 += kPlan) {
-        const int64_t c = c0 + tid, x = c < w.nchunks ? w.chunks[c] : 0;
-        int64_t mine;
-        plan_scan(c < (int64_t)blockIdx.x ? x : 0, sums, &mine);
-        before += mine;
-        plan_scan(x, sums, &total);
+        const int64_t c = c0 + tid;
+        const int32_t x = c < w.nchunks ? w.chunks[c] : 0;
+        // (one scan: what lies in front of this chunk's place in it is the sum in front of it)
+        __shared__ int32_t front;
+        const int32_t sum = plan_scan(x, sums, turn, &total);
+        if (c == (int64_t)blockIdx.x) front = all + sum;
+        __syncthreads();
+        if ((int64_t)blockIdx.x >= c0 && (int64_t)blockIdx.x < c0 + kPlan) before = front;
         all += total;
     }
     // the pages in use below index n = all: those stay
     const int64_t cn = all / kChunk;
-    int64_t stay = 0;
+    int32_t stay = 0;
     for (int64_t c0 = 0; c0 < cn; c0 += kPlan) {
         const int64_t c = c0 + tid;
-        plan_scan(c < cn ? w.chunks[c] : 0, sums, &total);
+        plan_scan(c < cn ? w.chunks[c] : 0, sums, turn, &total);
         stay += total;
     }
-    int64_t mine = 0;
-    for (int u = 0; u < 4; u++) {
-        const int64_t p = cn * kChunk + tid * 4 + u;
-        mine += p < all && in_use(a, p);
-    }
-    plan_scan(mine, sums, &total);
+    int32_t last[4], mine = 0;
+    const int64_t q0 = cn * kChunk + tid * 4;
+    uses(a, q0, last);
+#pragma unroll
+    for (int u = 0; u < 4; u++) mine += q0 + u < all && last[u];
+    plan_scan(mine, sums, turn, &total);
     stay += total;
-    if (blockIdx.x == 0 && tid == 0) *w.movers_n = (int32_t)(all - stay);
-    const int64_t p0 = (int64_t)blockIdx.x * kChunk + tid * 4;
-    int is[4];
-    mine = 0;
-    for (int u = 0; u < 4; u++) mine += is[u] = in_use(a, p0 + u);
-    int64_t live = before + plan_scan(mine, sums, &total);  // pages in use below p
+    if (blockIdx.x == 0 && tid == 0) *w.movers_n = all - stay;
+    int32_t live = before + plan_scan(is[0] + is[1] + is[2] + is[3], sums, turn, &total);  // pages in use below p
+#pragma unroll
     for (int u = 0; u < 4; u++) {
         const int64_t p = p0 + u;
         if (p >= a.num_pages) break;
@@ -302,9 +352,9 @@ __global__ __launch_bounds__(kPlan) void cache_compact_plan(CacheArgs a, Compact
             if (p < all) {
                 to = (int32_t)p;
             } else {
-                const int64_t k = live - stay;
+                const int32_t k = live - stay;
                 w.movers[k] = (int32_t)p;
-                to = (int32_t)(-2 - k);
+                to = -2 - k;
             }
             live++;
         } else if (p < all) {
@@ -359,17 +409,19 @@ __global__ __launch_bounds__(256) void cache_compact_apply(CacheArgs a, PoolArgs
 }
 
 static const int64_t kI31 = (int64_t)1 << 31;
+static const int64_t kMostPages = ((int64_t)1 << 21) - 1;  // a planning workgroup's sums of 1024 needs fit 32 bits
 static const int64_t kMostRows = (int64_t)1 << 22;  // rows of a call: a workgroup each, under 2^32 threads
 
 static bool table_sizes(const dm_cache_table *t) {
     return t && t->rows >= 0 && t->rows < kI31 && t->max_pages >= 0 && t->max_pages < kI31 && t->num_pages >= 0 &&
-           t->num_pages < kI31 - 8192 && t->page_size >= 1 && t->page_size < kI31;
+           t->num_pages < kMostPages && t->page_size >= 1 && t->page_size < kI31;
 }
 
 static int check_table(const std::string &op, const dm_cache_table *t) {
     if (!t) return refuse(op + ": null table");
     if (!table_sizes(t))
-        return refuse(op + ": page_size must be positive, rows, max_pages and num_pages not negative");
+        return refuse(op + ": page_size must be positive, rows, max_pages and num_pages not negative, the pages "
+                           "fewer than 2^21");
     if ((t->rows > 0 && !t->lengths) || (t->rows * t->max_pages > 0 && !t->block_table) ||
         (t->num_pages > 0 && !t->refcounts))
         return refuse(op + ": the block table, the lengths or the page counts are missing");
@@ -455,7 +507,10 @@ int dm_cache_fork(const dm_cache_table *t, const dm_cache_pool *pools, int64_t n
     int32_t *held = (int32_t *)workspace;
     int32_t *claim = (int32_t *)((char *)workspace + align_up((size_t)n * 4));
     int32_t *list = (int32_t *)((char *)claim + align_up((size_t)t->rows * 4));
-    cache_fork_plan<<<1, kPlan, 0, st>>>(a, parents, children, n, fresh, held, claim, list);
+    if (t->rows <= kClaims)
+        cache_fork_plan<true><<<1, kPlan, 0, st>>>(a, parents, children, n, fresh, held, claim, list);
+    else
+        cache_fork_plan<false><<<1, kPlan, 0, st>>>(a, parents, children, n, fresh, held, claim, list);
     for (int64_t at = 0; at == 0 || at < npools; at += kPoolsPerLaunch) {
         bool wide;
         int64_t pieces;

@@ -792,20 +792,27 @@ def _cache_pools(op, pools, num_pages, device):
     each contiguous."""
     if isinstance(pools, torch.Tensor) or len(pools) == 0:
         raise Unsupported(f"{op}: the pools are a list of at least one tensor [P, page_size, ...]")
-    page_size = pools[0].shape[1] if pools[0].dim() >= 2 else 0
-    values = []
+    first = pools[0]
+    shape, page_size = first.shape, first.shape[1] if first.dim() >= 2 else 0
+    values, same = [], None  # (the values of a contiguous pool of the first one's shape and type)
     for t in pools:
+        if same is not None and t.shape == shape and t.dtype == first.dtype and t.is_contiguous() and t.device == device:
+            values += (t.data_ptr(), same, same)
+            continue
         if t.dim() < 2 or t.shape[0] != num_pages or t.shape[1] != page_size or t.device != device:
             raise Unsupported(f"{op}: the pools are [P, page_size, ...] with P = {num_pages} and one page_size, "
                               f"on {device}")
         if page_size < 1:
             raise Unsupported(f"{op}: pages hold at least one key")
-        each = t.numel() // num_pages if num_pages else 0
-        if not t.is_contiguous():  # (a slice of a wider pool, say: whole pages, apart)
-            if num_pages and t.numel() and not (t[0].is_contiguous() and
-                                                (num_pages == 1 or t.stride(0) >= each)):
-                raise Unsupported(f"{op}: the pools' pages must each be contiguous and apart")
-        size = t.element_size()
+        each, size = t.numel() // num_pages if num_pages else 0, t.element_size()
+        if t.is_contiguous():
+            if t is first:
+                same = each * size
+            values += (t.data_ptr(), each * size, each * size)
+            continue
+        # (a slice of a wider pool, say: whole pages, apart)
+        if num_pages and t.numel() and not (t[0].is_contiguous() and (num_pages == 1 or t.stride(0) >= each)):
+            raise Unsupported(f"{op}: the pools' pages must each be contiguous and apart")
         values += (t.data_ptr(), each * size, (t.stride(0) if num_pages > 1 else each) * size)
     arr = (_lib.CachePool * len(pools))()
     struct.pack_into(f"{len(values)}q", arr, 0, *values)
