@@ -446,7 +446,7 @@ def attention_decode_paged(query, key_pages, value_pages, block_table, lengths=N
 # (The calls of these operators take a few microseconds on the GPU, as long as the host takes for a dozen
 # attribute look-ups: pointers go to the library as numbers, strides into a descriptor by one
 # ``pack_into``, and the device is switched only where it is another.)
-_STRIDES = {n: struct.Struct(f"{n}q") for n in (3, 6, 9, 12, 15)}
+_STRIDES = {n: struct.Struct(f"{n}q") for n in (6, 9)}
 
 
 def _run(op, device, fn, *args):
@@ -484,9 +484,17 @@ def _whole(t):
     return t if t.is_contiguous() and not t.data_ptr() % 16 else _readable(t)
 
 
-def _put_strides(desc, first, *values):
-    """The ``dm_strides`` of ``desc`` from the field ``first`` on."""
-    _STRIDES[len(values)].pack_into(desc, getattr(type(desc), first).offset, *values)
+def _put_strides(desc, offset, *values):
+    """The ``dm_strides`` of ``desc`` from the byte ``offset`` on."""
+    _STRIDES[len(values)].pack_into(desc, offset, *values)
+
+
+_ROPE_SQ, _ROPE_SGQ = _lib.QkNormRopeDesc.sq.offset, _lib.QkNormRopeDesc.sgq.offset
+_PAGES_SK, _ATTENTION_SQ = _lib.KvPages.sk.offset, _lib.AttentionDesc.sq.offset
+
+
+def _contiguous_like(t):
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 _INTS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
@@ -574,8 +582,8 @@ def qk_norm_rope(query, key, q_weight, k_weight, inv_freq, positions=None,
     dev = query.device
     at = _positions(op, desc, positions, dev)
     q, k, wq, wk, freq = _whole(query), _whole(key), _flat(q_weight), _flat(k_weight), _flat(inv_freq)
-    _put_strides(desc, "sq", *q.stride()[:3], *k.stride()[:3])
-    qo, ko = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k))
+    _put_strides(desc, _ROPE_SQ, *q.stride()[:3], *k.stride()[:3])
+    qo, ko = _contiguous_like(q), _contiguous_like(k)
     _run(op, dev, _lib.lib().dm_qk_norm_rope, ctypes.byref(desc), q.data_ptr(), k.data_ptr(), _at(wq), _at(wk),
          freq.data_ptr(), qo.data_ptr(), ko.data_ptr())
     return qo, ko
@@ -596,10 +604,10 @@ def qk_norm_rope_backward(query, key, q_weight, k_weight, inv_freq, grad_query, 
     at = _positions(op, desc, positions, dev)
     q, k, wq, wk, freq = _whole(query), _whole(key), _flat(q_weight), _flat(k_weight), _flat(inv_freq)
     gq, gk = _whole(grad_query.to(q.dtype)), _whole(grad_key.to(q.dtype))
-    _put_strides(desc, "sq", *q.stride()[:3], *k.stride()[:3])
-    _put_strides(desc, "sgq", *gq.stride()[:3], *gk.stride()[:3])
-    dq, dk = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k))
-    dwq, dwk = (None if w is None else torch.empty(w.shape, dtype=w.dtype, device=dev) for w in (wq, wk))
+    _put_strides(desc, _ROPE_SQ, *q.stride()[:3], *k.stride()[:3])
+    _put_strides(desc, _ROPE_SGQ, *gq.stride()[:3], *gk.stride()[:3])
+    dq, dk = _contiguous_like(q), _contiguous_like(k)
+    dwq, dwk = (None if w is None else torch.empty_like(w) for w in (wq, wk))
     nbytes = _lib.lib().dm_qk_norm_rope_bwd_workspace(ctypes.byref(desc))
     ws = _workspace(nbytes, dev)
     _run(op, dev, _lib.lib().dm_qk_norm_rope_bwd, ctypes.byref(desc), q.data_ptr(), k.data_ptr(), _at(wq), _at(wk),
@@ -673,10 +681,11 @@ def qk_norm_rope_paged(query, key, value, q_weight, k_weight, inv_freq, key_page
                           f"{nseq} sequences")
     q, k, v = _whole(query), _whole(key), _whole(value)
     wq, wk, freq = _flat(q_weight), _flat(k_weight), _flat(inv_freq)
-    _put_strides(desc, "sq", 0, *q.stride()[:2], 0, *k.stride()[:2], 0, *v.stride()[:2])
+    (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.stride(), k.stride(), v.stride()
+    _put_strides(desc, _ROPE_SQ, 0, qt, qh, 0, kt, kh, 0, vt, vh)
     pages = _lib.KvPages(ps[0], ps[1], bt.shape[1], nseq, bt.data_ptr(), ln.data_ptr(), _at(cu))
-    _put_strides(pages, "sk", *key_pages.stride()[:3], *value_pages.stride()[:3])
-    qo = torch.empty(q.shape, dtype=dtype, device=dev)
+    _put_strides(pages, _PAGES_SK, *key_pages.stride()[:3], *value_pages.stride()[:3])
+    qo = _contiguous_like(q)
     _run(op, dev, _lib.lib().dm_qk_norm_rope_paged, ctypes.byref(desc), ctypes.byref(pages), q.data_ptr(),
          k.data_ptr(), v.data_ptr(), _at(wq), _at(wk), freq.data_ptr(), qo.data_ptr(), key_pages.data_ptr(),
          value_pages.data_ptr())
@@ -722,8 +731,8 @@ def attention_decode_shared(query, key_pages, value_pages, block_table, lengths,
         _decode_options(desc.options, options)
     desc.strided = 1
     sq = q.stride()
-    _put_strides(desc, "sq", sq[0], 0, sq[1], *k.stride()[:3], *v.stride()[:3])
-    out = torch.empty(qs, dtype=dtype, device=dev)
+    _put_strides(desc, _ATTENTION_SQ, sq[0], 0, sq[1], *k.stride()[:3], *v.stride()[:3])
+    out = _contiguous_like(q)
     ng = cu.shape[0] - 1
     nbytes = _lib.lib().dm_attention_decode_shared_workspace(ctypes.byref(desc), page_size, ng)
     ws = _workspace(nbytes, dev)
@@ -839,7 +848,7 @@ def cache_reserve(block_table, lengths, refcounts, new_lengths, page_size):
     new = _rows_i32(op, new_lengths, dev, "the new lengths")
     if new.shape[0] != desc.rows:
         raise Unsupported(f"{op}: the new lengths are [R] = [{desc.rows}]")
-    granted = torch.empty(desc.rows, dtype=torch.bool, device=dev)
+    granted = torch.empty_like(new, dtype=torch.bool)
     nbytes = _lib.lib().dm_cache_reserve_workspace(ctypes.byref(desc))
     ws = _workspace(nbytes, dev)
     _run(op, dev, _lib.lib().dm_cache_reserve, ctypes.byref(desc), new.data_ptr(), granted.data_ptr(), ws.data_ptr(), nbytes)
@@ -863,7 +872,7 @@ def cache_fork(pools, block_table, lengths, refcounts, parents, children):
     n = pa.shape[0]
     if ch.shape[0] != n:
         raise Unsupported(f"{op}: the parents and children are [N], one N")
-    fresh = torch.empty(n, dtype=torch.int32, device=dev)
+    fresh = torch.empty_like(pa)
     nbytes = _lib.lib().dm_cache_fork_workspace(ctypes.byref(desc), n)
     ws = _workspace(nbytes, dev)
     _run(op, dev, _lib.lib().dm_cache_fork, ctypes.byref(desc), arr, len(arr), pa.data_ptr(), ch.data_ptr(), n,
@@ -891,7 +900,7 @@ def cache_compact(pools, block_table, lengths, refcounts):
     dev = block_table.device
     arr, page_size = _cache_pools(op, pools, refcounts.shape[0], dev)
     desc = _cache_table(op, block_table, lengths, refcounts, page_size)
-    moved = torch.empty(desc.num_pages, dtype=torch.int32, device=dev)
+    moved = torch.empty_like(refcounts)
     nbytes = _lib.lib().dm_cache_compact_workspace(ctypes.byref(desc))
     ws = _workspace(nbytes, dev)
     _run(op, dev, _lib.lib().dm_cache_compact, ctypes.byref(desc), arr, len(arr), moved.data_ptr(), ws.data_ptr(), nbytes)
