@@ -30,12 +30,15 @@ FLAGS = [
 # wavefront per SIMD: with the products' accumulators in ordinary vector registers, the state's
 # decay and conversions work on them in place instead of moving every value out of and back into
 # the accumulator registers at each step.
+# The shared decode at head width 256 the same (8 answers to a prompt of 6144 tokens 35 -> 28 us; widths 64 and
+# 128 keep their times).
 # The attention kernels are scheduled with the strategy that keeps memory instructions together
 # (measured at head width 256, one wavefront per SIMD: forward 288 -> 262 us, dK/dV 759 -> 723 us,
 # dQ 359 -> 346 us on the reference's T = 6144 shape; the same at widths 64 and 128 within noise),
 # but for the head width 256 dK/dV kernel, whose occupancy-driven iterative scheduling took it to
 # 690 us.
 EXTRA = {"gdr_chunk_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+         "decode_shared.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "attention_fwd.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
          "attention_mfma_bwd.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
          "attention_bwd_w4.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-maxocc"]}

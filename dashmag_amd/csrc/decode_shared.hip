@@ -50,11 +50,11 @@ __device__ __forceinline__ int64_t shared_page(const SharedArgs &a, int64_t m, i
     return pg >= 0 && pg < a.num_pages ? pg : -1;
 }
 
-// What a team of wavefronts does: range `slot` of the rows r0 .. r0 + nrow - 1 (row r: member
+// What a workgroup or a wavefront does: range `slot` of the rows r0 .. r0 + nrow - 1 (row r: member
 // m0 + r / rep, query head kh rep + r % rep) over the keys [s0, s1), which lie on `table`'s pages; a
 // member sees those of its own range that lie in front of `cap`. Every field is the wavefront's.
 struct SharedItem {
-    int32_t m0, table, s0, s1, cap, r0, nrow, kh, slot;
+    int32_t m0, m1, table, s0, s1, base, cap, len, r0, nrow, kh, slot;
     bool prefix;
 };
 
@@ -67,31 +67,41 @@ __device__ __forceinline__ int32_t first_tile(int32_t s, int32_t g) {
     return ((s - g) >> shift) + g;
 }
 
-// The item of `index`; false: it has no keys (where it is a row's to say so, that is written down). A
-// whole wavefront; with several in a team each does the same, and the first (`writes`) writes.
-// unit: ranges are multiples of this many keys (a multiple of 16). RT: rows of a prefix tile.
+// Row r of an item: its member, its query head and its place among the partial results.
+__device__ __forceinline__ void head_of(const SharedArgs &a, const SharedItem &it, int r, int32_t *member, int32_t *head) {
+    const uint32_t rr = it.r0 + r;
+    *member = it.m0 + (it.prefix ? (int32_t)(rr / (uint32_t)a.rep) : 0);
+    *head = it.kh * a.rep + (int32_t)(it.prefix ? rr % (uint32_t)a.rep : rr);
+}
+__device__ __forceinline__ int64_t part_of(const SharedArgs &a, const SharedItem &it, int r) {
+    int32_t member, head;
+    head_of(a, it, r, &member, &head);
+    return ((int64_t)member * a.hq + head) * (a.nsp + a.nso) + it.slot;
+}
+
+// Which rows the item of `index` has (false: none, or there is no such item), and for a prefix its group's
+// last row; its keys come with range_of. A whole wavefront; with several for an item each does the same, and the
+// first (`writes`) writes. RT: rows of a prefix tile.
 template <int RT>
-__device__ __forceinline__ bool item_of(const SharedArgs &a, int32_t index, int unit, bool writes, SharedItem &it) {
+__device__ __forceinline__ bool rows_of(const SharedArgs &a, int32_t index, bool writes, SharedItem &it) {
     const int lane = threadIdx.x & 63;
     const int32_t np = a.ptiles * a.nsp;
     uint32_t x = (uint32_t)index;
     it.kh = (int32_t)(x % (uint32_t)a.hkv);
     x /= (uint32_t)a.hkv;
     it.prefix = x < (uint32_t)np;
-    int32_t b = 0, tile = 0, split, ot = 0, len = 0;
+    int32_t b = 0, tile = 0, ot = 0;
     if (it.prefix) {
-        tile = (int32_t)(x % (uint32_t)a.ptiles), split = (int32_t)(x / (uint32_t)a.ptiles);
-        it.slot = split;
+        tile = (int32_t)(x % (uint32_t)a.ptiles), it.slot = (int32_t)(x / (uint32_t)a.ptiles);
     } else {
         x -= np;
         b = (int32_t)(x % (uint32_t)a.B);
         x /= (uint32_t)a.B;
-        ot = (int32_t)(x % (uint32_t)a.otiles), split = (int32_t)(x / (uint32_t)a.otiles);
-        it.slot = a.nsp + split;
-        len = len_of(a, b);
+        ot = (int32_t)(x % (uint32_t)a.otiles), it.slot = a.nsp + (int32_t)(x / (uint32_t)a.otiles);
+        it.len = len_of(a, b);
     }
-    // the group (the first of those that hold the tile or the row), if the groups go up from 0 at least
-    // to B at most: 64 of them at a time, a lane each
+    // the group (the last that starts at the tile or in front of it, the first that holds the row), if the
+    // groups go up from 0 at least to B at most: 64 of them at a time, a lane each
     bool ok = true;
     int32_t g = -1, m0 = 0, m1 = 0, plen = 0;
     for (int32_t g0 = 0; g0 < a.ngroups; g0 += 64) {
@@ -109,15 +119,32 @@ __device__ __forceinline__ bool item_of(const SharedArgs &a, int32_t index, int 
         }
     }
     ok = __all(ok);
-    int32_t lo, hi;
     if (it.prefix) {
         if (!ok || g < 0) return false;
         const int32_t first = (tile - first_tile<RT>(m0 * a.rep, g)) * RT, rows = (m1 - m0) * a.rep;
         if (first >= rows) return false;
-        it.m0 = m0, it.r0 = first, it.nrow = min(RT, rows - first), it.cap = plen;
+        it.m0 = m0, it.m1 = m1, it.r0 = first, it.nrow = min(RT, rows - first), it.cap = plen;
+        return true;
+    }
+    const bool grouped = ok && g >= 0;
+    it.m0 = it.table = b;
+    it.r0 = ot * kOwnRows, it.nrow = min(kOwnRows, a.rep - it.r0);
+    it.base = grouped ? plen : 0, it.cap = a.S;
+    if (!grouped && it.slot == a.nsp && writes)  // the prefix's ranges, which nobody else writes
+        for (int i = lane; i < it.nrow * a.nsp; i += 64)
+            a.part_lse[((int64_t)b * a.hq + it.kh * a.rep + it.r0 + i / a.nsp) * (a.nsp + a.nso) + i % a.nsp] = -INFINITY;
+    return true;
+}
+
+// The item's keys: false where there are none, which is then written down. unit: ranges are multiples of
+// this many keys (a multiple of 16).
+__device__ __forceinline__ bool range_of(const SharedArgs &a, int unit, bool writes, SharedItem &it) {
+    const int lane = threadIdx.x & 63;
+    int32_t lo, hi;
+    if (it.prefix) {
         // the longest member, and the shortest that sees any key
         int32_t most = -1, least = INT32_MAX, at = 0;
-        for (int32_t m = m0 + lane; m < m1; m += 64) {
+        for (int32_t m = it.m0 + lane; m < it.m1; m += 64) {
             const int32_t l = len_of(a, m);
             if (l > most) most = l, at = m;
             if (l > 0) least = min(least, l);
@@ -127,7 +154,7 @@ __device__ __forceinline__ bool item_of(const SharedArgs &a, int32_t index, int 
         for (int o = 32; o >= 1; o >>= 1) longest = max(longest, __shfl_xor(longest, o, 64));
         longest = uniform(longest);
         it.table = __builtin_amdgcn_readlane(at, __builtin_ctzll(__ballot(most == longest)));
-        hi = min(plen, longest);
+        hi = min(it.cap, longest);
         lo = 0;
         if (a.left >= 0 && longest > 0) {
 #pragma unroll
@@ -135,53 +162,18 @@ __device__ __forceinline__ bool item_of(const SharedArgs &a, int32_t index, int 
             lo = low_of(a, uniform(least));
         }
     } else {
-        const bool grouped = ok && g >= 0;
-        it.m0 = it.table = b;
-        it.r0 = ot * kOwnRows, it.nrow = min(kOwnRows, a.rep - it.r0);
-        it.cap = a.S;
-        if (!grouped && split == 0 && writes)  // the prefix's ranges, which no other team writes
-            for (int i = lane; i < it.nrow * a.nsp; i += 64)
-                a.part_lse[((int64_t)b * a.hq + it.kh * a.rep + it.r0 + i / a.nsp) * (a.nsp + a.nso) + i % a.nsp] =
-                    -INFINITY;
-        hi = uniform(len);
-        lo = max(grouped ? plen : 0, low_of(a, hi));
+        hi = uniform(it.len);
+        lo = max(it.base, low_of(a, hi));
     }
-    const int32_t from = lo & ~15, n = it.prefix ? a.nsp : a.nso;
+    const int32_t from = lo & ~15, n = it.prefix ? a.nsp : a.nso, split = it.prefix ? it.slot : it.slot - a.nsp;
     const int32_t each = hi > from ? (int32_t)(((uint32_t)(hi - from) + n - 1) / (uint32_t)n + unit - 1) / unit * unit : 0;
     const int64_t start = from + (int64_t)split * each;
     it.s0 = (int32_t)max((int64_t)lo, min(start, (int64_t)hi));
     it.s1 = (int32_t)min((int64_t)hi, start + each);
     if (it.s0 < it.s1) return true;
     if (writes)
-        for (int r = lane; r < it.nrow; r += 64) {
-            const int rr = it.r0 + r;
-            const int64_t row = (int64_t)(it.m0 + rr / a.rep) * a.hq + it.kh * a.rep + rr % a.rep;
-            a.part_lse[row * (a.nsp + a.nso) + it.slot] = -INFINITY;
-        }
+        for (int r = lane; r < it.nrow; r += 64) a.part_lse[part_of(a, it, r)] = -INFINITY;
     return false;
-}
-
-// Row r of an item (it may be past its rows): its place among the partial results, and the keys of
-// the item that it sees.
-struct SharedRow {
-    int32_t member, head, lo, hi;
-    int64_t part;
-};
-__device__ __forceinline__ SharedRow row_of(const SharedArgs &a, const SharedItem &it, int r) {
-    SharedRow w;
-    const bool on = r < it.nrow;
-    const uint32_t rr = it.r0 + (on ? r : 0);
-    w.member = it.m0 + (it.prefix ? (int32_t)(rr / (uint32_t)a.rep) : 0);
-    w.head = it.kh * a.rep + (int32_t)(it.prefix ? rr % (uint32_t)a.rep : rr);
-    w.part = ((int64_t)w.member * a.hq + w.head) * (a.nsp + a.nso) + it.slot;
-    w.lo = it.s0, w.hi = it.s1;
-    if (it.prefix) {
-        const int32_t len = len_of(a, w.member);
-        w.lo = max(low_of(a, len), it.s0);
-        w.hi = min(min(len, it.cap), it.s1);
-    }
-    if (!on) w.hi = 0;
-    return w;
 }
 
 // The simple form, for every type, head width, page size and stride: 32 rows and 16 keys at a time in
@@ -193,9 +185,15 @@ __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const
                                                              const void *__restrict__ v) {
     __shared__ float qs[32][257], kv[kGenKeys][257], ps[32][kGenKeys + 1];
     SharedItem it;
-    if (!item_of<32>(a, blockIdx.x, kGenKeys, threadIdx.x < 64, it)) return;
+    if (!rows_of<32>(a, blockIdx.x, threadIdx.x < 64, it) || !range_of(a, kGenKeys, threadIdx.x < 64, it)) return;
     const int tid = threadIdx.x, r = tid >> 3, c = tid & 7;
-    const SharedRow row = row_of(a, it, r);
+    int32_t member, head, low = it.s0, high = r < it.nrow ? it.s1 : 0;
+    head_of(a, it, r < it.nrow ? r : 0, &member, &head);
+    const int64_t part = part_of(a, it, r < it.nrow ? r : 0);
+    if (it.prefix) {
+        const int32_t len = len_of(a, member);
+        low = max(low_of(a, len), it.s0), high = min(min(len, it.cap), high);
+    }
     for (int i = tid; i < 32 * a.d; i += 256) {
         const int x = i / a.d, e = i - x * a.d;
         const int rr = it.r0 + (x < it.nrow ? x : 0);
@@ -219,7 +217,7 @@ __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const
             const int x = c + 8 * u;
             const int64_t j = j0 + x;
             s[u] = -INFINITY;
-            if (j >= row.lo && j < row.hi) {
+            if (j >= low && j < high) {
                 float t = 0.f;
                 for (int e = 0; e < a.d; e++) t += qs[r][e] * kv[x][e];
                 s[u] = t;
@@ -236,7 +234,7 @@ __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const
         for (int u = 0; u < 2; u++) {
             // (a masked key's weight is a marker below zero: what its value holds stays out)
             const int64_t j = j0 + c + 8 * u;
-            const bool seen = j >= row.lo && j < row.hi;
+            const bool seen = j >= low && j < high;
             const float p = seen ? expf(s[u] - mn) : 0.f;
             ps[r][c + 8 * u] = seen ? p : -1.f;
             l += p;
@@ -265,8 +263,8 @@ __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const
     const bool none = l == 0.f;
 #pragma unroll
     for (int i = 0; i < 32; i++)
-        if (!none && c + 8 * i < a.d) a.part_o[row.part * a.d + c + 8 * i] = acc[i] / l;
-    if (c == 0) a.part_lse[row.part] = none ? -INFINITY : m + logf(l);
+        if (!none && c + 8 * i < a.d) a.part_o[part * a.d + c + 8 * i] = acc[i] / l;
+    if (c == 0) a.part_lse[part] = none ? -INFINITY : m + logf(l);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -291,7 +289,6 @@ __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const
 
 template <int D, bool WIDE>
 constexpr int shared_waves() { return D == 256 || !WIDE ? 4 : 8; }
-constexpr int kTeam = 4;  // wavefronts that take a narrow item
 
 // Where the keys of an item lie: byte strides of a page and of a row (keys' and values' alike).
 struct PageMap {
@@ -343,7 +340,7 @@ struct SharedSmem {
     union {
         Narrow narrow[NW];
         Wide wide[WIDE];
-        alignas(16) float join[NW / kTeam][kTeam * 32 * (D + 2)];
+        alignas(16) float join[WIDE ? 1 : NW * 32 * (D + 2)];
     };
     int32_t lo[NW], hi[NW], bad;
     uint64_t blocks[WIDE ? 512 : 1];  // wide: the offsets of 128 tiles' blocks, see fill
@@ -353,41 +350,56 @@ struct SharedSmem {
 template <int D>
 struct RowState {
     Frag8 qf[D / 16];
+    int32_t len;       // prefix: the member's
     int32_t lo, hi;    // this lane's row
     int32_t flo, fhi;  // the keys that all of the wavefront's rows see
     bool on;
 };
 
+// The loads of row r's query (and length), which need no key; nothing here waits for them.
 template <int DT, int D>
 __device__ __forceinline__ void load_rows(const SharedArgs &a, const SharedItem &it, const void *q, int r,
                                           bool slots, RowState<D> &w) {
     const int half = (threadIdx.x >> 5) & 1;
-    const SharedRow row = row_of(a, it, r);
     w.on = r < it.nrow;
-    w.lo = row.lo, w.hi = row.hi;
-    const uint16_t *qp = (const uint16_t *)q + row.member * a.qb + row.head * a.qh;
-    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // (the softmax below takes a scale above 0)
+    int32_t member, head;
+    head_of(a, it, w.on ? r : 0, &member, &head);
+    w.len = it.prefix ? len_of(a, member) : 0;
+    const uint16_t *qp = (const uint16_t *)q + member * a.qb + head * a.qh;
 #pragma unroll
     for (int s = 0; s < D / 16; s++) {
-        uint4 x = zero4();
-        if (w.on) {
-            if (slots) {  // narrow: the slots 4 h + e and 8 + 4 h + e of row_frag
-                const uint2 l = *(const uint2 *)(qp + s * 16 + half * 4), u = *(const uint2 *)(qp + s * 16 + 8 + half * 4);
-                x = make_uint4(l.x, l.y, u.x, u.y);
-            } else {
-                x = *(const uint4 *)(qp + s * 16 + half * 8);
-            }
+        // (a lane without a row takes the first row's query; nobody reads what becomes of it)
+        if (slots) {  // narrow: the slots 4 h + e and 8 + 4 h + e of row_frag
+            const uint2 l = *(const uint2 *)(qp + s * 16 + half * 4), u = *(const uint2 *)(qp + s * 16 + 8 + half * 4);
+            w.qf[s].u = make_uint4(l.x, l.y, u.x, u.y);
+        } else {
+            w.qf[s].u = *(const uint4 *)(qp + s * 16 + half * 8);
         }
-        w.qf[s].u = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
     }
+}
+
+// The keys that the rows see, once the item's are known.
+template <int D>
+__device__ __forceinline__ void bound_rows(const SharedArgs &a, const SharedItem &it, RowState<D> &w) {
+    w.lo = it.s0, w.hi = it.s1;
+    if (it.prefix) w.lo = max(low_of(a, w.len), it.s0), w.hi = min(min(w.len, it.cap), it.s1);
+    if (!w.on) w.hi = 0;
     int32_t flo = w.on ? w.lo : INT32_MIN, fhi = w.on ? w.hi : INT32_MAX;
+    if (it.prefix) {
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-        flo = max(flo, __shfl_xor(flo, o, 64));
-        fhi = min(fhi, __shfl_xor(fhi, o, 64));
+        for (int o = 16; o >= 1; o >>= 1) {
+            flo = max(flo, __shfl_xor(flo, o, 64));
+            fhi = min(fhi, __shfl_xor(fhi, o, 64));
+        }
     }
-    w.flo = __builtin_amdgcn_readfirstlane(flo);
-    w.fhi = __builtin_amdgcn_readfirstlane(fhi);
+    w.flo = uniform(flo), w.fhi = uniform(fhi);
+    if (a.scale < 0.f) {  // (the softmax takes a scale above 0: the queries' signs instead)
+#pragma unroll
+        for (int s = 0; s < D / 16; s++) {
+            uint4 &x = w.qf[s].u;
+            x = make_uint4(x.x ^ 0x80008000u, x.y ^ 0x80008000u, x.z ^ 0x80008000u, x.w ^ 0x80008000u);
+        }
+    }
 }
 
 // The values that were taken out, added for the rows that see them: every key of [j0, j1) again, one
@@ -422,16 +434,35 @@ struct Partial {
     float m, l;
 };
 
-// (`has`: the team has an item. Teams of a workgroup meet at its barriers, so one without passes them too.)
-template <int DT, int D, bool WIDE>
-__device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedItem &it, bool has, const PageMap &map,
-                                              const void *q, SharedSmem<D, WIDE> &sm) {
-    constexpr int NW = kTeam, KS = SharedSmem<D, WIDE>::KS, VS = SharedSmem<D, WIDE>::VS;
+// A wavefront's rows (this lane's: r) with the sums l over both halves: normalised partial results.
+template <int D>
+__device__ __forceinline__ void put_rows(const SharedArgs &a, const SharedItem &it, const RowState<D> &rs, int r,
+                                         const Partial<D> &p, float l) {
+    const int half = (threadIdx.x >> 5) & 1;
+    if (!rs.on) return;
+    const int64_t part = part_of(a, it, r);
+    if (l != 0.f) {  // (NaN is not 0)
+        const float inv = 1.f / l;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+            for (int g4 = 0; g4 < 4; g4++)
+                *(float4 *)(a.part_o + part * D + dt * 32 + g4 * 8 + half * 4) =
+                    make_float4(p.acc[dt][g4 * 4] * inv, p.acc[dt][g4 * 4 + 1] * inv, p.acc[dt][g4 * 4 + 2] * inv,
+                                p.acc[dt][g4 * 4 + 3] * inv);
+    }
+    if (half == 0) a.part_lse[part] = l == 0.f ? -INFINITY : (p.m + log2f(l)) * 0.6931471805599453f;
+}
+
+// TEAM: the wavefronts that share the item's keys, the whole workgroup or one.
+template <int DT, int D, bool WIDE, int TEAM>
+__device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedItem &it, const PageMap &map,
+                                              RowState<D> &rs, SharedSmem<D, WIDE> &sm) {
+    constexpr int NW = TEAM, KS = SharedSmem<D, WIDE>::KS, VS = SharedSmem<D, WIDE>::VS;
     constexpr int LPR = D / 8, RPL = 64 / LPR, NLD = 32 / RPL;  // lanes a row, rows a load, loads
     constexpr int KST = D / 16, DTN = D / 32;
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    const int wave = uniform(threadIdx.x >> 6) % kTeam, team = uniform(threadIdx.x >> 6) / kTeam;
-    RowState<D> rs;
+    const int slot = uniform(threadIdx.x >> 6), wave = TEAM == 1 ? 0 : slot;
     const float qscale = fabsf(a.scale) * 1.4426950408889634f;
     Partial<D> p;
     p.m = -INFINITY, p.l = 0.f;
@@ -439,8 +470,8 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
     for (int dt = 0; dt < DTN; dt++) p.acc[dt] = zero16();
     const int32_t s0 = it.s0, s1 = it.s1, a0 = s0 & ~15;
     const int32_t per = ((s1 - a0 + NW - 1) / NW + 31) & ~31;
-    const int32_t w0 = max(s0, a0 + wave * per), w1 = has ? min(s1, a0 + (wave + 1) * per) : 0, b0 = w0 & ~15;
-    typename SharedSmem<D, WIDE>::Narrow &t = sm.narrow[team * kTeam + wave];
+    const int32_t w0 = max(s0, a0 + wave * per), w1 = min(s1, a0 + (wave + 1) * per), b0 = w0 & ~15;
+    typename SharedSmem<D, WIDE>::Narrow &t = sm.narrow[slot];
     uint4 sk[NLD], sv[NLD];
     // the offsets of 64 blocks of 16 keys from block `from` on, a lane each
     uint64_t at;
@@ -469,19 +500,24 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
         const int nblk = (w1 - b0 + 31) / 32;
         look_up(0);
         load(0);
-        load_rows<DT, D>(a, it, q, col, true, rs);
+        bound_rows<D>(a, it, rs);
         for (int n = 0; n < nblk; n++) {
             const int32_t j0 = b0 + n * 32;
             const bool cut = j0 < rs.flo || j0 + 32 > rs.fhi;
-            if (cut) {
-#pragma unroll
-                for (int u = 0; u < NLD; u++) bad |= take_out<DT>(sv[u]);
-            }
 #pragma unroll
             for (int u = 0; u < NLD; u++) {
                 const int r = RPL * u + lane / LPR, c = (lane % LPR) * 8;
                 *(uint4 *)(t.k + r * KS + c) = sk[u];
                 *(uint4 *)(t.v + r * VS + c) = sv[u];
+            }
+            if (cut) {  // (in LDS: the loads' registers are full)
+#pragma unroll 1
+                for (int u = 0; u < NLD; u++) {
+                    uint4 *x = (uint4 *)(t.v + (RPL * u + lane / LPR) * VS + (lane % LPR) * 8), y = *x;
+                    const uint32_t m = take_out<DT>(y);
+                    if (m) *x = y;
+                    bad |= m;
+                }
             }
             if ((n & 31) == 31) look_up(2 * n + 2);
             load(n + 1);
@@ -529,10 +565,14 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
                 add_back<DT, D>(a, map, max(j0, w0), min(j0 + 32, w1), rs.lo, rs.hi, p.acc);
     }
     const float l = p.l + __shfl_xor(p.l, 32, 64);
+    if constexpr (TEAM == 1) {
+        put_rows<D>(a, it, rs, col, p, l);
+        return;
+    }
     // the wavefronts' results joined through LDS: [wave][row][D], their references and sums behind
     __syncthreads();
-    float *sa = sm.join[team], *sm_m = sa + NW * 32 * D, *sm_l = sm_m + NW * 32;
-    if (has && col < it.nrow) {
+    float *sa = sm.join, *sm_m = sa + NW * 32 * D, *sm_l = sm_m + NW * 32;
+    if (col < it.nrow) {
 #pragma unroll
         for (int dt = 0; dt < DTN; dt++)
 #pragma unroll
@@ -542,8 +582,7 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
         if (half == 0) sm_m[wave * 32 + col] = p.m, sm_l[wave * 32 + col] = l;
     }
     __syncthreads();
-    if (!has) return;
-    for (int x = wave * 64 + lane; x < it.nrow * (D / 4); x += NW * 64) {
+    for (int x = threadIdx.x; x < it.nrow * (D / 4); x += NW * 64) {
         const int r = x / (D / 4), d = x % (D / 4) * 4;
         float M = -INFINITY;
         for (int w = 0; w < NW; w++) M = fmaxf(M, sm_m[w * 32 + r]);
@@ -557,18 +596,18 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
                 L += sm_l[w * 32 + r] * f;
                 o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
             }
-        const SharedRow row = row_of(a, it, r);
+        const int64_t part = part_of(a, it, r);
         if (L != 0.f) {  // (NaN is not 0)
             const float inv = 1.f / L;
-            *(float4 *)(a.part_o + row.part * D + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            *(float4 *)(a.part_o + part * D + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
         }
-        if (d == 0) a.part_lse[row.part] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+        if (d == 0) a.part_lse[part] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
     }
 }
 
 template <int DT, int D>
 __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedItem &it, const PageMap &map,
-                                            const void *q, SharedSmem<D, true> &sm) {
+                                            RowState<D> &rs, SharedSmem<D, true> &sm) {
     constexpr int NW = shared_waves<D, true>(), NT = NW * 64, KS = SharedSmem<D, true>::KS, VS = SharedSmem<D, true>::VS;
     constexpr int CPR = D / 8, RSTEP = NT / CPR, NCH = 64 / RSTEP;  // pieces a row, rows at a time, pieces a thread
     constexpr int KST = D / 16, DTN = D / 32;
@@ -579,16 +618,15 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
     auto fill = [&](int32_t block) __attribute__((always_inline)) {
         sm.blocks[block & 511] = block_at(a, map, k0 + 16 * block, s1);
     };
-    RowState<D> rs;
-    load_rows<DT, D>(a, it, q, wave * 32 + col, false, rs);
+    fill(threadIdx.x);
+    if (NT < 512) fill(threadIdx.x + 256);
+    bound_rows<D>(a, it, rs);
     // (the queries are waited for here: behind the tiles' loads they would leave a wait for all of
     // those in the loop)
     __builtin_amdgcn_s_waitcnt(0x0F70);
     const bool rows = wave * 32 < it.nrow;  // this wavefront has rows
     if (lane == 0) sm.lo[wave] = rs.flo, sm.hi[wave] = rs.fhi;
     if (threadIdx.x == 0) sm.bad = 0;
-    fill(threadIdx.x);
-    if (NT < 512) fill(threadIdx.x + 256);
     __syncthreads();
     int32_t tlo = INT32_MIN, thi = INT32_MAX;  // the keys that every row of the tile sees
 #pragma unroll
@@ -619,9 +657,6 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
             x[u] = *(const uint4 *)(base + (ok[u] ? at[u] : 0) + ((uint32_t)(r & 15) * map.row + lc * 16));
         }
     };
-    auto zeroed = [](const uint4 &x, bool ok) {
-        return make_uint4(ok ? x.x : 0u, ok ? x.y : 0u, ok ? x.z : 0u, ok ? x.w : 0u);
-    };
     auto load_v = [&](int32_t j) __attribute__((always_inline)) { load(j, map.v, av, rv, okv); };
     // the keys of tile j, then the offsets of the tile behind it
     auto load_k = [&](int32_t j) __attribute__((always_inline)) {
@@ -630,9 +665,13 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
         for (int u = 0; u < NCH; u++) av[u] = ak[u];
         offsets(j + 1);
     };
+    auto zeroed = [](const uint4 &x, bool ok) {
+        return make_uint4(ok ? x.x : 0u, ok ? x.y : 0u, ok ? x.z : 0u, ok ? x.w : 0u);
+    };
     auto store_k = [&](int32_t j) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < NCH; u++) *(uint4 *)(sm.wide[0].k[j & 1] + (row0 + u * RSTEP) * KS + lc * 8) = zeroed(rk[u], okk[u]);
+        for (int u = 0; u < NCH; u++)
+            *(uint4 *)(sm.wide[0].k[j & 1] + (row0 + u * RSTEP) * KS + lc * 8) = zeroed(rk[u], okk[u]);
     };
     auto store_v = [&](int32_t j) __attribute__((always_inline)) {
         const int32_t t = k0 + j * 64;
@@ -760,19 +799,7 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
             if (j0 < tlo || j0 + 64 > thi)
                 add_back<DT, D>(a, map, max(j0, s0), min(j0 + 64, s1), rs.lo, rs.hi, p.acc);
     const float l = p.l + __shfl_xor(p.l, 32, 64);
-    if (!rs.on) return;
-    const SharedRow row = row_of(a, it, wave * 32 + col);
-    if (l != 0.f) {
-        const float inv = 1.f / l;
-#pragma unroll
-        for (int dt = 0; dt < DTN; dt++)
-#pragma unroll
-            for (int g4 = 0; g4 < 4; g4++)
-                *(float4 *)(a.part_o + row.part * D + dt * 32 + g4 * 8 + half * 4) =
-                    make_float4(p.acc[dt][g4 * 4] * inv, p.acc[dt][g4 * 4 + 1] * inv, p.acc[dt][g4 * 4 + 2] * inv,
-                                p.acc[dt][g4 * 4 + 3] * inv);
-    }
-    if (half == 0) a.part_lse[row.part] = l == 0.f ? -INFINITY : (p.m + log2f(l)) * 0.6931471805599453f;
+    put_rows<D>(a, it, rs, wave * 32 + col, p, l);
 }
 
 template <int DT, int D, bool WIDE>
@@ -780,16 +807,20 @@ __global__ __launch_bounds__((64 * shared_waves<D, WIDE>()), (D == 256 ? 1 : 2))
                                                                                         const void *__restrict__ q,
                                                                                         const void *__restrict__ k,
                                                                                         const void *__restrict__ v) {
-    constexpr int TEAMS = shared_waves<D, WIDE>() / kTeam, RT = WIDE ? 32 * shared_waves<D, WIDE>() : 32;
+    constexpr int NW = shared_waves<D, WIDE>(), RT = WIDE ? 32 * NW : 32;
     __shared__ SharedSmem<D, WIDE> sm;
-    // the wide items first, a workgroup each, then the others, a team each
-    const int32_t np = WIDE ? a.ptiles * a.nsp * a.hkv : 0;
+    // the prefixes' items first, a workgroup each, then the rows' own keys, a wavefront each
+    const int32_t np = a.ptiles * a.nsp * a.hkv;
     const int wave = uniform(threadIdx.x >> 6);
-    const bool wide = WIDE && (int32_t)blockIdx.x < np;
-    const int32_t index = wide ? (int32_t)blockIdx.x : np + ((int32_t)blockIdx.x - np) * TEAMS + wave / kTeam;
+    const bool prefix = (int32_t)blockIdx.x < np, writes = !prefix || wave == 0;
+    const int32_t index = prefix ? (int32_t)blockIdx.x : np + ((int32_t)blockIdx.x - np) * NW + wave;
     SharedItem it{};
-    const bool has = uniform(index < items && item_of<RT>(a, index, wide ? 64 : 32, wave % (wide ? 8 : kTeam) == 0, it));
-    if (wide && !has) return;
+    RowState<D> rs;
+    if (!uniform(index < items && rows_of<RT>(a, index, writes, it))) return;
+    // (the queries' loads are in flight while the item's keys are found)
+    const bool wide = WIDE && prefix;
+    load_rows<DT, D>(a, it, q, (wide ? wave * 32 : 0) + (threadIdx.x & 31), !wide, rs);
+    if (!uniform(range_of(a, wide ? 64 : 32, writes, it))) return;
     // (the wavefront's, which the compiler does not see of every one: the loads below take scalar bases)
     it.m0 = uniform(it.m0), it.table = uniform(it.table), it.s0 = uniform(it.s0), it.s1 = uniform(it.s1);
     it.cap = uniform(it.cap), it.r0 = uniform(it.r0), it.nrow = uniform(it.nrow), it.kh = uniform(it.kh);
@@ -799,13 +830,14 @@ __global__ __launch_bounds__((64 * shared_waves<D, WIDE>()), (D == 256 ? 1 : 2))
     map.v = (const char *)v + (int64_t)it.kh * a.vh * 2;
     map.table = a.block_table + it.table * a.max_pages;
     map.page = (uint32_t)(a.kb * 2), map.row = (uint32_t)(a.kt * 2), map.size = (uint32_t)a.page_size;
-    if constexpr (WIDE) {
-        if (wide) {
-            shared_wide<DT, D>(a, it, map, q, sm);
-            return;
-        }
+    if (!prefix) {
+        shared_narrow<DT, D, WIDE, 1>(a, it, map, rs, sm);
+        return;
     }
-    shared_narrow<DT, D, WIDE>(a, it, has, map, q, sm);
+    if constexpr (WIDE)
+        shared_wide<DT, D>(a, it, map, rs, sm);
+    else
+        shared_narrow<DT, D, WIDE, NW>(a, it, map, rs, sm);
 }
 
 // The ranges of a row joined, a workgroup a row: the ranges that hold keys are listed with their
@@ -894,9 +926,11 @@ static bool shared_mfma_takes(const dm_attention_desc *d, int64_t page_size) {
            k.b == v.b && k.t == v.t && k.t >= d->d && k.b < most && k.t < most / page_size;
 }
 
-// The split of a call: ranges of the prefixes and of the rows' own keys, so that there are about
-// kSharedTarget workgroups of each kind where the cache is long enough for ranges of 128 keys.
-constexpr int64_t kSharedTarget = 256;
+// The split of a call. A prefix's item is a workgroup: about kPrefixItems of them, so that some compute
+// units are left to the rows' own keys meanwhile (one reads, the other multiplies). A row's own item
+// is a wavefront (the generic kernel: a workgroup): about kOwnItems of them. No range is meant for fewer
+// than 128 keys of a prefix, 32 of a row's own, by the longest that the table can hold.
+constexpr int64_t kPrefixItems = 192, kOwnItems = 2048, kGenericItems = 1024;
 struct SharedPlan {
     bool wide;
     int32_t rows;  // rows of a prefix tile
@@ -912,12 +946,12 @@ static SharedPlan shared_plan(const dm_attention_desc *d, bool mfma, int64_t ngr
     // (first_tile of the group behind the last)
     p.ptiles = ngroups > 0 && d->b * rep > 0 ? std::max<int64_t>(0, (d->b * rep - ngroups) / p.rows) + ngroups : 0;
     p.otiles = (int32_t)((rep + kOwnRows - 1) / kOwnRows);
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kSharedSplits / 2, (d->tk + 127) / 128));
-    auto split = [&](int64_t tiles) {
-        return tiles > 0 ? (int32_t)std::min(most, std::max<int64_t>(1, kSharedTarget / tiles)) : 0;
+    auto split = [&](int64_t tiles, int64_t target, int64_t keys) {
+        const int64_t most = std::min<int64_t>(kSharedSplits / 2, (d->tk + keys - 1) / keys);
+        return tiles > 0 ? (int32_t)std::max<int64_t>(1, std::min(most, target / tiles)) : 0;
     };
-    p.nsp = split(p.ptiles * d->hkv);
-    p.nso = split(d->b * p.otiles * d->hkv);
+    p.nsp = split(p.ptiles * d->hkv, mfma ? kPrefixItems : kGenericItems, 128);
+    p.nso = split(d->b * p.otiles * d->hkv, mfma ? kOwnItems : kGenericItems, mfma ? 32 : 128);
     p.items = (p.ptiles * p.nsp + d->b * p.otiles * p.nso) * d->hkv;
     return p;
 }
@@ -998,9 +1032,9 @@ int dm_attention_decode_shared(const dm_attention_desc *d, const void *q, const 
     a.part_o = (float *)workspace;
     a.part_lse = (float *)((char *)workspace + align_up(parts * d->d * sizeof(float)));
     const int32_t items = (int32_t)p.items;
-    // (a workgroup of two teams takes two narrow items, see decode_shared_mfma)
-    const int64_t np = p.wide ? p.ptiles * p.nsp * d->hkv : 0, teams = p.wide && d->d != 256 ? 2 : 1;
-    const unsigned g = (unsigned)(np + (p.items - np + teams - 1) / teams);
+    // (the 16-bit kernel: a workgroup a prefix's item, a wavefront a row's, see decode_shared_mfma)
+    const int64_t np = p.ptiles * p.nsp * d->hkv, waves = !mfma ? 1 : (p.wide && d->d != 256 ? 8 : 4);
+    const unsigned g = (unsigned)(np + (p.items - np + waves - 1) / waves);
 #define SHARED_W(DT, D)                                                                            \
     if (p.wide)                                                                                    \
         decode_shared_mfma<DT, D, true><<<g, 64 * shared_waves<D, true>(), 0, st>>>(a, items, q, k_pages, v_pages); \
