@@ -588,14 +588,13 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
         for (int w = 0; w < NW; w++) M = fmaxf(M, sm_m[w * 32 + r]);
         float L = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (M != -INFINITY)
-            for (int w = 0; w < NW; w++) {
-                if (sm_m[w * 32 + r] == -INFINITY) continue;
-                const float f = fast_exp2(sm_m[w * 32 + r] - M);
-                const float4 y = *(const float4 *)(sa + (w * 32 + r) * D + d);
-                L += sm_l[w * 32 + r] * f;
-                o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
-            }
+        for (int w = 0; w < NW; w++) {
+            // (a reference of -inf: the wavefront's sums are 0, or NaN where all scores are)
+            const float f = sm_m[w * 32 + r] == M ? 1.f : fast_exp2(sm_m[w * 32 + r] - M);
+            const float4 y = *(const float4 *)(sa + (w * 32 + r) * D + d);
+            L += sm_l[w * 32 + r] * f;
+            o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
+        }
         const int64_t part = part_of(a, it, r);
         if (L != 0.f) {  // (NaN is not 0)
             const float inv = 1.f / L;
@@ -633,7 +632,8 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
     for (int w = 0; w < NW; w++) tlo = max(tlo, sm.lo[w]), thi = min(thi, sm.hi[w]);
     tlo = __builtin_amdgcn_readfirstlane(tlo), thi = __builtin_amdgcn_readfirstlane(thi);
     const int32_t nt = (s1 - k0 + 63) / 64;
-    const float c2 = fabsf(a.scale) * 1.4426950408889634f;
+    // (a scale of 0 as the smallest: a masked score stays -inf, the others' weights are alike)
+    const float c2 = a.scale == 0.f ? 1.2e-38f : fabsf(a.scale) * 1.4426950408889634f;
 
     // staging: NCH pieces of a tile's K and of its V a thread. The offsets of the tiles' blocks lie in
     // LDS, a ring of 128 tiles: 64 of them are looked up 64 steps before they are read.
@@ -956,11 +956,11 @@ static SharedPlan shared_plan(const dm_attention_desc *d, bool mfma, int64_t ngr
     return p;
 }
 
-// sizes whose products below fit 64 bits, and grids of fewer than 2^32 threads
+// sizes whose products below fit 64 bits, keys whose ranges fit 32, and grids of fewer than 2^32 threads
 static bool shared_sizes(const dm_attention_desc *d, int64_t ngroups) {
     const int64_t big = (int64_t)1 << 31;
     return d && d->hkv > 0 && d->b >= 0 && d->b < big && d->hq >= 0 && d->hq < 65536 && d->tk >= 0 &&
-           d->tk < big && d->d >= 0 && d->d <= 256 && ngroups >= 0 && ngroups < big &&
+           d->tk <= (big >> 1) && d->d >= 0 && d->d <= 256 && ngroups >= 0 && ngroups < big &&
            (d->b + ngroups) * std::max<int64_t>(d->hq, d->hkv) < ((int64_t)1 << 23);
 }
 

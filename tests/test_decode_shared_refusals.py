@@ -42,6 +42,7 @@ def _call(ws=1 << 40, ps=16, mp=4, bt=256, g=256, ng=1, pl=256, **kw):
     (dict(mp=3), "desc->tk (64)"), (dict(bt=None), "block table"), (dict(g=None), "groups is [G + 1]"),
     (dict(pl=None), "groups is [G + 1]"), (dict(ws=0), "workspace"), (dict(cu_seqlens_k=256), "not cu_seqlens_k"),
     (dict(b=1 << 40), "more rows"), (dict(b=1 << 30, hq=64), "more rows"), (dict(ng=1 << 40), "more rows"),
+    (dict(tk=(1 << 30) + 16, mp=(1 << 26) + 1), "more rows"),
     (dict(strided=1, sk=_lib.Strides(0, -1, 0)), "strides")])
 def test_the_library_refuses(kw, what):
     rc, msg = _call(**kw)

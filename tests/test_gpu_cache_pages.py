@@ -165,6 +165,26 @@ def test_pools(dtype, shapes, views):
     c.compact()
 
 
+def test_pools_past_four_gigabytes():
+    """Pages whose bytes lie past 32 bits are copied and moved: 5 GB, the last pages in use."""
+    pages, page, width = 5 * 2 ** 30 // 65536, 16, 4096
+    pool = torch.empty(pages, page, width, dtype=torch.int8, device="cuda")
+    table = torch.full((3, 4), -1, dtype=torch.int32, device="cuda")
+    table[0, :2] = _i32([pages - 1, pages - 3])
+    lengths, counts = _i32([21, 0, 0]), torch.zeros(pages, dtype=torch.int32, device="cuda")
+    counts[pages - 1] = counts[pages - 3] = 1
+    counts[1] = 1  # (nobody's here, in use all the same)
+    keys = torch.randint(-128, 128, (2, page, width), dtype=torch.int8, device="cuda")
+    pool[pages - 1], pool[pages - 3] = keys[0], keys[1]
+    assert dm.cache_fork([pool], table, lengths, counts, _i32([0]), _i32([2])).tolist() == [0]
+    assert table[2].tolist() == [pages - 1, 0, -1, -1] and torch.equal(pool[0, :5], keys[1, :5])
+    moved = dm.cache_compact([pool], table, lengths, counts)
+    assert counts.nonzero()[:, 0].tolist() == [0, 1, 2, 3]
+    assert table.tolist() == [[3, 2, -1, -1], [-1] * 4, [3, 0, -1, -1]]
+    assert torch.equal(pool[3], keys[0]) and torch.equal(pool[2], keys[1]) and torch.equal(pool[0, :5], keys[1, :5])
+    assert moved[pages - 1] == 3 and moved[pages - 3] == 2 and moved[[0, 1, 2]].tolist() == [0, 1, -1]
+
+
 def test_entries_outside_the_pages_are_passed_over():
     c = Both(4, 5, 20, 4, seed=10)
     c.reserve([15, 9, 0, 0])

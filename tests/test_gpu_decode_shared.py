@@ -121,6 +121,69 @@ def test_what_a_row_does_not_see_stays_out_of_it(dtype, d, page):
                     held(f"row {r}", out[r], want[r], bound[r])
 
 
+@pytest.mark.parametrize("dtype,d,window", [(BF, 128, None), (F16, 64, 100), (BF, 256, None), (BF, 128, 40)])
+def test_what_a_row_of_many_does_not_see_stays_out_of_it(dtype, d, window):
+    """The same in a group of many rows, whose prefix is swept by all of them together."""
+    lens = [300 + 7 * (i % 30) for i in range(40)]
+    b = Batch(dtype, d, 1, 4, 16, [(0, lens, 480)], {}, len(lens), seed=d, window=window)
+    opts = dm.AttentionOptions(window=None if window is None else dm.Window(window, 0))
+    bad = 371
+    want, bound = b.want()
+    q, k, v, table, *rest = b.cuda()
+    sees = [bool(n > bad and (window is None or n - 1 - window <= bad)) for n in lens]
+    assert any(sees) and not all(sees)
+    pg, row = int(table[lens.index(max(lens)), bad // 16]), bad % 16
+    for x in (float("nan"), float("inf"), -float("inf")):
+        v[pg, row, 0, 3] = x
+        if x != x:
+            k[pg, row, 0, 5] = x
+        out = dm.attention_decode_shared(q, k, v, table, *rest, opts)
+        if x != x:
+            k[pg, row, 0, 5] = 0.5
+        for r, s in enumerate(sees):
+            if s:
+                assert not torch.isfinite(out[r, :, 3]).any()
+            else:
+                held(f"row {r}", out[r], want[r], bound[r])
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F16, 64), (BF, 256), (F32, 64)])
+@pytest.mark.parametrize("rows", [3, 60])
+def test_a_query_that_is_nan_gives_nan(dtype, d, rows):
+    """In its own row and head, in groups of few rows and of many; the others are what they were."""
+    b = Batch(dtype, d, 1, 4, 16, [(0, [600 + i for i in range(rows)], 590)], {}, rows, seed=4)
+    want, bound = b.want()
+    b.q[1, 2, 7] = float("nan")
+    out = _run(b)
+    assert torch.isnan(out[1, 2]).all()
+    keep = torch.ones(out.shape[:2], dtype=torch.bool)
+    keep[1, 2] = False
+    held("others", out[keep.cuda()], want[keep], bound[keep])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F16, 64), (BF, 256), (F32, 64)])
+@pytest.mark.parametrize("shape", ["ragged", "many rows", "two large groups"])
+def test_scales_of_zero_and_below(shape, dtype, d, scale):
+    groups, lone, rows, _ = SHAPES[shape]
+    b = Batch(dtype, d, 1, 4, 16, groups, lone, rows, seed=6)
+    held("out", _run(b, dm.AttentionOptions(scale=scale)), *b.want(scale))
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_pages_past_four_gigabytes(rows):
+    """The last pages of a pool of 5 GB are the ones that are read."""
+    b = Batch(BF, 128, 2, 4, 16, [(0, [200 + i for i in range(rows)], 180)], {}, rows, seed=9)
+    q, k, v, table, *rest = b.cuda()
+    n, pages = len(k), 5 * 2 ** 30 // (k[0].numel() * 2)
+    far = [torch.empty(pages, *k.shape[1:], dtype=BF, device="cuda") for _ in range(2)]
+    far[0][-n:], far[1][-n:] = k, v
+    for pool in far:
+        pool[:1].fill_(float("nan"))
+    table = torch.where(table >= 0, table + (pages - n), table)
+    held("out", dm.attention_decode_shared(q, *far, table, *rest), *b.want())
+
+
 def test_pages_outside_read_as_zeros():
     """A page index outside the pages is a page of zeros, in the prefix and behind it."""
     b = Batch(BF, 128, 2, 4, 16, [(0, [200, 230], 160)], {}, 2, seed=5)

@@ -263,6 +263,23 @@ def test_paged_tokens_without_a_place():
     rc.held("q", qo[~zero], want[~zero], bound[~zero])
 
 
+def test_paged_past_four_gigabytes():
+    """Rows in the last pages of pools of 5 GB."""
+    page, hq, hkv, d, n = 16, 4, 2, 128, 64
+    c = _paged_case(BF, [20, 1, 3], [7, 8, 0], page, hq, hkv, d, 6)
+    q, k, v, pages, table, lengths, cut = c
+    used, total = len(pages[0]), 5 * 2 ** 30 // (pages[0][0].numel() * 2)
+    far = [torch.empty(total, *x.shape[1:], dtype=x.dtype, device="cuda") for x in pages]
+    for x, y in zip(far, pages):
+        x[-used:] = y.cuda()
+    freq = (100.0 ** (-torch.arange(n, dtype=torch.float64) / n)).float()
+    opts = dm.QkNormRopeOptions()
+    at = torch.where(table >= 0, table + (total - used), table)
+    qo = dm.qk_norm_rope_paged(*_cuda(q, k, v), None, None, freq.cuda(), *far, at.cuda(), lengths.cuda(),
+                               cut.cuda(), opts)
+    _check_paged(c, page, opts, (None, None), freq, n, (qo, far[0][-used:], far[1][-used:]))
+
+
 def test_paged_offsets_that_do_not_go_up():
     """Offsets and lengths are read on the GPU whatever they hold: no row outside is touched."""
     page, hq, hkv, d = 16, 2, 1, 64
