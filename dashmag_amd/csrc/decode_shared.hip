@@ -52,10 +52,11 @@ __device__ __forceinline__ int64_t shared_page(const SharedArgs &a, int64_t m, i
 
 // What a workgroup or a wavefront does: range `slot` of the rows r0 .. r0 + nrow - 1 (row r: member
 // m0 + r / rep, query head kh rep + r % rep) over the keys [s0, s1), which lie on `table`'s pages; a
-// member sees those of its own range that lie in front of `cap`. Every field is the wavefront's.
+// member sees those of its own range that lie in front of `cap`. Every field but len is the wavefront's.
 struct SharedItem {
-    int32_t m0, m1, table, s0, s1, base, cap, len, r0, nrow, kh, slot;
+    int32_t m0, m1, table, s0, s1, base, cap, r0, nrow, kh, slot;
     bool prefix;
+    int32_t len;  // own keys: the member's; prefix: a lane's of the members m0 + lane (-1 past the last)
 };
 
 // The first tile of group g, whose rows start at row s (of all rows of a key-value head): behind every
@@ -124,6 +125,7 @@ __device__ __forceinline__ bool rows_of(const SharedArgs &a, int32_t index, bool
         const int32_t first = (tile - first_tile<RT>(m0 * a.rep, g)) * RT, rows = (m1 - m0) * a.rep;
         if (first >= rows) return false;
         it.m0 = m0, it.m1 = m1, it.r0 = first, it.nrow = min(RT, rows - first), it.cap = plen;
+        it.len = m0 + lane < m1 ? len_of(a, m0 + lane) : -1;
         return true;
     }
     const bool grouped = ok && g >= 0;
@@ -145,7 +147,7 @@ __device__ __forceinline__ bool range_of(const SharedArgs &a, int unit, bool wri
         // the longest member, and the shortest that sees any key
         int32_t most = -1, least = INT32_MAX, at = 0;
         for (int32_t m = it.m0 + lane; m < it.m1; m += 64) {
-            const int32_t l = len_of(a, m);
+            const int32_t l = m < it.m0 + 64 ? it.len : len_of(a, m);
             if (l > most) most = l, at = m;
             if (l > 0) least = min(least, l);
         }
@@ -337,13 +339,15 @@ struct SharedSmem {
     struct Wide {
         alignas(16) uint16_t k[2][64 * KS], v[2][64 * VS];
     };
+    static_assert(!WIDE || NW * 32 * KS * 2 <= (int)sizeof(Wide), "the queries go through the tiles' places");
     union {
         Narrow narrow[NW];
         Wide wide[WIDE];
-        alignas(16) float join[WIDE ? 1 : NW * 32 * (D + 2)];
+        alignas(16) float join[WIDE ? 1 : NW * 32 * (D + 6)];
     };
     int32_t lo[NW], hi[NW], bad;
     uint64_t blocks[WIDE ? 512 : 1];  // wide: the offsets of 128 tiles' blocks, see fill
+    int64_t places[WIDE ? 1 : 32];    // narrow: the rows' places among the partial results
 };
 
 // What the lanes of a wavefront know of their rows: the queries as the second operand, and the keys seen.
@@ -356,26 +360,44 @@ struct RowState {
     bool on;
 };
 
-// The loads of row r's query (and length), which need no key; nothing here waits for them.
+// The loads of 32 rows' queries (and of this lane's row's length), which need no key; nothing here waits for
+// them. The lanes go along the rows, so that a load touches few cache lines: settle_rows sorts the pieces.
 template <int DT, int D>
-__device__ __forceinline__ void load_rows(const SharedArgs &a, const SharedItem &it, const void *q, int r,
-                                          bool slots, RowState<D> &w) {
-    const int half = (threadIdx.x >> 5) & 1;
+__device__ __forceinline__ void load_rows(const SharedArgs &a, const SharedItem &it, const void *q, int first, RowState<D> &w) {
+    constexpr int LPR = D / 8, RPL = 64 / LPR;  // lanes a row, rows a load
+    const int lane = threadIdx.x & 63, r = first + (lane & 31);
     w.on = r < it.nrow;
     int32_t member, head;
-    head_of(a, it, w.on ? r : 0, &member, &head);
+    head_of(a, it, w.on ? r : 0, &member, &head);  // (without a row: the first row's, nobody reads what becomes of it)
     w.len = it.prefix ? len_of(a, member) : 0;
-    const uint16_t *qp = (const uint16_t *)q + member * a.qb + head * a.qh;
+    const int64_t off = member * a.qb + head * a.qh;
+#pragma unroll
+    for (int u = 0; u < D / 16; u++) {
+        const int x = u * RPL + lane / LPR;
+        const int64_t at = ((int64_t)__shfl((int)(off >> 32), x, 64) << 32) | (uint32_t)__shfl((int)off, x, 64);
+        w.qf[u].u = *(const uint4 *)((const uint16_t *)q + at + (lane % LPR) * 8);
+    }
+}
+// Through the wavefront's own rows of LDS, 32 of KS values, into operands; slots: in the order of row_frag
+// (4 h + e and 8 + 4 h + e).
+template <int D>
+__device__ __forceinline__ void settle_rows(uint16_t *rows, bool slots, RowState<D> &w) {
+    constexpr int LPR = D / 8, RPL = 64 / LPR, KS = D + 8;
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int u = 0; u < D / 16; u++) *(uint4 *)(rows + (u * RPL + lane / LPR) * KS + (lane % LPR) * 8) = w.qf[u].u;
+    __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS accesses complete in order)
+    const uint16_t *mine = rows + col * KS;
 #pragma unroll
     for (int s = 0; s < D / 16; s++) {
-        // (a lane without a row takes the first row's query; nobody reads what becomes of it)
-        if (slots) {  // narrow: the slots 4 h + e and 8 + 4 h + e of row_frag
-            const uint2 l = *(const uint2 *)(qp + s * 16 + half * 4), u = *(const uint2 *)(qp + s * 16 + 8 + half * 4);
+        if (slots) {
+            const uint2 l = *(const uint2 *)(mine + s * 16 + half * 4), u = *(const uint2 *)(mine + s * 16 + 8 + half * 4);
             w.qf[s].u = make_uint4(l.x, l.y, u.x, u.y);
         } else {
-            w.qf[s].u = *(const uint4 *)(qp + s * 16 + half * 8);
+            w.qf[s].u = *(const uint4 *)(mine + s * 16 + half * 8);
         }
     }
+    __builtin_amdgcn_wave_barrier();
 }
 
 // The keys that the rows see, once the item's are known.
@@ -500,6 +522,7 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
         const int nblk = (w1 - b0 + 31) / 32;
         look_up(0);
         load(0);
+        settle_rows<D>(t.k, true, rs);
         bound_rows<D>(a, it, rs);
         for (int n = 0; n < nblk; n++) {
             const int32_t j0 = b0 + n * 32;
@@ -569,38 +592,51 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
         put_rows<D>(a, it, rs, col, p, l);
         return;
     }
-    // the wavefronts' results joined through LDS: [wave][row][D], their references and sums behind
+    // the wavefronts' results joined through LDS: [wave][row][D] (rows four banks apart), their references
+    // and sums behind, which become the factors of the sum
+    constexpr int JS = D + 4;
     __syncthreads();
-    float *sa = sm.join, *sm_m = sa + NW * 32 * D, *sm_l = sm_m + NW * 32;
+    float *sa = sm.join, *sm_m = sa + NW * 32 * JS, *sm_l = sm_m + NW * 32;
     if (col < it.nrow) {
 #pragma unroll
         for (int dt = 0; dt < DTN; dt++)
 #pragma unroll
             for (int g4 = 0; g4 < 4; g4++)
-                *(float4 *)(sa + (wave * 32 + col) * D + dt * 32 + g4 * 8 + half * 4) =
+                *(float4 *)(sa + (wave * 32 + col) * JS + dt * 32 + g4 * 8 + half * 4) =
                     make_float4(p.acc[dt][g4 * 4], p.acc[dt][g4 * 4 + 1], p.acc[dt][g4 * 4 + 2], p.acc[dt][g4 * 4 + 3]);
         if (half == 0) sm_m[wave * 32 + col] = p.m, sm_l[wave * 32 + col] = l;
     }
     __syncthreads();
-    for (int x = threadIdx.x; x < it.nrow * (D / 4); x += NW * 64) {
-        const int r = x / (D / 4), d = x % (D / 4) * 4;
-        float M = -INFINITY;
+    const int r = threadIdx.x;
+    if (r < it.nrow) {
+        float M = -INFINITY, L = 0.f, f[NW];
+#pragma unroll
         for (int w = 0; w < NW; w++) M = fmaxf(M, sm_m[w * 32 + r]);
-        float L = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
         for (int w = 0; w < NW; w++) {
             // (a reference of -inf: the wavefront's sums are 0, or NaN where all scores are)
-            const float f = sm_m[w * 32 + r] == M ? 1.f : fast_exp2(sm_m[w * 32 + r] - M);
-            const float4 y = *(const float4 *)(sa + (w * 32 + r) * D + d);
-            L += sm_l[w * 32 + r] * f;
+            const float m = sm_m[w * 32 + r];
+            f[w] = m == M ? 1.f : fast_exp2(m - M);
+            L += sm_l[w * 32 + r] * f[w];
+        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;  // (NaN is not 0)
+#pragma unroll
+        for (int w = 0; w < NW; w++) sm_l[w * 32 + r] = f[w] * inv;
+        const int64_t part = part_of(a, it, r);
+        sm.places[r] = part;
+        a.part_lse[part] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < it.nrow * (D / 4); x += NW * 64) {
+        const int r = x / (D / 4), d = x % (D / 4) * 4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float f = sm_l[w * 32 + r];
+            const float4 y = *(const float4 *)(sa + (w * 32 + r) * JS + d);
             o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
         }
-        const int64_t part = part_of(a, it, r);
-        if (L != 0.f) {  // (NaN is not 0)
-            const float inv = 1.f / L;
-            *(float4 *)(a.part_o + part * D + d) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        }
-        if (d == 0) a.part_lse[part] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+        *(float4 *)(a.part_o + sm.places[r] * D + d) = o;
     }
 }
 
@@ -609,7 +645,7 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
                                             RowState<D> &rs, SharedSmem<D, true> &sm) {
     constexpr int NW = shared_waves<D, true>(), NT = NW * 64, KS = SharedSmem<D, true>::KS, VS = SharedSmem<D, true>::VS;
     constexpr int CPR = D / 8, RSTEP = NT / CPR, NCH = 64 / RSTEP;  // pieces a row, rows at a time, pieces a thread
-    constexpr int KST = D / 16, DTN = D / 32;
+    constexpr int KST = D / 16, DTN = D / 32, AHEAD = 2;
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool first = NW == 4 || wave < 4;  // products first in each step
@@ -619,10 +655,8 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
     };
     fill(threadIdx.x);
     if (NT < 512) fill(threadIdx.x + 256);
+    settle_rows<D>((uint16_t *)&sm.wide[0] + wave * 32 * KS, false, rs);  // (read whole before the barrier below)
     bound_rows<D>(a, it, rs);
-    // (the queries are waited for here: behind the tiles' loads they would leave a wait for all of
-    // those in the loop)
-    __builtin_amdgcn_s_waitcnt(0x0F70);
     const bool rows = wave * 32 < it.nrow;  // this wavefront has rows
     if (lane == 0) sm.lo[wave] = rs.flo, sm.hi[wave] = rs.fhi;
     if (threadIdx.x == 0) sm.bad = 0;
@@ -692,31 +726,42 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
     for (int dt = 0; dt < DTN; dt++) p.acc[dt] = zero16();
     f32x16_t s[2];
     Frag8 pf[2][2];
+    // O^T of step j - 1 first, whose operands are dead when S^T's take their registers; each fragment is
+    // read from LDS ahead of the products in front of it.
     auto products = [&](int32_t j) __attribute__((always_inline)) {
+        const uint16_t *tk = sm.wide[0].k[j & 1] + col * KS + half * 8, *tv = sm.wide[0].v[(j - 1) & 1];
+        Frag8 vf[2][DTN], kf[AHEAD + 1][2];
+        auto read_v = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+            for (int dt = 0; dt < DTN; dt++) vf[g & 1][dt] = lds_tr_frag(tv, VS, g * 16, dt * 32, lane);
+        };
+        auto read_k = [&](int st) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) kf[st % (AHEAD + 1)][t].u = *(const uint4 *)(tk + t * 32 * KS + st * 16);
+        };
         __builtin_amdgcn_s_setprio(1);
+        read_v(0);  // (of a step without a tile, too: whatever lies there, unused)
+        if (rows && j > 0) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                if (g < 3) read_v(g + 1);
+#pragma unroll
+                for (int dt = 0; dt < DTN; dt++) p.acc[dt] = mfma32<DT>(vf[g & 1][dt], pf[g >> 1][g & 1], p.acc[dt]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
         if (rows && j < nt) {
-            const uint16_t *sk = sm.wide[0].k[j & 1];
+#pragma unroll
+            for (int st = 0; st < AHEAD; st++) read_k(st);
 #pragma unroll
             for (int t = 0; t < 2; t++) s[t] = zero16();
 #pragma unroll
-            for (int st = 0; st < KST; st++)
+            for (int st = 0; st < KST; st++) {
+                if (st + AHEAD < KST) read_k(st + AHEAD);
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    Frag8 x;
-                    x.u = *(const uint4 *)(sk + (t * 32 + col) * KS + half * 8 + st * 16);
-                    s[t] = mfma32<DT>(x, rs.qf[st], s[t]);
-                }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (rows && j > 0) {
-            const uint16_t *v = sm.wide[0].v[(j - 1) & 1];
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int dt = 0; dt < DTN; dt++)
-                        p.acc[dt] = mfma32<DT>(lds_tr_frag(v, VS, t * 32 + u * 16, dt * 32, lane), pf[t][u], p.acc[dt]);
+                for (int t = 0; t < 2; t++) s[t] = mfma32<DT>(kf[st % (AHEAD + 1)][t], rs.qf[st], s[t]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         __builtin_amdgcn_s_setprio(0);
     };
@@ -819,7 +864,7 @@ __global__ __launch_bounds__((64 * shared_waves<D, WIDE>()), (D == 256 ? 1 : 2))
     if (!uniform(index < items && rows_of<RT>(a, index, writes, it))) return;
     // (the queries' loads are in flight while the item's keys are found)
     const bool wide = WIDE && prefix;
-    load_rows<DT, D>(a, it, q, (wide ? wave * 32 : 0) + (threadIdx.x & 31), !wide, rs);
+    load_rows<DT, D>(a, it, q, wide ? wave * 32 : 0, rs);
     if (!uniform(range_of(a, wide ? 64 : 32, writes, it))) return;
     // (the wavefront's, which the compiler does not see of every one: the loads below take scalar bases)
     it.m0 = uniform(it.m0), it.table = uniform(it.table), it.s0 = uniform(it.s0), it.s1 = uniform(it.s1);
@@ -912,6 +957,64 @@ __global__ __launch_bounds__(256) void decode_shared_merge(SharedArgs a, void *_
             st<DT>(o, row * a.d + tid * V + c, nan ? NAN : t * inv);
         }
     }
+}
+
+// The same for rows of at most 64 ranges and a D of pieces of 4, a wavefront a row: lane i has the weight of
+// range i, and the lanes are D / 4 columns by 64 / (D / 4) groups.
+template <int DT>
+__global__ __launch_bounds__(256) void decode_shared_merge_few(SharedArgs a, int64_t rows, void *__restrict__ o) {
+    __shared__ float w[4][64];
+    __shared__ int32_t list[4][64];
+    __shared__ float4 red[4][64];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), n = a.nsp + a.nso;
+    const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+    if (row >= rows) return;
+    const float x = lane < n ? a.part_lse[row * n + lane] : -INFINITY;
+    const bool nan = __any(x != x);
+    const float top = wave_max(x);
+    const float f = x == -INFINITY ? 0.f : (x == top ? 1.f : expf(x - top));
+    const float sum = wave_sum(f);
+    const unsigned long long has = __ballot(f != 0.f);
+    const int m = __popcll(has);
+    if (f != 0.f) {
+        const int i = __popcll(has & (((unsigned long long)1 << lane) - 1));
+        list[wave][i] = lane, w[wave][i] = f;
+    }
+    __builtin_amdgcn_wave_barrier();
+    const int pieces = a.d / 4, groups = 64 / pieces, p = lane % pieces, g = lane / pieces;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (g < groups) {
+        const float *po = a.part_o + row * n * a.d + p * 4;
+        for (int i = g; i < m; i += 8 * groups) {
+            float4 y[8];
+            float fu[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int k = i + u * groups;
+                fu[u] = k < m ? w[wave][k] : 0.f;
+                y[u] = *(const float4 *)(po + (int64_t)list[wave][k < m ? k : i] * a.d);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const bool on = fu[u] != 0.f;
+                acc.x += on ? fu[u] * y[u].x : 0.f, acc.y += on ? fu[u] * y[u].y : 0.f;
+                acc.z += on ? fu[u] * y[u].z : 0.f, acc.w += on ? fu[u] * y[u].w : 0.f;
+            }
+        }
+    }
+    red[wave][lane] = acc;
+    __builtin_amdgcn_wave_barrier();
+    if (lane >= pieces) return;
+    for (int i = 1; i < groups; i++) {
+        const float4 y = red[wave][i * pieces + lane];
+        acc.x += y.x, acc.y += y.y, acc.z += y.z, acc.w += y.w;
+    }
+    const float inv = nan ? NAN : (sum > 0.f ? 1.f / sum : 0.f);
+    const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+    if constexpr (DT == DM_F32)
+        *(float4 *)((float *)o + row * a.d + lane * 4) = make_float4(y[0], y[1], y[2], y[3]);
+    else
+        *(uint2 *)((uint16_t *)o + row * a.d + lane * 4) = make_uint2(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]));
 }
 
 // The 16-bit kernel's calls: 16-byte pieces, keys' and values' pages laid out alike, a page under 2 GB.
@@ -1035,6 +1138,8 @@ int dm_attention_decode_shared(const dm_attention_desc *d, const void *q, const 
     // (the 16-bit kernel: a workgroup a prefix's item, a wavefront a row's, see decode_shared_mfma)
     const int64_t np = p.ptiles * p.nsp * d->hkv, waves = !mfma ? 1 : (p.wide && d->d != 256 ? 8 : 4);
     const unsigned g = (unsigned)(np + (p.items - np + waves - 1) / waves);
+    // (a row of few ranges is a wavefront's, in 16-byte pieces; on 8192 rows of 7 ranges ... )
+    const bool few = p.nsp + p.nso <= 64 && d->d % 4 == 0 && aligned_16b(o);
 #define SHARED_W(DT, D)                                                                            \
     if (p.wide)                                                                                    \
         decode_shared_mfma<DT, D, true><<<g, 64 * shared_waves<D, true>(), 0, st>>>(a, items, q, k_pages, v_pages); \
@@ -1052,7 +1157,9 @@ int dm_attention_decode_shared(const dm_attention_desc *d, const void *q, const 
             SHARED_W(DT, 256);                                                 \
         }                                                                      \
     }                                                                          \
-    if (d->d % 4 == 0)                                                         \
+    if (few)                                                                   \
+        decode_shared_merge_few<DT><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a, rows, o); \
+    else if (d->d % 4 == 0)                                                    \
         decode_shared_merge<DT, 4><<<(unsigned)rows, 256, 0, st>>>(a, o);      \
     else                                                                       \
         decode_shared_merge<DT, 1><<<(unsigned)rows, 256, 0, st>>>(a, o)
