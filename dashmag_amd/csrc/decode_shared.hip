@@ -456,24 +456,31 @@ struct Partial {
     float m, l;
 };
 
-// A wavefront's rows (this lane's: r) with the sums l over both halves: normalised partial results.
+// A wavefront's rows (n from r0 on) with the sums l over both halves: normalised partial results, through its
+// own `rows` of LDS so that the lanes go along the rows. (A range whose weights are 0 is zeros that nobody reads.)
 template <int D>
-__device__ __forceinline__ void put_rows(const SharedArgs &a, const SharedItem &it, const RowState<D> &rs, int r,
-                                         const Partial<D> &p, float l) {
-    const int half = (threadIdx.x >> 5) & 1;
-    if (!rs.on) return;
-    const int64_t part = part_of(a, it, r);
-    if (l != 0.f) {  // (NaN is not 0)
-        const float inv = 1.f / l;
+__device__ __forceinline__ void put_rows(const SharedArgs &a, const SharedItem &it, int r0, const Partial<D> &p, float l,
+                                         float *rows) {
+    constexpr int JS = D + 4, LPR = D / 4, RPL = 64 / LPR;
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, n = min(32, it.nrow - r0);
+    const int64_t part = part_of(a, it, r0 + (col < n ? col : 0));
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // (NaN is not 0)
 #pragma unroll
-        for (int dt = 0; dt < D / 32; dt++)
+    for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
-            for (int g4 = 0; g4 < 4; g4++)
-                *(float4 *)(a.part_o + part * D + dt * 32 + g4 * 8 + half * 4) =
-                    make_float4(p.acc[dt][g4 * 4] * inv, p.acc[dt][g4 * 4 + 1] * inv, p.acc[dt][g4 * 4 + 2] * inv,
-                                p.acc[dt][g4 * 4 + 3] * inv);
+        for (int g4 = 0; g4 < 4; g4++)
+            *(float4 *)(rows + col * JS + dt * 32 + g4 * 8 + half * 4) =
+                make_float4(p.acc[dt][g4 * 4] * inv, p.acc[dt][g4 * 4 + 1] * inv, p.acc[dt][g4 * 4 + 2] * inv,
+                            p.acc[dt][g4 * 4 + 3] * inv);
+    __builtin_amdgcn_wave_barrier();
+    if (half == 0 && col < n) a.part_lse[part] = l == 0.f ? -INFINITY : (p.m + log2f(l)) * 0.6931471805599453f;
+#pragma unroll 4
+    for (int r = 0; r < n; r += RPL) {
+        const int x = r + lane / LPR, y = min(x, 31);
+        const int64_t to = ((int64_t)__shfl((int)(part >> 32), y, 64) << 32) | (uint32_t)__shfl((int)part, y, 64);
+        const float4 o = *(const float4 *)(rows + y * JS + lane % LPR * 4);
+        if (x < n) *(float4 *)(a.part_o + to * D + lane % LPR * 4) = o;
     }
-    if (half == 0) a.part_lse[part] = l == 0.f ? -INFINITY : (p.m + log2f(l)) * 0.6931471805599453f;
 }
 
 // TEAM: the wavefronts that share the item's keys, the whole workgroup or one.
@@ -589,7 +596,9 @@ __device__ __forceinline__ void shared_narrow(const SharedArgs &a, const SharedI
     }
     const float l = p.l + __shfl_xor(p.l, 32, 64);
     if constexpr (TEAM == 1) {
-        put_rows<D>(a, it, rs, col, p, l);
+        static_assert(sizeof(t) >= 32 * (D + 4) * sizeof(float), "the results go through the tile's place");
+        __builtin_amdgcn_wave_barrier();
+        put_rows<D>(a, it, 0, p, l, (float *)&t);
         return;
     }
     // the wavefronts' results joined through LDS: [wave][row][D] (rows four banks apart), their references
@@ -844,7 +853,9 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
             if (j0 < tlo || j0 + 64 > thi)
                 add_back<DT, D>(a, map, max(j0, s0), min(j0 + 64, s1), rs.lo, rs.hi, p.acc);
     const float l = p.l + __shfl_xor(p.l, 32, 64);
-    put_rows<D>(a, it, rs, wave * 32 + col, p, l);
+    // (every wavefront is past its last tile)
+    static_assert(sizeof(sm.narrow) >= NW * 32 * (D + 4) * sizeof(float), "the results go through the tiles' places");
+    put_rows<D>(a, it, wave * 32, p, l, (float *)&sm.narrow[0] + wave * 32 * (D + 4));
 }
 
 template <int DT, int D, bool WIDE>
