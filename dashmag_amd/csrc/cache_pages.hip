@@ -5,6 +5,11 @@
 // one that keeps the pages in use together. The bookkeeping is a walk over the counts with prefix
 // sums, by one workgroup (it is a few KB to a few hundred KB, and pages are handed out in order);
 // copying pages is what costs bandwidth, and is spread over the card in 16 KB pieces.
+//
+// The walks are bound by latency: with 4096 pages and 128 rows, 64 forks are planned in 4.4 us and made
+// (four layers' last pages, 16 MB at most) in 6.8, 128 rows' pages reserved in 4.6, 64 rows freed in 3.3,
+// about 3 us of each a launch. Compaction is bound by its copies: 6000 pages of 32 KB in four pools half in use,
+// 5.1 us of plan and 4.6 of counts in front of 68-80 us at 4.9 to 5.7 TB/s.
 #include <algorithm>
 #include <string>
 
@@ -156,7 +161,7 @@ __global__ __launch_bounds__(kPlan) void cache_reserve_kernel(CacheArgs a, const
 
 // Which forks are made, and the pages of their own: held [n] is the keys that the child takes over, -1
 // for a fork that is not made. The first fork that names a child has it: claim [rows], in LDS for tables
-// of up to kClaims rows.
+// of up to kClaims rows (its 16 KB; larger tables claim in the workspace, through the cache).
 constexpr int kClaims = 4096;
 template <bool LDS>
 __global__ __launch_bounds__(kPlan) void cache_fork_plan(CacheArgs a, const int32_t *__restrict__ parents,
@@ -281,7 +286,7 @@ __global__ __launch_bounds__(256) void cache_free_kernel(CacheArgs a, const int3
     }
 }
 
-// Compaction in three launches: the pages in use counted by chunk; each chunk's holes and movers put
+// Compaction in three launches (two for a single chunk): the pages in use counted by chunk; each chunk's holes and movers put
 // in their places of the two lists (moved holds -2 - place for a mover until the last launch); the
 // pages, counts and entries moved.
 constexpr int kChunk = kPlan * 4;
@@ -315,7 +320,8 @@ __global__ __launch_bounds__(kPlan) void cache_compact_plan(CacheArgs a, Compact
     int32_t is[4], total;
     uses(a, p0, is);
     int32_t before = 0, all = 0;  // the pages in use in front of this chunk, and altogether
-    for (int64_t c0 = 0; c0 < w.nchunks; c0 += kPlan) {
+    if (w.nchunks == 1) plan_scan(is[0] + is[1] + is[2] + is[3], sums, turn, &all);
+    for (int64_t c0 = 0; w.nchunks > 1 && c0 < w.nchunks; c0 += kPlan) {
         const int64_t c = c0 + tid;
         const int32_t x = c < w.nchunks ? w.chunks[c] : 0;
         // (one scan: what lies in front of this chunk's place in it is the sum in front of it)
@@ -331,7 +337,7 @@ __global__ __launch_bounds__(kPlan) void cache_compact_plan(CacheArgs a, Compact
     int32_t stay = 0;
     for (int64_t c0 = 0; c0 < cn; c0 += kPlan) {
         const int64_t c = c0 + tid;
-        plan_scan(c < cn ? w.chunks[c] : 0, sums, turn, &total);
+        plan_scan(c < cn ? (w.nchunks > 1 ? w.chunks[c] : all) : 0, sums, turn, &total);
         stay += total;
     }
     int32_t last[4], mine = 0;
@@ -562,7 +568,7 @@ int dm_cache_compact(const dm_cache_table *t, const dm_cache_pool *pools, int64_
     w.chunks = (int32_t *)(at += 256);
     w.holes = (int32_t *)(at += align_up((size_t)w.nchunks * 4));
     w.movers = (int32_t *)(at += align_up((size_t)t->num_pages * 4));
-    cache_compact_count<<<(unsigned)w.nchunks, kPlan, 0, st>>>(a, w);
+    if (w.nchunks > 1) cache_compact_count<<<(unsigned)w.nchunks, kPlan, 0, st>>>(a, w);  // (one: the plan counts it)
     cache_compact_plan<<<(unsigned)w.nchunks, kPlan, 0, st>>>(a, w, moved);
     for (int64_t i = 0; i == 0 || i < npools; i += kPoolsPerLaunch) {
         bool wide;

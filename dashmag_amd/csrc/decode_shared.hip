@@ -10,6 +10,16 @@
 // A workgroup takes one range of keys for a tile of rows of one key-value head. The ranges are cut on
 // the device, evenly over the keys that there are, so the grid needs no length on the host and a
 // call reads nothing back. A call whose groups do not go up runs with every row's keys its own.
+//
+// Measured in bf16, with the merge, MFMA rates counting 4 D a (row, key) pair (a large product on this card
+// runs at 1240 TFLOP/s, a large copy at 5.0 TB/s):
+//   256 rows, a prefix of 32768 keys, 512 of their own, 32 heads of 128 over 8: 220 us, 630 TFLOP/s. Bound by
+//     the prefix's products: alone they reach 670 TFLOP/s on 192 compute units and 725 on all 256, where the
+//     clock falls; a 64-key step of 256 rows takes 3900 cycles, 2060 of them MFMA issue.
+//   64 rows, 16384 and 1024 keys, the same heads: 75 us: 216 MB, 43 us at a copy's rate, and about 6 us until
+//     the first keys arrive (the groups, the lengths, the page, the keys: each waits for the one in front).
+//   8 rows, 6144 and 200 keys, 8 heads of 256 over 2: 20 us; 45 rows in 5 groups, 16 heads of 64 over 2 in f16,
+//     window 6000: 23 us: the same chain, one or a few steps, the ranges' join and the merge's launch.
 #include <algorithm>
 #include <string>
 
@@ -179,7 +189,9 @@ __device__ __forceinline__ bool range_of(const SharedArgs &a, int unit, bool wri
 }
 
 // The simple form, for every type, head width, page size and stride: 32 rows and 16 keys at a time in
-// LDS as f32, eight threads a row, each two of its scores and every eighth column of its output.
+// LDS as f32, eight threads a row, each two of its scores and every eighth column of its output. Bound by
+// its LDS reads, two for a multiply-add: 256 bf16 rows of 32768 + 512 keys, 32 heads of 128, take 21 ms
+// here against 0.22 below.
 constexpr int kGenKeys = 16;
 template <int DT>
 __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const void *__restrict__ q,
@@ -283,7 +295,8 @@ __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const
 //
 // WIDE items (the prefix of a group of many rows): the rows are shared out, 32 a wavefront, and all
 // sweep the same keys in tiles of 64. Wavefronts w and w + 4 of a SIMD run half a step apart, so
-// that one's products and the other's softmax run side by side.
+// that one's products and the other's softmax run side by side. (At D = 256 a wavefront a SIMD: its outputs
+// and queries alone are 192 registers.)
 //
 // Keys arrive in 16-key blocks, each on one page: a buffer resource of the block's rows up to the
 // item's end reads zeros behind it, and a page outside the pages, or in front of the item's start,
@@ -1040,10 +1053,19 @@ static bool shared_mfma_takes(const dm_attention_desc *d, int64_t page_size) {
            k.b == v.b && k.t == v.t && k.t >= d->d && k.b < most && k.t < most / page_size;
 }
 
-// The split of a call. A prefix's item is a workgroup: about kPrefixItems of them, so that some compute
-// units are left to the rows' own keys meanwhile (one reads, the other multiplies). A row's own item
-// is a wavefront (the generic kernel: a workgroup): about kOwnItems of them. No range is meant for fewer
-// than 128 keys of a prefix, 32 of a row's own, by the longest that the table can hold.
+// The split of a call.
+//
+// Wide where a group has more than 32 rows a key-value head in the mean, a narrow tile's. (One group, 16384
+// keys, 4 key-value heads, narrow and wide: 16 and 32 rows of 128: 19.1 and 20.1 us, 23.4 and 24.1; 48 and 64:
+// 25.3 and 24.6, 25.0 and 25.2; 128: 31.6, 27.3. Rows of 64: 32 16.1, 19.1, 128 23.5, 20.9; rows of 256: 32 30.9,
+// 35.0, 48 38.9, 35.9.)
+//
+// A prefix's item is a workgroup: about kPrefixItems of them, so that some compute units are left to the rows'
+// own keys meanwhile (one reads, the other multiplies). (256 rows, 32768 + 512 keys and 64 rows, 16384 + 1024:
+// 160 236 and 73 us, 192 222 and 75, 224 239 and 77, 256 239 and 80.) A row's own item is a wavefront (the
+// generic kernel: a workgroup): about kOwnItems of them. (1024: 227 and 91 us; the small calls are alike.) No
+// range is meant for fewer than 128 keys of a prefix (64: 8 rows of 6144 + 200 keys of 256 26 us, 128 20), 32 of a
+// row's own, by the longest that the table can hold.
 constexpr int64_t kPrefixItems = 192, kOwnItems = 2048, kGenericItems = 1024;
 struct SharedPlan {
     bool wide;
@@ -1149,7 +1171,7 @@ int dm_attention_decode_shared(const dm_attention_desc *d, const void *q, const 
     // (the 16-bit kernel: a workgroup a prefix's item, a wavefront a row's, see decode_shared_mfma)
     const int64_t np = p.ptiles * p.nsp * d->hkv, waves = !mfma ? 1 : (p.wide && d->d != 256 ? 8 : 4);
     const unsigned g = (unsigned)(np + (p.items - np + waves - 1) / waves);
-    // (a row of few ranges is a wavefront's, in 16-byte pieces; on 8192 rows of 7 ranges ... )
+    // (8192 rows of 7 ranges: 10 us by wavefronts, 28 by workgroups; of more than 64, a workgroup)
     const bool few = p.nsp + p.nso <= 64 && d->d % 4 == 0 && aligned_16b(o);
 #define SHARED_W(DT, D)                                                                            \
     if (p.wide)                                                                                    \

@@ -138,10 +138,11 @@ def test_many_rows_and_forks():
 
 
 @pytest.mark.parametrize("in_use", ["none", "all", "low", "high", "one"])
-def test_compaction_of(in_use):
-    pages = 9000
+@pytest.mark.parametrize("pages", [9000, 1, 100, 4095, 4096, 4097, 8192])
+def test_compaction_of(in_use, pages):
+    """Pools around the pages that a planning workgroup takes at a time (4096)."""
     c = Both(4, 4096, pages, 2, shapes=((8,),), seed=8)
-    n = {"none": 0, "all": pages, "low": 3000, "high": 3000, "one": 1}[in_use]
+    n = {"none": 0, "all": pages, "low": pages // 3, "high": pages // 3, "one": 1}[in_use]
     start = pages - n if in_use in ("high", "one") else 0
     ids = list(range(start, start + n))
     for r in range(4):
