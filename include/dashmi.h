@@ -214,7 +214,8 @@ typedef struct {
  * is free), int32 on the device, changed in place. A row of n keys holds its first
  * ceil(n / page_size) entries. Only whole pages are ever shared, so what a row appends to its last,
  * partly filled page no other row holds. Whatever the arrays hold, no page outside the pools and no
- * entry outside the table is touched. */
+ * entry outside the table is touched. num_pages is at most 2^21 - 2; the calls that take n forks or
+ * rows take at most 2^22. */
 typedef struct {
     int64_t rows, max_pages, num_pages, page_size;
     int32_t *block_table, *lengths, *refcounts;
@@ -378,11 +379,12 @@ int dm_attention_decode_paged(const dm_attention_desc *desc, const void *q, cons
 /* dm_attention_decode_paged for sequences that share prefixes: rows groups[g] .. groups[g + 1] - 1
  * of the batch hold the same first prefix_lengths[g] keys, which are read once for the group, through
  * the block table of its longest row (one of them), which has to hold all of the prefix that
- * any row of the group sees; each row's own keys behind them through its own. Results are the paged decode's of the same arguments wherever that holds. groups
+ * any row of the group sees; each row's own keys behind them through its own. Wherever that holds
+ * the results are those of the paged decode on the same arguments, up to rounding. groups
  * [ngroups + 1] and prefix_lengths [ngroups] are int32 on the device, as block_table and lengths,
  * and are read there only. Rows in front of the first group or behind the last share nothing, and
  * no row does if groups does not go up from 0 at least to B at most; a prefix length is taken
- * between 0 and desc->tk. */
+ * between 0 and desc->tk. Refused: (B + ngroups) * max(Hq, Hkv) of 2^23 or more, tk above 2^30. */
 size_t dm_attention_decode_shared_workspace(const dm_attention_desc *desc, int64_t page_size,
                                             int64_t ngroups);
 int dm_attention_decode_shared(const dm_attention_desc *desc, const void *q, const void *k_pages,
