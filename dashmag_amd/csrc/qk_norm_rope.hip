@@ -16,6 +16,7 @@
 // loads (the length, its page, the heads): 7.7 us.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "attention_kernels.h"
 #include "dm_common.h"
@@ -259,15 +260,23 @@ __global__ __launch_bounds__(256) void rope_bwd_generic(RopeArgs a, const void *
     }
 }
 
-// The kernels for heads of 64, 128 and 256 in 16-byte pieces of V values: D / (2 V) lanes take a head,
-// each the pieces at V li and n + V li, the first and the second elements of its pairs (half style), or
-// of adjacent ones (interleaved); past the rotated 2 n the rest of the head in the same manner. So a
-// pair never leaves its lane, and a head's sums are moves within 16 lanes (32 in f32).
+// The kernels for heads of 64, 80, 96, 128, 192 and 256 in 16-byte pieces of V values: D / (2 V) lanes take a
+// head, each the pieces at V li and n + V li, the first and the second elements of its pairs (half style),
+// or of adjacent ones (interleaved); past the rotated 2 n the rest of the head in the same manner. So a
+// pair never leaves its lane, and a head's sums are moves within 16 lanes (32 in f32). Lanes come in powers
+// of two: of a head of 96 two of eight are idle, with values of 0. (8192 tokens of 40 heads in bf16,
+// replayed, forward and backward: 80 wide 27 and 39 us, 96 27 and 41, 192 51 and 87; 112, by the simple
+// kernels, 184 and 376.)
 //
 // A workgroup takes `tile` tokens: the angles of all of them go to LDS first, one a thread, since every
 // head of a token turns by the same ones, then its lanes go through the tokens' heads.
 template <int DT>
 constexpr int rope_v() { return DT == DM_F32 ? 4 : 8; }
+
+// Lanes with pieces of a head, and lanes of a head.
+template <int DT, int D>
+constexpr int rope_pieces() { return D / (2 * rope_v<DT>()); }
+constexpr int rope_lanes(int pieces) { return pieces <= 1 ? 1 : 2 * rope_lanes((pieces + 1) / 2); }
 
 template <int DT>
 __device__ __forceinline__ uint4 raw_piece(const void *p, int64_t at) {
@@ -283,6 +292,11 @@ __device__ __forceinline__ void unpack_piece(const uint4 &a, float (&x)[V]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) x[2 * i] = unpack_lo<DT>(w[i]), x[2 * i + 1] = unpack_hi<DT>(w[i]);
     }
+}
+template <int V>
+__device__ __forceinline__ void zero_pieces(float (&a)[V], float (&b)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) a[i] = b[i] = 0.f;
 }
 template <int DT, int V>
 __device__ __forceinline__ void put_piece(void *p, int64_t at, const float (&x)[V]) {
@@ -402,14 +416,15 @@ template <int DT, int D, int MODE, bool INTER>
 __global__ __launch_bounds__(256) void rope_fast(RopeArgs a, RopePages pg, int tile, const void *__restrict__ q,
                                                  const void *__restrict__ k, const void *__restrict__ v,
                                                  void *__restrict__ qo, void *__restrict__ ko, void *__restrict__ vo) {
-    constexpr int V = rope_v<DT>(), LPH = D / (2 * V), BY = 256 / LPH, U = 2;
+    constexpr int V = rope_v<DT>(), PIECES = rope_pieces<DT, D>(), LPH = rope_lanes(PIECES), BY = 256 / LPH, U = 2;
     constexpr bool PAGED = MODE == kRopePaged;
     extern __shared__ __align__(16) float lds[];  // the weights [2, D], two tiles' angles
     __shared__ RopePlaces places[PAGED ? 3 : 1];
     const int tid = threadIdx.x, li = tid % LPH, r0 = tid / LPH, n = a.n;
     float *angles = lds + 2 * D;
     const int64_t step = (int64_t)gridDim.x * tile, start = (int64_t)blockIdx.x * tile;
-    const HeadLane<D, V, INTER> hl(li, n);
+    const bool part = PIECES == LPH || li < PIECES;  // (an idle lane reads the first pieces and holds zeros)
+    const HeadLane<D, V, INTER> hl(part ? li : 0, n);
     uint4 ra[U], rb[U];
     auto load = [&](int64_t first, int r, RowWalk &w, int rows, const void *src, const Strd &sd) __attribute__((always_inline)) {
 #pragma unroll
@@ -460,6 +475,7 @@ __global__ __launch_bounds__(256) void rope_fast(RopeArgs a, RopePages pg, int t
                         float pa[V], pb[V], ss = 0.f;
                         unpack_piece<DT, V>(ra[u], pa);
                         unpack_piece<DT, V>(rb[u], pb);
+                        if (!part) zero_pieces<V>(pa, pb);
 #pragma unroll
                         for (int i = 0; i < V; i++) ss += pa[i] * pa[i] + pb[i] * pb[i];
                         const float rs = rsqrtf(head_sum<LPH>(ss) * (1.f / D) + a.eps);
@@ -478,7 +494,7 @@ __global__ __launch_bounds__(256) void rope_fast(RopeArgs a, RopePages pg, int t
                                 for (int i = 0; i < V; i++) pa[i] = pb[i] = 0.f;
                             }
                         }
-                        if (on) {
+                        if (on && part) {
                             put_piece<DT, V>(dst, to + hl.a, pa);
                             put_piece<DT, V>(dst, to + hl.b, pb);
                         }
@@ -491,11 +507,11 @@ __global__ __launch_bounds__(256) void rope_fast(RopeArgs a, RopePages pg, int t
             constexpr int E = DT == DM_F32 ? 4 : 2;
             RowWalk w(r0, BY, max(a.hkv, 1));
             for (int r = r0; r < here * a.hkv; r += BY, w.next()) {
-                if (place.vrow[w.t] < 0) continue;
+                if (place.vrow[w.t] < 0 || !part) continue;
                 const uint4 *from = (const uint4 *)((const char *)v + ((first + w.t) * a.v.t + w.h * a.v.h) * E);
                 uint4 *to = (uint4 *)((char *)vo + (place.vrow[w.t] + w.h * pg.v.h) * E);
-                const uint4 y = from[li], z = from[li + LPH];
-                to[li] = y, to[li + LPH] = z;
+                const uint4 y = from[li], z = from[li + PIECES];
+                to[li] = y, to[li + PIECES] = z;
             }
         }
         if (next >= start && next < a.tokens) {
@@ -517,11 +533,12 @@ __global__ __launch_bounds__(256) void rope_bwd_fast(RopeArgs a, int tile, const
                                                      const void *__restrict__ k, const void *__restrict__ gq,
                                                      const void *__restrict__ gk, void *__restrict__ dq,
                                                      void *__restrict__ dk, float *__restrict__ parts) {
-    constexpr int V = rope_v<DT>(), LPH = D / (2 * V), BY = 256 / LPH;
+    constexpr int V = rope_v<DT>(), PIECES = rope_pieces<DT, D>(), LPH = rope_lanes(PIECES), BY = 256 / LPH;
     extern __shared__ __align__(16) float lds[];  // the weights [2, D], two tiles' angles; at the end the lanes' sums [BY, D]
     const int tid = threadIdx.x, li = tid % LPH, r0 = tid / LPH, n = a.n;
     float *angles = lds + 2 * D;
-    const HeadLane<D, V, INTER> hl(li, n);
+    const bool part = PIECES == LPH || li < PIECES;
+    const HeadLane<D, V, INTER> hl(part ? li : 0, n);
     float da[2][V] = {}, db[2][V] = {};  // of the heads that are gone through now, and of the others
     const int64_t step = (int64_t)gridDim.x * tile, start = (int64_t)blockIdx.x * tile;
     int buf = 0;
@@ -546,11 +563,13 @@ __global__ __launch_bounds__(256) void rope_bwd_fast(RopeArgs a, int tile, const
                 float xa[V], xb[V], za[V], zb[V], ss = 0.f, gh = 0.f;
                 unpack_piece<DT, V>(rxa, xa);
                 unpack_piece<DT, V>(rxb, xb);
+                if (!part) zero_pieces<V>(xa, xb);
 #pragma unroll
                 for (int i = 0; i < V; i++) ss += xa[i] * xa[i] + xb[i] * xb[i];
                 const float rs = rsqrtf(head_sum<LPH>(ss) * (1.f / D) + a.eps);
                 unpack_piece<DT, V>(rza, za);
                 unpack_piece<DT, V>(rzb, zb);
+                if (!part) zero_pieces<V>(za, zb);
                 if (hl.turns) turn_pieces<V, INTER, true>(za, zb, cs + w.t * n, sn + w.t * n, hl.ja, hl.jb);
 #pragma unroll
                 for (int i = 0; i < V; i++) {
@@ -566,8 +585,10 @@ __global__ __launch_bounds__(256) void rope_bwd_fast(RopeArgs a, int tile, const
                     zb[i] = rs * (zb[i] - xb[i] * mean);
                 }
                 const int64_t to = ((first + w.t) * heads + w.h) * D;
-                put_piece<DT, V>(dst, to + hl.a, za);
-                put_piece<DT, V>(dst, to + hl.b, zb);
+                if (part) {
+                    put_piece<DT, V>(dst, to + hl.a, za);
+                    put_piece<DT, V>(dst, to + hl.b, zb);
+                }
             }
 #pragma unroll
             for (int i = 0; i < V; i++) {
@@ -582,7 +603,8 @@ __global__ __launch_bounds__(256) void rope_bwd_fast(RopeArgs a, int tile, const
     for (int x = 0; x < 2; x++) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < V; i++) lds[r0 * D + hl.a + i] = da[x][i], lds[r0 * D + hl.b + i] = db[x][i];
+        for (int i = 0; i < V; i++)
+            if (part) lds[r0 * D + hl.a + i] = da[x][i], lds[r0 * D + hl.b + i] = db[x][i];
         __syncthreads();
         for (int e = tid; e < D; e += 256) {
             float t = 0.f;
@@ -670,7 +692,8 @@ static RopeArgs rope_args(const dm_qk_norm_rope_desc *d, const void *wq, const v
 static bool fast_takes(const dm_qk_norm_rope_desc *d, const RopeArgs &a, const void *const *ptrs, int n,
                        const Strd *strides, int ns) {
     const int v = d->dtype == DM_F32 ? 4 : 8;
-    if ((d->d != 64 && d->d != 128 && d->d != 256) || d->n % v != 0) return false;
+    if ((d->d != 64 && d->d != 80 && d->d != 96 && d->d != 128 && d->d != 192 && d->d != 256) || d->n % v != 0)
+        return false;
     for (int i = 0; i < n; i++)
         if (!aligned_16b(ptrs[i])) return false;
     for (int i = 0; i < ns; i++)
@@ -693,20 +716,29 @@ static int rope_tile(const RopeArgs &a, int by) {
 constexpr int64_t kRopeGrid = 4096;
 static size_t rope_lds(const RopeArgs &a, int tile) { return ((size_t)2 * a.d + (size_t)4 * tile * a.n) * sizeof(float); }
 
-#define ROPE_D(KERNEL, DT, MODE_, GRID, LDS, ...)                                                           \
-    do {                                                                                                    \
-        if (d->d == 64) {                                                                                   \
-            if (a.interleaved) KERNEL<DT, 64 MODE_, true><<<GRID, 256, LDS, st>>>(__VA_ARGS__);             \
-            else KERNEL<DT, 64 MODE_, false><<<GRID, 256, LDS, st>>>(__VA_ARGS__);                          \
-        } else if (d->d == 128) {                                                                           \
-            if (a.interleaved) KERNEL<DT, 128 MODE_, true><<<GRID, 256, LDS, st>>>(__VA_ARGS__);            \
-            else KERNEL<DT, 128 MODE_, false><<<GRID, 256, LDS, st>>>(__VA_ARGS__);                         \
-        } else {                                                                                            \
-            if (a.interleaved) KERNEL<DT, 256 MODE_, true><<<GRID, 256, LDS, st>>>(__VA_ARGS__);            \
-            else KERNEL<DT, 256 MODE_, false><<<GRID, 256, LDS, st>>>(__VA_ARGS__);                         \
-        }                                                                                                   \
-    } while (0)
-#define ROPE_COMMA ,
+// f(type, width, interleaved) as constants, for the fast kernels' widths.
+template <int X>
+using Int = std::integral_constant<int, X>;
+template <typename F>
+static void rope_dispatch(const dm_qk_norm_rope_desc *d, F f) {
+    auto inter = [&](auto dt, auto width) {
+        if (d->interleaved) f(dt, width, Int<1>{});
+        else f(dt, width, Int<0>{});
+    };
+    auto of = [&](auto dt) {
+        switch (d->d) {
+            case 64: return inter(dt, Int<64>{});
+            case 80: return inter(dt, Int<80>{});
+            case 96: return inter(dt, Int<96>{});
+            case 128: return inter(dt, Int<128>{});
+            case 192: return inter(dt, Int<192>{});
+            default: return inter(dt, Int<256>{});
+        }
+    };
+    if (d->dtype == DM_F32) of(Int<DM_F32>{});
+    else if (d->dtype == DM_BF16) of(Int<DM_BF16>{});
+    else of(Int<DM_F16>{});
+}
 
 template <int MODE>
 static int run_rope(const char *op, const dm_qk_norm_rope_desc *d, const RopeArgs &a, const RopePages &pg,
@@ -716,15 +748,13 @@ static int run_rope(const char *op, const dm_qk_norm_rope_desc *d, const RopeArg
     const Strd strides[] = {a.q, a.k, a.v, pg.k, pg.v};
     constexpr bool paged = MODE == kRopePaged;
     if (fast_takes(d, a, ptrs, paged ? 6 : 4, strides, paged ? 5 : 2)) {
-        const int by = 256 / (int)(d->d / (d->dtype == DM_F32 ? 8 : 16)), tile = rope_tile(a, by);
+        const int by = 256 / rope_lanes((int)(d->d / (d->dtype == DM_F32 ? 8 : 16))), tile = rope_tile(a, by);
         const unsigned grid = (unsigned)std::min((a.tokens + tile - 1) / tile, kRopeGrid);
         const size_t lds = rope_lds(a, tile);
-        if (d->dtype == DM_F32)
-            ROPE_D(rope_fast, DM_F32, ROPE_COMMA MODE, grid, lds, a, pg, tile, q, k, v, qo, ko, vo);
-        else if (d->dtype == DM_BF16)
-            ROPE_D(rope_fast, DM_BF16, ROPE_COMMA MODE, grid, lds, a, pg, tile, q, k, v, qo, ko, vo);
-        else
-            ROPE_D(rope_fast, DM_F16, ROPE_COMMA MODE, grid, lds, a, pg, tile, q, k, v, qo, ko, vo);
+        rope_dispatch(d, [&](auto dt, auto width, auto inter) {
+            rope_fast<decltype(dt)::value, decltype(width)::value, MODE, decltype(inter)::value != 0>
+                <<<grid, 256, lds, st>>>(a, pg, tile, q, k, v, qo, ko, vo);
+        });
     } else {
         const int64_t rows = a.tokens * (a.hq + a.hkv * (paged ? 2 : 1));
         const unsigned grid = (unsigned)std::min<int64_t>((rows + 3) / 4, 16384);
@@ -777,16 +807,14 @@ int dm_qk_norm_rope_bwd(const dm_qk_norm_rope_desc *d, const void *q, const void
         const void *ptrs[] = {q, k, grad_q, grad_k, dq, dk};
         const Strd strides[] = {a.q, a.k, a.gq, a.gk};
         if (fast_takes(d, a, ptrs, 6, strides, 4)) {
-            const int by = 256 / (int)(d->d / (d->dtype == DM_F32 ? 8 : 16)), tile = rope_tile(a, by);
+            const int by = 256 / rope_lanes((int)(d->d / (d->dtype == DM_F32 ? 8 : 16))), tile = rope_tile(a, by);
             nparts = std::min<int64_t>((a.tokens + tile - 1) / tile, kRopeParts);
             const unsigned grid = (unsigned)nparts;
             const size_t lds = std::max(rope_lds(a, tile), (size_t)by * d->d * sizeof(float));
-            if (d->dtype == DM_F32)
-                ROPE_D(rope_bwd_fast, DM_F32, , grid, lds, a, tile, q, k, grad_q, grad_k, dq, dk, parts);
-            else if (d->dtype == DM_BF16)
-                ROPE_D(rope_bwd_fast, DM_BF16, , grid, lds, a, tile, q, k, grad_q, grad_k, dq, dk, parts);
-            else
-                ROPE_D(rope_bwd_fast, DM_F16, , grid, lds, a, tile, q, k, grad_q, grad_k, dq, dk, parts);
+            rope_dispatch(d, [&](auto dt, auto width, auto inter) {
+                rope_bwd_fast<decltype(dt)::value, decltype(width)::value, decltype(inter)::value != 0>
+                    <<<grid, 256, lds, st>>>(a, tile, q, k, grad_q, grad_k, dq, dk, parts);
+            });
         } else {
             nparts = bwd_workgroups(d);
             const unsigned grid = (unsigned)nparts;

@@ -20,7 +20,17 @@ CASES = [
     (F32, F32, 1, 40, 3, 1, 128, 16, True, True, "far"),
     (F32, None, 1, 33, 2, 2, 256, 128, False, False, "negative"),
     (BF, BF, 1, 1, 1, 1, 64, 8, False, False, "none"),
-    (BF, F32, 2, 31, 3, 1, 96, 48, False, False, "i32"),   # the simple kernels: widths
+    (BF, F32, 2, 31, 3, 1, 96, 48, False, False, "i32"),   # lanes without pieces
+    (F16, F16, 1, 70, 5, 2, 80, 40, False, True, "far"),
+    (BF, BF, 2, 333, 6, 3, 80, 16, True, False, "i32"),
+    (F32, F32, 1, 45, 3, 3, 80, 8, False, False, "i64"),
+    (F32, None, 2, 19, 4, 2, 96, 36, True, True, "far"),
+    (BF, BF, 1, 2300, 12, 4, 96, 16, True, False, "none"),
+    (F16, F32, 1, 61, 4, 2, 192, 96, False, False, "negative"),
+    (BF, BF, 1, 200, 5, 1, 192, 32, True, True, "i32"),
+    (F32, F32, 1, 26, 2, 1, 192, 64, False, False, "far"),
+    (F16, F32, 1, 30, 3, 2, 104, 12, True, True, "i64"),    # the simple kernels: widths
+    (BF, BF, 1, 30, 3, 2, 112, 56, False, False, "i64"),
     (F16, F32, 1, 30, 3, 2, 96, 12, True, True, "i64"),
     (F32, F32, 1, 9, 2, 1, 7, 3, False, False, "i32"),
     (BF, BF, 1, 64, 7, 3, 128, 20, False, False, "i32"),    # pairs of no whole piece
@@ -205,6 +215,10 @@ PAGED = [
     (F32, [3, 9], [0, 8], 32, 2, 1, 128, 64, False),
     (BF, [1, 4], [6, 0], 16, 3, 3, 96, 12, True),
     (BF, [1500, 1], [17, 30], 64, 4, 1, 64, 8, False),
+    (F16, [40, 3], [9, 0], 16, 4, 2, 80, 40, False),
+    (BF, [7, 21], [0, 50], 16, 4, 2, 96, 48, True),
+    (F32, [7, 21], [0, 50], 16, 2, 2, 96, 48, False),
+    (BF, [90, 5], [0, 50], 16, 6, 2, 192, 32, False),
 ]
 
 
