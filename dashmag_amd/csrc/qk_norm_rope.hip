@@ -103,27 +103,23 @@ __device__ __forceinline__ void pair_of(int e, int n, int interleaved, int *j, i
     }
 }
 
-// The simple forms, for any width, alignment and number of pairs: a wavefront takes a head, four
-// elements 64 apart in a lane, and finds a pair's other element in the wavefront's row of LDS. Bound by
-// the angles, in 64 bits for every head: 380 us forward and 856 backward on 16384 tokens of 40 heads of
-// 128 in bf16, against 63 and 106 of the kernels below.
+// The simple forms, for any width, alignment and number of pairs: a workgroup takes a token, whose angles go
+// to LDS, and a wavefront a head of it at a time (block (x, y): every gridDim.y-th four), four elements 64
+// apart in a lane, a pair's other element found in the wavefront's row of LDS. Bound by the chain of a
+// head (single elements loaded, their sum, the row, the result) that a wavefront goes through one at a time:
+// 8192 tokens of 40 heads of 112 in bf16 take 125 us forward and 270 backward (with angles for every head 183
+// and 377), where the kernels below take 27 and 41 for a width of 96.
 template <int DT, int MODE>
 __global__ __launch_bounds__(256) void rope_generic(RopeArgs a, RopePages pg, const void *__restrict__ q,
                                                     const void *__restrict__ k, const void *__restrict__ v,
                                                     void *__restrict__ qo, void *__restrict__ ko,
                                                     void *__restrict__ vo) {
     __shared__ float rows[4][256];
+    __shared__ float2 angles[128];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float *row = rows[wave];
     const int heads = a.hq + a.hkv * (MODE == kRopePaged ? 2 : 1);
-    const int64_t total = a.tokens * heads;
-    const int64_t each = (int64_t)gridDim.x * 4;
-    // (every wavefront makes the same number of rounds: the barriers below are the workgroup's)
-    for (int64_t base = (int64_t)blockIdx.x * 4; base < total; base += each) {
-        const int64_t w = base + wave;
-        const bool on = w < total;
-        const int64_t token = on ? w / heads : 0;
-        const int h = on ? (int)(w - token * heads) : 0;
+    for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
         const int64_t b = token / a.T, t = token - b * a.T;
         int64_t p, krow = -1, vrow = -1;
         bool is = true;
@@ -131,53 +127,58 @@ __global__ __launch_bounds__(256) void rope_generic(RopeArgs a, RopePages pg, co
             is = place_paged(pg, token, &p, &krow, &vrow);
         else
             p = place_plain(a, b, t);
-        if (MODE == kRopePaged && h >= a.hq + a.hkv) {  // a value head: as it is
-            const int hv = h - a.hq - a.hkv;
-            if (on && is && vrow >= 0)
-                for (int e = lane; e < a.d; e += 64)
-                    st<DT>(vo, vrow + hv * pg.v.h + e, ld<DT>(v, b * a.v.b + t * a.v.t + hv * a.v.h + e));
-        }
-        const bool isq = h < a.hq;
-        const int hh = isq ? h : h - a.hq;
-        const bool head = on && h < a.hq + a.hkv;
-        const void *src = isq ? q : k;
-        const Strd sd = isq ? a.q : a.k;
-        const void *wt = isq ? a.wq : a.wk;
-        const int64_t from = b * sd.b + t * sd.t + hh * sd.h;
-        float x[4], ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int e = lane + 64 * i;
-            x[i] = head && e < a.d ? ld<DT>(src, from + e) : 0.f;
-            ss += x[i] * x[i];
-        }
-        const float r = rsqrtf(wave_sum(ss) / a.d + a.eps);
+        __syncthreads();  // (the last token's angles have been read)
+        for (int j = threadIdx.x; j < a.n; j += 256) angles[j] = turn_of(p, a.inv_freq[j]);
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int e = lane + 64 * i;
-            const float wv = wt && e < a.d ? ld_any(a.weight_dtype, wt, e) + a.unit : 1.f;
-            x[i] *= r * wv;
-            row[e] = x[i];
-        }
-        __syncthreads();
-        if (!head || (MODE == kRopePaged && !isq && krow < 0)) continue;
-        void *dst = isq ? qo : ko;
-        const int64_t to = isq ? (token * a.hq + hh) * a.d
-                               : (MODE == kRopePaged ? krow + hh * pg.k.h : (token * a.hkv + hh) * a.d);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int e = lane + 64 * i;
-            if (e >= a.d) continue;
-            float y = x[i];
-            if (e < 2 * a.n) {
-                int j, other;
-                bool first;
-                pair_of(e, a.n, a.interleaved, &j, &other, &first);
-                const float2 cs = turn_of(p, a.inv_freq[j]);
-                y = first ? y * cs.x - row[other] * cs.y : row[other] * cs.y + y * cs.x;
+        for (int h = blockIdx.y * 4 + wave; h < heads; h += 4 * gridDim.y) {
+            if (MODE == kRopePaged && h >= a.hq + a.hkv) {  // a value head: as it is
+                const int hv = h - a.hq - a.hkv;
+                if (is && vrow >= 0)
+                    for (int e = lane; e < a.d; e += 64)
+                        st<DT>(vo, vrow + hv * pg.v.h + e, ld<DT>(v, b * a.v.b + t * a.v.t + hv * a.v.h + e));
+                continue;
             }
-            st<DT>(dst, to + e, MODE == kRopePaged && !is ? 0.f : y);
+            const bool isq = h < a.hq;
+            if (MODE == kRopePaged && !isq && krow < 0) continue;
+            const int hh = isq ? h : h - a.hq;
+            const void *src = isq ? q : k;
+            const Strd sd = isq ? a.q : a.k;
+            const void *wt = isq ? a.wq : a.wk;
+            const int64_t from = b * sd.b + t * sd.t + hh * sd.h;
+            float x[4], ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = lane + 64 * i;
+                x[i] = e < a.d ? ld<DT>(src, from + e) : 0.f;
+                ss += x[i] * x[i];
+            }
+            const float r = rsqrtf(wave_sum(ss) / a.d + a.eps);
+            __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS accesses complete in order)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = lane + 64 * i;
+                const float wv = wt && e < a.d ? ld_any(a.weight_dtype, wt, e) + a.unit : 1.f;
+                x[i] *= r * wv;
+                row[e] = x[i];
+            }
+            __builtin_amdgcn_wave_barrier();
+            void *dst = isq ? qo : ko;
+            const int64_t to = isq ? (token * a.hq + hh) * a.d
+                                   : (MODE == kRopePaged ? krow + hh * pg.k.h : (token * a.hkv + hh) * a.d);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = lane + 64 * i;
+                if (e >= a.d) continue;
+                float y = x[i];
+                if (e < 2 * a.n) {
+                    int j, other;
+                    bool first;
+                    pair_of(e, a.n, a.interleaved, &j, &other, &first);
+                    const float2 cs = angles[j];
+                    y = first ? y * cs.x - row[other] * cs.y : row[other] * cs.y + y * cs.x;
+                }
+                st<DT>(dst, to + e, MODE == kRopePaged && !is ? 0.f : y);
+            }
         }
     }
 }
@@ -191,61 +192,61 @@ __global__ __launch_bounds__(256) void rope_bwd_generic(RopeArgs a, const void *
                                                         const void *__restrict__ gk, void *__restrict__ dq,
                                                         void *__restrict__ dk, float *__restrict__ parts) {
     __shared__ float rows[4][256], sums[4][2][256];
+    __shared__ float2 angles[128];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float *row = rows[wave];
     const int heads = a.hq + a.hkv;
-    const int64_t total = a.tokens * heads;
-    const int64_t each = (int64_t)gridDim.x * 4;
     float dw[2][4] = {};
-    for (int64_t base = (int64_t)blockIdx.x * 4; base < total; base += each) {
-        const int64_t w = base + wave;
-        const bool on = w < total;
-        const int64_t token = on ? w / heads : 0;
-        const int h = on ? (int)(w - token * heads) : 0;
+    for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
         const int64_t b = token / a.T, t = token - b * a.T, p = place_plain(a, b, t);
-        const bool isq = h < a.hq;
-        const int hh = isq ? h : h - a.hq;
-        const void *src = isq ? q : k, *grad = isq ? gq : gk, *wt = isq ? a.wq : a.wk;
-        const Strd sd = isq ? a.q : a.k, sg = isq ? a.gq : a.gk;
-        const int64_t from = b * sd.b + t * sd.t + hh * sd.h, gfrom = b * sg.b + t * sg.t + hh * sg.h;
-        float x[4], z[4], ss = 0.f;
+        __syncthreads();  // (the last token's angles have been read)
+        for (int j = threadIdx.x; j < a.n; j += 256) angles[j] = turn_of(p, a.inv_freq[j]);
         __syncthreads();
+        for (int h = blockIdx.y * 4 + wave; h < heads; h += 4 * gridDim.y) {
+            const bool isq = h < a.hq;
+            const int hh = isq ? h : h - a.hq;
+            const void *src = isq ? q : k, *grad = isq ? gq : gk, *wt = isq ? a.wq : a.wk;
+            const Strd sd = isq ? a.q : a.k, sg = isq ? a.gq : a.gk;
+            const int64_t from = b * sd.b + t * sd.t + hh * sd.h, gfrom = b * sg.b + t * sg.t + hh * sg.h;
+            float x[4], z[4], ss = 0.f;
+            __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS accesses complete in order)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int e = lane + 64 * i;
-            x[i] = on && e < a.d ? ld<DT>(src, from + e) : 0.f;
-            z[i] = on && e < a.d ? ld<DT>(grad, gfrom + e) : 0.f;
-            ss += x[i] * x[i];
-            row[e] = z[i];
-        }
-        const float r = rsqrtf(wave_sum(ss) / a.d + a.eps);
-        __syncthreads();
-        float gx = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int e = lane + 64 * i;
-            if (e < 2 * a.n) {
-                int j, other;
-                bool first;
-                pair_of(e, a.n, a.interleaved, &j, &other, &first);
-                const float2 cs = turn_of(p, a.inv_freq[j]);
-                z[i] = first ? z[i] * cs.x + row[other] * cs.y : z[i] * cs.x - row[other] * cs.y;
+            for (int i = 0; i < 4; i++) {
+                const int e = lane + 64 * i;
+                x[i] = e < a.d ? ld<DT>(src, from + e) : 0.f;
+                z[i] = e < a.d ? ld<DT>(grad, gfrom + e) : 0.f;
+                ss += x[i] * x[i];
+                row[e] = z[i];
             }
-            const float add = on ? z[i] * (x[i] * r) : 0.f;
-            if (isq)
-                dw[0][i] += add;
-            else
-                dw[1][i] += add;
-            z[i] *= wt && e < a.d ? ld_any(a.weight_dtype, wt, e) + a.unit : 1.f;
-            gx += z[i] * (x[i] * r);
-        }
-        const float mean = wave_sum(gx) / a.d;
-        void *dst = isq ? dq : dk;
-        const int64_t to = (token * (isq ? a.hq : a.hkv) + hh) * a.d;
+            const float r = rsqrtf(wave_sum(ss) / a.d + a.eps);
+            __builtin_amdgcn_wave_barrier();
+            float gx = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int e = lane + 64 * i;
-            if (on && e < a.d) st<DT>(dst, to + e, r * (z[i] - x[i] * r * mean));
+            for (int i = 0; i < 4; i++) {
+                const int e = lane + 64 * i;
+                if (e < 2 * a.n) {
+                    int j, other;
+                    bool first;
+                    pair_of(e, a.n, a.interleaved, &j, &other, &first);
+                    const float2 cs = angles[j];
+                    z[i] = first ? z[i] * cs.x + row[other] * cs.y : z[i] * cs.x - row[other] * cs.y;
+                }
+                const float add = z[i] * (x[i] * r);
+                if (isq)
+                    dw[0][i] += add;
+                else
+                    dw[1][i] += add;
+                z[i] *= wt && e < a.d ? ld_any(a.weight_dtype, wt, e) + a.unit : 1.f;
+                gx += z[i] * (x[i] * r);
+            }
+            const float mean = wave_sum(gx) / a.d;
+            void *dst = isq ? dq : dk;
+            const int64_t to = (token * (isq ? a.hq : a.hkv) + hh) * a.d;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = lane + 64 * i;
+                if (e < a.d) st<DT>(dst, to + e, r * (z[i] - x[i] * r * mean));
+            }
         }
     }
 #pragma unroll
@@ -253,10 +254,10 @@ __global__ __launch_bounds__(256) void rope_bwd_generic(RopeArgs a, const void *
 #pragma unroll
         for (int i = 0; i < 4; i++) sums[wave][x][lane + 64 * i] = dw[x][i];
     __syncthreads();
+    const int64_t part = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     for (int e = threadIdx.x; e < 2 * a.d; e += 256) {
         const int x = e / a.d, c = e - x * a.d;
-        parts[(int64_t)blockIdx.x * 2 * a.d + e] =
-            (sums[0][x][c] + sums[1][x][c]) + (sums[2][x][c] + sums[3][x][c]);
+        parts[part * 2 * a.d + e] = (sums[0][x][c] + sums[1][x][c]) + (sums[2][x][c] + sums[3][x][c]);
     }
 }
 
@@ -265,8 +266,7 @@ __global__ __launch_bounds__(256) void rope_bwd_generic(RopeArgs a, const void *
 // or of adjacent ones (interleaved); past the rotated 2 n the rest of the head in the same manner. So a
 // pair never leaves its lane, and a head's sums are moves within 16 lanes (32 in f32). Lanes come in powers
 // of two: of a head of 96 two of eight are idle, with values of 0. (8192 tokens of 40 heads in bf16,
-// replayed, forward and backward: 80 wide 27 and 39 us, 96 27 and 41, 192 51 and 87; 112, by the simple
-// kernels, 184 and 376.)
+// replayed, forward and backward: 80 wide 27 and 39 us, 96 27 and 41, 192 51 and 85.)
 //
 // A workgroup takes `tile` tokens: the angles of all of them go to LDS first, one a thread, since every
 // head of a token turns by the same ones, then its lanes go through the tokens' heads.
@@ -642,9 +642,11 @@ __global__ __launch_bounds__(1024) void rope_weights(const float *__restrict__ p
 // of 256: 49.0, 49.0, 53.9.)
 constexpr int64_t kRopeParts = 768;
 
-static int64_t bwd_workgroups(const dm_qk_norm_rope_desc *d) {
-    const int64_t tokens = d->b * d->t;
-    return std::max<int64_t>(1, std::min(tokens, kRopeParts));
+// The simple kernels' grid: a workgroup a token up to `most`, and where those are few the tokens' heads, four a
+// workgroup, shared out too.
+static dim3 generic_grid(int64_t tokens, int64_t heads, int64_t most) {
+    const int64_t x = std::max<int64_t>(1, std::min(tokens, most));
+    return dim3((unsigned)x, (unsigned)std::max<int64_t>(1, std::min((heads + 3) / 4, most / x)));
 }
 
 static Strd strd(const dm_strides &s) { return Strd{s.b, s.t, s.h}; }
@@ -756,8 +758,7 @@ static int run_rope(const char *op, const dm_qk_norm_rope_desc *d, const RopeArg
                 <<<grid, 256, lds, st>>>(a, pg, tile, q, k, v, qo, ko, vo);
         });
     } else {
-        const int64_t rows = a.tokens * (a.hq + a.hkv * (paged ? 2 : 1));
-        const unsigned grid = (unsigned)std::min<int64_t>((rows + 3) / 4, 16384);
+        const dim3 grid = generic_grid(a.tokens, a.hq + a.hkv * (paged ? 2 : 1), kRopeGrid);
         if (d->dtype == DM_F32)
             rope_generic<DM_F32, MODE><<<grid, 256, 0, st>>>(a, pg, q, k, v, qo, ko, vo);
         else if (d->dtype == DM_BF16)
@@ -816,8 +817,8 @@ int dm_qk_norm_rope_bwd(const dm_qk_norm_rope_desc *d, const void *q, const void
                     <<<grid, 256, lds, st>>>(a, tile, q, k, grad_q, grad_k, dq, dk, parts);
             });
         } else {
-            nparts = bwd_workgroups(d);
-            const unsigned grid = (unsigned)nparts;
+            const dim3 grid = generic_grid(a.tokens, a.hq + a.hkv, kRopeParts);
+            nparts = (int64_t)grid.x * grid.y;
             if (d->dtype == DM_F32)
                 rope_bwd_generic<DM_F32><<<grid, 256, 0, st>>>(a, q, k, grad_q, grad_k, dq, dk, parts);
             else if (d->dtype == DM_BF16)
