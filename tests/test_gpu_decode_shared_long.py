@@ -1,0 +1,142 @@
+"""The decode over shared prefixes on its long paths and in groups of many rows, against the 64-bit
+softmax of each row (shared_cases.py): ranges of keys past what a kernel looks up at once, the checks of
+groups, pages, views and captured calls in groups of many rows.
+
+A call's ranges follow from the number of its tiles, so each long batch has enough short groups or rows
+beside the long one that its keys are one range."""
+import pytest
+import torch
+
+import dashmag_amd as dm
+from rope_cases import held
+from shared_cases import Batch
+
+pytestmark = pytest.mark.gpu
+
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _options(window):
+    return dm.AttentionOptions(window=None if window is None else dm.Window(window, 0))
+
+
+def _checked(b, window=None):
+    out = dm.attention_decode_shared(*b.cuda(), _options(window))
+    assert torch.equal(out, dm.attention_decode_shared(*b.cuda(), _options(window)))
+    held("out", out, *b.want())
+
+
+def _beside(long, groups, members):
+    """The group ``long`` and short ones of ``members`` rows behind it."""
+    n = len(long[1])
+    return [long] + [(n + members * i, [5 + (i + j) % 13 for j in range(members)], 4) for i in range(groups)]
+
+
+# 120 (at D = 256: 136) tiles and one range of 16700 keys: 261 tiles of 64 keys, two rounds of the 128 whose
+# pages a workgroup holds. With the window a range of 14 tiles fewer that begins inside a page.
+@pytest.mark.parametrize("window", [None, 15800])
+@pytest.mark.parametrize("dtype,d,hkv,short", [(BF, 128, 8, 12), (F16, 64, 8, 12), (BF, 256, 4, 24)], ids=str)
+def test_long_prefixes_of_groups_of_many_rows(dtype, d, hkv, short, window):
+    groups = _beside((0, [16750, 16701, 9001], 16700), short, 3)
+    b = Batch(dtype, d, hkv, 16, 16, groups, {}, 3 + 3 * short, seed=d, window=window)
+    _checked(b, window)
+
+
+# 124 tiles and one range of 9000 keys: four wavefronts of 2250, whose pages are looked up for 1024 at a time.
+@pytest.mark.parametrize("window", [None, 8000])
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F16, 64), (BF, 256)], ids=str)
+def test_long_prefixes_of_groups_of_few_rows(dtype, d, window):
+    groups = _beside((0, [9040, 9001], 9000), 25, 2)
+    b = Batch(dtype, d, 4, 4, 16, groups, {}, 52, seed=d, window=window)
+    _checked(b, window)
+
+
+# 1040 tiles of own keys, so one range a row, a wavefront's: 5000 and 2049 keys. As rows of no group, and
+# (many) beside a group of many rows.
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F16, 64), (BF, 256)], ids=str)
+def test_long_own_keys(dtype, d, many):
+    lone = {r: r % 4 for r in range(80 if many else 0, 260)}
+    lone[100], lone[259] = 5000, 2049
+    groups = [(0, [40 + r % 5 for r in range(80)], 37)] if many else []
+    b = Batch(dtype, d, 4, 4, 16, groups, lone, 260, seed=d)
+    _checked(b)
+
+
+def test_groups_of_many_rows_with_bad_groups():
+    """Groups that do not go up within the batch share nothing, in a call that is planned for many rows."""
+    rows = 70
+    b = Batch(BF, 128, 2, 4, 16, [(0, [513 + 7 * (i % 5) for i in range(rows)], 512)], {}, rows, seed=2)
+    q, k, v, table, ln, cu, pl = b.cuda()
+    want = b.want()
+    for bad in ([3, 1], [-1, 2], [0, rows + 1], [rows, 0], [1 << 30, 1 << 30]):
+        at = torch.tensor(bad, dtype=torch.int32).cuda()
+        held(f"groups {bad}", dm.attention_decode_shared(q, k, v, table, ln, at, pl), *want)
+    held("negative prefix", dm.attention_decode_shared(q, k, v, table, ln, cu, -pl), *want)
+    held("a longer prefix than the table", dm.attention_decode_shared(q, k, v, table[:1].expand(rows, -1), ln[:1].expand(rows),
+                                                                      cu, pl + (1 << 30))[:1], want[0][:1], want[1][:1])
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F16, 64), (BF, 256)], ids=str)
+def test_groups_of_many_rows_with_pages_outside(dtype, d):
+    """A page index outside the pages is a page of zeros, in the prefix of many rows and behind it."""
+    rows = 44
+    b = Batch(dtype, d, 2, 4, 16, [(0, [600 + i for i in range(rows)], 592)], {}, rows, seed=5)
+    q, k, v, table, *rest = b.cuda()
+    table[:, 3], table[:, 36], table[7, 37] = 1 << 20, -5, 1 << 30
+    for r in range(rows):
+        for c in (3, 36, 37) if r == 7 else (3, 36):
+            for x in b.keys[r][:2]:
+                x[16 * c:16 * c + 16] = 0
+    held("out", dm.attention_decode_shared(q, k, v, table, *rest), *b.want())
+
+
+def test_groups_of_many_rows_in_views():
+    """Queries of a wider row, keys and values of one pool, heads ahead of the page's rows: the bits of the
+    contiguous call."""
+    rows = 70
+    b = Batch(BF, 128, 2, 4, 16, [(0, [513 + 7 * (i % 5) for i in range(rows)], 512)], {}, rows, seed=3)
+    q, k, v, *rest = b.cuda()
+    want = dm.attention_decode_shared(q, k, v, *rest)
+    held("contiguous", want, *b.want())
+    wide = torch.cat([q, q, q], 1)[:, 8:16]
+    both = torch.stack([k, v], 1)
+    ahead = both.transpose(2, 3).contiguous()
+    assert torch.equal(dm.attention_decode_shared(wide, both[:, 0], both[:, 1], *rest), want)
+    assert torch.equal(dm.attention_decode_shared(q, ahead[:, 0].transpose(1, 2), ahead[:, 1].transpose(1, 2), *rest), want)
+
+
+@pytest.mark.parametrize("dtype,d,groups,rows", [
+    (BF, 128, [(0, [1500 + 3 * i for i in range(66)], 1481)], 66),          # many rows
+    (BF, 256, [(0, [900 + 3 * i for i in range(40)], 887)], 40),
+    (BF, 128, [(1, [300], 256), (2, [90, 700, 91, 95, 400, 89], 89)], 9),   # few
+    (F32, 64, [(0, [200, 190, 313], 180)], 3)], ids=str)
+def test_a_captured_call_follows_its_lengths(dtype, d, groups, rows):
+    """Lengths that move on between the replays, to shorter rows and to none, and the prefixes and groups
+    with them: each replay has the eager call's bits and the 64-bit result of these lengths."""
+    b = Batch(dtype, d, 2, 4, 16, groups, {}, rows, seed=2)
+    q, k, v, table, ln, cu, pl = b.cuda()
+    call = lambda: dm.attention_decode_shared(q, k, v, table, ln, cu, pl)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    full = b.keys
+    for i, (cut, first) in enumerate(((0, -1), (37, 0), (0, -1), (150, 2))):
+        # every row `cut` keys shorter, row `first` without any
+        lens = [0 if r == first else max(0, len(x[0]) - cut) for r, x in enumerate(full)]
+        b.keys = [(x[0][:n], x[1][:n], 0) for x, n in zip(full, lens)]
+        ln.copy_(torch.tensor(lens, dtype=torch.int32))
+        if i == 3:
+            cu.zero_()
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, call()), i
+        held(f"replay {i}", got, *b.want())
