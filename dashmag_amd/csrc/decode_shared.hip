@@ -240,7 +240,8 @@ __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const
         }
 #pragma unroll
         for (int o = 4; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-        const float mn = fmaxf(m, mx);
+        // (while every score that the row has seen is -inf, their weights are 0 and not e^(-inf + inf))
+        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
         const float alpha = mn == -INFINITY ? 1.f : expf(m - mn);
         m = mn;
         l *= alpha;
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const
             // (a masked key's weight is a marker below zero: what its value holds stays out)
             const int64_t j = j0 + c + 8 * u;
             const bool seen = j >= low && j < high;
-            const float p = seen ? expf(s[u] - mn) : 0.f;
+            const float p = seen ? expf(s[u] - ref) : 0.f;
             ps[r][c + 8 * u] = seen ? p : -1.f;
             l += p;
         }

@@ -1,6 +1,6 @@
 """The decode over shared prefixes on its long paths and in groups of many rows, against the 64-bit
 softmax of each row (shared_cases.py): ranges of keys past what a kernel looks up at once, the checks of
-groups, pages, views and captured calls in groups of many rows.
+groups, pages, views and captured calls in groups of many rows, scores of minus infinity.
 
 A call's ranges follow from the number of its tiles, so each long batch has enough short groups or rows
 beside the long one that its keys are one range."""
@@ -140,3 +140,28 @@ def test_a_captured_call_follows_its_lengths(dtype, d, groups, rows):
         got = out.clone()
         assert torch.equal(got, call()), i
         held(f"replay {i}", got, *b.want())
+
+
+# ------------------------------------------------------------------------------------------
+# Scores of minus infinity
+# ------------------------------------------------------------------------------------------
+
+ALL = [(BF, 128, 16), (F16, 64, 16), (BF, 256, 16), (F32, 64, 16), (BF, 96, 16), (BF, 128, 7)]
+
+
+@pytest.mark.parametrize("rows", [3, 60])
+@pytest.mark.parametrize("dtype,d,page", ALL, ids=str)
+def test_keys_of_minus_infinity_have_no_weight(dtype, d, page, rows):
+    """Keys that a program has switched off with an element of minus infinity (the queries' are above 0
+    there), the first ones of the prefix and the first ones behind it: the row's result is that of its other keys."""
+    p = 592
+    b = Batch(dtype, d, 1, 4, page, [(0, [p + 70 + i for i in range(rows)], p)], {}, rows, seed=4)
+    b.q[:, :, 2] = b.q[:, :, 2].abs() + 0.125
+    off = list(range(0, 150)) + list(range(p, p + 40))
+    for r in range(rows):
+        for j in off:
+            b.k[int(b.table[r, j // page]), j % page, 0, 2] = -float("inf")
+    on = torch.ones(p + 70 + rows, dtype=torch.bool)
+    on[off] = False
+    b.keys = [(k[on[:len(k)]], v[on[:len(v)]], 0) for k, v, _ in b.keys]
+    held("out", dm.attention_decode_shared(*b.cuda()), *b.want())
