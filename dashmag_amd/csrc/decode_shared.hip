@@ -250,10 +250,10 @@ __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const
             // (a masked key's weight is a marker below zero: what its value holds stays out)
             const int64_t j = j0 + c + 8 * u;
             const bool seen = j >= low && j < high;
-            const float p = seen ? expf(s[u] - ref) : 0.f;
-            ps[r][c + 8 * u] = seen ? p : -1.f;
-            l += p;
+            s[u] = seen ? expf(s[u] - ref) : 0.f;
+            ps[r][c + 8 * u] = seen ? s[u] : -1.f;
         }
+        l += s[0] + s[1];
         __syncthreads();
         for (int i = tid; i < n * a.d; i += 256) {
             const int x = i / a.d, e = i - x * a.d;
@@ -261,14 +261,18 @@ __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const
             kv[x][e] = pg >= 0 ? ld<DT>(v, pg * a.vb + (j0 + x) % a.page_size * a.vt + it.kh * a.vh + e) : 0.f;
         }
         __syncthreads();
+        // (the step's 16 products first: with one addition a key a sum over 2^14 keys of like weights is off by
+        // as much as 2^-12)
+        float w[kGenKeys];
 #pragma unroll
-        for (int i = 0; i < 32; i++) acc[i] *= alpha;
-        for (int x = 0; x < n; x++) {
-            const float p = ps[r][x];
-            if (p < 0.f) continue;
+        for (int x = 0; x < kGenKeys; x++) w[x] = ps[r][x];
 #pragma unroll
-            for (int i = 0; i < 32; i++)
-                if (c + 8 * i < a.d) acc[i] += p * kv[x][c + 8 * i];
+        for (int i = 0; i < 32; i++) {
+            if (c + 8 * i >= a.d) continue;
+            float t = 0.f;
+#pragma unroll
+            for (int x = 0; x < kGenKeys; x++) t += w[x] < 0.f ? 0.f : w[x] * kv[x][c + 8 * i];
+            acc[i] = acc[i] * alpha + t;
         }
     }
 #pragma unroll

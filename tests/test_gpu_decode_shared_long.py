@@ -1,6 +1,6 @@
 """The decode over shared prefixes on its long paths and in groups of many rows, against the 64-bit
 softmax of each row (shared_cases.py): ranges of keys past what a kernel looks up at once, the checks of
-groups, pages, views and captured calls in groups of many rows, scores of minus infinity.
+groups, pages, views and captured calls in groups of many rows, scores of minus infinity, long sums.
 
 A call's ranges follow from the number of its tiles, so each long batch has enough short groups or rows
 beside the long one that its keys are one range."""
@@ -9,7 +9,7 @@ import torch
 
 import dashmag_amd as dm
 from rope_cases import held
-from shared_cases import Batch
+from shared_cases import U, Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -165,3 +165,53 @@ def test_keys_of_minus_infinity_have_no_weight(dtype, d, page, rows):
     on[off] = False
     b.keys = [(k[on[:len(k)]], v[on[:len(v)]], 0) for k, v, _ in b.keys]
     held("out", dm.attention_decode_shared(*b.cuda()), *b.want())
+
+
+# ------------------------------------------------------------------------------------------
+# Sums over many keys
+# ------------------------------------------------------------------------------------------
+#
+# A key of score `scale`, then n - 1 of score 0: all weights but the first are w = e^-scale, so that every
+# addition to a sum of them is off to the same side. Rounded sums of equal positive terms are off by at most
+# u / 2 times their number of additions (the sum grows evenly), u = 2^-24.
+
+def _equal_keys(dtype, d, n, w, values, rows, groups, rep):
+    """Row 0 has n such keys, in its own pages if groups is None and as the prefix of a group otherwise; the
+    other rows have one key. Returns (arrays, options, the result of row 0 in 64 bits)."""
+    page = 16
+    k, v = (torch.zeros(n // page + 1, page, 1, d, dtype=dtype, device="cuda") for _ in range(2))
+    k[0, 0, 0, 0] = 1.0
+    v[:] = values.to(dtype).cuda()
+    table = torch.full((rows, n // page), -1, dtype=torch.int32, device="cuda")
+    table[0] = torch.arange(n // page, dtype=torch.int32)
+    table[1:, 0] = n // page
+    lengths = torch.ones(rows, dtype=torch.int32, device="cuda")
+    lengths[0] = n
+    q = torch.zeros(rows, rep, d, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1.0
+    if groups:
+        cu = torch.arange(rows + 1, dtype=torch.int32, device="cuda")
+        pl = torch.ones(rows, dtype=torch.int32, device="cuda")
+        pl[0] = n
+    else:
+        cu, pl = (torch.zeros(i, dtype=torch.int32, device="cuda") for i in (1, 0))
+    scale = float(-torch.log(torch.tensor(w, dtype=torch.float64)))
+    return (q, k, v, table, lengths, cu, pl), dm.AttentionOptions(scale=scale), v[0, 0, 0].double().cpu()
+
+
+def _sum_held(args, opts, want, bound):
+    out = dm.attention_decode_shared(*args, opts)[0].flatten(0, -2)
+    held("row 0", out, want.expand_as(out), bound * want.abs().expand_as(out))
+
+
+@pytest.mark.parametrize("groups", [True, False])
+@pytest.mark.parametrize("dtype,d", [(F32, 64), (F32, 36), (BF, 96)], ids=str)
+def test_sums_of_the_simple_form(dtype, d, groups):
+    """2^14 keys in one range (520 tiles), 16 of them at a time. Off by: the sums of 16 keys' products and n / 16
+    additions of those; the weights' sums, each of 8 threads' n / 16 additions of two; 128 u for the scores, the
+    weights and the rest. (A result in bf16 is rounded once: the weights stay in f32 here.) With one addition a key
+    the products' sums in f32 are 2.3e-4 short: a column's terms are a whole number and 0.49 of a step of them."""
+    n, w = 1 << 14, 0.992
+    values = (1000.49 + torch.arange(d, dtype=torch.float64)) / 1024 / w
+    args = _equal_keys(dtype, d, n, w, values, 520, groups, 1)
+    _sum_held(*args, (n / 32 + n / 32 + 128) * U)
