@@ -822,6 +822,7 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
                 for (int i = 0; i < 16; i++) p.acc[dt][i] *= alpha;
         }
         const float mneg = p.m == -INFINITY ? 0.f : -p.m;
+        float ps = 0.f;  // (the tile's weights first: one at a time 2^19 like ones were summed 2^-8 short)
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -830,11 +831,12 @@ __device__ __forceinline__ void shared_wide(const SharedArgs &a, const SharedIte
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     e[i] = fast_exp2(fmaf(s[t][8 * u + i], c2, mneg));
-                    p.l += e[i];
+                    ps += e[i];
                 }
                 pf[t][u].u = make_uint4(pack2<DT>(e[0], e[1]), pack2<DT>(e[2], e[3]), pack2<DT>(e[4], e[5]),
                                         pack2<DT>(e[6], e[7]));
             }
+        p.l += ps;
     };
     // Wavefronts 0-3 store K_{j+1} and V_j during their softmax of step j, wavefronts 4-7, half a step
     // later, K_{j+2} and V_{j+1}: each tile is whole before its first reader's step.

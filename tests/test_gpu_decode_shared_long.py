@@ -204,6 +204,16 @@ def _sum_held(args, opts, want, bound):
     held("row 0", out, want.expand_as(out), bound * want.abs().expand_as(out))
 
 
+def test_sums_of_a_long_prefix_of_many_rows():
+    """2^19 keys in one range (100 groups, 115 tiles). Off by: the weights' rounding for the products, half a
+    step; the products' sums over 16 keys a time, n / 16 additions; the weights' sum, in which a lane takes
+    32 keys of a tile (at most 32 u) and n / 64 tiles; 64 u for the rest. w is 63.49 steps of a sum between 2^17 and 2^18: added
+    one at a time the weights' sum is 0.4% short."""
+    n = 1 << 19
+    args = _equal_keys(F16, 64, n, 63.49 / 64, torch.ones(64), 100, True, 40)
+    _sum_held(*args, 2.0 ** -11 + (n / 32 + n / 128 + 96) * U)
+
+
 @pytest.mark.parametrize("groups", [True, False])
 @pytest.mark.parametrize("dtype,d", [(F32, 64), (F32, 36), (BF, 96)], ids=str)
 def test_sums_of_the_simple_form(dtype, d, groups):
