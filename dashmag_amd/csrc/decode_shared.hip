@@ -917,8 +917,9 @@ __global__ __launch_bounds__((64 * shared_waves<D, WIDE>()), (D == 256 ? 1 : 2))
 }
 
 // The ranges of a row joined, a workgroup a row: the ranges that hold keys are listed with their
-// weights, and thread t sums, for the columns of its piece t % pieces (four of them where D is a multiple of
-// 4, one otherwise), every groups-th of the list, eight loads in flight; the groups are added in order.
+// weights (those of weight 0 too: zero times a result that is not finite is NaN), and thread t sums, for
+// the columns of its piece t % pieces (four of them where D is a multiple of 4, one otherwise), every
+// groups-th of the list, eight loads in flight; the groups are added in order.
 constexpr int kSharedSplits = 512;  // most ranges of a row
 template <int DT, int V>
 __global__ __launch_bounds__(256) void decode_shared_merge(SharedArgs a, void *__restrict__ o) {
@@ -935,7 +936,8 @@ __global__ __launch_bounds__(256) void decode_shared_merge(SharedArgs a, void *_
     auto weight = [&](float x) { return x == -INFINITY ? 0.f : (x == top ? 1.f : expf(x - top)); };
     const float w0 = weight(x0), w1 = weight(x1);
     const float part = wave_sum(w0 + w1);
-    const unsigned long long b0 = __ballot(w0 != 0.f), b1 = __ballot(w1 != 0.f);
+    const bool has0 = x0 != -INFINITY, has1 = x1 != -INFINITY;
+    const unsigned long long b0 = __ballot(has0), b1 = __ballot(has1);
     if (lane == 0) sums[wave] = part, counts[wave] = __popcll(b0) + __popcll(b1);
     __syncthreads();
     const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
@@ -945,11 +947,11 @@ __global__ __launch_bounds__(256) void decode_shared_merge(SharedArgs a, void *_
         m += counts[i];
     }
     const unsigned long long below = ((unsigned long long)1 << lane) - 1;
-    if (w0 != 0.f) {
+    if (has0) {
         const int i = at + __popcll(b0 & below);
         list[i] = tid, w[i] = w0;
     }
-    if (w1 != 0.f) {
+    if (has1) {
         const int i = at + __popcll(b0) + __popcll(b1 & below);
         list[i] = tid + 256, w[i] = w1;
     }
@@ -973,7 +975,7 @@ __global__ __launch_bounds__(256) void decode_shared_merge(SharedArgs a, void *_
 #pragma unroll
             for (int u = 0; u < 8; u++)
 #pragma unroll
-                for (int c = 0; c < V; c++) acc[c] += f[u] != 0.f ? f[u] * x[u][c] : 0.f;
+                for (int c = 0; c < V; c++) acc[c] += i + u * groups < m ? f[u] * x[u][c] : 0.f;
         }
     }
 #pragma unroll
@@ -1005,9 +1007,9 @@ __global__ __launch_bounds__(256) void decode_shared_merge_few(SharedArgs a, int
     const float top = wave_max(x);
     const float f = x == -INFINITY ? 0.f : (x == top ? 1.f : expf(x - top));
     const float sum = wave_sum(f);
-    const unsigned long long has = __ballot(f != 0.f);
+    const unsigned long long has = __ballot(x != -INFINITY);
     const int m = __popcll(has);
-    if (f != 0.f) {
+    if (x != -INFINITY) {
         const int i = __popcll(has & (((unsigned long long)1 << lane) - 1));
         list[wave][i] = lane, w[wave][i] = f;
     }
@@ -1027,7 +1029,7 @@ __global__ __launch_bounds__(256) void decode_shared_merge_few(SharedArgs a, int
             }
 #pragma unroll
             for (int u = 0; u < 8; u++) {
-                const bool on = fu[u] != 0.f;
+                const bool on = i + u * groups < m;
                 acc.x += on ? fu[u] * y[u].x : 0.f, acc.y += on ? fu[u] * y[u].y : 0.f;
                 acc.z += on ? fu[u] * y[u].z : 0.f, acc.w += on ? fu[u] * y[u].w : 0.f;
             }

@@ -1,6 +1,7 @@
 """The decode over shared prefixes on its long paths and in groups of many rows, against the 64-bit
 softmax of each row (shared_cases.py): ranges of keys past what a kernel looks up at once, the checks of
-groups, pages, views and captured calls in groups of many rows, scores of minus infinity, long sums.
+groups, pages, views and captured calls in groups of many rows, scores of minus infinity,
+values that are not finite, long sums.
 
 A call's ranges follow from the number of its tiles, so each long batch has enough short groups or rows
 beside the long one that its keys are one range."""
@@ -143,7 +144,7 @@ def test_a_captured_call_follows_its_lengths(dtype, d, groups, rows):
 
 
 # ------------------------------------------------------------------------------------------
-# Scores of minus infinity
+# Scores of minus infinity, values that are not finite
 # ------------------------------------------------------------------------------------------
 
 ALL = [(BF, 128, 16), (F16, 64, 16), (BF, 256, 16), (F32, 64, 16), (BF, 96, 16), (BF, 128, 7)]
@@ -165,6 +166,33 @@ def test_keys_of_minus_infinity_have_no_weight(dtype, d, page, rows):
     on[off] = False
     b.keys = [(k[on[:len(k)]], v[on[:len(v)]], 0) for k, v, _ in b.keys]
     held("out", dm.attention_decode_shared(*b.cuda()), *b.want())
+
+
+@pytest.mark.parametrize("rows", [3, 60])
+@pytest.mark.parametrize("dtype,d,page", ALL, ids=str)
+def test_a_value_that_is_not_finite_reaches_the_rows_that_see_it(dtype, d, page, rows):
+    """Whatever its key's weight: e^-400 of the others' here, 0 in 32 bits, and zero times NaN is NaN. The row's
+    other columns and the other rows are what they were."""
+    lens = [2000 + i for i in range(rows)]
+    b = Batch(dtype, d, 1, 4, page, [(0, lens, 1000)], {}, rows, seed=6)
+    b.q[:, :, 0] = 40.0
+    for k, _, _ in b.keys:
+        k[:, :, 0] = 0.0
+    b.k[:, :, :, 0] = torch.where(torch.isnan(b.k[:, :, :, 0].float()), b.k[:, :, :, 0], torch.zeros((), dtype=dtype))
+    opts = dm.AttentionOptions(scale=1.0)
+    b.q[:, :, 1:] *= 0.1
+    for r in (1, 2):  # whole ranges of such keys
+        for j in range(1400, lens[r]):
+            b.k[int(b.table[r, j // page]), j % page, 0, 0] = -10.0
+        b.keys[r][0][1400:, :, 0] = -10.0
+    want, bound = b.want(1.0)
+    b.v[int(b.table[1, 1990 // page]), 1990 % page, 0, 3] = float("nan")
+    b.v[int(b.table[2, 1500 // page]), 1500 % page, 0, 5] = float("nan")
+    out = dm.attention_decode_shared(*b.cuda(), opts)
+    assert torch.isnan(out[1, :, 3]).all() and torch.isnan(out[2, :, 5]).all()
+    keep = torch.ones(out.shape, dtype=torch.bool)
+    keep[1, :, 3] = keep[2, :, 5] = False
+    held("others", out[keep.cuda()], want[keep], bound[keep])
 
 
 # ------------------------------------------------------------------------------------------
