@@ -1,6 +1,6 @@
 """The decode over shared prefixes on its long paths and in groups of many rows, against the 64-bit
 softmax of each row (shared_cases.py): ranges of keys past what a kernel looks up at once, the checks of
-groups, pages, views and captured calls in groups of many rows, scores of minus infinity,
+groups, pages, views and captured calls in groups of many rows, odd widths, scores of minus infinity,
 values that are not finite, long sums.
 
 A call's ranges follow from the number of its tiles, so each long batch has enough short groups or rows
@@ -62,6 +62,13 @@ def test_long_own_keys(dtype, d, many):
     groups = [(0, [40 + r % 5 for r in range(80)], 37)] if many else []
     b = Batch(dtype, d, 4, 4, 16, groups, lone, 260, seed=d)
     _checked(b)
+
+
+@pytest.mark.parametrize("dtype,d,hkv,rep,page", [(F32, 7, 2, 3, 5), (BF, 50, 1, 2, 16), (F16, 249, 1, 40, 16), (BF, 1, 2, 2, 16)],
+                         ids=str)
+def test_widths_that_are_no_multiple_of_four(dtype, d, hkv, rep, page):
+    groups = [(1, [300], 256), (2, [90, 700, 91, 95, 400, 89], 89), (8, [2000, 1999], 1990)]
+    _checked(Batch(dtype, d, hkv, rep, page, groups, {0: 33, 10: 17, 11: 0}, 13, seed=d))
 
 
 def test_groups_of_many_rows_with_bad_groups():
