@@ -492,7 +492,6 @@ __device__ __forceinline__ void put_rows(const SharedArgs &a, const SharedItem &
                             p.acc[dt][g4 * 4 + 3] * inv);
     __builtin_amdgcn_wave_barrier();
     if (half == 0 && col < n) a.part_lse[part] = l == 0.f ? -INFINITY : (p.m + log2f(l)) * 0.6931471805599453f;
-#pragma unroll 4
     for (int r = 0; r < n; r += RPL) {
         const int x = r + lane / LPR, y = min(x, 31);
         const int64_t to = ((int64_t)__shfl((int)(part >> 32), y, 64) << 32) | (uint32_t)__shfl((int)part, y, 64);
