@@ -13,9 +13,11 @@
 //
 // Measured in bf16, with the merge, MFMA rates counting 4 D a (row, key) pair (a large product on this card
 // runs at 1240 TFLOP/s, a large copy at 5.0 TB/s):
-//   256 rows, a prefix of 32768 keys, 512 of their own, 32 heads of 128 over 8: 220 us, 630 TFLOP/s. Bound by
-//     the prefix's products: alone they reach 670 TFLOP/s on 192 compute units and 725 on all 256, where the
-//     clock falls; a 64-key step of 256 rows takes 3900 cycles, 2060 of them MFMA issue.
+//   256 rows, a prefix of 32768 keys, 512 of their own, 32 heads of 128 over 8: 197 us, 707 TFLOP/s. Bound by
+//     the prefix's products: alone they take 394 thousand cycles on 192 compute units (184 us at 2.14 GHz) and
+//     313 thousand on all 256 (154 us at 2.03 GHz, 893 TFLOP/s), the cycles of the attention forward for as many
+//     products (323 thousand); after some launches back to back the clock falls and they take 200 and 174 us. A
+//     64-key step of 256 rows takes 3900 cycles, 2060 of them MFMA issue.
 //   64 rows, 16384 and 1024 keys, the same heads: 75 us: 216 MB, 43 us at a copy's rate, and about 6 us until
 //     the first keys arrive (the groups, the lengths, the page, the keys: each waits for the one in front).
 //   8 rows, 6144 and 200 keys, 8 heads of 256 over 2: 20 us; 45 rows in 5 groups, 16 heads of 64 over 2 in f16,
@@ -190,8 +192,9 @@ __device__ __forceinline__ bool range_of(const SharedArgs &a, int unit, bool wri
 
 // The simple form, for every type, head width, page size and stride: 32 rows and 16 keys at a time in
 // LDS as f32, eight threads a row, each two of its scores and every eighth column of its output. Bound by
-// its LDS reads, two for a multiply-add: 256 bf16 rows of 32768 + 512 keys, 32 heads of 128, take 21 ms
-// here against 0.22 below.
+// its LDS reads, two for a multiply-add of the scores and one of the outputs: 256 bf16 rows of 32768 + 512
+// keys, 32 heads of 128, in pages of 8 take 26.7 ms here, in pages of 16 0.2 below. (64 rows of 4096 + 256 keys,
+// 32 heads over 8: f32 128 wide 0.85 ms, bf16 96 wide 0.67; row by row the paged decode takes 4.9 and 6.2.)
 constexpr int kGenKeys = 16;
 template <int DT>
 __global__ __launch_bounds__(256) void decode_shared_generic(SharedArgs a, const void *__restrict__ q,
@@ -1070,8 +1073,10 @@ static bool shared_mfma_takes(const dm_attention_desc *d, int64_t page_size) {
 //
 // A prefix's item is a workgroup: about kPrefixItems of them, so that some compute units are left to the rows'
 // own keys meanwhile (one reads, the other multiplies). (256 rows, 32768 + 512 keys and 64 rows, 16384 + 1024:
-// 160 236 and 73 us, 192 222 and 75, 224 239 and 77, 256 239 and 80.) A row's own item is a wavefront (the
-// generic kernel: a workgroup): about kOwnItems of them. (1024: 227 and 91 us; the small calls are alike.) No
+// 96 304 and 65 us, 128 238 and 66, 160 210 and 71, 192 197 and 72, 224 213 and 74, 256 218 and 77: the first call
+// is bound by the prefix's products, the second by its own keys.) A row's own item is a wavefront (the
+// generic kernel: a workgroup): about kOwnItems of them. (1024, with 192 at 222 and 75: 227 and 91 us; the small
+// calls are alike.) No
 // range is meant for fewer than 128 keys of a prefix (64: 8 rows of 6144 + 200 keys of 256 26 us, 128 20), 32 of a
 // row's own, by the longest that the table can hold.
 constexpr int64_t kPrefixItems = 192, kOwnItems = 2048, kGenericItems = 1024;

@@ -410,8 +410,9 @@ __device__ __forceinline__ void fill_angles(const RopeArgs &a, int64_t first, in
 // A workgroup goes through tiles of tokens. Each round fills in the next tile's angles (paged: and the
 // places of the one behind that) and begins the loads of its first heads, so that a tile costs one barrier and
 // every part of the code stands once: the first rounds have a tile before the first token, which is empty.
-// (A workgroup a tile, with its angles first and its heads behind a barrier: 89 us, not 63, on 16384
-// tokens of 40 heads of 128. Two heads a lane in flight, U: one and four measured the same or worse.)
+// (With the angles first and all heads behind a barrier: 89 us, not 63, on 16384 tokens of 40 heads of 128, where
+// a workgroup has an empty round and one tile: what it gains there is the loads begun in front of the barrier and
+// the weights in LDS. Two heads a lane in flight, U: one and four measured the same or worse.)
 template <int DT, int D, int MODE, bool INTER>
 __global__ __launch_bounds__(256) void rope_fast(RopeArgs a, RopePages pg, int tile, const void *__restrict__ q,
                                                  const void *__restrict__ k, const void *__restrict__ v,
@@ -714,7 +715,9 @@ static int rope_tile(const RopeArgs &a, int by) {
     return (int)tile;
 }
 // Workgroups at most, as many as are resident and a few rounds more. (The same two: 1024 of them 75.7 and 52.2
-// us, 4096 72.7 and 53.2; one a tile 71.9 and 53.3, without the loads ahead.)
+// us; 4096 are one a tile there, 72.7 and 53.2. Calls of more tiles, replayed, 4096 workgroups and one a tile: 65536
+// tokens of 40 heads of 128 263 and 242 us, 131072 of 10 134 and 130, of 5 heads of 64 49 and 52; into pages 65536 of
+// 48 323 and 307, 131072 of 12 173 and 169.)
 constexpr int64_t kRopeGrid = 4096;
 static size_t rope_lds(const RopeArgs &a, int tile) { return ((size_t)2 * a.d + (size_t)4 * tile * a.n) * sizeof(float); }
 

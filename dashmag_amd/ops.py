@@ -641,7 +641,9 @@ def qk_norm_rope_paged(query, key, value, q_weight, k_weight, inv_freq, key_page
     in place. ``lengths [S]`` are the sequences' lengths with these tokens, as the decode that follows
     takes them; the rows ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1`` are sequence ``s``'s last tokens
     (without ``cu_seqlens [S + 1]`` each sequence has one, N = S), each at its place in the sequence,
-    which is its position too; ``block_table [S, max_pages]`` holds the sequences' pages.
+    which is its position too; ``block_table [S, max_pages]`` holds the sequences' pages. The norm is
+    always taken (a weight of None leaves out the scale alone): a layer without norms of its queries and
+    keys writes its pages itself.
 
     int32 arrays on the GPU are not read back: what they hold is checked on the GPU. A token of no
     sequence, or with a position below zero (the padding of a batch: length 0), gets a query of zeros
