@@ -437,10 +437,10 @@ int dm_qk_norm_rope_bwd(const dm_qk_norm_rope_desc *desc, const void *q, const v
                         const void *grad_q, const void *grad_k, void *dq, void *dk,
                         void *dq_weight, void *dk_weight, void *workspace, size_t workspace_bytes,
                         void *stream);
-/* The same into a paged cache: q_out [N, Hq, D] contiguous; the keys, normalised and rotated (there is
- * no form without the norm), and the values as they are go to their rows of k_pages and v_pages. No two tokens of a call may have
- * one page row (sequences that share the page that they append to, a page twice in a row's table):
- * which of them it then holds is not said. */
+/* The same into a paged cache: q_out [N, Hq, D] contiguous; the keys, normalised and rotated (there
+ * is no form without the norm), and the values as they are go to their rows of k_pages and
+ * v_pages. No two tokens of a call may have one page row (sequences that share the page that they
+ * append to, a page twice in a row's table): which of them it then holds is not said. */
 int dm_qk_norm_rope_paged(const dm_qk_norm_rope_desc *desc, const dm_kv_pages *pages, const void *q,
                           const void *k, const void *v, const void *q_weight, const void *k_weight,
                           const float *inv_freq, void *q_out, void *k_pages, void *v_pages,
