@@ -19,7 +19,7 @@ PROBES = ["attn_fwd_mfma", "attn_fwd_generic", "attn_bwd_mfma", "attn_bwd_generi
           "conv1d_fwd", "conv1d_bwd", "conv1d_update", "logprob", "lce_fwd", "lce_bwd",
           "gdr_chunk_fwd_mfma", "gdr_chunk_bwd_mfma", "gdr_step_bwd", "qk_norm_rope",
           "qk_norm_rope_bwd", "decode_shared", "cache_reserve", "cache_fork", "cache_free",
-          "cache_compact"]
+          "cache_compact", "attn_paged", "attn_weights", "cache_evict"]
 DM_ACT_NONE, DM_ACT_SILU = 0, 1
 
 
@@ -174,6 +174,11 @@ SIGNATURES = {
     "dm_cache_free": (ctypes.c_int, [_TD, _VP, _I64, _VP]),
     "dm_cache_compact_workspace": (_SZ, [_TD]),
     "dm_cache_compact": (ctypes.c_int, [_TD, _LP, _I64, _VP, _VP, _SZ, _VP]),
+    "dm_attention_paged_workspace": (_SZ, [_AD, ctypes.c_int64, ctypes.c_int]),
+    "dm_attention_paged": (ctypes.c_int, [_AD, _VP, _VP, _VP, ctypes.c_int64, ctypes.c_int64, _VP,
+                                          ctypes.c_int64, _VP, _VP, _VP, _VP, _I64, _VP, _SZ, _VP]),
+    "dm_cache_evict_workspace": (_SZ, [_TD]),
+    "dm_cache_evict": (ctypes.c_int, [_TD, _LP, _I64, _VP, _I64, _VP, _I64, _VP, _VP, _SZ, _VP]),
     "dm_qk_norm_rope": (ctypes.c_int, [_QD] + [_VP] * 8),
     "dm_qk_norm_rope_bwd_workspace": (_SZ, [_QD]),
     "dm_qk_norm_rope_bwd": (ctypes.c_int, [_QD] + [_VP] * 12 + [_SZ, _VP]),

@@ -414,6 +414,189 @@ __global__ __launch_bounds__(256) void cache_compact_apply(CacheArgs a, PoolArgs
     }
 }
 
+// ------------------------------------------------------------------------------------------
+// Eviction
+// ------------------------------------------------------------------------------------------
+//
+// A row's plan is one workgroup's: what has to stay, the weight of the last key that stays of the others, by three
+// counts of 11, 11 and 10 bits of the weights' order, and one walk over the keys in order that gives each key that
+// stays its place. The keys then move down in every pool, a wavefront for 128 bytes of each: its loads of 128 keys
+// have all arrived before it stores one of them, and what it stores to lies in front of all that it has yet to
+// load, so that no order among wavefronts is needed.
+
+// What the plan leaves for the copies: of row r the keys first[r] .. count[r] - 1 move; key j comes from row
+// from[j] of the pool to row to[j] (page * page_size + row; kNoSlot: a page outside the pools).
+struct EvictWork {
+    int32_t *first, *count;  // [rows]
+    uint32_t *from, *to;     // [rows, max_pages * page_size]
+    int64_t cap;
+};
+constexpr uint32_t kNoSlot = 0xffffffffu;
+
+// A float's place in the order of weights: -0 as 0, NaN above all.
+__device__ __forceinline__ uint32_t weight_order(float x) {
+    if (x != x) return 0xffffffffu;
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__global__ __launch_bounds__(kPlan) void cache_evict_plan(CacheArgs a, float *weights, int64_t stride,
+                                                          const int32_t *__restrict__ budgets, int64_t recent,
+                                                          int32_t *__restrict__ kept, EvictWork w) {
+    __shared__ PlanSums sums;
+    __shared__ int32_t hist[2048], shared_to, chosen, above;
+    const int tid = threadIdx.x;
+    const int64_t r = blockIdx.x, cap = a.max_pages * a.page_size;
+    const int64_t held = keys_of(a, a.lengths[r]), budget = max(budgets[r], 0);
+    int32_t *row = a.table + r * a.max_pages, *out = kept + r * cap;
+    float *wr = weights + r * stride;
+    int turn = 0;
+    if (tid == 0) shared_to = 0;
+    __syncthreads();
+    // the pages up to the last that another row holds stay
+    const int64_t np = pages_of(a, held);
+    int32_t most = 0;
+    for (int64_t c = tid; c < np && held > budget; c += kPlan) {
+        const int32_t page = row[c];
+        if (page >= 0 && page < a.num_pages && a.counts[page] > 1) most = (int32_t)c + 1;
+    }
+    if (most) atomicMax(&shared_to, most);
+    __syncthreads();
+    const int64_t fixed = min(held, (int64_t)shared_to * a.page_size);
+    const int64_t until = max(fixed, held - min(recent, budget));  // the keys [fixed, until) may go
+    const int64_t must = held - (until - fixed), n = min(held, max(budget, must));
+    if (n == held) {
+        for (int64_t j = tid; j < cap; j += kPlan) out[j] = j < held ? (int32_t)j : -1;
+        if (tid == 0) w.first[r] = w.count[r] = 0;
+        return;
+    }
+    // of those the `need` largest weights: those above `bar`, and the first `ties` of those that equal it
+    const int32_t need = (int32_t)(n - must);
+    uint32_t bar = 0xffffffffu;
+    int32_t ties = 0;
+    if (need > 0) {
+        uint32_t prefix = 0, mask = 0;
+        int32_t left = need;
+        for (int pass = 0; pass < 3; pass++) {
+            const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
+            for (int i = tid; i < 2048; i += kPlan) hist[i] = 0;
+            __syncthreads();
+            for (int64_t j = fixed + tid; j < until; j += kPlan) {
+                const uint32_t x = weight_order(wr[j]);
+                if ((x & mask) == prefix) atomicAdd(&hist[(x >> shift) & (bins - 1)], 1);
+            }
+            __syncthreads();
+            // from the largest bin down: the one in which the count reaches `left`
+            const int b1 = 2047 - 2 * tid, b0 = b1 - 1;
+            const int32_t c1 = hist[b1], c0 = hist[b0];
+            int32_t total;
+            const int32_t before = plan_scan(c0 + c1, sums, turn, &total);
+            if (before < left && before + c1 >= left) chosen = b1, above = before;
+            if (before + c1 < left && before + c1 + c0 >= left) chosen = b0, above = before + c1;
+            __syncthreads();
+            prefix |= (uint32_t)chosen << shift;
+            mask |= (uint32_t)(bins - 1) << shift;
+            left -= above;
+            __syncthreads();
+        }
+        bar = prefix, ties = left;
+    }
+    // the keys in order, four a thread; a key's place: the keys above the bar in front of it, and the ties taken
+    int32_t over = 0, equal = 0;
+    if (tid == 0) chosen = (int32_t)n;
+    __syncthreads();
+    for (int64_t j0 = 0; j0 < held; j0 += kPlan * 4) {
+        float x[4];
+        int32_t is[4], eq[4], packed = 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int64_t j = j0 + tid * 4 + u;
+            x[u] = j < held ? wr[j] : 0.f;
+            const uint32_t y = weight_order(x[u]);
+            const bool stays = j < fixed || (j >= until && j < held), may = j >= fixed && j < until && need > 0;
+            is[u] = stays || (may && y > bar);
+            eq[u] = may && y == bar;
+            packed += is[u] | eq[u] << 16;
+        }
+        int32_t total;
+        const int32_t at = plan_scan(packed, sums, turn, &total);
+        int32_t o = over + (at & 0xffff), e = equal + (at >> 16);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int64_t j = j0 + tid * 4 + u;
+            if (is[u] || (eq[u] && e < ties)) {
+                const int64_t to = o + min(e, ties);
+                out[to] = (int32_t)j;
+                if (to != j) {
+                    wr[to] = x[u];
+                    const int64_t cf = j / a.page_size, ct = to / a.page_size;
+                    const int32_t pf = row[cf], pt = row[ct];
+                    const bool ok = pf >= 0 && pf < a.num_pages && pt >= 0 && pt < a.num_pages;
+                    w.from[r * cap + to] = ok ? (uint32_t)(pf * a.page_size + (j - cf * a.page_size)) : kNoSlot;
+                    w.to[r * cap + to] = (uint32_t)(pt * a.page_size + (to - ct * a.page_size));
+                }
+            } else if (j < held && j == o + min(e, ties)) {
+                chosen = (int32_t)j;  // (the first key that goes: no other has its own index for a place)
+            }
+            o += is[u], e += eq[u];
+        }
+        over += total & 0xffff, equal += total >> 16;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        w.first[r] = chosen, w.count[r] = (int32_t)n;
+        a.lengths[r] = (int32_t)n;
+    }
+    for (int64_t j = n + tid; j < cap; j += kPlan) {
+        out[j] = -1;
+        if (j < held) wr[j] = 0.f;
+    }
+    for (int64_t c = pages_of(a, n) + tid; c < np; c += kPlan) {
+        const int32_t page = row[c];
+        row[c] = -1;
+        if (page >= 0 && page < a.num_pages) atomicSub(a.counts + page, 1);
+    }
+}
+
+// Wavefront (row, pool, slice): `lanes` lanes a key, a T each, kEvictLoads loads in flight.
+constexpr int kEvictLoads = 16, kEvictLanes = 8;
+template <class T>
+__global__ __launch_bounds__(256) void cache_evict_move(EvictWork w, PoolArgs pools, int64_t page_size, int32_t slices,
+                                                        int64_t items) {
+    const int lane = threadIdx.x & 63;
+    int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= items) return;
+    const int32_t slice = (int32_t)(i % slices);
+    i /= slices;
+    const auto &pool = pools.at[i % pools.n];
+    const int64_t r = i / pools.n, bytes = pool.bytes / page_size;
+    const int64_t at = ((int64_t)slice * kEvictLanes + lane % kEvictLanes) * (int64_t)sizeof(T);
+    const int32_t first = w.first[r], count = w.count[r];
+    const uint32_t *from = w.from + r * w.cap, *to = w.to + r * w.cap;
+    if (!__any(at < bytes)) return;
+    constexpr int KEYS = 64 / kEvictLanes;
+    auto place = [&](uint32_t x) {
+        const uint32_t page = x / (uint32_t)page_size, k = x - page * (uint32_t)page_size;
+        return pool.pages + page * pool.stride + k * bytes + at;
+    };
+    for (int32_t j0 = first; j0 < count; j0 += KEYS * kEvictLoads) {
+        T x[kEvictLoads];
+        char *dst[kEvictLoads];
+#pragma unroll
+        for (int u = 0; u < kEvictLoads; u++) {
+            const int32_t j = j0 + u * KEYS + lane / kEvictLanes;
+            const uint32_t f = j < count && at < bytes ? from[j] : kNoSlot;
+            dst[u] = f != kNoSlot ? place(to[j]) : nullptr;
+            if (f != kNoSlot) x[u] = *(const T *)place(f);
+        }
+        // every load has arrived before the first store: a key may lie where another of these comes from
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int u = 0; u < kEvictLoads; u++)
+            if (dst[u]) *(T *)dst[u] = x[u];
+    }
+}
+
 static const int64_t kI31 = (int64_t)1 << 31;
 static const int64_t kMostPages = ((int64_t)1 << 21) - 1;  // a planning workgroup's sums of 1024 needs fit 32 bits
 static const int64_t kMostRows = (int64_t)1 << 22;  // rows of a call: a workgroup each, under 2^32 threads
@@ -586,6 +769,81 @@ int dm_cache_compact(const dm_cache_table *t, const dm_cache_pool *pools, int64_
     }
     probe_add(DM_PROBE_CACHE_COMPACT);
     DM_LAUNCH_CHECK("cache_compact: launch");
+    return DM_OK;
+}
+
+static EvictWork evict_work(const dm_cache_table *t, char *at, size_t *bytes) {
+    EvictWork w{};
+    w.cap = t->max_pages * t->page_size;
+    const size_t rows = align_up((size_t)t->rows * 4), keys = align_up((size_t)(t->rows * w.cap) * 4);
+    w.first = (int32_t *)at;
+    w.count = (int32_t *)(at + rows);
+    w.from = (uint32_t *)(at + 2 * rows);
+    w.to = (uint32_t *)(at + 2 * rows + keys);
+    *bytes = 2 * (rows + keys);
+    return w;
+}
+static bool evict_sizes(const dm_cache_table *t) {
+    return table_sizes(t) && t->rows <= kMostRows && t->max_pages <= ((int64_t)1 << 30) / t->page_size &&
+           t->num_pages < kI31 / t->page_size;
+}
+
+size_t dm_cache_evict_workspace(const dm_cache_table *t) {
+    size_t bytes = 0;
+    if (evict_sizes(t)) evict_work(t, nullptr, &bytes);
+    return bytes;
+}
+
+int dm_cache_evict(const dm_cache_table *t, const dm_cache_pool *pools, int64_t npools, float *weights,
+                   int64_t weights_stride, const int32_t *budgets, int64_t recent, int32_t *kept, void *workspace,
+                   size_t workspace_bytes, void *stream) {
+    const std::string op("cache_evict");
+    if (int rc = check_table(op, t)) return rc;
+    if (int rc = check_pools(op, t, pools, npools)) return rc;
+    if (!evict_sizes(t))
+        return refuse(op + ": a row holds at most 2^30 keys, the pools less than 2^31, rows are at most 2^22");
+    if (recent < 0) return refuse(op + ": recent must not be negative");
+    const int64_t cap = t->max_pages * t->page_size;
+    if (t->rows > 1 && weights_stride < cap)
+        return refuse(op + ": the weights are [R, max_pages * page_size], their rows apart");
+    if (workspace_bytes < dm_cache_evict_workspace(t))
+        return refuse(op + ": the workspace is smaller than dm_cache_evict_workspace");
+    if (t->rows == 0 || cap == 0) return DM_OK;
+    if (!weights || !budgets || !kept) return refuse(op + ": the weights, the budgets or the results' place are missing");
+    hipStream_t st = (hipStream_t)stream;
+    size_t bytes;
+    const EvictWork w = evict_work(t, (char *)workspace, &bytes);
+    cache_evict_plan<<<(unsigned)t->rows, kPlan, 0, st>>>(cache_args(t), weights, weights_stride, budgets, recent, kept, w);
+    for (int64_t i = 0; i < npools; i += kPoolsPerLaunch) {
+        bool wide;
+        int64_t pieces, most = 0, grain = 16;
+        const PoolArgs pa = pools_of(pools, npools, i, &wide, &pieces);
+        for (int x = 0; x < pa.n; x++) {
+            const int64_t row = pa.at[x].bytes / t->page_size;
+            const uint64_t bits = (uint64_t)pa.at[x].pages | (uint64_t)pa.at[x].stride | (uint64_t)row;
+            while (bits % grain) grain /= 2;
+            most = std::max(most, row);
+        }
+        const int64_t slices = (most + kEvictLanes * grain - 1) / (kEvictLanes * grain);
+        const int64_t items = t->rows * pa.n * slices;
+        if (items == 0) continue;
+        if (slices >= kI31 || items / 4 >= ((int64_t)1 << 24)) return refuse(op + ": more rows and bytes than one launch takes");
+        const unsigned g = (unsigned)((items + 3) / 4);
+#define EVICT_MOVE(T) cache_evict_move<T><<<g, 256, 0, st>>>(w, pa, t->page_size, (int32_t)slices, items)
+        if (grain == 16)
+            EVICT_MOVE(uint4);
+        else if (grain == 8)
+            EVICT_MOVE(uint2);
+        else if (grain == 4)
+            EVICT_MOVE(uint32_t);
+        else if (grain == 2)
+            EVICT_MOVE(uint16_t);
+        else
+            EVICT_MOVE(uint8_t);
+#undef EVICT_MOVE
+    }
+    probe_add(DM_PROBE_CACHE_EVICT);
+    DM_LAUNCH_CHECK("cache_evict: launch");
     return DM_OK;
 }
 

@@ -66,6 +66,12 @@ __device__ __forceinline__ f32x4_t mfma4(float a, float b, const f32x4_t &c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+// v_mfma_f32_32x32x2_f32: D[32x32] += A[32x2] B[2x32] in f32; lane l holds A's row (l % 32) and B's
+// column (l % 32) at k = l / 32; D as the 32x32x16 products'.
+__device__ __forceinline__ f32x16_t mfma2(float a, float b, const f32x16_t &c) {
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+
 // f32 -> 16-bit bits, two at a time: v_cvt_pk_bf16_f32 (round to nearest even) or
 // v_cvt_pk_f16_f32.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));

@@ -1,0 +1,257 @@
+// How a ragged batch of new tokens over a paged cache is shared out, worked out on the device.
+//
+// The query rows of a sequence (its new tokens x the query heads of one key-value head) lie in tiles, and a
+// tile sweeps the keys that its rows see. All tiles laid one after another, each as long as its keys and a
+// constant for its start, are a line; each of a fixed number of workers (workgroups or wavefronts) takes an
+// equal part of it, wherever that begins and ends. So every worker has the same work whatever the lengths are, no
+// length is needed on the host, and at most two of a worker's tiles are shared with others: a tile that a worker
+// has whole is written at once, the pieces of a shared one go to the worker's two places in the workspace and are
+// joined by a second launch. What a tile costs is linear in its number within the sequence, so a sequence's tiles are
+// summed in closed form and a worker finds its part by a scan over the sequences and a search within one.
+#pragma once
+
+#include "dm_common.h"
+
+namespace dm {
+
+struct PagedArgs {
+    int32_t S, N, cap, left;  // sequences, new tokens, keys that a table row holds, the window's left (-1: none)
+    int32_t hq, hkv, d, rep;  // rep: query heads of a key-value head
+    float scale;
+    const int32_t *lengths, *cu, *table;  // cu: NULL for one token a sequence
+    int64_t page_size, max_pages, num_pages;
+    int64_t qt, qh, kb, kt, kh, vb, vt, vh;  // strides in elements
+    void *o;
+    float *lse;  // [N, Hq] or NULL
+};
+
+// A shared tile's join: its rows, and the workers that have pieces of it.
+struct PagedJob {
+    int32_t tok, head, per, rows, first, last;
+};
+
+// One line: which sequences' tiles lie on it, and its workers.
+struct PagedLine {
+    int32_t rt, pitch;  // most rows of a tile, and of this call's tiles
+    int32_t m, hc, per; // tokens of a tile; tiles of a token (above rt heads); row r: token r / per, head r % per
+    int32_t over, upto; // the sequences of over < n rep <= upto rows
+    int32_t workers, unit;   // most workers; a piece's keys begin at multiples of unit from the tile's first
+    int32_t start, least;    // a tile's start in keys, and what a worker has at least
+    float *o;           // [2 workers, pitch, D]: unnormalised outputs
+    float2 *ml;         // [2 workers, pitch]: reference (log2 units) and sum
+    PagedJob *jobs;     // [workers]
+};
+
+struct PagedSeq {
+    int32_t first, n, len;  // first token, new tokens, keys with them
+    bool ok;                // its offsets go up within the tokens
+};
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs &a, int32_t s) {
+    PagedSeq q;
+    int32_t end = s + 1;
+    q.first = s;
+    if (a.cu) q.first = a.cu[s], end = a.cu[s + 1];
+    q.len = min(max(a.lengths[s], 0), a.cap);
+    q.ok = q.first >= 0 && q.first <= end && end <= a.N;
+    q.n = q.ok ? end - q.first : 0;
+    return q;
+}
+
+// sum over u < t of max(0, a + m u)
+__device__ __forceinline__ int64_t ramp(int64_t a, int64_t m, int64_t t) {
+    const int64_t u0 = a >= 0 ? 0 : min(t, (-a + m - 1) / m), c = t - u0;
+    return c * (a + m * u0) + m * (c * (c - 1) / 2);
+}
+
+// What the first t token tiles of a sequence cost: of each its start, and the keys between the first that its
+// first token sees and the last that its last one would see if the tile were full.
+__device__ __forceinline__ int64_t tiles_cost(const PagedArgs &a, const PagedLine &l, const PagedSeq &q, int32_t t) {
+    const int64_t p0 = (int64_t)q.len - q.n;
+    int64_t x = (int64_t)t * l.start + ramp(p0 + l.m, l.m, t);
+    if (a.left >= 0) x -= ramp(p0 - a.left, l.m, t);
+    return x;
+}
+__device__ __forceinline__ int32_t token_tiles(const PagedLine &l, const PagedSeq &q) { return (q.n + l.m - 1) / l.m; }
+__device__ __forceinline__ bool on_line(const PagedArgs &a, const PagedLine &l, const PagedSeq &q) {
+    const int64_t rows = (int64_t)q.n * a.rep;
+    return q.n > 0 && rows > l.over && rows <= l.upto;
+}
+
+// The exclusive prefix sums of the workgroup's x, and its total.
+template <int NT>
+struct PlanSmem {
+    int64_t pre[NT], waves[NT / 64];
+    int64_t base;
+};
+template <int NT>
+__device__ __forceinline__ int64_t scan64(int64_t x, PlanSmem<NT> &sm) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t in = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t y = __shfl_up((long long)in, o, 64);
+        if (lane >= o) in += y;
+    }
+    __syncthreads();  // (the last chunk's sums have been read)
+    if (lane == 63) sm.waves[wave] = in;
+    __syncthreads();
+    int64_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) {
+        before += w < wave ? sm.waves[w] : 0;
+        all += sm.waves[w];
+    }
+    sm.pre[threadIdx.x] = before + in - x;
+    __syncthreads();
+    return all;
+}
+template <int NT>
+__device__ __forceinline__ int64_t plan_chunk(const PagedArgs &a, const PagedLine &l, int32_t s0, PlanSmem<NT> &sm,
+                                              bool *ok) {
+    const int32_t s = s0 + (int32_t)threadIdx.x;
+    int64_t x = 0;
+    if (s < a.S) {
+        const PagedSeq q = paged_seq(a, s);
+        *ok = *ok && q.ok;
+        if (on_line(a, l, q)) x = (int64_t)a.hkv * l.hc * tiles_cost(a, l, q, token_tiles(l, q));
+    }
+    return scan64<NT>(x, sm);
+}
+
+// A worker's place on a line of length `total` with `workers` workers: worker w has [at(w), at(w + 1)).
+struct PagedShare {
+    int64_t total;
+    int32_t workers;
+    __device__ __forceinline__ int64_t at(int32_t w) const {
+        return total / workers * w + total % workers * w / workers;
+    }
+    // the last worker that begins in front of x > 0
+    __device__ __forceinline__ int32_t last_before(int64_t x) const {
+        int32_t w = (int32_t)min((int64_t)workers - 1, (x - 1) / max(total / workers, (int64_t)1));
+        while (w > 0 && at(w) >= x) w--;
+        return w;
+    }
+};
+
+// Where a worker stands: the tile x of sequence s and key-value head kh, which begins at `base` of the line.
+struct PagedWalk {
+    int32_t s, kh, c, t;  // c: which heads of a token, t: token tile
+    int32_t nt;           // token tiles of the sequence
+    PagedSeq q;
+    int64_t base;
+};
+
+// The whole workgroup: the line's total, 0 where offsets do not go up; and the walk of the worker at `p`
+// (wavefront-uniform; each wavefront its own), if it has anything. `where` maps (total) to p, or -1 for none.
+template <int NT, class Where>
+__device__ __forceinline__ PagedShare plan_line(const PagedArgs &a, const PagedLine &l, PlanSmem<NT> &sm, Where where,
+                                                PagedWalk *walk, int64_t *p, bool *valid) {
+    bool ok = true;
+    int64_t total = 0;
+    for (int32_t s0 = 0; s0 < a.S; s0 += NT) total += plan_chunk<NT>(a, l, s0, sm, &ok);
+    ok = __syncthreads_and(ok);
+    *valid = ok;
+    PagedShare sh;
+    sh.total = ok ? total : 0;
+    sh.workers = (int32_t)max((int64_t)1, min((int64_t)l.workers, sh.total / l.least));
+    *p = sh.total > 0 ? where(sh) : -1;
+    int64_t base = 0;
+    int32_t found = -1;
+    const int lane = threadIdx.x & 63;
+    for (int32_t s0 = 0; s0 < a.S && sh.total > 0; s0 += NT) {
+        int64_t all = sh.total;
+        if (a.S > NT) all = plan_chunk<NT>(a, l, s0, sm, &ok);
+        if (*p >= base && *p < base + all) {
+            int n = 0;
+#pragma unroll 1
+            for (int i = 0; i < NT; i += 64) n += __popcll(__ballot(sm.pre[i + lane] <= *p - base));
+            found = s0 + n - 1;
+            walk->base = base + sm.pre[n - 1];
+        }
+        base += all;
+    }
+    if (found < 0) {
+        *p = -1;
+        return sh;
+    }
+    walk->s = __builtin_amdgcn_readfirstlane(found);
+    walk->q = paged_seq(a, walk->s);
+    walk->nt = token_tiles(l, walk->q);
+    int64_t rem = *p - walk->base;
+    const int64_t chunk = tiles_cost(a, l, walk->q, walk->nt), head = chunk * l.hc;
+    const int64_t kh = rem / head;
+    rem -= kh * head;
+    const int64_t c = rem / chunk;
+    rem -= c * chunk;
+    // the last tile that begins at rem or in front of it: 64 probes at a time
+    int32_t lo = 0, hi = walk->nt;  // it lies in [lo, hi)
+    while (hi - lo > 1) {
+        const int32_t step = (hi - lo + 63) / 64, t = lo + lane * step;
+        const int n = __popcll(__ballot(t < hi && tiles_cost(a, l, walk->q, t) <= rem));
+        lo += (n - 1) * step;
+        hi = min(hi, lo + step);
+    }
+    walk->kh = (int32_t)kh, walk->c = (int32_t)c, walk->t = lo;
+    walk->base = *p - rem + tiles_cost(a, l, walk->q, lo);
+    return sh;
+}
+
+// A worker's next piece: rows of one tile, the keys [s0, s1) of those [lo, hi) that the tile sees.
+struct PagedPiece {
+    int32_t tok, head, per, rows;  // first token and query head; row r: token tok + r / per, head head + r % per
+    int32_t pos, kh, s;            // the position of tok; key-value head, sequence
+    int32_t s0, s1;
+    bool whole;
+    int32_t slot;                  // not whole: its place
+};
+
+template <class Args>
+__device__ __forceinline__ PagedPiece piece_of(const Args &a, const PagedLine &l, const PagedWalk &w, const PagedShare &sh,
+                                               int32_t worker, int64_t p, int64_t end, int64_t *next, int32_t *last) {
+    PagedPiece x;
+    const int32_t i0 = w.t * l.m, i1 = min(i0 + l.m, w.q.n);
+    const int64_t cost = tiles_cost(a, l, w.q, w.t + 1) - tiles_cost(a, l, w.q, w.t);
+    x.tok = w.q.first + i0;
+    x.head = w.kh * a.rep + w.c * l.rt;
+    x.per = l.per;
+    x.rows = l.hc > 1 ? min(l.rt, a.rep - w.c * l.rt) : (i1 - i0) * a.rep;
+    x.pos = w.q.len - w.q.n + i0;
+    x.kh = w.kh, x.s = w.s;
+    const int32_t hi = max(0, w.q.len - w.q.n + i1);
+    const int32_t lo = a.left >= 0 ? min(hi, max(0, x.pos - a.left)) : 0;
+    auto key = [&](int64_t off) -> int32_t {  // the key at `off` of the tile's part of the line
+        const int64_t k = (off - l.start) / l.unit * l.unit;
+        return off >= cost ? hi : (k <= 0 ? lo : (int32_t)min((int64_t)hi, lo + k));
+    };
+    const int64_t o0 = p - w.base, o1 = min(end - w.base, cost);
+    x.s0 = key(o0), x.s1 = key(o1);
+    x.whole = o0 == 0 && o1 == cost;
+    x.slot = 2 * worker + (o0 == 0 ? 1 : 0);
+    *next = w.base + cost;
+    // the worker that the tile's first border belongs to has it joined
+    *last = -1;
+    if (o0 > 0 && sh.at(worker - 1) <= w.base) *last = sh.last_before(w.base + cost);
+    return x;
+}
+
+// On to the next tile of the line (false: there is none).
+__device__ __forceinline__ bool walk_on(const PagedArgs &a, const PagedLine &l, PagedWalk &w, int64_t base) {
+    w.base = base;
+    if (++w.t < w.nt) return true;
+    w.t = 0;
+    if (++w.c < l.hc) return true;
+    w.c = 0;
+    if (++w.kh < a.hkv) return true;
+    w.kh = 0;
+    while (++w.s < a.S) {
+        w.q = paged_seq(a, w.s);
+        if (on_line(a, l, w.q)) {
+            w.nt = token_tiles(l, w.q);
+            return true;
+        }
+    }
+    return false;
+}
+
+}  // namespace dm

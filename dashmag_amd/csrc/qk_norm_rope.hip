@@ -92,6 +92,14 @@ __device__ __forceinline__ int64_t place_plain(const RopeArgs &a, int64_t b, int
     return a.positions_i64 ? ((const int64_t *)a.positions)[i] : (int64_t)((const int32_t *)a.positions)[i];
 }
 
+// place_paged, with the call's own positions where it has some.
+__device__ __forceinline__ bool place_turned(const RopeArgs &a, const RopePages &pg, int64_t token, int64_t *p,
+                                             int64_t *krow, int64_t *vrow) {
+    const bool is = place_paged(pg, token, p, krow, vrow);
+    if (a.positions && is) *p = place_plain(a, 0, token);
+    return is;
+}
+
 // A head's pair index and partner of element e (e < 2 n), and whether e is the pair's first.
 __device__ __forceinline__ void pair_of(int e, int n, int interleaved, int *j, int *other, bool *first) {
     if (interleaved) {
@@ -124,7 +132,7 @@ __global__ __launch_bounds__(256) void rope_generic(RopeArgs a, RopePages pg, co
         int64_t p, krow = -1, vrow = -1;
         bool is = true;
         if (MODE == kRopePaged)
-            is = place_paged(pg, token, &p, &krow, &vrow);
+            is = place_turned(a, pg, token, &p, &krow, &vrow);
         else
             p = place_plain(a, b, t);
         __syncthreads();  // (the last token's angles have been read)
@@ -385,7 +393,7 @@ __device__ __forceinline__ void fill_places(const RopeArgs &a, const RopePages &
     const int t = threadIdx.x;
     if (t < tile && first + t < a.tokens) {
         int64_t p, kr, vr;
-        o.is[t] = place_paged(pg, first + t, &p, &kr, &vr);
+        o.is[t] = place_turned(a, pg, first + t, &p, &kr, &vr);
         o.at[t] = p, o.krow[t] = kr, o.vrow[t] = vr;
     }
 }

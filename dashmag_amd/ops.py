@@ -634,14 +634,15 @@ def _block_table(op, block_table, rows, device):
 
 
 def qk_norm_rope_paged(query, key, value, q_weight, k_weight, inv_freq, key_pages, value_pages, block_table,
-                       lengths, cu_seqlens=None, options: Optional[QkNormRopeOptions] = None):
+                       lengths, cu_seqlens=None, options: Optional[QkNormRopeOptions] = None, positions=None):
     """:func:`qk_norm_rope` of the tokens that join a paged cache, prompts or one token a sequence:
     returns ``query [N, Hq, D]`` normalised and rotated, and writes ``key [N, Hkv, D]``, normalised and
     rotated, and ``value`` as it is to their rows of ``key_pages, value_pages [P, page_size, Hkv, D]``
     in place. ``lengths [S]`` are the sequences' lengths with these tokens, as the decode that follows
     takes them; the rows ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1`` are sequence ``s``'s last tokens
     (without ``cu_seqlens [S + 1]`` each sequence has one, N = S), each at its place in the sequence,
-    which is its position too; ``block_table [S, max_pages]`` holds the sequences' pages. The norm is
+    which is its position too unless ``positions [N]`` gives others (whole numbers: a sequence that has
+    given up keys, :func:`cache_evict`); ``block_table [S, max_pages]`` holds the sequences' pages. The norm is
     always taken (a weight of None leaves out the scale alone): a layer without norms of its queries and
     keys writes its pages itself.
 
@@ -668,6 +669,7 @@ def qk_norm_rope_paged(query, key, value, q_weight, k_weight, inv_freq, key_page
     _in_pages(op, key_pages, "key_pages")
     _in_pages(op, value_pages, "value_pages")
     dev, n = query.device, query.shape[0]
+    at = _positions(op, desc, positions, dev)
     ln = _device_i32(op, lengths, dev, "the cache lengths")
     if ln.dim() != 1:
         raise Unsupported(f"{op}: the cache lengths are [S]")
@@ -742,6 +744,111 @@ def attention_decode_shared(query, key_pages, value_pages, block_table, lengths,
          v.data_ptr(), npages, page_size, bt.data_ptr(), max_pages, _at(ln), cu.data_ptr(), ng, pl.data_ptr(),
          out.data_ptr(), ws.data_ptr(), nbytes)
     return out
+
+
+def attention_paged(query, key_pages, value_pages, block_table, lengths, cu_seqlens=None, options=None):
+    """The attention of new tokens over a paged cache that holds their keys and values already (as
+    :func:`qk_norm_rope_paged` leaves it): chunks of prompts, drafted tokens, single tokens, in one batch.
+    ``query [N, Hq, D]``; sequence ``s`` has the tokens ``cu_seqlens[s] .. cu_seqlens[s + 1] - 1`` as the last
+    ones of its ``lengths[s]`` keys (without ``cu_seqlens [S + 1]`` each sequence has one, N = S), and a token
+    sees the keys of its sequence up to its own, with a window no more than ``left`` in front of it.
+    ``key_pages, value_pages [P, page_size, Hkv, D]`` and ``block_table [S, max_pages]`` are
+    :func:`attention_decode_paged`'s. ``[N, Hq, D]`` in the queries' dtype.
+
+    int32 arrays on the GPU are not read back: a length counts as between 0 and the keys that a table row
+    holds, and with offsets that do not go up from 0 at least to N at most no token belongs to a sequence. Such
+    tokens, and those whose position is below zero, get zeros."""
+    return _attention_paged("attention_paged", query, key_pages, value_pages, block_table, lengths, None, cu_seqlens,
+                            options, False)[0]
+
+
+def attention_paged_with_lse(query, key_pages, value_pages, block_table, lengths, cu_seqlens=None, options=None):
+    """:func:`attention_paged`'s output and its log-sum-exp ``[N, Hq]`` f32 (natural log, -inf for a token
+    that sees no key)."""
+    return _attention_paged("attention_paged_with_lse", query, key_pages, value_pages, block_table, lengths, None,
+                            cu_seqlens, options, True)
+
+
+def attention_paged_with_weights(query, key_pages, value_pages, block_table, lengths, weights, cu_seqlens=None,
+                                 options=None):
+    """:func:`attention_paged_with_lse`, and the attention that each cached key gets added to ``weights
+    [S, max_pages * page_size]`` f32 in place: to key ``j`` of sequence ``s`` the sum of its softmax weights
+    over the tokens and query heads that see it, in a fixed order. What :func:`cache_evict` goes by; the layers
+    of a model, whose pools share a table, add to one such array."""
+    return _attention_paged("attention_paged_with_weights", query, key_pages, value_pages, block_table, lengths, weights,
+                            cu_seqlens, options, True)
+
+
+def _attention_paged(op, query, key_pages, value_pages, block_table, lengths, weights, cu_seqlens, options, want_lse):
+    options = options or AttentionOptions()
+    _one_device(op, query, key_pages, value_pages, weights)
+    qs, ps, dtype = query.shape, key_pages.shape, query.dtype
+    if len(qs) != 3:
+        raise Unsupported(f"{op}: query is [N, Hq, D]")
+    if len(ps) != 4 or ps != value_pages.shape:
+        raise Unsupported(f"{op}: the key and value pages are [P, page_size, Hkv, D], one shape")
+    (n, hq, d), (npages, page_size, hkv, dk) = qs, ps
+    if page_size < 1:
+        raise Unsupported(f"{op}: pages hold at least one key")
+    if d != dk:
+        raise Unsupported(f"{op}: query and key must have one head dimension")
+    if hkv == 0 or hq % hkv != 0:
+        raise Unsupported(f"{op}: the query heads ({hq}) must be a multiple of the key-value heads ({hkv})")
+    if not (dtype == key_pages.dtype == value_pages.dtype):
+        raise Unsupported(f"{op}: query, key and value must share one dtype")
+    dev = query.device
+    bt, ln, cu = _paged_arrays(op, block_table, lengths, cu_seqlens, n, dev)
+    nseq, max_pages = bt.shape
+    cap = max_pages * page_size
+    row = _paged_weights(op, weights, nseq, cap)
+    q, k, v = _whole(query), _whole(key_pages), _whole(value_pages)
+    desc = _lib.AttentionDesc(nseq, n, cap, hq, hkv, d, _dtype(op, query), _lib.DM_MASK_NONE, None, _at(cu))
+    if options.scale is not None or options.window is not None:
+        _decode_options(desc.options, options)
+    desc.strided = 1
+    sq = q.stride()
+    _put_strides(desc, _ATTENTION_SQ, 0, sq[0], sq[1], *k.stride()[:3], *v.stride()[:3])
+    out = _contiguous_like(q)
+    lse = torch.empty((n, hq), dtype=torch.float32, device=dev) if want_lse else None
+    nbytes = _lib.lib().dm_attention_paged_workspace(ctypes.byref(desc), page_size, 0 if weights is None else 1)
+    ws = _workspace(nbytes, dev)
+    _run(op, dev, _lib.lib().dm_attention_paged, ctypes.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), npages,
+         page_size, bt.data_ptr(), max_pages, ln.data_ptr(), out.data_ptr(), _at(lse), _at(weights), row, ws.data_ptr(),
+         nbytes)
+    return out, lse
+
+
+def _paged_arrays(op, block_table, lengths, cu_seqlens, n, device):
+    """The table, lengths and offsets as int32 device arrays; offsets that lie on the host are checked there."""
+    ln = _device_i32(op, lengths, device, "the cache lengths")
+    if ln.dim() != 1:
+        raise Unsupported(f"{op}: the cache lengths are [S]")
+    nseq = ln.shape[0]
+    bt = _block_table(op, block_table, nseq, device)
+    if cu_seqlens is None:
+        if nseq != n:
+            raise Unsupported(f"{op}: without cu_seqlens there is one token a sequence, got {n} tokens and {nseq} "
+                              "sequences")
+        return bt, ln, None
+    cu = _device_i32(op, cu_seqlens, device, "cu_seqlens")
+    if cu.shape != (nseq + 1,):
+        raise Unsupported(f"{op}: cu_seqlens is [S + 1] = [{nseq + 1}]")
+    if not (isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda):
+        at = torch.as_tensor(cu_seqlens).tolist()
+        if min(at) < 0 or max(at) > n or any(x > y for x, y in zip(at, at[1:])):
+            raise Unsupported(f"{op}: cu_seqlens must go from 0 or more to at most N = {n} without decreasing, got {at}")
+    return bt, ln, cu
+
+
+def _paged_weights(op, weights, rows, cap):
+    """The distance of two rows of the keys' weights ``[rows, cap]`` f32, written in place."""
+    if weights is None:
+        return 0
+    if tuple(weights.shape) != (rows, cap) or weights.dtype != torch.float32:
+        raise Unsupported(f"{op}: the weights are f32 and one a key that a table row holds, [{rows}, {cap}]")
+    if (cap > 1 and weights.stride(1) != 1) or (rows > 1 and weights.stride(0) < cap):
+        raise Unsupported(f"{op}: the weights must be a view whose rows are each contiguous and apart")
+    return weights.stride(0) if rows > 1 else cap
 
 
 def _decode_options(o, options):
@@ -907,6 +1014,39 @@ def cache_compact(pools, block_table, lengths, refcounts):
     ws = _workspace(nbytes, dev)
     _run(op, dev, _lib.lib().dm_cache_compact, ctypes.byref(desc), arr, len(arr), moved.data_ptr(), ws.data_ptr(), nbytes)
     return moved
+
+
+def cache_evict(pools, weights, block_table, lengths, refcounts, budgets, recent=0):
+    """Rows of more keys than ``budgets [R]`` give up keys, by the weights that
+    :func:`attention_paged_with_weights` has accumulated (``weights [R, max_pages * page_size]`` f32). A row keeps
+    what it has to: the keys of its pages up to the last that another row holds too, and its last
+    ``min(recent, budget)``; and of the others those of the largest weights (NaN above all, of equal ones the
+    first) until it holds its budget. So it ends with its budget of keys, or those that it has to keep where they are
+    more. The keys that stay stay in order, so that later tokens and windows see them as before; they move
+    down within the row's pages in every tensor of ``pools``, their weights with them (the weights behind become
+    0), and the pages behind them are given up, as in :func:`cache_free`. ``block_table``, ``lengths`` and
+    ``refcounts`` change in place, as in :func:`cache_reserve`.
+
+    Returns ``kept [R, max_pages * page_size]`` int32: where in its row the key now at ``j`` was, -1 from the
+    row's length on. Keys that were rotated by their positions keep those: give :func:`qk_norm_rope_paged` the
+    ``positions`` of what follows."""
+    op = "cache_evict"
+    _one_device(op, block_table, weights)
+    dev = block_table.device
+    arr, page_size = _cache_pools(op, pools, refcounts.shape[0], dev)
+    desc = _cache_table(op, block_table, lengths, refcounts, page_size)
+    row = _paged_weights(op, weights, desc.rows, desc.max_pages * page_size)
+    b = _rows_i32(op, budgets, dev, "the budgets")
+    if b.shape[0] != desc.rows:
+        raise Unsupported(f"{op}: the budgets are [R] = [{desc.rows}]")
+    if isinstance(recent, bool) or not isinstance(recent, int) or not 0 <= recent < 1 << 31:
+        raise Unsupported(f"{op}: recent is a whole number of keys, not negative")
+    kept = torch.empty(weights.shape, dtype=torch.int32, device=dev)
+    nbytes = _lib.lib().dm_cache_evict_workspace(ctypes.byref(desc))
+    ws = _workspace(nbytes, dev)
+    _run(op, dev, _lib.lib().dm_cache_evict, ctypes.byref(desc), arr, len(arr), weights.data_ptr(), row, b.data_ptr(),
+         recent, kept.data_ptr(), ws.data_ptr(), nbytes)
+    return kept
 
 
 # ------------------------------------------------------------------------------------------

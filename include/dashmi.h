@@ -9,7 +9,9 @@
  *   dm_attention_decode  AttentionBackend::attention_decode     crates/dash-ops/src/attention.rs:732
  *   dm_attention_decode_paged  (none: the decode over a paged cache)
  *   dm_attention_decode_shared  (none: the paged decode of sequences that share prefixes)
- *   dm_cache_reserve, _fork, _free, _compact  (none: the pages of a paged cache)
+ *   dm_attention_paged   (none: the attention of new tokens over a paged cache, and the weights that
+ *                        its keys get)
+ *   dm_cache_reserve, _fork, _free, _compact, _evict  (none: the pages of a paged cache)
  *   dm_qk_norm_rope{,_bwd,_paged}  (none: the norms and the rotation of queries and keys that
  *                        precede the attention; the reference's callers bring them rotated)
  *   dm_gdr_chunk_fwd     ChunkGatedDeltaBackend::chunk_gated_delta_forward
@@ -276,6 +278,9 @@ typedef enum {
     DM_PROBE_CACHE_FORK,
     DM_PROBE_CACHE_FREE,
     DM_PROBE_CACHE_COMPACT,
+    DM_PROBE_ATTN_PAGED,         /* new tokens over a paged cache (one with its join and weights) */
+    DM_PROBE_ATTN_WEIGHTS,       /* those of them that accumulate the keys' weights */
+    DM_PROBE_CACHE_EVICT,
     DM_PROBE_COUNT
 } dm_probe;
 uint64_t dm_probe_count(int probe);
@@ -394,6 +399,28 @@ int dm_attention_decode_shared(const dm_attention_desc *desc, const void *q, con
                                const int32_t *prefix_lengths, void *o, void *workspace,
                                size_t workspace_bytes, void *stream);
 
+/* The attention of new tokens over a paged cache that holds their keys and values already: q [N, Hq, D]
+ * (desc->tq = N), sequence s (desc->b = S of them) having the tokens cu_seqlens_q[s] ..
+ * cu_seqlens_q[s + 1] - 1 (NULL: one token a sequence, N = S) as the last ones of its lengths[s] keys, so that
+ * the token in front of i others sits at position p = lengths[s] - 1 - i and sees the keys
+ * max(0, p - window_left) .. p, in the pages of dm_attention_decode_paged. o [N, Hq, D] in dtype,
+ * lse [N, Hq] f32 or NULL (natural log); a token that sees no key (a position below zero) gets zeros and
+ * -inf, and so does one of no sequence. The options' scale and window_left apply. desc->tk must be
+ * max_pages * page_size, mask_kind DM_MASK_NONE and cu_seqlens_k NULL; desc->strided reads sq.t, sq.h and the
+ * pages' sk, sv (b = page).
+ * weights [S, tk] f32 with rows weights_stride elements apart, or NULL: key j of sequence s is given, on top of
+ * what is there, the sum over the tokens and the query heads that see it of e^(scale q k - lse), in a fixed
+ * order.
+ * All int32 arrays are read on the device only: a length counts as between 0 and tk, offsets that do not go up
+ * between 0 and N leave every token without a sequence, a page outside [0, num_pages) reads as zeros.
+ * Refused: N * Hq of 2^26 or more, tk above 2^30. */
+size_t dm_attention_paged_workspace(const dm_attention_desc *desc, int64_t page_size, int weights);
+int dm_attention_paged(const dm_attention_desc *desc, const void *q, const void *k_pages,
+                       const void *v_pages, int64_t num_pages, int64_t page_size,
+                       const int32_t *block_table, int64_t max_pages, const int32_t *lengths,
+                       void *o, float *lse, float *weights, int64_t weights_stride, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
 /* Pages for what rows are about to hold: row r grows to new_lengths[r] keys (unchanged where that is
  * no more than it holds), taking the free pages of the lowest indices, the rows in order, each page
  * counted 1. granted [rows] (bytes): 0 where the row was left as it was, because the table has no
@@ -422,6 +449,18 @@ int dm_cache_free(const dm_cache_table *table, const int32_t *rows, int64_t n, v
 size_t dm_cache_compact_workspace(const dm_cache_table *table);
 int dm_cache_compact(const dm_cache_table *table, const dm_cache_pool *pools, int64_t npools,
                      int32_t *moved, void *workspace, size_t workspace_bytes, void *stream);
+/* Rows give up keys: a row of more than budgets[r] keys (L of them) keeps n = max(budgets[r], those that it has to
+ * keep). It has to keep the keys of its pages up to the last that another row holds too, and its last
+ * min(recent, budgets[r]); of the others it keeps those of the largest weights [rows, max_pages * page_size] f32
+ * (rows weights_stride elements apart; NaN above all, of equal ones the first). They stay in order and move down to
+ * 0 .. n - 1 in every pool, their weights with them, and the weights of n .. L - 1 become 0; the pages
+ * behind ceil(n / page_size) are given up as by dm_cache_free. kept [rows, max_pages * page_size]: where each key
+ * of a row, now at j, was before (j itself in a row that gives up none), -1 from its length on. A key on a page
+ * outside the pools is not moved. Refused: pools of 2^31 keys or more. */
+size_t dm_cache_evict_workspace(const dm_cache_table *table);
+int dm_cache_evict(const dm_cache_table *table, const dm_cache_pool *pools, int64_t npools, float *weights,
+                   int64_t weights_stride, const int32_t *budgets, int64_t recent, int32_t *kept,
+                   void *workspace, size_t workspace_bytes, void *stream);
 
 /* The queries' and keys' norms and rotation: q_out [B, T, Hq, D] and k_out [B, T, Hkv, D],
  * contiguous. q_weight and k_weight [D] may be NULL (no weight). */
@@ -440,7 +479,9 @@ int dm_qk_norm_rope_bwd(const dm_qk_norm_rope_desc *desc, const void *q, const v
 /* The same into a paged cache: q_out [N, Hq, D] contiguous; the keys, normalised and rotated (there
  * is no form without the norm), and the values as they are go to their rows of k_pages and
  * v_pages. No two tokens of a call may have one page row (sequences that share the page that they
- * append to, a page twice in a row's table): which of them it then holds is not said. */
+ * append to, a page twice in a row's table): which of them it then holds is not said. With
+ * desc->positions [N] the tokens turn by those and not by their places in the sequences (a cache whose
+ * rows have given up keys: dm_cache_evict). */
 int dm_qk_norm_rope_paged(const dm_qk_norm_rope_desc *desc, const dm_kv_pages *pages, const void *q,
                           const void *k, const void *v, const void *q_weight, const void *k_weight,
                           const float *inv_freq, void *q_out, void *k_pages, void *v_pages,
