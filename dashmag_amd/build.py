@@ -39,6 +39,7 @@ FLAGS = [
 # 690 us.
 EXTRA = {"gdr_chunk_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "decode_shared.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+         "attention_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "attention_fwd.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
          "attention_mfma_bwd.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
          "attention_bwd_w4.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-maxocc"]}

@@ -263,6 +263,613 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
     }
 }
 
+// ------------------------------------------------------------------------------------------
+// The 16-bit kernels (D = 64, 128 or 256, any page size)
+// ------------------------------------------------------------------------------------------
+//
+// Both products run on MFMA: S^T = K q^T (keys x 32 rows) and O^T += V^T P^T, S^T's output layout being P^T's
+// operand; the weights are rounded to the inputs' type for the second product (half a step a weight, as in the other
+// attention kernels), scores, maxima, sums and outputs stay in f32.
+//
+// NARROW tiles, of up to 32 rows: a wavefront is a worker and sweeps its keys in blocks of 32 through its own LDS
+// tiles. WIDE tiles, of up to 256 rows (128 at D = 256): a workgroup is a worker, its wavefronts have 32 rows each
+// and sweep the same keys in tiles of 64; wavefronts w and w + 4 of a SIMD run half a step apart, so that one's
+// products and the other's softmax run side by side. A sequence's rows lie in wide tiles where they are more than
+// kNarrowRows.
+//
+// Keys are read by their rows: a key's place in the pool, in 16-byte units, is looked up well ahead of its load (64 keys
+// ahead in registers; wide: 8 tiles ahead in an LDS ring), so any page size costs the same. A key of no
+// page, or behind the piece, is loaded from the pool's start and zeroed on its way into LDS.
+
+constexpr int kNarrowRows = 64;
+template <int D>
+constexpr int paged_waves() { return D == 256 ? 4 : 8; }
+constexpr uint32_t kNoKey = 0xffffffffu;
+
+struct PoolMap {
+    const char *k, *v;     // at the piece's key-value head
+    const int32_t *table;  // the sequence's
+    uint32_t page, row;    // 16-byte units of a page and of a row, keys' and values' alike
+    uint32_t size, pages;
+};
+__device__ __forceinline__ PoolMap pool_of(const PagedArgs &a, const PagedPiece &x, const void *k, const void *v) {
+    PoolMap m;
+    m.k = (const char *)k + (int64_t)x.kh * a.kh * 2;
+    m.v = (const char *)v + (int64_t)x.kh * a.vh * 2;
+    m.table = a.table + x.s * a.max_pages;
+    m.page = (uint32_t)(a.kb / 8), m.row = (uint32_t)(a.kt / 8);
+    m.size = (uint32_t)a.page_size, m.pages = (uint32_t)a.num_pages;
+    return m;
+}
+// Key j's entry in the table (-1 behind `end`), and its place from that.
+__device__ __forceinline__ int32_t entry_of(const PoolMap &m, int32_t j, int32_t end) {
+    return j < end ? m.table[(uint32_t)j / m.size] : -1;
+}
+__device__ __forceinline__ uint32_t place_of(const PoolMap &m, int32_t j, int32_t entry) {
+    return (uint32_t)entry < m.pages ? (uint32_t)entry * m.page + ((uint32_t)j % m.size) * m.row : kNoKey;
+}
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 load_nt(const char *p) {
+    const u32x4 x = __builtin_nontemporal_load((const u32x4 *)p);
+    return make_uint4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ uint4 only(bool ok, const uint4 &x) {
+    return make_uint4(ok ? x.x : 0u, ok ? x.y : 0u, ok ? x.z : 0u, ok ? x.w : 0u);
+}
+
+// 32 rows' queries: loaded along the rows (a load then touches few cache lines), sorted into operands through the
+// wavefront's own 32 rows of LDS. slots: in the order of row_frag. Nothing is waited for before settle_q.
+template <int D>
+struct QueryRows {
+    Frag8 f[D / 16];
+};
+template <int D>
+__device__ __forceinline__ void load_q(const PagedArgs &a, const RowKeys &k, const void *q, QueryRows<D> &w) {
+    constexpr int LPR = D / 8, RPL = 64 / LPR;  // lanes a row, rows a load
+    const int lane = threadIdx.x & 63;
+    const int64_t off = (int64_t)k.tok * a.qt + (int64_t)k.head * a.qh;  // (without a row: the piece's first)
+#pragma unroll
+    for (int u = 0; u < D / 16; u++) {
+        const int x = u * RPL + lane / LPR;
+        const int64_t at = __shfl((long long)off, x, 64);
+        w.f[u].u = *(const uint4 *)((const uint16_t *)q + at + (lane % LPR) * 8);
+    }
+}
+template <int D>
+__device__ __forceinline__ void settle_q(const PagedArgs &a, uint16_t *rows, bool slots, QueryRows<D> &w) {
+    constexpr int LPR = D / 8, RPL = 64 / LPR, KS = D + 8;
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int u = 0; u < D / 16; u++) *(uint4 *)(rows + (u * RPL + lane / LPR) * KS + (lane % LPR) * 8) = w.f[u].u;
+    __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS accesses complete in order)
+    const uint16_t *mine = rows + col * KS;
+    const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;  // (the softmax takes a scale above 0)
+#pragma unroll
+    for (int s = 0; s < D / 16; s++) {
+        uint4 x;
+        if (slots) {
+            const uint2 l = *(const uint2 *)(mine + s * 16 + half * 4), u = *(const uint2 *)(mine + s * 16 + 8 + half * 4);
+            x = make_uint4(l.x, l.y, u.x, u.y);
+        } else {
+            x = *(const uint4 *)(mine + s * 16 + half * 8);
+        }
+        w.f[s].u = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The values that were taken out of V, added for the rows that see them: the keys of [j0, j1) again, one at a time.
+template <int DT, int D>
+__device__ __forceinline__ void add_back16(const PoolMap &m, int32_t j0, int32_t j1, const RowKeys &rk, f32x16_t (&acc)[D / 32]) {
+    const int lane = threadIdx.x & 63;
+    for (int32_t j = j0; j < j1; j++) {
+        const uint32_t at = place_of(m, j, entry_of(m, j, j1));
+        if (at == kNoKey || j < rk.lo || j >= rk.hi) continue;
+        const uint16_t *row = (const uint16_t *)(m.v + (uint64_t)at * 16);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                uint32_t x = *(const uint32_t *)(row + dt * 32 + crow(i, lane));  // elements i and i + 1
+                x &= not_finite<DT>(x);
+                acc[dt][i] += unpack_lo<DT>(x);
+                acc[dt][i + 1] += unpack_hi<DT>(x);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (with every load of a row up front the registers run out)
+        }
+    }
+}
+
+// A wavefront's 32 rows from `first` on: outputs and log-sum-exps of a whole tile, or its place in the workspace, the
+// lanes along the rows through its own LDS (32 rows of D + 4 floats).
+template <int DT, int D>
+__device__ __forceinline__ void finish_rows(const PagedArgs &a, const PagedLine &l, const PagedPiece &x, const RowKeys &rk,
+                                            int first, const f32x16_t (&acc)[D / 32], float m, float sum, float *rows) {
+    constexpr int JS = D + 4, LPR = D / 4, RPL = 64 / LPR;
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, n = min(32, x.rows - first);
+    const float f = !x.whole ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);  // (NaN is not 0)
+#pragma unroll
+    for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *(float4 *)(rows + col * JS + dt * 32 + g * 8 + half * 4) =
+                make_float4(acc[dt][g * 4] * f, acc[dt][g * 4 + 1] * f, acc[dt][g * 4 + 2] * f, acc[dt][g * 4 + 3] * f);
+    __builtin_amdgcn_wave_barrier();
+    const int64_t place = (int64_t)x.slot * l.pitch + first;
+    if (half == 0 && rk.on) {
+        if (!x.whole)
+            l.ml[place + col] = make_float2(m, sum);
+        else if (a.lse)
+            a.lse[(int64_t)rk.tok * a.hq + rk.head] = lse_of(m, sum);
+    }
+    const int64_t mine = (int64_t)rk.tok * a.hq + rk.head;
+    for (int r = 0; r < n; r += RPL) {
+        const int y = r + lane / LPR, z = min(y, 31), c = lane % LPR * 4;
+        const int64_t row = __shfl((long long)mine, z, 64);
+        const float4 o = *(const float4 *)(rows + z * JS + c);
+        if (y >= n) continue;
+        if (x.whole)
+            *(uint2 *)((uint16_t *)a.o + row * D + c) = make_uint2(pack2<DT>(o.x, o.y), pack2<DT>(o.z, o.w));
+        else
+            *(float4 *)(l.o + (place + y) * D + c) = o;
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <int D>
+struct NarrowTile {
+    static constexpr int KS = D + 8, VS = D + 32;
+    alignas(16) uint16_t k[32 * KS], v[32 * VS];
+};
+static_assert(sizeof(NarrowTile<64>) >= 32 * 68 * 4 && sizeof(NarrowTile<256>) >= 32 * 260 * 4,
+              "a tile's results go through its place");
+
+template <int DT, int D>
+__device__ __forceinline__ void paged_narrow(const PagedArgs &a, const PagedLine &l, const PagedPiece &x, const PoolMap &map,
+                                             const void *q, NarrowTile<D> &t) {
+    constexpr int KS = NarrowTile<D>::KS, VS = NarrowTile<D>::VS, KST = D / 16, DTN = D / 32;
+    constexpr int LPR = D / 8, RPL = 64 / LPR, NLD = 32 / RPL;  // lanes a row, rows a load, loads
+    const int lane = threadIdx.x & 63, col = lane & 31;
+    const int32_t s0 = x.s0, s1 = x.s1;
+    const float qscale = fabsf(a.scale) * kLog2e;
+    // the entries and places of the 64 keys at hand, a lane each, and the entries of the 64 behind them
+    int32_t ahead = entry_of(map, s0 + lane, s1);
+    const RowKeys rk = row_keys(a, x, 0);
+    QueryRows<D> qr;
+    load_q<D>(a, rk, q, qr);
+    uint32_t at = place_of(map, s0 + lane, ahead);
+    ahead = entry_of(map, s0 + 64 + lane, s1);
+    uint4 sk[NLD], sv[NLD];
+    uint32_t have = 0;  // the loads of this lane that are keys'
+    auto load = [&](int32_t n) __attribute__((always_inline)) {  // the n-th 32 keys
+        have = 0;
+#pragma unroll
+        for (int u = 0; u < NLD; u++) {
+            const uint32_t p = __shfl(at, (n & 1) * 32 + RPL * u + lane / LPR, 64);
+            const bool ok = p != kNoKey;
+            have |= (uint32_t)ok << u;
+            const uint64_t off = (uint64_t)(ok ? p : 0u) * 16 + (lane % LPR) * 16;
+            sk[u] = load_nt(map.k + off);
+            sv[u] = load_nt(map.v + off);
+        }
+    };
+    f32x16_t acc[DTN];
+#pragma unroll
+    for (int dt = 0; dt < DTN; dt++) acc[dt] = zero16();
+    float m = -INFINITY, sum = 0.f;
+    uint32_t bad = 0;
+    const int32_t blocks = (s1 - s0 + 31) / 32;
+    if (blocks > 0) {
+        load(0);
+        settle_q<D>(a, t.k, true, qr);
+        for (int32_t n = 0; n < blocks; n++) {
+            const int32_t j0 = s0 + n * 32;
+            const bool cut = j0 < rk.flo || j0 + 32 > rk.fhi;
+            if (!__all(have == (1u << NLD) - 1)) {
+#pragma unroll
+                for (int u = 0; u < NLD; u++) {
+                    const bool ok = have >> u & 1;
+                    sk[u] = only(ok, sk[u]), sv[u] = only(ok, sv[u]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < NLD; u++) {
+                const int r = RPL * u + lane / LPR, c = (lane % LPR) * 8;
+                *(uint4 *)(t.k + r * KS + c) = sk[u];
+                *(uint4 *)(t.v + r * VS + c) = sv[u];
+            }
+            if (cut) {  // (in LDS: the loads' registers are full)
+#pragma unroll 1
+                for (int u = 0; u < NLD; u++) {
+                    uint4 *p = (uint4 *)(t.v + (RPL * u + lane / LPR) * VS + (lane % LPR) * 8), y = *p;
+                    const uint32_t out = take_out<DT>(y);
+                    if (out) *p = y;
+                    bad |= out;
+                }
+            }
+            if (n & 1) {
+                at = place_of(map, j0 + 32 + lane, ahead);
+                ahead = entry_of(map, j0 + 96 + lane, s1);
+            }
+            load(n + 1);  // (past the last: the pool's start, unused)
+            f32x16_t sc = zero16();
+#pragma unroll
+            for (int st = 0; st < KST; st++) sc = mfma32<DT>(row_frag(t.k, KS, 0, st * 16, lane), qr.f[st], sc);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int32_t key = j0 + crow(i, lane);
+                sc[i] = !cut || (key >= rk.lo && key < rk.hi) ? sc[i] * qscale : -INFINITY;
+                mx = fmaxf(mx, sc[i]);
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const bool grow = mx > m + 8.f;
+            if (__any(grow)) {
+                const float mn = grow ? mx : m, alpha = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+                m = mn;
+                sum *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DTN; dt++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) acc[dt][i] *= alpha;
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
+            float ps = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                sc[i] = fast_exp2(sc[i] - ref);
+                ps += sc[i];
+            }
+            sum += ps;
+            const Frag8 p0 = c_frag<DT>(sc, 0), p1 = c_frag<DT>(sc, 1);
+#pragma unroll
+            for (int dt = 0; dt < DTN; dt++) {
+                acc[dt] = mfma32<DT>(lds_tr_frag(t.v, VS, 0, dt * 32, lane), p0, acc[dt]);
+                acc[dt] = mfma32<DT>(lds_tr_frag(t.v, VS, 16, dt * 32, lane), p1, acc[dt]);
+            }
+        }
+    }
+    if (__any(bad))
+        for (int32_t j0 = s0; j0 < s1; j0 += 32)
+            if (j0 < rk.flo || j0 + 32 > rk.fhi) add_back16<DT, D>(map, j0, min(j0 + 32, s1), rk, acc);
+    finish_rows<DT, D>(a, l, x, rk, 0, acc, m, sum + __shfl_xor(sum, 32, 64), (float *)&t);
+}
+
+template <int D>
+struct WideTiles {
+    static constexpr int KS = D + 8, VS = D + 32, NW = paged_waves<D>();
+    alignas(16) uint16_t k[2][64 * KS], v[2][64 * VS];
+    uint32_t places[1024];  // of 16 tiles' keys, see `fill`
+    int32_t lo[NW], hi[NW], bad;
+};
+
+template <int DT, int D>
+__device__ __forceinline__ void paged_wide(const PagedArgs &a, const PagedLine &l, const PagedPiece &x, const PoolMap &map,
+                                           const void *q, WideTiles<D> &sm, NarrowTile<D> *area) {
+    constexpr int NW = paged_waves<D>(), NT = NW * 64, KS = WideTiles<D>::KS, VS = WideTiles<D>::VS;
+    constexpr int CPR = D / 8, RSTEP = NT / CPR, NCH = 64 / RSTEP;  // pieces a row, rows at a time, pieces a thread
+    constexpr int KST = D / 16, DTN = D / 32, AHEAD = 2, PK = 512 / NT;
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, wave = uni(threadIdx.x >> 6);
+    const bool first = NW == 4 || wave < 4;  // products first in each step
+    const int32_t s0 = x.s0, s1 = x.s1, nt = (s1 - s0 + 63) / 64;
+    int32_t entry[PK], entry1[PK];
+    auto look_up = [&](int32_t key, int32_t (&entry)[PK]) __attribute__((always_inline)) {  // of 512 keys from `key` on
+#pragma unroll
+        for (int u = 0; u < PK; u++) entry[u] = entry_of(map, s0 + key + u * NT + (int32_t)threadIdx.x, s1);
+    };
+    auto fill = [&](int32_t key, const int32_t (&entry)[PK]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < PK; u++) {
+            const int32_t j = key + u * NT + (int32_t)threadIdx.x;
+            sm.places[j & 1023] = place_of(map, s0 + j, entry[u]);
+        }
+    };
+    look_up(0, entry);
+    look_up(512, entry1);
+    const RowKeys rk = row_keys(a, x, wave * 32);
+    QueryRows<D> qr;
+    load_q<D>(a, rk, q, qr);
+    // the keys that any of the wavefront's rows sees
+    int32_t wlo = rk.on ? rk.lo : INT32_MAX, whi = rk.hi;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        wlo = min(wlo, __shfl_xor(wlo, o, 64));
+        whi = max(whi, __shfl_xor(whi, o, 64));
+    }
+    wlo = uni(wlo), whi = uni(whi);
+    __syncthreads();  // (the last piece's results have left LDS)
+    settle_q<D>(a, (uint16_t *)&area[wave], false, qr);
+    __syncthreads();  // (the queries' way through LDS is what the places and tiles lie in)
+    fill(0, entry);
+    fill(512, entry1);
+    if (lane == 0) sm.lo[wave] = rk.flo, sm.hi[wave] = rk.fhi;
+    if (threadIdx.x == 0) sm.bad = 0;
+    __syncthreads();
+    int32_t tlo = INT32_MIN, thi = INT32_MAX;  // the keys that every row of the tile sees
+#pragma unroll
+    for (int w = 0; w < NW; w++) tlo = max(tlo, sm.lo[w]), thi = min(thi, sm.hi[w]);
+    tlo = uni(tlo), thi = uni(thi);
+    // (a scale of 0 as the smallest: a masked score stays -inf, the others' weights are alike)
+    const float c2 = a.scale == 0.f ? 1.2e-38f : fabsf(a.scale) * kLog2e;
+
+    // staging: NCH pieces of a tile's K and of its V a thread; a tile's places are read from LDS a step before its
+    // keys are loaded, and kept for its values
+    const int row0 = threadIdx.x / CPR, lc = threadIdx.x % CPR;
+    uint4 rk4[NCH], rv4[NCH];
+    uint32_t ak[NCH], av[NCH];
+    bool okk[NCH], okv[NCH];
+    auto offsets = [&](int32_t j) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < NCH; u++) ak[u] = sm.places[(j * 64 + row0 + u * RSTEP) & 1023];
+    };
+    auto load = [&](const char *base, const uint32_t (&at)[NCH], uint4 (&y)[NCH], bool (&ok)[NCH]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < NCH; u++) {
+            ok[u] = at[u] != kNoKey;
+            y[u] = *(const uint4 *)(base + (uint64_t)(ok[u] ? at[u] : 0u) * 16 + lc * 16);
+        }
+    };
+    auto load_v = [&]() __attribute__((always_inline)) { load(map.v, av, rv4, okv); };
+    // the keys of tile j, then the places of the tile behind it
+    auto load_k = [&](int32_t j) __attribute__((always_inline)) {
+        load(map.k, ak, rk4, okk);
+#pragma unroll
+        for (int u = 0; u < NCH; u++) av[u] = ak[u];
+        offsets(j + 1);
+    };
+    auto store_k = [&](int32_t j) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < NCH; u++)
+            *(uint4 *)(sm.k[j & 1] + (row0 + u * RSTEP) * KS + lc * 8) = only(okk[u], rk4[u]);
+    };
+    auto store_v = [&](int32_t j) __attribute__((always_inline)) {
+        const int32_t t = s0 + j * 64;
+#pragma unroll
+        for (int u = 0; u < NCH; u++) rv4[u] = only(okv[u], rv4[u]);
+        if (t < tlo || t + 64 > thi) {  // (a tile that some row does not see all of)
+            uint32_t bad = 0;
+#pragma unroll
+            for (int u = 0; u < NCH; u++) bad |= take_out<DT>(rv4[u]);
+            if (__any(bad) && lane == 0) sm.bad = 1;
+        }
+#pragma unroll
+        for (int u = 0; u < NCH; u++) *(uint4 *)(sm.v[j & 1] + (row0 + u * RSTEP) * VS + lc * 8) = rv4[u];
+    };
+    auto sees = [&](int32_t j) __attribute__((always_inline)) {
+        const int32_t j0 = s0 + j * 64;
+        return j >= 0 && j < nt && j0 < whi && j0 + 64 > wlo;
+    };
+    f32x16_t acc[DTN], s[2];
+    Frag8 pf[2][2];
+    float m = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DTN; dt++) acc[dt] = zero16();
+    // O^T of step j - 1 first, whose operands are dead when S^T's take their registers; each fragment is
+    // read from LDS ahead of the products in front of it.
+    auto products = [&](int32_t j) __attribute__((always_inline)) {
+        const uint16_t *tk = sm.k[j & 1] + col * KS + half * 8, *tv = sm.v[(j - 1) & 1];
+        Frag8 vf[2][DTN], kf[AHEAD + 1][2];
+        auto read_v = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+            for (int dt = 0; dt < DTN; dt++) vf[g & 1][dt] = lds_tr_frag(tv, VS, g * 16, dt * 32, lane);
+        };
+        auto read_k = [&](int st) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) kf[st % (AHEAD + 1)][t].u = *(const uint4 *)(tk + t * 32 * KS + st * 16);
+        };
+        __builtin_amdgcn_s_setprio(1);
+        read_v(0);  // (of a step without a tile, too: whatever lies there, unused)
+        if (sees(j - 1)) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                if (g < 3) read_v(g + 1);
+#pragma unroll
+                for (int dt = 0; dt < DTN; dt++) acc[dt] = mfma32<DT>(vf[g & 1][dt], pf[g >> 1][g & 1], acc[dt]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (sees(j)) {
+#pragma unroll
+            for (int st = 0; st < AHEAD; st++) read_k(st);
+#pragma unroll
+            for (int t = 0; t < 2; t++) s[t] = zero16();
+#pragma unroll
+            for (int st = 0; st < KST; st++) {
+                if (st + AHEAD < KST) read_k(st + AHEAD);
+#pragma unroll
+                for (int t = 0; t < 2; t++) s[t] = mfma32<DT>(kf[st % (AHEAD + 1)][t], qr.f[st], s[t]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        __builtin_amdgcn_s_setprio(0);
+    };
+    auto softmax = [&](int32_t jj) __attribute__((always_inline)) {
+        const int32_t j0 = s0 + jj * 64;
+        if (j0 < rk.flo || j0 + 64 > rk.fhi) {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int32_t j = j0 + t * 32 + crow(i, lane);
+                    s[t][i] = ((j >= rk.lo) & (j < rk.hi)) ? s[t][i] : -INFINITY;
+                }
+        }
+        float tmax = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) tmax = fmaxf(tmax, s[t][i]);
+        tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
+        const float tmc = tmax * c2;
+        const bool grow = tmc - m > 8.f;  // false while both are -inf
+        if (__any(grow)) {
+            const float mnew = grow ? tmc : m, alpha = grow ? fast_exp2(m - mnew) : 1.f;  // 0 from -inf
+            m = mnew;
+            sum *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DTN; dt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[dt][i] *= alpha;
+        }
+        const float mneg = m == -INFINITY ? 0.f : -m;
+        float ps = 0.f;  // (the tile's weights first: one at a time, long sums of like ones come out short)
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    e[i] = fast_exp2(fmaf(s[t][8 * u + i], c2, mneg));
+                    ps += e[i];
+                }
+                pf[t][u].u = make_uint4(pack2<DT>(e[0], e[1]), pack2<DT>(e[2], e[3]), pack2<DT>(e[4], e[5]),
+                                        pack2<DT>(e[6], e[7]));
+            }
+        sum += ps;
+    };
+    // Wavefronts 0-3 store K_{j+1} and V_j during their softmax of step j, wavefronts 4-7, half a step
+    // later, K_{j+2} and V_{j+1}: each tile is whole before its first reader's step.
+    const int32_t ahead = first ? 0 : 1;
+    auto stage = [&](int32_t j) __attribute__((always_inline)) {
+        store_k(j + 1 + ahead);
+        store_v(j + ahead);
+        load_v();
+        load_k(j + 2 + ahead);
+        // The ring's half of the tiles j - 8 .. j - 1, whose places all have read, goes to j + 8 .. j + 15: looked up
+        // now and written two steps later, three steps before any of them is read.
+        if (j > 0 && (j & 7) == 0) look_up(64 * (j + 8), entry);
+        if (j > 2 && (j & 7) == 2) fill(64 * (j + 6), entry);
+    };
+    if (nt > 0) {
+        offsets(0);
+        load_k(0);
+        load_v();
+        store_k(0);
+        load_k(1);
+    }
+    __syncthreads();
+    if (!first) {
+        if (nt > 0) stage(-1);
+        __syncthreads();
+    }
+    for (int32_t j = 0; j <= nt; j++) {
+        products(j);
+        __syncthreads();
+        if (sees(j)) softmax(j);
+        if (j < nt) stage(j);
+        __syncthreads();
+    }
+    if (first) __syncthreads();
+    const bool rows = wave * 32 < x.rows;
+    if (rows && sm.bad)
+        for (int32_t j0 = s0; j0 < s1; j0 += 64)
+            if (j0 < tlo || j0 + 64 > thi) add_back16<DT, D>(map, j0, min(j0 + 64, s1), rk, acc);
+    __syncthreads();  // (every wavefront is past its last tile, and has read whether there was a bad one)
+    if (rows) finish_rows<DT, D>(a, l, x, rk, wave * 32, acc, m, sum + __shfl_xor(sum, 32, 64), (float *)&area[wave]);
+}
+
+// Everything uniform in a wavefront that the loads' scalar bases come from.
+__device__ __forceinline__ void settle_piece(PagedPiece &x) {
+    x.tok = uni(x.tok), x.head = uni(x.head), x.rows = uni(x.rows), x.pos = uni(x.pos), x.kh = uni(x.kh), x.s = uni(x.s);
+    x.s0 = uni(x.s0), x.s1 = uni(x.s1), x.slot = uni(x.slot), x.whole = uni(x.whole);
+}
+
+// A call whose sequences all have few rows: every wavefront a worker.
+template <int DT, int D>
+__device__ __forceinline__ void narrow_share(const PagedArgs &a, const PagedLine &l, const PagedShare &sh, int32_t worker,
+                                             PagedWalk &walk, int64_t p, const void *q, const void *k, const void *v,
+                                             NarrowTile<D> &tile) {
+    if ((threadIdx.x & 63) == 0 && worker < l.workers) l.jobs[worker].rows = 0;
+    if (p < 0) return;
+    const int64_t end = sh.at(worker + 1);
+    for (;;) {
+        int64_t next;
+        int32_t last;
+        PagedPiece x = piece_of(a, l, walk, sh, worker, p, end, &next, &last);
+        settle_piece(x);
+        if (last >= 0 && (threadIdx.x & 63) == 0) l.jobs[worker] = PagedJob{x.tok, x.head, x.per, x.rows, worker - 1, last};
+        paged_narrow<DT, D>(a, l, x, pool_of(a, x, k, v), q, tile);
+        p = next;
+        if (p >= end || !walk_on(a, l, walk, next)) return;
+    }
+}
+template <int DT, int D>
+__global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void paged_narrow_kernel(PagedArgs a, PagedLine l, const void *__restrict__ q,
+                                                                              const void *__restrict__ k,
+                                                                              const void *__restrict__ v) {
+    __shared__ union {
+        PlanSmem<256> plan;
+        NarrowTile<D> tiles[4];
+    } sm;
+    const int wave = uni(threadIdx.x >> 6);
+    const int32_t worker = blockIdx.x * 4 + wave;
+    PagedWalk walk;
+    int64_t p;
+    bool valid;
+    const PagedShare sh = plan_line<256>(
+        a, l, sm.plan, [&](const PagedShare &s) { return worker < s.workers ? s.at(worker) : -1; }, &walk, &p, &valid);
+    fill_outside<DT>(a, valid);
+    narrow_share<DT, D>(a, l, sh, worker, walk, p, q, k, v, sm.tiles[wave]);
+}
+
+// Any call: the wide tiles' line, a workgroup a worker, and the narrow tiles', a wavefront a worker. Every other
+// workgroup begins with its narrow share, so that reading and multiplying go on side by side.
+template <int DT, int D>
+__global__ __launch_bounds__((64 * paged_waves<D>()), (D == 256 ? 1 : 2)) void paged_mixed_kernel(PagedArgs a, PagedLine wide, PagedLine narrow,
+                                                                                   const void *__restrict__ q,
+                                                                                   const void *__restrict__ k,
+                                                                                   const void *__restrict__ v) {
+    constexpr int NW = paged_waves<D>();
+    __shared__ union {
+        PlanSmem<64 * NW> plan;
+        WideTiles<D> wide;
+        NarrowTile<D> tiles[NW];
+    } sm;
+    const int wave = uni(threadIdx.x >> 6);
+    for (int turn = 0; turn < 2; turn++) {
+        PagedWalk walk;
+        int64_t p;
+        bool valid;
+        if ((turn ^ (int)(blockIdx.x >> 3)) & 1) {
+            const int32_t worker = blockIdx.x * NW + wave;
+            const PagedShare sh = plan_line<64 * NW>(
+                a, narrow, sm.plan, [&](const PagedShare &s) { return worker < s.workers ? s.at(worker) : -1; }, &walk, &p,
+                &valid);
+            narrow_share<DT, D>(a, narrow, sh, worker, walk, p, q, k, v, sm.tiles[wave]);
+            __syncthreads();
+            continue;
+        }
+        // workgroups go to the XCDs in turn: each XCD has a part of the line of its own
+        int32_t worker = blockIdx.x;
+        const PagedShare sh = plan_line<64 * NW>(
+            a, wide, sm.plan,
+            [&](const PagedShare &s) {
+                if (s.workers == (int32_t)gridDim.x && s.workers % 8 == 0)
+                    worker = blockIdx.x % 8 * (s.workers / 8) + blockIdx.x / 8;
+                return worker < s.workers ? s.at(worker) : -1;
+            },
+            &walk, &p, &valid);
+        fill_outside<DT>(a, valid);
+        if (threadIdx.x == 0) wide.jobs[worker].rows = 0;
+        if (p < 0) continue;
+        const int64_t end = sh.at(worker + 1);
+        for (;;) {
+            int64_t next;
+            int32_t last;
+            PagedPiece x = piece_of(a, wide, walk, sh, worker, p, end, &next, &last);
+            settle_piece(x);
+            if (last >= 0 && threadIdx.x == 0)
+                wide.jobs[worker] = PagedJob{x.tok, x.head, x.per, x.rows, worker - 1, last};
+            paged_wide<DT, D>(a, wide, x, pool_of(a, x, k, v), q, sm.wide, sm.tiles);
+            p = next;
+            if (p >= end || !walk_on(a, wide, walk, next)) break;
+        }
+        __syncthreads();
+    }
+}
+
 // The pieces of a shared tile joined, a wavefront a row: the largest reference, then the outputs and sums by it, in
 // the order of the workers.
 template <int DT>
@@ -388,8 +995,23 @@ static PagedLine line_of(const dm_attention_desc *d, int32_t rt, int32_t over, i
     return l;
 }
 
+// The 16-bit kernels' calls: 16-byte pieces, keys' and values' pages laid out alike, places that 32 bits of
+// 16-byte units hold. (A size query comes without the pool.)
+static bool paged_fast_shape(const dm_attention_desc *d) {
+    if ((d->dtype != DM_BF16 && d->dtype != DM_F16) || (d->d != 64 && d->d != 128 && d->d != 256)) return false;
+    if (!d->strided) return true;
+    const dm_strides &k = d->sk, &v = d->sv;
+    return d->sq.t % 8 == 0 && d->sq.h % 8 == 0 && k.b % 8 == 0 && k.t % 8 == 0 && k.h % 8 == 0 && v.h % 8 == 0 &&
+           k.b == v.b && k.t == v.t;
+}
+static bool paged_fast_pool(const PagedArgs &a) {
+    const int64_t most = ((int64_t)1 << 32) * 8 - 8;  // elements
+    return a.num_pages > 0 && a.kb < most / a.num_pages / 2 && a.kt < most / a.page_size / 2;
+}
+
 struct PagedPlan {
-    PagedLine line;
+    bool fast, mixed;
+    PagedLine wide, narrow;  // the simple kernel's: narrow
     size_t bytes;
     size_t lse;  // where the weights' own log-sum-exps lie
 };
@@ -402,14 +1024,26 @@ static size_t place_line(const dm_attention_desc *d, PagedLine *l, char *base, s
     l->jobs = (PagedJob *)(base + at);
     return at + align_up((size_t)l->workers * sizeof(PagedJob));
 }
-static PagedPlan paged_plan(const dm_attention_desc *d, char *base, bool weights) {
+static PagedPlan paged_plan(const dm_attention_desc *d, char *base, bool weights, bool fast) {
     PagedPlan p{};
-    p.line = line_of(d, 32, 0, INT32_MAX);
-    p.line.workers = d->d > 128 ? 1024 : 2048;
-    p.line.unit = 32;
-    p.line.start = 64;
-    p.line.least = 192;
-    p.bytes = place_line(d, &p.line, base, 0);
+    const int64_t rep = d->hq / d->hkv;
+    p.fast = fast;
+    // (whether a sequence has more rows than a narrow one's is known only on the device, but for calls that cannot)
+    p.mixed = fast && (d->cu_seqlens_q ? d->tq : 1) * rep > kNarrowRows;
+    if (p.mixed) {
+        p.wide = line_of(d, d->d == 256 ? 128 : 256, kNarrowRows, INT32_MAX);
+        p.wide.workers = 256;
+        p.wide.unit = 64;
+        p.wide.start = 192;
+        p.wide.least = 512;
+        p.bytes = place_line(d, &p.wide, base, p.bytes);
+    }
+    p.narrow = line_of(d, 32, 0, p.mixed ? kNarrowRows : INT32_MAX);
+    p.narrow.workers = d->d > 128 ? 1024 : 2048;
+    p.narrow.unit = 32;
+    p.narrow.start = 64;
+    p.narrow.least = 192;
+    p.bytes = place_line(d, &p.narrow, base, p.bytes);
     p.lse = p.bytes;
     if (weights) p.bytes += align_up((size_t)(d->tq * d->hq) * sizeof(float));
     return p;
@@ -431,7 +1065,9 @@ extern "C" {
 
 size_t dm_attention_paged_workspace(const dm_attention_desc *d, int64_t page_size, int weights) {
     if (!paged_sizes(d) || page_size < 1 || d->hq == 0) return 0;
-    return paged_plan(d, nullptr, weights != 0).bytes;
+    // (which kernel runs also depends on the pool and the pointers' alignment)
+    return std::max(paged_plan(d, nullptr, weights != 0, false).bytes,
+                    paged_plan(d, nullptr, weights != 0, paged_fast_shape(d)).bytes);
 }
 
 int dm_attention_paged(const dm_attention_desc *d, const void *q, const void *k_pages, const void *v_pages,
@@ -467,7 +1103,6 @@ int dm_attention_paged(const dm_attention_desc *d, const void *q, const void *k_
         DM_LAUNCH_CHECK("attention_paged: fill");
         return DM_OK;
     }
-    const PagedPlan p = paged_plan(d, (char *)workspace, weights != nullptr);
     PagedArgs a{};
     a.S = (int32_t)d->b, a.N = (int32_t)d->tq, a.cap = (int32_t)d->tk, a.left = (int32_t)left_of(d);
     a.hq = (int32_t)d->hq, a.hkv = (int32_t)d->hkv, a.d = (int32_t)d->d, a.rep = (int32_t)(d->hq / d->hkv);
@@ -483,21 +1118,33 @@ int dm_attention_paged(const dm_attention_desc *d, const void *q, const void *k_
         a.qt = d->hq * d->d, a.qh = d->d;
         a.kb = a.vb = page_size * row, a.kt = a.vt = row, a.kh = a.vh = d->d;
     }
+    const bool fast = paged_fast_shape(d) && paged_fast_pool(a) && aligned_16b(q) && aligned_16b(k_pages) &&
+                      aligned_16b(v_pages) && aligned_16b(o);
+    const PagedPlan p = paged_plan(d, (char *)workspace, weights != nullptr, fast);
     a.o = o;
     a.lse = lse ? lse : (weights ? (float *)((char *)workspace + p.lse) : nullptr);
     // (four elements at a time where rows and bases allow it)
     const int64_t eb = dtype_bytes(d->dtype);
     const bool vec = ((d->d | a.kb | a.kt | a.kh | a.vb | a.vt | a.vh) & 3) == 0 &&
                      (((uintptr_t)k_pages | (uintptr_t)v_pages) & (4 * eb - 1)) == 0;
-    const PagedLine &l = p.line;
+    const PagedLine &l = p.narrow;
     const unsigned g = l.workers / 4;
-#define PAGED_V(DT, DP)                                                              \
-    if (vec)                                                                         \
-        paged_simple<DT, DP, 4><<<g, 256, 0, st>>>(a, l, q, k_pages, v_pages);       \
-    else                                                                             \
-        paged_simple<DT, DP, 1><<<g, 256, 0, st>>>(a, l, q, k_pages, v_pages);       \
-    paged_join<DT><<<dim3(l.workers, (l.pitch + 3) / 4), 256, 0, st>>>(a, l);        \
+#define PAGED_W(DT, DP)                                                                                       \
     if (weights) paged_weights_simple<DT, DP><<<1024, 256, 0, st>>>(a, q, k_pages, weights, weights_stride)
+#define PAGED_V(DT, DP)                                                                                       \
+    if constexpr (DT != DM_F32) {                                                                             \
+        if (p.mixed)                                                                                          \
+            paged_mixed_kernel<DT, DP><<<256, 64 * paged_waves<DP>(), 0, st>>>(a, p.wide, l, q, k_pages, v_pages); \
+        else if (fast)                                                                                        \
+            paged_narrow_kernel<DT, DP><<<g, 256, 0, st>>>(a, l, q, k_pages, v_pages);                        \
+    }                                                                                                         \
+    if (!fast && vec)                                                                                         \
+        paged_simple<DT, DP, 4><<<g, 256, 0, st>>>(a, l, q, k_pages, v_pages);                                \
+    else if (!fast)                                                                                           \
+        paged_simple<DT, DP, 1><<<g, 256, 0, st>>>(a, l, q, k_pages, v_pages);                                \
+    paged_join<DT><<<dim3(l.workers, (l.pitch + 3) / 4), 256, 0, st>>>(a, l);                                 \
+    if (p.mixed) paged_join<DT><<<dim3(p.wide.workers, (p.wide.pitch + 3) / 4), 256, 0, st>>>(a, p.wide);     \
+    PAGED_W(DT, DP)
 #define PAGED(DT)               \
     if (padded(d->d) == 64) {   \
         PAGED_V(DT, 64);        \
@@ -515,6 +1162,7 @@ int dm_attention_paged(const dm_attention_desc *d, const void *q, const void *k_
     }
 #undef PAGED
 #undef PAGED_V
+#undef PAGED_W
     probe_add(DM_PROBE_ATTN_PAGED);
     if (weights) probe_add(DM_PROBE_ATTN_WEIGHTS);
     DM_LAUNCH_CHECK("attention_paged: launch");

@@ -332,27 +332,6 @@ __device__ __forceinline__ uint64_t block_at(const SharedArgs &a, const PageMap 
     return pg >= 0 && pg < a.num_pages ? (uint64_t)(uint32_t)pg * m.page + ((uint32_t)j - e * m.size) * m.row : kNoBlock;
 }
 
-// All ones in each 16-bit half of w that is not finite: its exponent plus one carries into the sign's
-// place. (Arithmetic alone: a comparison an element would hold a mask of lanes for each.)
-template <int DT>
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-    constexpr uint32_t e = DT == DM_BF16 ? 0x7f807f80u : 0x7c007c00u, one = DT == DM_BF16 ? 0x00800080u : 0x04000400u;
-    const uint32_t m = ((w & e) + one) & 0x80008000u;
-    return (m - (m >> 15)) | m;
-}
-// Values that are not finite taken out of a piece of V (whoever sees them adds them at the end).
-template <int DT>
-__device__ __forceinline__ uint32_t take_out(uint4 &x) {
-    uint32_t *w = (uint32_t *)&x, any = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t m = not_finite<DT>(w[i]);
-        w[i] &= ~m;
-        any |= m;
-    }
-    return any;
-}
-
 template <int D, bool WIDE>
 struct SharedSmem {
     static constexpr int NW = shared_waves<D, WIDE>(), KS = D + 8, VS = D + 32;

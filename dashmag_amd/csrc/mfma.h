@@ -165,6 +165,27 @@ __device__ __forceinline__ float unpack_hi(uint32_t w) {
     }
 }
 
+// All ones in each 16-bit half of w that is not finite: its exponent plus one carries into the sign's
+// place. (Arithmetic alone: a comparison an element would hold a mask of lanes for each.)
+template <int DT>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    constexpr uint32_t e = DT == DM_BF16 ? 0x7f807f80u : 0x7c007c00u, one = DT == DM_BF16 ? 0x00800080u : 0x04000400u;
+    const uint32_t m = ((w & e) + one) & 0x80008000u;
+    return (m - (m >> 15)) | m;
+}
+// Values that are not finite taken out of a piece of V (whoever sees them adds them at the end).
+template <int DT>
+__device__ __forceinline__ uint32_t take_out(uint4 &x) {
+    uint32_t *w = (uint32_t *)&x, any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t m = not_finite<DT>(w[i]);
+        w[i] &= ~m;
+        any |= m;
+    }
+    return any;
+}
+
 // Raw buffer loads: out-of-range offsets (>= the resource's byte count) return zeros, so tile
 // loads need no bounds branches. The offsets are 32-bit byte offsets from the resource's base.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void *base, uint32_t bytes) {

@@ -171,6 +171,7 @@ __device__ __forceinline__ PagedShare plan_line(const PagedArgs &a, const PagedL
         }
         base += all;
     }
+    __syncthreads();  // (the sums have been read)
     if (found < 0) {
         *p = -1;
         return sh;
