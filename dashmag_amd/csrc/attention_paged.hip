@@ -974,6 +974,213 @@ __global__ __launch_bounds__(256) void paged_weights_simple(PagedArgs a, const v
     }
 }
 
+// The 16-bit kernel: a workgroup takes a tile of keys, 64 of them a wavefront (32 at D = 256) in registers as the second
+// operand, and sweeps the rows that see them, 64 at a time through LDS, head by head. A key's sum over a step's 32
+// rows is taken first, then over a head's, then over the heads (one at a time, a long sum would lose bits).
+template <int D>
+constexpr int key_cols() { return D == 256 ? 1 : 2; }  // 32-key columns of a wavefront
+template <int D>
+constexpr int key_tile() { return 8 * 32 * key_cols<D>(); }
+template <int D>
+union KeyTiles {
+    static constexpr int KS = D + 8;
+    PlanSmem<512> plan;
+    struct {
+        alignas(16) uint16_t q[2][64 * KS];
+        alignas(16) float ref[2][64];  // -lse in log2 units, -inf for a row that is none or sees no key
+        alignas(16) int32_t pos[2][64];
+    } rows;
+    alignas(16) uint16_t keys[8][32 * KS];
+};
+
+template <int DT, int D>
+__global__ __launch_bounds__(512, 2) void paged_weights_kernel(PagedArgs a, KeyLine l, const void *__restrict__ q,
+                                                              const void *__restrict__ k, float *__restrict__ weights,
+                                                              int64_t stride) {
+    constexpr int KS = KeyTiles<D>::KS, COLS = key_cols<D>(), KST = D / 16, LPR = D / 8, RPL = 64 / LPR, NLD = 32 / RPL;
+    constexpr int RSTEP = 512 / LPR, NCH = 64 / RSTEP;  // rows at a time, 16-byte pieces a thread, of a step's queries
+    __shared__ KeyTiles<D> sm;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), col = lane & 31, half = lane >> 5;
+    const int32_t worker = blockIdx.x;
+    PagedWalk walk;
+    int64_t p;
+    bool valid;
+    const PagedShare sh = plan_line<512>(
+        a, l, sm.plan, [&](const PagedShare &s) { return worker < s.workers ? s.at(worker) : -1; }, &walk, &p, &valid);
+    if (tid == 0) l.jobs[worker].rows = 0;
+    if (p < 0) return;
+    const int64_t end = sh.at(worker + 1);
+    const float c2 = a.scale * kLog2e;
+    const int32_t rep = a.rep, more = 64 / rep, rest = 64 - more * rep;  // 64 rows on: tokens and heads
+    for (;;) {
+        int64_t next;
+        int32_t last;
+        const KeyPiece x = key_piece(a, l, walk, sh, worker, p, end, &next, &last);
+        if (last >= 0 && tid == 0) l.jobs[worker] = PagedJob{x.s, walk.t, 0, 1, worker - 1, last};
+        const int32_t s = uni(x.s), len = uni(walk.q.len), p0 = uni(walk.q.len - walk.q.n), tok0 = uni(walk.q.first);
+        const int32_t from = uni(x.from), to = uni(x.to), steps = uni(x.steps);
+        const int32_t w0 = uni(x.k0) + wave * 32 * COLS;  // the wavefront's first key
+        const int32_t *entries = a.table + s * a.max_pages;
+        uint32_t at = kNoKey;  // the place of key w0 + lane
+        if (w0 + lane < len && lane < 32 * COLS) {
+            const uint32_t e = (uint32_t)(w0 + lane) / (uint32_t)a.page_size, row = (uint32_t)(w0 + lane) - e * (uint32_t)a.page_size;
+            const int32_t pg = entries[e];
+            if ((uint32_t)pg < (uint32_t)a.num_pages) at = (uint32_t)pg * (uint32_t)(a.kb / 8) + row * (uint32_t)(a.kt / 8);
+        }
+        float total[COLS];
+#pragma unroll
+        for (int c = 0; c < COLS; c++) total[c] = 0.f;
+        for (int32_t r = uni(x.r0), r1 = uni(x.r1); r < r1;) {
+            const int32_t kh = uni(r / steps), n = min(r1, (kh + 1) * steps) - r;  // this head's steps
+            const int32_t first = from + (r - kh * steps) * 64;                     // its first row
+            const char *base = (const char *)k + (int64_t)kh * a.kh * 2;
+            uint4 sk[COLS][NLD];
+#pragma unroll
+            for (int c = 0; c < COLS; c++)
+#pragma unroll
+                for (int u = 0; u < NLD; u++) {
+                    const uint32_t y = __shfl(at, c * 32 + RPL * u + lane / LPR, 64);
+                    const bool ok = y != kNoKey;
+                    sk[c][u] = only(ok, *(const uint4 *)(base + (uint64_t)(ok ? y : 0u) * 16 + (lane % LPR) * 16));
+                }
+            // this thread's rows of a step: token and head of each, moved on by 64 rows a step
+            int32_t t[NCH + 1], h[NCH + 1];
+#pragma unroll
+            for (int u = 0; u <= NCH; u++) {
+                const int32_t y = first + (u < NCH ? tid / LPR + u * RSTEP : lane);
+                t[u] = y / rep, h[u] = y - t[u] * rep;
+            }
+            int32_t ts = uni(first / rep), hs = uni(first - ts * rep);  // the step's first row
+            uint4 sq[NCH];
+            float ref = 0.f;
+            int32_t pos = 0;
+            auto load = [&](int32_t i) __attribute__((always_inline)) {  // step i's queries
+#pragma unroll
+                for (int u = 0; u < NCH; u++) {
+                    const bool ok = first + i * 64 + tid / LPR + u * RSTEP < to;
+                    const int64_t y = (int64_t)(tok0 + (ok ? t[u] : 0)) * a.qt + (int64_t)(kh * rep + (ok ? h[u] : 0)) * a.qh;
+                    sq[u] = only(ok, *(const uint4 *)((const uint16_t *)q + y + (tid % LPR) * 8));
+                }
+                if (wave == 0) {
+                    const bool ok = first + i * 64 + lane < to;
+                    const float ls = ok ? a.lse[(int64_t)(tok0 + t[NCH]) * a.hq + kh * rep + h[NCH]] : -INFINITY;
+                    ref = ls == -INFINITY ? ls : -ls * kLog2e;
+                    pos = p0 + t[NCH];
+                }
+#pragma unroll
+                for (int u = 0; u <= NCH; u++) {
+                    t[u] += more, h[u] += rest;
+                    if (h[u] >= rep) t[u]++, h[u] -= rep;
+                }
+            };
+            auto store = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+                for (int u = 0; u < NCH; u++)
+                    *(uint4 *)(sm.rows.q[b] + (tid / LPR + u * RSTEP) * KS + (tid % LPR) * 8) = sq[u];
+                if (wave == 0) sm.rows.ref[b][lane] = ref, sm.rows.pos[b][lane] = pos;
+            };
+            load(0);
+            Frag8 kf[COLS][KST];
+            __syncthreads();  // (the last head's rows have been read)
+#pragma unroll
+            for (int c = 0; c < COLS; c++) {
+                uint16_t *rows = sm.keys[wave];
+#pragma unroll
+                for (int u = 0; u < NLD; u++) *(uint4 *)(rows + (RPL * u + lane / LPR) * KS + (lane % LPR) * 8) = sk[c][u];
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int st = 0; st < KST; st++) kf[c][st].u = *(const uint4 *)(rows + col * KS + st * 16 + half * 8);
+                __builtin_amdgcn_wave_barrier();
+            }
+            __syncthreads();
+            store(0);
+            __syncthreads();
+            float sub[COLS];
+#pragma unroll
+            for (int c = 0; c < COLS; c++) sub[c] = 0.f;
+            for (int32_t i = 0; i < n; i++) {
+                const int b = i & 1;
+                if (i + 1 < n) load(i + 1);
+                // all of the step's rows see all of the wavefront's keys (those of the last token may be fewer)
+                const bool full = p0 + ts >= w0 + 32 * COLS - 1 && (a.left < 0 || p0 + ts + more + 1 - a.left <= w0);
+                const int tiles = first + i * 64 + 32 < to ? 2 : 1;
+                const uint16_t *tq = sm.rows.q[b] + col * KS + half * 8;
+                for (int y = 0; y < tiles; y++) {
+                    f32x16_t sc[COLS];
+#pragma unroll
+                    for (int c = 0; c < COLS; c++) sc[c] = zero16();
+#pragma unroll
+                    for (int st = 0; st < KST; st++) {
+                        Frag8 f;
+                        f.u = *(const uint4 *)(tq + y * 32 * KS + st * 16);
+#pragma unroll
+                        for (int c = 0; c < COLS; c++) sc[c] = mfma32<DT>(f, kf[c][st], sc[c]);
+                    }
+                    float part[COLS];
+#pragma unroll
+                    for (int c = 0; c < COLS; c++) part[c] = 0.f;
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const float4 rf = *(const float4 *)(sm.rows.ref[b] + y * 32 + g * 8 + half * 4);
+                        const float f4[4] = {rf.x, rf.y, rf.z, rf.w};
+                        if (full) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+#pragma unroll
+                                for (int c = 0; c < COLS; c++) part[c] += fast_exp2(fmaf(sc[c][g * 4 + e], c2, f4[e]));
+                        } else {
+                            const int4 ps = *(const int4 *)(sm.rows.pos[b] + y * 32 + g * 8 + half * 4);
+                            const int32_t p4[4] = {ps.x, ps.y, ps.z, ps.w};
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+#pragma unroll
+                                for (int c = 0; c < COLS; c++) {
+                                    const int32_t key = w0 + c * 32 + col;
+                                    const bool seen = key <= p4[e] && (a.left < 0 || key >= p4[e] - a.left) && f4[e] != -INFINITY;
+                                    part[c] += seen ? fast_exp2(fmaf(sc[c][g * 4 + e], c2, f4[e])) : 0.f;
+                                }
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < COLS; c++) sub[c] += part[c];
+                }
+                ts += more, hs += rest;
+                if (hs >= rep) ts++, hs -= rep;
+                if (i + 1 < n) store(b ^ 1);
+                __syncthreads();
+            }
+#pragma unroll
+            for (int c = 0; c < COLS; c++) total[c] += sub[c];
+            r += n;
+        }
+#pragma unroll
+        for (int c = 0; c < COLS; c++) {
+            const float y = total[c] + __shfl_xor(total[c], 32, 64);
+            const int32_t i = wave * 32 * COLS + c * 32 + col;
+            if (half == 0) {
+                if (!x.whole)
+                    l.sums[(int64_t)x.slot * l.keys + i] = y;
+                else if (w0 + c * 32 + col < len && x.r1 > 0)
+                    weights[s * stride + w0 + c * 32 + col] += y;
+            }
+        }
+        p = next;
+        if (p >= end || !walk_on(a, l, walk, next)) return;
+        __syncthreads();
+    }
+}
+
+// The pieces of a shared tile's sums, in the order of the workers.
+__global__ __launch_bounds__(256) void paged_weights_join(PagedArgs a, KeyLine l, float *__restrict__ weights, int64_t stride) {
+    const PagedJob job = l.jobs[blockIdx.x];
+    if (job.rows == 0) return;
+    const int32_t i = blockIdx.y * 256 + threadIdx.x, key = job.head * l.keys + i;
+    if (i >= l.keys || key >= paged_seq(a, job.tok).len) return;
+    float y = 0.f;
+    for (int32_t w = job.first; w <= job.last; w++) y += l.sums[(int64_t)(2 * w + (w == job.first ? 1 : 0)) * l.keys + i];
+    weights[job.tok * stride + key] += y;
+}
+
 // ------------------------------------------------------------------------------------------
 // Host
 // ------------------------------------------------------------------------------------------
@@ -1013,7 +1220,8 @@ struct PagedPlan {
     bool fast, mixed;
     PagedLine wide, narrow;  // the simple kernel's: narrow
     size_t bytes;
-    size_t lse;  // where the weights' own log-sum-exps lie
+    KeyLine keys;            // with weights
+    size_t lse;              // where their own log-sum-exps lie
 };
 static size_t place_line(const dm_attention_desc *d, PagedLine *l, char *base, size_t at) {
     const size_t rows = (size_t)2 * l->workers * l->pitch;
@@ -1045,7 +1253,19 @@ static PagedPlan paged_plan(const dm_attention_desc *d, char *base, bool weights
     p.narrow.least = 192;
     p.bytes = place_line(d, &p.narrow, base, p.bytes);
     p.lse = p.bytes;
-    if (weights) p.bytes += align_up((size_t)(d->tq * d->hq) * sizeof(float));
+    if (weights) {
+        p.bytes += align_up((size_t)(d->tq * d->hq) * sizeof(float));
+        KeyLine &l = p.keys;
+        l.keys = d->d == 256 ? key_tile<256>() : key_tile<128>();
+        l.workers = 256;
+        l.unit = 64;
+        l.start = 256;
+        l.least = 1024;
+        l.sums = (float *)(base + p.bytes);
+        p.bytes += align_up((size_t)2 * l.workers * l.keys * sizeof(float));
+        l.jobs = (PagedJob *)(base + p.bytes);
+        p.bytes += align_up((size_t)l.workers * sizeof(PagedJob));
+    }
     return p;
 }
 
@@ -1130,7 +1350,13 @@ int dm_attention_paged(const dm_attention_desc *d, const void *q, const void *k_
     const PagedLine &l = p.narrow;
     const unsigned g = l.workers / 4;
 #define PAGED_W(DT, DP)                                                                                       \
-    if (weights) paged_weights_simple<DT, DP><<<1024, 256, 0, st>>>(a, q, k_pages, weights, weights_stride)
+    if (weights && !fast)                                                                                     \
+        paged_weights_simple<DT, DP><<<1024, 256, 0, st>>>(a, q, k_pages, weights, weights_stride);           \
+    else if (weights) {                                                                                       \
+        if constexpr (DT != DM_F32)                                                                           \
+            paged_weights_kernel<DT, DP><<<p.keys.workers, 512, 0, st>>>(a, p.keys, q, k_pages, weights, weights_stride); \
+        paged_weights_join<<<dim3(p.keys.workers, p.keys.keys / 256), 256, 0, st>>>(a, p.keys, weights, weights_stride); \
+    }
 #define PAGED_V(DT, DP)                                                                                       \
     if constexpr (DT != DM_F32) {                                                                             \
         if (p.mixed)                                                                                          \

@@ -64,6 +64,12 @@ __device__ __forceinline__ int64_t ramp(int64_t a, int64_t m, int64_t t) {
     return c * (a + m * u0) + m * (c * (c - 1) / 2);
 }
 
+// sum over u < t of max(0, b - m u)
+__device__ __forceinline__ int64_t slope(int64_t b, int64_t m, int64_t t) {
+    const int64_t c = b <= 0 ? 0 : min(t, (b + m - 1) / m);
+    return c * b - m * (c * (c - 1) / 2);
+}
+
 // What the first t token tiles of a sequence cost: of each its start, and the keys between the first that its
 // first token sees and the last that its last one would see if the tile were full.
 __device__ __forceinline__ int64_t tiles_cost(const PagedArgs &a, const PagedLine &l, const PagedSeq &q, int32_t t) {
@@ -72,10 +78,40 @@ __device__ __forceinline__ int64_t tiles_cost(const PagedArgs &a, const PagedLin
     if (a.left >= 0) x -= ramp(p0 - a.left, l.m, t);
     return x;
 }
-__device__ __forceinline__ int32_t token_tiles(const PagedLine &l, const PagedSeq &q) { return (q.n + l.m - 1) / l.m; }
+__device__ __forceinline__ int32_t tiles_of(const PagedArgs &a, const PagedLine &l, const PagedSeq &q) {
+    return (q.n + l.m - 1) / l.m;
+}
+// how often the tiles of a sequence stand on the line
+__device__ __forceinline__ int32_t turns_of(const PagedArgs &a, const PagedLine &l) { return a.hkv * l.hc; }
 __device__ __forceinline__ bool on_line(const PagedArgs &a, const PagedLine &l, const PagedSeq &q) {
     const int64_t rows = (int64_t)q.n * a.rep;
     return q.n > 0 && rows > l.over && rows <= l.upto;
+}
+
+// The line of the weights that keys get: a tile is `keys` keys of a sequence, and costs, for each key-value head,
+// its start and the rows that see any of them.
+struct KeyLine {
+    int32_t keys, workers, start, least, unit;
+    int32_t over;     // the sequences of more than `over` rows
+    float *sums;      // [2 workers, keys]
+    PagedJob *jobs;   // [workers]: tok = sequence, head = tile
+};
+__device__ __forceinline__ int64_t tiles_cost(const PagedArgs &a, const KeyLine &l, const PagedSeq &q, int32_t t) {
+    // tokens of tile u: those from max(0, keys u - p0) on and, with a window, in front of keys (u + 1) + left - p0
+    const int64_t p0 = (int64_t)q.len - q.n;
+    int64_t x = (int64_t)t * q.n - ramp(-p0, l.keys, t);
+    if (a.left >= 0) {
+        const int64_t y = p0 - l.keys - a.left;
+        x -= slope(q.n + y, l.keys, t) - slope(y, l.keys, t);
+    }
+    return ((int64_t)t * l.start + x * a.rep) * a.hkv;
+}
+__device__ __forceinline__ int32_t tiles_of(const PagedArgs &a, const KeyLine &l, const PagedSeq &q) {
+    return (q.len + l.keys - 1) / l.keys;
+}
+__device__ __forceinline__ int32_t turns_of(const PagedArgs &a, const KeyLine &l) { return 1; }
+__device__ __forceinline__ bool on_line(const PagedArgs &a, const KeyLine &l, const PagedSeq &q) {
+    return q.n > 0 && q.len > 0 && (int64_t)q.n * a.rep > l.over;
 }
 
 // The exclusive prefix sums of the workgroup's x, and its total.
@@ -106,15 +142,15 @@ __device__ __forceinline__ int64_t scan64(int64_t x, PlanSmem<NT> &sm) {
     __syncthreads();
     return all;
 }
-template <int NT>
-__device__ __forceinline__ int64_t plan_chunk(const PagedArgs &a, const PagedLine &l, int32_t s0, PlanSmem<NT> &sm,
+template <int NT, class Line>
+__device__ __forceinline__ int64_t plan_chunk(const PagedArgs &a, const Line &l, int32_t s0, PlanSmem<NT> &sm,
                                               bool *ok) {
     const int32_t s = s0 + (int32_t)threadIdx.x;
     int64_t x = 0;
     if (s < a.S) {
         const PagedSeq q = paged_seq(a, s);
         *ok = *ok && q.ok;
-        if (on_line(a, l, q)) x = (int64_t)a.hkv * l.hc * tiles_cost(a, l, q, token_tiles(l, q));
+        if (on_line(a, l, q)) x = turns_of(a, l) * tiles_cost(a, l, q, tiles_of(a, l, q));
     }
     return scan64<NT>(x, sm);
 }
@@ -134,18 +170,18 @@ struct PagedShare {
     }
 };
 
-// Where a worker stands: the tile x of sequence s and key-value head kh, which begins at `base` of the line.
+// Where a worker stands: tile t of sequence s, in its u-th turn, which begins at `base` of the line.
 struct PagedWalk {
-    int32_t s, kh, c, t;  // c: which heads of a token, t: token tile
-    int32_t nt;           // token tiles of the sequence
+    int32_t s, u, t;
+    int32_t nt;  // tiles of the sequence
     PagedSeq q;
     int64_t base;
 };
 
 // The whole workgroup: the line's total, 0 where offsets do not go up; and the walk of the worker at `p`
 // (wavefront-uniform; each wavefront its own), if it has anything. `where` maps (total) to p, or -1 for none.
-template <int NT, class Where>
-__device__ __forceinline__ PagedShare plan_line(const PagedArgs &a, const PagedLine &l, PlanSmem<NT> &sm, Where where,
+template <int NT, class Line, class Where>
+__device__ __forceinline__ PagedShare plan_line(const PagedArgs &a, const Line &l, PlanSmem<NT> &sm, Where where,
                                                 PagedWalk *walk, int64_t *p, bool *valid) {
     bool ok = true;
     int64_t total = 0;
@@ -178,13 +214,10 @@ __device__ __forceinline__ PagedShare plan_line(const PagedArgs &a, const PagedL
     }
     walk->s = __builtin_amdgcn_readfirstlane(found);
     walk->q = paged_seq(a, walk->s);
-    walk->nt = token_tiles(l, walk->q);
+    walk->nt = tiles_of(a, l, walk->q);
     int64_t rem = *p - walk->base;
-    const int64_t chunk = tiles_cost(a, l, walk->q, walk->nt), head = chunk * l.hc;
-    const int64_t kh = rem / head;
-    rem -= kh * head;
-    const int64_t c = rem / chunk;
-    rem -= c * chunk;
+    const int64_t turn = tiles_cost(a, l, walk->q, walk->nt), u = rem / turn;
+    rem -= u * turn;
     // the last tile that begins at rem or in front of it: 64 probes at a time
     int32_t lo = 0, hi = walk->nt;  // it lies in [lo, hi)
     while (hi - lo > 1) {
@@ -193,7 +226,7 @@ __device__ __forceinline__ PagedShare plan_line(const PagedArgs &a, const PagedL
         lo += (n - 1) * step;
         hi = min(hi, lo + step);
     }
-    walk->kh = (int32_t)kh, walk->c = (int32_t)c, walk->t = lo;
+    walk->u = (int32_t)u, walk->t = lo;
     walk->base = *p - rem + tiles_cost(a, l, walk->q, lo);
     return sh;
 }
@@ -207,18 +240,19 @@ struct PagedPiece {
     int32_t slot;                  // not whole: its place
 };
 
-template <class Args>
-__device__ __forceinline__ PagedPiece piece_of(const Args &a, const PagedLine &l, const PagedWalk &w, const PagedShare &sh,
+__device__ __forceinline__ PagedPiece piece_of(const PagedArgs &a, const PagedLine &l, const PagedWalk &w, const PagedShare &sh,
                                                int32_t worker, int64_t p, int64_t end, int64_t *next, int32_t *last) {
     PagedPiece x;
     const int32_t i0 = w.t * l.m, i1 = min(i0 + l.m, w.q.n);
     const int64_t cost = tiles_cost(a, l, w.q, w.t + 1) - tiles_cost(a, l, w.q, w.t);
+    x.kh = w.u / l.hc;
+    const int32_t c = w.u - x.kh * l.hc;  // which heads of a token
     x.tok = w.q.first + i0;
-    x.head = w.kh * a.rep + w.c * l.rt;
+    x.head = x.kh * a.rep + c * l.rt;
     x.per = l.per;
-    x.rows = l.hc > 1 ? min(l.rt, a.rep - w.c * l.rt) : (i1 - i0) * a.rep;
+    x.rows = l.hc > 1 ? min(l.rt, a.rep - c * l.rt) : (i1 - i0) * a.rep;
     x.pos = w.q.len - w.q.n + i0;
-    x.kh = w.kh, x.s = w.s;
+    x.s = w.s;
     const int32_t hi = max(0, w.q.len - w.q.n + i1);
     const int32_t lo = a.left >= 0 ? min(hi, max(0, x.pos - a.left)) : 0;
     auto key = [&](int64_t off) -> int32_t {  // the key at `off` of the tile's part of the line
@@ -237,22 +271,51 @@ __device__ __forceinline__ PagedPiece piece_of(const Args &a, const PagedLine &l
 }
 
 // On to the next tile of the line (false: there is none).
-__device__ __forceinline__ bool walk_on(const PagedArgs &a, const PagedLine &l, PagedWalk &w, int64_t base) {
+template <class Line>
+__device__ __forceinline__ bool walk_on(const PagedArgs &a, const Line &l, PagedWalk &w, int64_t base) {
     w.base = base;
     if (++w.t < w.nt) return true;
     w.t = 0;
-    if (++w.c < l.hc) return true;
-    w.c = 0;
-    if (++w.kh < a.hkv) return true;
-    w.kh = 0;
+    if (++w.u < turns_of(a, l)) return true;
+    w.u = 0;
     while (++w.s < a.S) {
         w.q = paged_seq(a, w.s);
         if (on_line(a, l, w.q)) {
-            w.nt = token_tiles(l, w.q);
+            w.nt = tiles_of(a, l, w.q);
             return true;
         }
     }
     return false;
+}
+
+// A worker's next part of a tile of keys: its steps [r0, r1) of `unit` rows, counted through the key-value heads
+// (each of them `steps`), rows from row `from` of a head on to `to`.
+struct KeyPiece {
+    int32_t s, k0;          // sequence, first key
+    int32_t from, to, steps;
+    int32_t r0, r1;
+    bool whole;
+    int32_t slot;
+};
+__device__ __forceinline__ KeyPiece key_piece(const PagedArgs &a, const KeyLine &l, const PagedWalk &w, const PagedShare &sh,
+                                              int32_t worker, int64_t p, int64_t end, int64_t *next, int32_t *last) {
+    KeyPiece x;
+    const int64_t cost = tiles_cost(a, l, w.q, w.t + 1) - tiles_cost(a, l, w.q, w.t);
+    const int32_t p0 = w.q.len - w.q.n;
+    x.s = w.s, x.k0 = w.t * l.keys;
+    const int32_t t0 = max(0, x.k0 - p0);
+    const int32_t t1 = a.left >= 0 ? (int32_t)max((int64_t)t0, min((int64_t)w.q.n, (int64_t)x.k0 + l.keys + a.left - p0)) : w.q.n;
+    x.from = t0 * a.rep, x.to = t1 * a.rep;
+    x.steps = (x.to - x.from + l.unit - 1) / l.unit;
+    const int64_t o0 = p - w.base, o1 = min(end - w.base, cost), all = (int64_t)x.steps * a.hkv;
+    auto step = [&](int64_t off) { return off >= cost ? (int32_t)all : (int32_t)(off * all / cost); };
+    x.r0 = step(o0), x.r1 = step(o1);
+    x.whole = o0 == 0 && o1 == cost;
+    x.slot = 2 * worker + (o0 == 0 ? 1 : 0);
+    *next = w.base + cost;
+    *last = -1;
+    if (o0 > 0 && sh.at(worker - 1) <= w.base) *last = sh.last_before(w.base + cost);
+    return x;
 }
 
 }  // namespace dm
