@@ -420,18 +420,20 @@ __global__ __launch_bounds__(256) void cache_compact_apply(CacheArgs a, PoolArgs
 //
 // A row's plan is one workgroup's: what has to stay, the weight of the last key that stays of the others, by three
 // counts of 11, 11 and 10 bits of the weights' order, and one walk over the keys in order that gives each key that
-// stays its place. The keys then move down in every pool, a wavefront for 128 bytes of each: its loads of 128 keys
-// have all arrived before it stores one of them, and what it stores to lies in front of all that it has yet to
-// load, so that no order among wavefronts is needed.
+// stays its place. The keys then move down in every pool, a wavefront for a column of each: its loads of a step's
+// keys have all arrived before it stores one of them, and what it stores to lies in front of all that it has yet to
+// load, so that no order among wavefronts is needed. A column is 16 to 128 bytes wide: narrow ones are more wavefronts
+// with more keys a step, wide ones touch fewer cache lines a load.
 
-// What the plan leaves for the copies: of row r the keys first[r] .. count[r] - 1 move; key j comes from row
-// from[j] of the pool to row to[j] (page * page_size + row; kNoSlot: a page outside the pools).
+// What the plan leaves for the copies: of row r the keys first[r] .. count[r] - 1 move; key j comes from page and
+// row from[j] of the pool to to[j] (page kNoPage: one outside the pools).
 struct EvictWork {
     int32_t *first, *count;  // [rows]
-    uint32_t *from, *to;     // [rows, max_pages * page_size]
+    uint2 *from, *to;        // [rows, max_pages * page_size]
     int64_t cap;
 };
-constexpr uint32_t kNoSlot = 0xffffffffu;
+constexpr uint32_t kNoPage = 0xffffffffu;
+typedef float f32x4_unaligned __attribute__((ext_vector_type(4), aligned(4)));
 
 // A float's place in the order of weights: -0 as 0, NaN above all.
 __device__ __forceinline__ uint32_t weight_order(float x) {
@@ -481,10 +483,17 @@ __global__ __launch_bounds__(kPlan) void cache_evict_plan(CacheArgs a, float *we
             const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
             for (int i = tid; i < 2048; i += kPlan) hist[i] = 0;
             __syncthreads();
-            for (int64_t j = fixed + tid; j < until; j += kPlan) {
-                const uint32_t x = weight_order(wr[j]);
+            auto count = [&](float y) {
+                const uint32_t x = weight_order(y);
                 if ((x & mask) == prefix) atomicAdd(&hist[(x >> shift) & (bins - 1)], 1);
+            };
+            const int64_t whole = fixed + (until - fixed) / (4 * kPlan) * (4 * kPlan);
+#pragma unroll 4
+            for (int64_t j = fixed; j < whole; j += 4 * kPlan) {
+                const f32x4_unaligned y = *(const f32x4_unaligned *)(wr + j + 4 * tid);
+                count(y[0]), count(y[1]), count(y[2]), count(y[3]);
             }
+            for (int64_t j = whole + tid; j < until; j += kPlan) count(wr[j]);
             __syncthreads();
             // from the largest bin down: the one in which the count reaches `left`
             const int b1 = 2047 - 2 * tid, b0 = b1 - 1;
@@ -508,10 +517,16 @@ __global__ __launch_bounds__(kPlan) void cache_evict_plan(CacheArgs a, float *we
     for (int64_t j0 = 0; j0 < held; j0 += kPlan * 4) {
         float x[4];
         int32_t is[4], eq[4], packed = 0;
+        if (j0 + 4 * kPlan <= held) {
+            const f32x4_unaligned y = *(const f32x4_unaligned *)(wr + j0 + 4 * tid);
+            x[0] = y[0], x[1] = y[1], x[2] = y[2], x[3] = y[3];
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; u++) x[u] = j0 + tid * 4 + u < held ? wr[j0 + tid * 4 + u] : 0.f;
+        }
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int64_t j = j0 + tid * 4 + u;
-            x[u] = j < held ? wr[j] : 0.f;
             const uint32_t y = weight_order(x[u]);
             const bool stays = j < fixed || (j >= until && j < held), may = j >= fixed && j < until && need > 0;
             is[u] = stays || (may && y > bar);
@@ -529,11 +544,11 @@ __global__ __launch_bounds__(kPlan) void cache_evict_plan(CacheArgs a, float *we
                 out[to] = (int32_t)j;
                 if (to != j) {
                     wr[to] = x[u];
-                    const int64_t cf = j / a.page_size, ct = to / a.page_size;
+                    const uint32_t cf = (uint32_t)j / (uint32_t)a.page_size, ct = (uint32_t)to / (uint32_t)a.page_size;
                     const int32_t pf = row[cf], pt = row[ct];
                     const bool ok = pf >= 0 && pf < a.num_pages && pt >= 0 && pt < a.num_pages;
-                    w.from[r * cap + to] = ok ? (uint32_t)(pf * a.page_size + (j - cf * a.page_size)) : kNoSlot;
-                    w.to[r * cap + to] = (uint32_t)(pt * a.page_size + (to - ct * a.page_size));
+                    w.from[r * cap + to] = make_uint2(ok ? (uint32_t)pf : kNoPage, (uint32_t)(j - cf * a.page_size));
+                    w.to[r * cap + to] = make_uint2((uint32_t)pt, (uint32_t)(to - ct * a.page_size));
                 }
             } else if (j < held && j == o + min(e, ties)) {
                 chosen = (int32_t)j;  // (the first key that goes: no other has its own index for a place)
@@ -558,37 +573,45 @@ __global__ __launch_bounds__(kPlan) void cache_evict_plan(CacheArgs a, float *we
     }
 }
 
-// Wavefront (row, pool, slice): `lanes` lanes a key, a T each, kEvictLoads loads in flight.
-constexpr int kEvictLoads = 16, kEvictLanes = 8;
-template <class T>
-__global__ __launch_bounds__(256) void cache_evict_move(EvictWork w, PoolArgs pools, int64_t page_size, int32_t slices,
+// Wavefront (row, pool, column): LANES lanes a key, a T each, kEvictLoads loads in flight.
+constexpr int kEvictLoads = 16;
+template <class T, int LANES>
+__global__ __launch_bounds__(512) void cache_evict_move(EvictWork w, PoolArgs pools, int64_t page_size, int32_t columns,
                                                         int64_t items) {
+    constexpr int KEYS = 64 / LANES, STEP = KEYS * kEvictLoads;
     const int lane = threadIdx.x & 63;
-    int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 6);
     if (i >= items) return;
-    const int32_t slice = (int32_t)(i % slices);
-    i /= slices;
+    const int32_t column = (int32_t)(i % columns);
+    i /= columns;
     const auto &pool = pools.at[i % pools.n];
     const int64_t r = i / pools.n, bytes = pool.bytes / page_size;
-    const int64_t at = ((int64_t)slice * kEvictLanes + lane % kEvictLanes) * (int64_t)sizeof(T);
+    const int64_t at = ((int64_t)column * LANES + lane % LANES) * (int64_t)sizeof(T);
     const int32_t first = w.first[r], count = w.count[r];
-    const uint32_t *from = w.from + r * w.cap, *to = w.to + r * w.cap;
-    if (!__any(at < bytes)) return;
-    constexpr int KEYS = 64 / kEvictLanes;
-    auto place = [&](uint32_t x) {
-        const uint32_t page = x / (uint32_t)page_size, k = x - page * (uint32_t)page_size;
-        return pool.pages + page * pool.stride + k * bytes + at;
+    const uint2 *from = w.from + r * w.cap, *to = w.to + r * w.cap;
+    if (first >= count || !__any(at < bytes)) return;
+    // (a lane past the row's end reads the row's first bytes, one without a key the pool's, and stores nothing)
+    char *base = pool.pages + (at < bytes ? at : 0);
+    auto place = [&](const uint2 &x) { return base + (int64_t)x.x * pool.stride + (int64_t)x.y * bytes; };
+    uint2 f[kEvictLoads], t[kEvictLoads];
+    auto look = [&](int32_t j0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < kEvictLoads; u++) {
+            const int32_t j = min(j0 + u * KEYS + lane / LANES, count - 1);
+            f[u] = from[j], t[u] = to[j];
+        }
     };
-    for (int32_t j0 = first; j0 < count; j0 += KEYS * kEvictLoads) {
+    look(first);
+    for (int32_t j0 = first; j0 < count; j0 += STEP) {
         T x[kEvictLoads];
         char *dst[kEvictLoads];
 #pragma unroll
         for (int u = 0; u < kEvictLoads; u++) {
-            const int32_t j = j0 + u * KEYS + lane / kEvictLanes;
-            const uint32_t f = j < count && at < bytes ? from[j] : kNoSlot;
-            dst[u] = f != kNoSlot ? place(to[j]) : nullptr;
-            if (f != kNoSlot) x[u] = *(const T *)place(f);
+            const bool ok = f[u].x != kNoPage;
+            x[u] = *(const T *)place(ok ? f[u] : make_uint2(0, 0));
+            dst[u] = ok && at < bytes && j0 + u * KEYS + lane / LANES < count ? place(t[u]) : nullptr;
         }
+        if (j0 + STEP < count) look(j0 + STEP);
         // every load has arrived before the first store: a key may lie where another of these comes from
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
@@ -775,17 +798,18 @@ int dm_cache_compact(const dm_cache_table *t, const dm_cache_pool *pools, int64_
 static EvictWork evict_work(const dm_cache_table *t, char *at, size_t *bytes) {
     EvictWork w{};
     w.cap = t->max_pages * t->page_size;
-    const size_t rows = align_up((size_t)t->rows * 4), keys = align_up((size_t)(t->rows * w.cap) * 4);
+    const size_t rows = align_up((size_t)t->rows * 4), keys = align_up((size_t)(t->rows * w.cap) * sizeof(uint2));
     w.first = (int32_t *)at;
     w.count = (int32_t *)(at + rows);
-    w.from = (uint32_t *)(at + 2 * rows);
-    w.to = (uint32_t *)(at + 2 * rows + keys);
+    w.from = (uint2 *)(at + 2 * rows);
+    w.to = (uint2 *)(at + 2 * rows + keys);
     *bytes = 2 * (rows + keys);
     return w;
 }
+constexpr int64_t kEvictWaves = 2048;
 static bool evict_sizes(const dm_cache_table *t) {
     return table_sizes(t) && t->rows <= kMostRows && t->max_pages <= ((int64_t)1 << 30) / t->page_size &&
-           t->num_pages < kI31 / t->page_size;
+           t->rows * t->max_pages * t->page_size < kI31 * 16;
 }
 
 size_t dm_cache_evict_workspace(const dm_cache_table *t) {
@@ -801,7 +825,7 @@ int dm_cache_evict(const dm_cache_table *t, const dm_cache_pool *pools, int64_t 
     if (int rc = check_table(op, t)) return rc;
     if (int rc = check_pools(op, t, pools, npools)) return rc;
     if (!evict_sizes(t))
-        return refuse(op + ": a row holds at most 2^30 keys, the pools less than 2^31, rows are at most 2^22");
+        return refuse(op + ": a row holds at most 2^30 keys, the rows less than 2^35, rows are at most 2^22");
     if (recent < 0) return refuse(op + ": recent must not be negative");
     const int64_t cap = t->max_pages * t->page_size;
     if (t->rows > 1 && weights_stride < cap)
@@ -824,23 +848,38 @@ int dm_cache_evict(const dm_cache_table *t, const dm_cache_pool *pools, int64_t 
             while (bits % grain) grain /= 2;
             most = std::max(most, row);
         }
-        const int64_t slices = (most + kEvictLanes * grain - 1) / (kEvictLanes * grain);
-        const int64_t items = t->rows * pa.n * slices;
+        // the widest columns that make kEvictWaves wavefronts
+        int lanes = 8;
+        auto columns = [&](int n) { return (most + n * grain - 1) / (n * grain); };
+        while (lanes > 1 && t->rows * pa.n * columns(lanes) < kEvictWaves) lanes /= 2;
+        const int64_t items = t->rows * pa.n * columns(lanes);
         if (items == 0) continue;
-        if (slices >= kI31 || items / 4 >= ((int64_t)1 << 24)) return refuse(op + ": more rows and bytes than one launch takes");
-        const unsigned g = (unsigned)((items + 3) / 4);
-#define EVICT_MOVE(T) cache_evict_move<T><<<g, 256, 0, st>>>(w, pa, t->page_size, (int32_t)slices, items)
-        if (grain == 16)
+        if (columns(lanes) >= kI31 || items >= ((int64_t)1 << 25))
+            return refuse(op + ": more rows and bytes than one launch takes");
+        const unsigned g = (unsigned)((items + 7) / 8);
+#define EVICT_L(T, L) cache_evict_move<T, L><<<g, 512, 0, st>>>(w, pa, t->page_size, (int32_t)columns(L), items)
+#define EVICT_MOVE(T)     \
+    if (lanes == 8)       \
+        EVICT_L(T, 8);    \
+    else if (lanes == 4)  \
+        EVICT_L(T, 4);    \
+    else if (lanes == 2)  \
+        EVICT_L(T, 2);    \
+    else                  \
+        EVICT_L(T, 1)
+        if (grain == 16) {
             EVICT_MOVE(uint4);
-        else if (grain == 8)
+        } else if (grain == 8) {
             EVICT_MOVE(uint2);
-        else if (grain == 4)
+        } else if (grain == 4) {
             EVICT_MOVE(uint32_t);
-        else if (grain == 2)
+        } else if (grain == 2) {
             EVICT_MOVE(uint16_t);
-        else
+        } else {
             EVICT_MOVE(uint8_t);
+        }
 #undef EVICT_MOVE
+#undef EVICT_L
     }
     probe_add(DM_PROBE_CACHE_EVICT);
     DM_LAUNCH_CHECK("cache_evict: launch");

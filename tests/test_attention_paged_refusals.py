@@ -99,7 +99,7 @@ def _evict(ws=1 << 40, pools=(), w=256, stride=64, b=256, kept=256, recent=0, **
     (dict(lengths=None), "missing"), (dict(refcounts=None), "missing"), (dict(block_table=None), "missing"),
     (dict(w=None), "missing"), (dict(b=None), "missing"), (dict(kept=None), "missing"), (dict(ws=0), "workspace"),
     (dict(recent=-1), "recent"), (dict(stride=63), "their rows apart"), (dict(rows=(1 << 22) + 1), "at most 2^22"),
-    (dict(max_pages=(1 << 26) + 1), "at most 2^30"), (dict(num_pages=(1 << 21) - 3, page_size=2048), "less than 2^31"),
+    (dict(max_pages=(1 << 26) + 1), "at most 2^30"), (dict(rows=1 << 22, max_pages=1 << 13, page_size=1), "less than 2^35"),
     (dict(pools=[_lib.CachePool(256, 24, 24)]), "a pool's pages"), (dict(pools=[_lib.CachePool(None, 32, 32)]), "missing")])
 def test_the_eviction_refuses(kw, what):
     rc, msg = _evict(**kw)
