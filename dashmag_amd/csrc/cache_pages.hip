@@ -420,10 +420,10 @@ __global__ __launch_bounds__(256) void cache_compact_apply(CacheArgs a, PoolArgs
 //
 // A row's plan is one workgroup's: what has to stay, the weight of the last key that stays of the others, by three
 // counts of 11, 11 and 10 bits of the weights' order, and one walk over the keys in order that gives each key that
-// stays its place. The keys then move down in every pool, a wavefront for a column of each: its loads of a step's
+// stays its place. The keys then move down in every pool, a workgroup for a column of each: its loads of a step's
 // keys have all arrived before it stores one of them, and what it stores to lies in front of all that it has yet to
-// load, so that no order among wavefronts is needed. A column is 16 to 128 bytes wide: narrow ones are more wavefronts
-// with more keys a step, wide ones touch fewer cache lines a load.
+// load, so that no order among workgroups is needed. Wide columns read memory in long runs, narrow ones are more
+// workgroups with more keys a step.
 
 // What the plan leaves for the copies: of row r the keys first[r] .. count[r] - 1 move; key j comes from page and
 // row from[j] of the pool to to[j] (page kNoPage: one outside the pools).
@@ -433,6 +433,8 @@ struct EvictWork {
     int64_t cap;
 };
 constexpr uint32_t kNoPage = 0xffffffffu;
+typedef uint32_t u32x2_vec __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_vec __attribute__((ext_vector_type(4)));
 typedef float f32x4_unaligned __attribute__((ext_vector_type(4), aligned(4)));
 
 // A float's place in the order of weights: -0 as 0, NaN above all.
@@ -573,50 +575,73 @@ __global__ __launch_bounds__(kPlan) void cache_evict_plan(CacheArgs a, float *we
     }
 }
 
-// Wavefront (row, pool, column): LANES lanes a key, a T each, kEvictLoads loads in flight.
-constexpr int kEvictLoads = 16;
-template <class T, int LANES>
-__global__ __launch_bounds__(512) void cache_evict_move(EvictWork w, PoolArgs pools, int64_t page_size, int32_t columns,
-                                                        int64_t items) {
-    constexpr int KEYS = 64 / LANES, STEP = KEYS * kEvictLoads;
-    const int lane = threadIdx.x & 63;
-    int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 6);
-    if (i >= items) return;
+// Workgroup (row, pool, column): 2^shift threads a key, a T each. Two steps of kEvictLoads loads are in flight: a
+// step's keys are stored while the next one's arrive.
+#ifndef KEL
+#define KEL 8
+#endif
+constexpr int kEvictLoads = KEL, kEvictThreads = 512;
+template <class T>
+__global__ __launch_bounds__(kEvictThreads) void cache_evict_move(EvictWork w, PoolArgs pools, int64_t page_size,
+                                                                  int32_t columns, int32_t shift) {
+    const int32_t keys = kEvictThreads >> shift, step = keys * kEvictLoads, mine = threadIdx.x >> shift;
+    int64_t i = blockIdx.x;
     const int32_t column = (int32_t)(i % columns);
     i /= columns;
-    const auto &pool = pools.at[i % pools.n];
-    const int64_t r = i / pools.n, bytes = pool.bytes / page_size;
-    const int64_t at = ((int64_t)column * LANES + lane % LANES) * (int64_t)sizeof(T);
+    const int x = (int)(i % pools.n);
+    const int64_t r = i / pools.n, bytes = pools.at[x].bytes / page_size, stride = pools.at[x].stride;
+    const int64_t at = (((int64_t)column << shift) + (threadIdx.x & ((1 << shift) - 1))) * (int64_t)sizeof(T);
     const int32_t first = w.first[r], count = w.count[r];
     const uint2 *from = w.from + r * w.cap, *to = w.to + r * w.cap;
-    if (first >= count || !__any(at < bytes)) return;
-    // (a lane past the row's end reads the row's first bytes, one without a key the pool's, and stores nothing)
-    char *base = pool.pages + (at < bytes ? at : 0);
-    auto place = [&](const uint2 &x) { return base + (int64_t)x.x * pool.stride + (int64_t)x.y * bytes; };
+    if (first >= count || ((int64_t)column << shift) * (int64_t)sizeof(T) >= bytes) return;
+    // (a thread past the row's end reads the row's first bytes, one without a key the pool's, and stores nothing)
+    char *base = pools.at[x].pages + (at < bytes ? at : 0);
+    auto place = [&](uint32_t page, uint32_t row) { return base + (int64_t)page * stride + (int64_t)row * bytes; };
+    T even[kEvictLoads], odd[kEvictLoads];
+    uint32_t page0[kEvictLoads], row0[kEvictLoads], page1[kEvictLoads], row1[kEvictLoads];
     uint2 f[kEvictLoads], t[kEvictLoads];
     auto look = [&](int32_t j0) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kEvictLoads; u++) {
-            const int32_t j = min(j0 + u * KEYS + lane / LANES, count - 1);
+            const int32_t j = min(j0 + u * keys + mine, count - 1);
             f[u] = from[j], t[u] = to[j];
         }
     };
-    look(first);
-    for (int32_t j0 = first; j0 < count; j0 += STEP) {
-        T x[kEvictLoads];
-        char *dst[kEvictLoads];
+    auto load = [&](int32_t j0, T(&x)[kEvictLoads], uint32_t(&page)[kEvictLoads], uint32_t(&row)[kEvictLoads])
+                    __attribute__((always_inline)) {  // and the places of the step behind
 #pragma unroll
         for (int u = 0; u < kEvictLoads; u++) {
             const bool ok = f[u].x != kNoPage;
-            x[u] = *(const T *)place(ok ? f[u] : make_uint2(0, 0));
-            dst[u] = ok && at < bytes && j0 + u * KEYS + lane / LANES < count ? place(t[u]) : nullptr;
+            x[u] = *(const T *)place(ok ? f[u].x : 0u, ok ? f[u].y : 0u);
+            page[u] = ok && at < bytes && j0 + u * keys + mine < count ? t[u].x : kNoPage;
+            row[u] = t[u].y;
         }
-        if (j0 + STEP < count) look(j0 + STEP);
-        // every load has arrived before the first store: a key may lie where another of these comes from
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        look(j0 + step);
+    };
+    auto store = [&](T(&x)[kEvictLoads], uint32_t(&page)[kEvictLoads], uint32_t(&row)[kEvictLoads])
+                     __attribute__((always_inline)) {
+        // every load of the step has arrived before its first store: a key may lie where another of these comes from
+#pragma unroll
+        for (int u = 0; u < kEvictLoads; u++) {
+            if constexpr (sizeof(T) > 4)
+                asm volatile("" ::"v"(x[u][0]) : "memory");
+            else
+                asm volatile("" ::"v"((uint32_t)x[u]) : "memory");
+        }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
 #pragma unroll
         for (int u = 0; u < kEvictLoads; u++)
-            if (dst[u]) *(T *)dst[u] = x[u];
+            if (page[u] != kNoPage) *(T *)place(page[u], row[u]) = x[u];
+    };
+    look(first);
+    load(first, even, page0, row0);
+    for (int32_t j0 = first; j0 < count; j0 += 2 * step) {
+        load(j0 + step, odd, page1, row1);
+        store(even, page0, row0);
+        if (j0 + step >= count) break;
+        load(j0 + 2 * step, even, page0, row0);
+        store(odd, page1, row1);
     }
 }
 
@@ -806,7 +831,10 @@ static EvictWork evict_work(const dm_cache_table *t, char *at, size_t *bytes) {
     *bytes = 2 * (rows + keys);
     return w;
 }
-constexpr int64_t kEvictWaves = 2048;
+#ifndef KEG
+#define KEG 256
+#endif
+constexpr int64_t kEvictGroups = KEG;
 static bool evict_sizes(const dm_cache_table *t) {
     return table_sizes(t) && t->rows <= kMostRows && t->max_pages <= ((int64_t)1 << 30) / t->page_size &&
            t->rows * t->max_pages * t->page_size < kI31 * 16;
@@ -848,38 +876,27 @@ int dm_cache_evict(const dm_cache_table *t, const dm_cache_pool *pools, int64_t 
             while (bits % grain) grain /= 2;
             most = std::max(most, row);
         }
-        // the widest columns that make kEvictWaves wavefronts
-        int lanes = 8;
-        auto columns = [&](int n) { return (most + n * grain - 1) / (n * grain); };
-        while (lanes > 1 && t->rows * pa.n * columns(lanes) < kEvictWaves) lanes /= 2;
-        const int64_t items = t->rows * pa.n * columns(lanes);
-        if (items == 0) continue;
-        if (columns(lanes) >= kI31 || items >= ((int64_t)1 << 25))
+        // the widest columns that make kEvictGroups workgroups
+        int shift = 9;
+        auto columns = [&](int n) { return (most + (grain << n) - 1) / (grain << n); };
+        while (shift > 0 && (t->rows * pa.n * columns(shift) < kEvictGroups || (most <= grain << (shift - 1)))) shift--;
+        const int64_t items = t->rows * pa.n * columns(shift);
+        if (most == 0) continue;
+        if (columns(shift) >= kI31 || items >= ((int64_t)1 << 23))
             return refuse(op + ": more rows and bytes than one launch takes");
-        const unsigned g = (unsigned)((items + 7) / 8);
-#define EVICT_L(T, L) cache_evict_move<T, L><<<g, 512, 0, st>>>(w, pa, t->page_size, (int32_t)columns(L), items)
-#define EVICT_MOVE(T)     \
-    if (lanes == 8)       \
-        EVICT_L(T, 8);    \
-    else if (lanes == 4)  \
-        EVICT_L(T, 4);    \
-    else if (lanes == 2)  \
-        EVICT_L(T, 2);    \
-    else                  \
-        EVICT_L(T, 1)
-        if (grain == 16) {
-            EVICT_MOVE(uint4);
-        } else if (grain == 8) {
-            EVICT_MOVE(uint2);
-        } else if (grain == 4) {
+#define EVICT_MOVE(T) \
+    cache_evict_move<T><<<(unsigned)items, kEvictThreads, 0, st>>>(w, pa, t->page_size, (int32_t)columns(shift), shift)
+        if (grain == 16)
+            EVICT_MOVE(u32x4_vec);
+        else if (grain == 8)
+            EVICT_MOVE(u32x2_vec);
+        else if (grain == 4)
             EVICT_MOVE(uint32_t);
-        } else if (grain == 2) {
+        else if (grain == 2)
             EVICT_MOVE(uint16_t);
-        } else {
+        else
             EVICT_MOVE(uint8_t);
-        }
 #undef EVICT_MOVE
-#undef EVICT_L
     }
     probe_add(DM_PROBE_CACHE_EVICT);
     DM_LAUNCH_CHECK("cache_evict: launch");
