@@ -418,18 +418,25 @@ __global__ __launch_bounds__(256) void cache_compact_apply(CacheArgs a, PoolArgs
 // Eviction
 // ------------------------------------------------------------------------------------------
 //
-// A row's plan is one workgroup's: what has to stay, the weight of the last key that stays of the others, by three
-// counts of 11, 11 and 10 bits of the weights' order, and one walk over the keys in order that gives each key that
-// stays its place. The keys then move down in every pool, a workgroup for a column of each: its loads of a step's
-// keys have all arrived before it stores one of them, and what it stores to lies in front of all that it has yet to
-// load, so that no order among workgroups is needed. Wide columns read memory in long runs, narrow ones are more
-// workgroups with more keys a step.
+// Three launches. A workgroup a row finds what has to stay and the weight of the last key that stays of the others, by
+// three counts of 11, 11 and 10 bits of the weights' order. Then a workgroup for every kPlan * 4 keys or more of a row
+// gives the keys that stay their places, counting those in front of its own for itself (a walk by one workgroup was
+// 27 us of 55 for 31000 keys, all of it instructions). At last the keys move down in every pool, a workgroup for a
+// column of each: its loads of a step's keys have all arrived before it stores one of them, and what it stores to
+// lies in front of all that it has yet to load, so that no order among workgroups is needed. Wide columns read memory
+// in long runs, narrow ones are more workgroups with more keys a step.
 
-// What the plan leaves for the copies: of row r the keys first[r] .. count[r] - 1 move; key j comes from page and
-// row from[j] of the pool to to[j] (page kNoPage: one outside the pools).
+// What the first launch leaves of a row, and the second for the copies: key j of [first, n) comes from page and row
+// from[j] of the pool to to[j] (page kNoPage: one outside the pools), its weight is weight[j].
+struct EvictRow {
+    int32_t held, n, fixed, until;  // keys, those that stay; the keys [fixed, until) may go,
+    uint32_t bar;                   // of which those above the bar stay and the first `ties` that equal it
+    int32_t ties, first;
+};
 struct EvictWork {
-    int32_t *first, *count;  // [rows]
-    uint2 *from, *to;        // [rows, max_pages * page_size]
+    EvictRow *rows;
+    uint2 *from, *to;  // [rows, max_pages * page_size]
+    float *weight;
     int64_t cap;
 };
 constexpr uint32_t kNoPage = 0xffffffffu;
@@ -444,41 +451,35 @@ __device__ __forceinline__ uint32_t weight_order(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__global__ __launch_bounds__(kPlan) void cache_evict_plan(CacheArgs a, float *weights, int64_t stride,
-                                                          const int32_t *__restrict__ budgets, int64_t recent,
-                                                          int32_t *__restrict__ kept, EvictWork w) {
+__global__ __launch_bounds__(kPlan) void cache_evict_select(CacheArgs a, const float *__restrict__ weights, int64_t stride,
+                                                            const int32_t *__restrict__ budgets, int64_t recent,
+                                                            EvictWork w) {
     __shared__ PlanSums sums;
     __shared__ int32_t hist[2048], shared_to, chosen, above;
     const int tid = threadIdx.x;
-    const int64_t r = blockIdx.x, cap = a.max_pages * a.page_size;
-    const int64_t held = keys_of(a, a.lengths[r]), budget = max(budgets[r], 0);
-    int32_t *row = a.table + r * a.max_pages, *out = kept + r * cap;
-    float *wr = weights + r * stride;
+    const int64_t r = blockIdx.x;
+    const int32_t held = (int32_t)keys_of(a, a.lengths[r]), budget = max(budgets[r], 0);
+    const int32_t *row = a.table + r * a.max_pages;
+    const float *wr = weights + r * stride;
     int turn = 0;
     if (tid == 0) shared_to = 0;
     __syncthreads();
     // the pages up to the last that another row holds stay
-    const int64_t np = pages_of(a, held);
+    const int32_t np = (int32_t)pages_of(a, held);
     int32_t most = 0;
-    for (int64_t c = tid; c < np && held > budget; c += kPlan) {
+    for (int32_t c = tid; c < np && held > budget; c += kPlan) {
         const int32_t page = row[c];
-        if (page >= 0 && page < a.num_pages && a.counts[page] > 1) most = (int32_t)c + 1;
+        if (page >= 0 && page < a.num_pages && a.counts[page] > 1) most = c + 1;
     }
     if (most) atomicMax(&shared_to, most);
     __syncthreads();
-    const int64_t fixed = min(held, (int64_t)shared_to * a.page_size);
-    const int64_t until = max(fixed, held - min(recent, budget));  // the keys [fixed, until) may go
-    const int64_t must = held - (until - fixed), n = min(held, max(budget, must));
-    if (n == held) {
-        for (int64_t j = tid; j < cap; j += kPlan) out[j] = j < held ? (int32_t)j : -1;
-        if (tid == 0) w.first[r] = w.count[r] = 0;
-        return;
-    }
-    // of those the `need` largest weights: those above `bar`, and the first `ties` of those that equal it
-    const int32_t need = (int32_t)(n - must);
+    const int32_t fixed = (int32_t)min((int64_t)held, shared_to * a.page_size);
+    const int32_t until = max(fixed, held - (int32_t)min(recent, (int64_t)budget));
+    const int32_t must = held - (until - fixed), n = min(held, max(budget, must));
+    const int32_t need = n - must;
     uint32_t bar = 0xffffffffu;
     int32_t ties = 0;
-    if (need > 0) {
+    if (n < held && need > 0) {
         uint32_t prefix = 0, mask = 0;
         int32_t left = need;
         for (int pass = 0; pass < 3; pass++) {
@@ -489,13 +490,13 @@ __global__ __launch_bounds__(kPlan) void cache_evict_plan(CacheArgs a, float *we
                 const uint32_t x = weight_order(y);
                 if ((x & mask) == prefix) atomicAdd(&hist[(x >> shift) & (bins - 1)], 1);
             };
-            const int64_t whole = fixed + (until - fixed) / (4 * kPlan) * (4 * kPlan);
+            const int32_t whole = fixed + (until - fixed) / (4 * kPlan) * (4 * kPlan);
 #pragma unroll 4
-            for (int64_t j = fixed; j < whole; j += 4 * kPlan) {
+            for (int32_t j = fixed; j < whole; j += 4 * kPlan) {
                 const f32x4_unaligned y = *(const f32x4_unaligned *)(wr + j + 4 * tid);
                 count(y[0]), count(y[1]), count(y[2]), count(y[3]);
             }
-            for (int64_t j = whole + tid; j < until; j += kPlan) count(wr[j]);
+            for (int32_t j = whole + tid; j < until; j += kPlan) count(wr[j]);
             __syncthreads();
             // from the largest bin down: the one in which the count reaches `left`
             const int b1 = 2047 - 2 * tid, b0 = b1 - 1;
@@ -512,86 +513,140 @@ __global__ __launch_bounds__(kPlan) void cache_evict_plan(CacheArgs a, float *we
         }
         bar = prefix, ties = left;
     }
-    // the keys in order, four a thread; a key's place: the keys above the bar in front of it, and the ties taken
-    int32_t over = 0, equal = 0;
-    if (tid == 0) chosen = (int32_t)n;
-    __syncthreads();
-    for (int64_t j0 = 0; j0 < held; j0 += kPlan * 4) {
+    if (tid == 0) w.rows[r] = EvictRow{held, n, fixed, until, bar, ties, n};
+}
+
+// Workgroup (share, row): the keys of the row's share, a wavefront 256 of a step's 4096 in four rows of its lanes (so
+// that the lanes' stores lie side by side). A key's place: the keys above the bar in front of it, and the ties taken.
+constexpr int kEvictShares = 64;  // most shares of a row
+__global__ __launch_bounds__(kPlan) void cache_evict_place(CacheArgs a, const float *__restrict__ weights, int64_t stride,
+                                                           int32_t *__restrict__ kept, EvictWork w) {
+    __shared__ int4 sums[2][kPlan / 64 / 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t r = blockIdx.y;
+    const EvictRow er = w.rows[r];
+    const int32_t size = (int32_t)min(a.page_size, (int64_t)1 << 30);
+    const int32_t steps = (er.held + 4 * kPlan - 1) / (4 * kPlan), share = (steps + gridDim.x - 1) / gridDim.x * 4 * kPlan;
+    const int64_t from = (int64_t)blockIdx.x * share, cap = w.cap;
+    int32_t *out = kept + r * cap;
+    // behind the row, a part for each workgroup
+    for (int64_t j = er.n + (int64_t)blockIdx.x * kPlan + tid; j < cap; j += (int64_t)gridDim.x * kPlan) out[j] = -1;
+    if (from >= er.held) return;
+    const int32_t begin = (int32_t)from, end = (int32_t)min((int64_t)er.held, from + share);
+    if (er.n == er.held) {
+        for (int32_t j = begin + tid; j < end; j += kPlan) out[j] = j;
+        return;
+    }
+    const float *wr = weights + r * stride;
+    const int32_t *row = a.table + r * a.max_pages;
+    // the keys in front of the share: those that have to stay in closed form, the others counted
+    int32_t over = min(begin, er.fixed) + max(0, begin - er.until), equal = 0;
+    const bool takes = er.n > er.held - (er.until - er.fixed);  // some of those that may go stay
+    int turn = 0;
+    auto meet = [&](int32_t packed, int32_t *before, int32_t *total) __attribute__((always_inline)) {
+        int32_t *all = (int32_t *)sums[turn];
+        turn ^= 1;
+        if (lane == 0) all[wave] = packed;
+        __syncthreads();
+        *before = *total = 0;
+#pragma unroll
+        for (int i = 0; i < kPlan / 64; i++) {
+            *before += i < wave ? all[i] : 0;
+            *total += all[i];
+        }
+    };
+    if (takes && begin > er.fixed) {
+        int32_t mine = 0, same = 0;
+        const int32_t to = min(begin, er.until);
+#pragma unroll 4
+        for (int32_t j = er.fixed + tid; j < to; j += kPlan) {
+            const uint32_t y = weight_order(wr[j]);
+            mine += y > er.bar, same += y == er.bar;
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) mine += __shfl_xor(mine, o, 64), same += __shfl_xor(same, o, 64);
+        int32_t before, total;
+        meet(mine, &before, &total);
+        over += total;
+        meet(same, &before, &total);
+        equal += total;
+    }
+    const unsigned long long below = ((unsigned long long)1 << lane) - 1;
+    for (int32_t j0 = begin; j0 < end; j0 += kPlan * 4) {
         float x[4];
-        int32_t is[4], eq[4], packed = 0;
-        if (j0 + 4 * kPlan <= held) {
-            const f32x4_unaligned y = *(const f32x4_unaligned *)(wr + j0 + 4 * tid);
-            x[0] = y[0], x[1] = y[1], x[2] = y[2], x[3] = y[3];
-        } else {
+        unsigned long long is[4], eq[4];
+        int32_t packed = 0, before, total;
 #pragma unroll
-            for (int u = 0; u < 4; u++) x[u] = j0 + tid * 4 + u < held ? wr[j0 + tid * 4 + u] : 0.f;
-        }
+        for (int u = 0; u < 4; u++) x[u] = wr[min(j0 + wave * 256 + u * 64 + lane, er.held - 1)];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const int64_t j = j0 + tid * 4 + u;
+            const int32_t j = j0 + wave * 256 + u * 64 + lane;
             const uint32_t y = weight_order(x[u]);
-            const bool stays = j < fixed || (j >= until && j < held), may = j >= fixed && j < until && need > 0;
-            is[u] = stays || (may && y > bar);
-            eq[u] = may && y == bar;
-            packed += is[u] | eq[u] << 16;
+            const bool may = j >= er.fixed && j < er.until;
+            is[u] = __ballot(may ? takes && y > er.bar : j < er.held);
+            eq[u] = __ballot(may && takes && y == er.bar);
+            packed += __popcll(is[u]) | __popcll(eq[u]) << 16;
         }
-        int32_t total;
-        const int32_t at = plan_scan(packed, sums, turn, &total);
-        int32_t o = over + (at & 0xffff), e = equal + (at >> 16);
+        meet(packed, &before, &total);
+        int32_t o = over + (before & 0xffff), e = equal + (before >> 16);
+        over += total & 0xffff, equal += total >> 16;
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const int64_t j = j0 + tid * 4 + u;
-            if (is[u] || (eq[u] && e < ties)) {
-                const int64_t to = o + min(e, ties);
-                out[to] = (int32_t)j;
-                if (to != j) {
-                    wr[to] = x[u];
-                    const uint32_t cf = (uint32_t)j / (uint32_t)a.page_size, ct = (uint32_t)to / (uint32_t)a.page_size;
-                    const int32_t pf = row[cf], pt = row[ct];
-                    const bool ok = pf >= 0 && pf < a.num_pages && pt >= 0 && pt < a.num_pages;
-                    w.from[r * cap + to] = make_uint2(ok ? (uint32_t)pf : kNoPage, (uint32_t)(j - cf * a.page_size));
-                    w.to[r * cap + to] = make_uint2((uint32_t)pt, (uint32_t)(to - ct * a.page_size));
-                }
-            } else if (j < held && j == o + min(e, ties)) {
-                chosen = (int32_t)j;  // (the first key that goes: no other has its own index for a place)
+            const int32_t j = j0 + wave * 256 + u * 64 + lane;
+            const int32_t mine = e + __popcll(eq[u] & below), to = o + __popcll(is[u] & below) + min(mine, er.ties);
+            if ((is[u] >> lane & 1) || ((eq[u] >> lane & 1) && mine < er.ties)) {
+                out[to] = j;
+                w.weight[r * cap + to] = x[u];
+                const int32_t jc = j / size, tc = to / size, pf = row[jc], pt = row[tc];
+                const bool ok = pf >= 0 && pf < a.num_pages && pt >= 0 && pt < a.num_pages;
+                w.from[r * cap + to] = make_uint2(ok ? (uint32_t)pf : kNoPage, (uint32_t)(j - jc * size));
+                w.to[r * cap + to] = make_uint2((uint32_t)pt, (uint32_t)(to - tc * size));
+            } else if (j < er.held && j == to) {
+                w.rows[r].first = j;  // (the first key that goes: no other has its own index for a place)
             }
-            o += is[u], e += eq[u];
+            o += __popcll(is[u]), e += __popcll(eq[u]);
         }
-        over += total & 0xffff, equal += total >> 16;
     }
-    __syncthreads();
-    if (tid == 0) {
-        w.first[r] = chosen, w.count[r] = (int32_t)n;
-        a.lengths[r] = (int32_t)n;
-    }
-    for (int64_t j = n + tid; j < cap; j += kPlan) {
-        out[j] = -1;
-        if (j < held) wr[j] = 0.f;
-    }
-    for (int64_t c = pages_of(a, n) + tid; c < np; c += kPlan) {
+}
+
+// What else changes of a row that gives up keys, a workgroup's: its weights, its length, its entries and the counts of the
+// pages behind.
+__device__ __forceinline__ void evict_finish(const CacheArgs &a, const EvictWork &w, float *weights, int64_t stride, int64_t r) {
+    const EvictRow er = w.rows[r];
+    if (er.n == er.held) return;
+    float *wr = weights + r * stride;
+    for (int32_t j = er.first + threadIdx.x; j < er.held; j += blockDim.x) wr[j] = j < er.n ? w.weight[r * w.cap + j] : 0.f;
+    int32_t *row = a.table + r * a.max_pages;
+    const int64_t np = pages_of(a, er.held);
+    for (int64_t c = pages_of(a, er.n) + threadIdx.x; c < np; c += blockDim.x) {
         const int32_t page = row[c];
         row[c] = -1;
         if (page >= 0 && page < a.num_pages) atomicSub(a.counts + page, 1);
     }
+    if (threadIdx.x == 0) a.lengths[r] = er.n;
 }
 
-// Workgroup (row, pool, column): 2^shift threads a key, a T each. Two steps of kEvictLoads loads are in flight: a
-// step's keys are stored while the next one's arrive.
-#ifndef KEL
-#define KEL 8
-#endif
-constexpr int kEvictLoads = KEL, kEvictThreads = 512;
+// The first workgroups finish a row each (in the first launch of a call). Workgroup (row, pool, column): 2^shift threads
+// a key, a T each. Two steps of kEvictLoads loads are in flight: a step's keys are stored while the next one's arrive.
+constexpr int kEvictLoads = 8, kEvictThreads = 512;
 template <class T>
-__global__ __launch_bounds__(kEvictThreads) void cache_evict_move(EvictWork w, PoolArgs pools, int64_t page_size,
-                                                                  int32_t columns, int32_t shift) {
-    const int32_t keys = kEvictThreads >> shift, step = keys * kEvictLoads, mine = threadIdx.x >> shift;
+__global__ __launch_bounds__(kEvictThreads) void cache_evict_move(CacheArgs a, EvictWork w, float *weights, int64_t weights_stride,
+                                                                  int32_t finish, PoolArgs pools, int32_t columns,
+                                                                  int32_t shift) {
     int64_t i = blockIdx.x;
+    if (i < finish) {
+        evict_finish(a, w, weights, weights_stride, i);
+        return;
+    }
+    i -= finish;
+    const int64_t page_size = a.page_size;
+    const int32_t keys = kEvictThreads >> shift, step = keys * kEvictLoads, mine = threadIdx.x >> shift;
     const int32_t column = (int32_t)(i % columns);
     i /= columns;
     const int x = (int)(i % pools.n);
     const int64_t r = i / pools.n, bytes = pools.at[x].bytes / page_size, stride = pools.at[x].stride;
     const int64_t at = (((int64_t)column << shift) + (threadIdx.x & ((1 << shift) - 1))) * (int64_t)sizeof(T);
-    const int32_t first = w.first[r], count = w.count[r];
+    const int32_t first = w.rows[r].first, count = w.rows[r].n;
     const uint2 *from = w.from + r * w.cap, *to = w.to + r * w.cap;
     if (first >= count || ((int64_t)column << shift) * (int64_t)sizeof(T) >= bytes) return;
     // (a thread past the row's end reads the row's first bytes, one without a key the pool's, and stores nothing)
@@ -823,18 +878,15 @@ int dm_cache_compact(const dm_cache_table *t, const dm_cache_pool *pools, int64_
 static EvictWork evict_work(const dm_cache_table *t, char *at, size_t *bytes) {
     EvictWork w{};
     w.cap = t->max_pages * t->page_size;
-    const size_t rows = align_up((size_t)t->rows * 4), keys = align_up((size_t)(t->rows * w.cap) * sizeof(uint2));
-    w.first = (int32_t *)at;
-    w.count = (int32_t *)(at + rows);
-    w.from = (uint2 *)(at + 2 * rows);
-    w.to = (uint2 *)(at + 2 * rows + keys);
-    *bytes = 2 * (rows + keys);
+    const size_t rows = align_up((size_t)t->rows * sizeof(EvictRow)), keys = (size_t)(t->rows * w.cap);
+    w.rows = (EvictRow *)at;
+    w.from = (uint2 *)(at + rows);
+    w.to = (uint2 *)(at + rows + align_up(keys * sizeof(uint2)));
+    w.weight = (float *)(at + rows + 2 * align_up(keys * sizeof(uint2)));
+    *bytes = rows + 2 * align_up(keys * sizeof(uint2)) + align_up(keys * sizeof(float));
     return w;
 }
-#ifndef KEG
-#define KEG 256
-#endif
-constexpr int64_t kEvictGroups = KEG;
+constexpr int64_t kEvictGroups = 256;
 static bool evict_sizes(const dm_cache_table *t) {
     return table_sizes(t) && t->rows <= kMostRows && t->max_pages <= ((int64_t)1 << 30) / t->page_size &&
            t->rows * t->max_pages * t->page_size < kI31 * 16;
@@ -862,11 +914,27 @@ int dm_cache_evict(const dm_cache_table *t, const dm_cache_pool *pools, int64_t 
         return refuse(op + ": the workspace is smaller than dm_cache_evict_workspace");
     if (t->rows == 0 || cap == 0) return DM_OK;
     if (!weights || !budgets || !kept) return refuse(op + ": the weights, the budgets or the results' place are missing");
+    for (int64_t i = 0; i < npools; i += kPoolsPerLaunch) {  // (workgroups of a launch: a row each, and columns of 512 bytes or more)
+        int64_t groups = t->rows;
+        for (int64_t x = i; x < std::min(npools, i + kPoolsPerLaunch); x++)
+            groups += t->rows * (pools[x].page_bytes / t->page_size / 512 + 1);
+        if (groups >= ((int64_t)1 << 23)) return refuse(op + ": more rows and bytes than one launch takes");
+    }
     hipStream_t st = (hipStream_t)stream;
     size_t bytes;
     const EvictWork w = evict_work(t, (char *)workspace, &bytes);
-    cache_evict_plan<<<(unsigned)t->rows, kPlan, 0, st>>>(cache_args(t), weights, weights_stride, budgets, recent, kept, w);
-    for (int64_t i = 0; i < npools; i += kPoolsPerLaunch) {
+    const CacheArgs ca = cache_args(t);
+    cache_evict_select<<<(unsigned)t->rows, kPlan, 0, st>>>(ca, weights, weights_stride, budgets, recent, w);
+    const unsigned shares = (unsigned)std::min<int64_t>(kEvictShares, (cap + 4 * kPlan - 1) / (4 * kPlan));
+    for (int64_t r = 0; r < t->rows; r += 65535) {  // (rows of a launch)
+        EvictWork part = w;
+        part.rows += r, part.from += r * cap, part.to += r * cap, part.weight += r * cap;
+        CacheArgs pa = ca;
+        pa.table += r * t->max_pages;
+        cache_evict_place<<<dim3(shares, (unsigned)std::min<int64_t>(65535, t->rows - r)), kPlan, 0, st>>>(
+            pa, weights + r * weights_stride, weights_stride, kept + r * cap, part);
+    }
+    for (int64_t i = 0; i == 0 || i < npools; i += kPoolsPerLaunch) {
         bool wide;
         int64_t pieces, most = 0, grain = 16;
         const PoolArgs pa = pools_of(pools, npools, i, &wide, &pieces);
@@ -881,11 +949,11 @@ int dm_cache_evict(const dm_cache_table *t, const dm_cache_pool *pools, int64_t 
         auto columns = [&](int n) { return (most + (grain << n) - 1) / (grain << n); };
         while (shift > 0 && (t->rows * pa.n * columns(shift) < kEvictGroups || (most <= grain << (shift - 1)))) shift--;
         const int64_t items = t->rows * pa.n * columns(shift);
-        if (most == 0) continue;
-        if (columns(shift) >= kI31 || items >= ((int64_t)1 << 23))
-            return refuse(op + ": more rows and bytes than one launch takes");
-#define EVICT_MOVE(T) \
-    cache_evict_move<T><<<(unsigned)items, kEvictThreads, 0, st>>>(w, pa, t->page_size, (int32_t)columns(shift), shift)
+        const int64_t finish = i == 0 ? t->rows : 0;
+        if (finish + items == 0) continue;
+#define EVICT_MOVE(T)                                                                                             \
+    cache_evict_move<T><<<(unsigned)(finish + items), kEvictThreads, 0, st>>>(ca, w, weights, weights_stride,     \
+                                                                              (int32_t)finish, pa, (int32_t)columns(shift), shift)
         if (grain == 16)
             EVICT_MOVE(u32x4_vec);
         else if (grain == 8)

@@ -100,6 +100,8 @@ def _evict(ws=1 << 40, pools=(), w=256, stride=64, b=256, kept=256, recent=0, **
     (dict(w=None), "missing"), (dict(b=None), "missing"), (dict(kept=None), "missing"), (dict(ws=0), "workspace"),
     (dict(recent=-1), "recent"), (dict(stride=63), "their rows apart"), (dict(rows=(1 << 22) + 1), "at most 2^22"),
     (dict(max_pages=(1 << 26) + 1), "at most 2^30"), (dict(rows=1 << 22, max_pages=1 << 13, page_size=1), "less than 2^35"),
+    (dict(rows=1 << 22, pools=[_lib.CachePool(256, 32, 32)]), "more rows and bytes"),
+    (dict(rows=1 << 20, pools=[_lib.CachePool(256, 1 << 16, 1 << 16)]), "more rows and bytes"),
     (dict(pools=[_lib.CachePool(256, 24, 24)]), "a pool's pages"), (dict(pools=[_lib.CachePool(None, 32, 32)]), "missing")])
 def test_the_eviction_refuses(kw, what):
     rc, msg = _evict(**kw)
