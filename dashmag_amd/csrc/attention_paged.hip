@@ -870,39 +870,86 @@ __global__ __launch_bounds__((64 * paged_waves<D>()), (D == 256 ? 1 : 2)) void p
     }
 }
 
-// The pieces of a shared tile joined, a wavefront a row: the largest reference, then the outputs and sums by it, in
-// the order of the workers.
-template <int DT>
-__global__ __launch_bounds__(256) void paged_join(PagedArgs a, PagedLine l) {
-    const PagedJob job = l.jobs[blockIdx.x];
-    const int lane = threadIdx.x & 63, r = blockIdx.y * 4 + uni(threadIdx.x >> 6);
-    if (r >= job.rows) return;
-    const int n = job.last - job.first + 1;
-    auto place = [&](int i) { return (int64_t)(2 * (job.first + i) + (i == 0 ? 1 : 0)) * l.pitch + r; };
-    float top = -INFINITY;
-    for (int i = lane; i < n; i += 64) top = fmaxf(top, l.ml[place(i)].x);
-    top = wave_max(top);
-    float sum = 0.f, acc[4] = {};
-    for (int i0 = 0; i0 < n; i0 += 64) {
-        const float2 ml = i0 + lane < n ? l.ml[place(i0 + lane)] : make_float2(-INFINITY, 0.f);
-        const float f = ml.x == top ? 1.f : fast_exp2(ml.x - top), s = ml.y * f;
-        for (int i = 0; i < min(64, n - i0); i++) {
-            const float y = __shfl(s, i, 64), g = __shfl(f, i, 64);
-            if (__shfl(ml.y, i, 64) == 0.f) continue;  // (no key of the piece has a weight)
-            sum += y;
-            const float *o = l.o + place(i0 + i) * a.d;
+// The pieces of shared tiles joined: D / V threads a row, V columns each, the workgroup's other threads take other rows,
+// or share out the pieces of one where they are more than kJoinMany (each every so-many-th of them, added in order). A
+// thread needs nothing but its own loads: its reference moves as in the sweep.
+constexpr int kJoinMany = 48, kJoinFew = 4;  // and the pieces that a thread has in flight
+template <int V>
+struct Joined {
+    float m, sum, acc[V];
+};
+template <int V>
+__device__ __forceinline__ void join_one(Joined<V> &j, float m, float sum, const float *o) {
+    const float top = fmaxf(j.m, m);
+    // (a piece without weight: zeros, and a reference of -inf that may be the largest all the same)
+    const float f = j.m == top ? 1.f : fast_exp2(j.m - top), g = m == top ? 1.f : fast_exp2(m - top);
+    j.m = top;
+    j.sum = j.sum * f + sum * g;
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-                if (lane + 64 * u < a.d) acc[u] += g * o[lane + 64 * u];
+    for (int c = 0; c < V; c++) j.acc[c] = j.acc[c] * f + o[c] * g;
+}
+template <int DT, int V>
+__global__ __launch_bounds__(256) void paged_join(PagedArgs a, PagedLine narrow, PagedLine wide, int32_t nblocks) {
+    __shared__ float red[256 * (V + 2)];
+    const int tid = threadIdx.x, per = a.d / V, slots = 256 / per, slot = tid / per, c = (tid - slot * per) * V;
+    // (narrow tiles' workgroups first: y of them a job)
+    const bool w = (int32_t)blockIdx.x >= nblocks;
+    const PagedLine &l = w ? wide : narrow;
+    const int32_t y = (l.pitch + slots - 1) / slots, i = blockIdx.x - (w ? nblocks : 0), jb = i / y, r0 = (i - jb * y) * slots;
+    const PagedJob job = l.jobs[jb];
+    if (r0 >= job.rows) return;
+    const int32_t n = job.last - job.first + 1;
+    const bool few = n <= kJoinMany;
+    const int32_t rows = min(slots, job.rows - r0);
+    for (int32_t x = 0; x < (few ? 1 : rows); x++) {
+        const int32_t r = r0 + (few ? slot : x), step = few ? 1 : slots;
+        const bool on = slot < slots && r < job.rows;
+        Joined<V> j{-INFINITY, 0.f, {}};
+        for (int32_t p0 = few ? 0 : slot; on && p0 < n; p0 += kJoinFew * step) {
+            float2 ml[kJoinFew];
+            float o[kJoinFew][V];
+#pragma unroll
+            for (int u = 0; u < kJoinFew; u++) {
+                const int32_t p = min(p0 + u * step, n - 1);  // (past the last: read again, left out)
+                const int64_t at = (int64_t)(2 * (job.first + p) + (p == 0 ? 1 : 0)) * l.pitch + r;
+                ml[u] = l.ml[at];
+                if constexpr (V == 4)
+                    *(float4 *)o[u] = *(const float4 *)(l.o + at * a.d + c);
+                else
+                    o[u][0] = l.o[at * a.d + c];
+            }
+#pragma unroll
+            for (int u = 0; u < kJoinFew; u++)
+                if (p0 + u * step < n) join_one<V>(j, ml[u].x, ml[u].y, o[u]);
         }
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int32_t i = r / job.per;
-    const int64_t row = (int64_t)(job.tok + i) * a.hq + job.head + (r - i * job.per);
+        if (!few) {
+            __syncthreads();
+            float *mine = red + tid * (V + 2);
+            mine[0] = j.m, mine[1] = j.sum;
 #pragma unroll
-    for (int u = 0; u < 4; u++)
-        if (lane + 64 * u < a.d) st<DT>(a.o, row * a.d + lane + 64 * u, acc[u] * inv);
-    if (lane == 0 && a.lse) a.lse[row] = lse_of(top, sum);
+            for (int u = 0; u < V; u++) mine[2 + u] = j.acc[u];
+            __syncthreads();
+            if (slot != 0) continue;
+            for (int k = 1; k < min(slots, n); k++) {
+                const float *other = red + (tid + k * per) * (V + 2);
+                join_one<V>(j, other[0], other[1], other + 2);
+            }
+        }
+        if (!on) continue;
+        const float inv = j.sum == 0.f ? 0.f : 1.f / j.sum;  // (NaN is not 0)
+        const int32_t t = r / job.per;
+        const int64_t row = (int64_t)(job.tok + t) * a.hq + job.head + (r - t * job.per);
+        if constexpr (V == 4 && DT != DM_F32) {
+            *(uint2 *)((uint16_t *)a.o + row * a.d + c) =
+                make_uint2(pack2<DT>(j.acc[0] * inv, j.acc[1] * inv), pack2<DT>(j.acc[2] * inv, j.acc[3] * inv));
+        } else if constexpr (V == 4) {
+            *(float4 *)((float *)a.o + row * a.d + c) =
+                make_float4(j.acc[0] * inv, j.acc[1] * inv, j.acc[2] * inv, j.acc[3] * inv);
+        } else {
+            st<DT>(a.o, row * a.d + c, j.acc[0] * inv);
+        }
+        if (c == 0 && a.lse) a.lse[row] = lse_of(j.m, j.sum);
+    }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1349,6 +1396,9 @@ int dm_attention_paged(const dm_attention_desc *d, const void *q, const void *k_
                      (((uintptr_t)k_pages | (uintptr_t)v_pages) & (4 * eb - 1)) == 0;
     const PagedLine &l = p.narrow;
     const unsigned g = l.workers / 4;
+    const int slots = 256 / (int)(d->d % 4 == 0 && aligned_16b(o) ? d->d / 4 : d->d);  // rows of a joining workgroup
+    const int nb = l.workers * ((l.pitch + slots - 1) / slots);
+    const int wb = p.mixed ? p.wide.workers * ((p.wide.pitch + slots - 1) / slots) : 0;
 #define PAGED_W(DT, DP)                                                                                       \
     if (weights && !fast)                                                                                     \
         paged_weights_simple<DT, DP><<<1024, 256, 0, st>>>(a, q, k_pages, weights, weights_stride);           \
@@ -1368,8 +1418,10 @@ int dm_attention_paged(const dm_attention_desc *d, const void *q, const void *k_
         paged_simple<DT, DP, 4><<<g, 256, 0, st>>>(a, l, q, k_pages, v_pages);                                \
     else if (!fast)                                                                                           \
         paged_simple<DT, DP, 1><<<g, 256, 0, st>>>(a, l, q, k_pages, v_pages);                                \
-    paged_join<DT><<<dim3(l.workers, (l.pitch + 3) / 4), 256, 0, st>>>(a, l);                                 \
-    if (p.mixed) paged_join<DT><<<dim3(p.wide.workers, (p.wide.pitch + 3) / 4), 256, 0, st>>>(a, p.wide);     \
+    if (d->d % 4 == 0 && aligned_16b(o))                                                                      \
+        paged_join<DT, 4><<<nb + wb, 256, 0, st>>>(a, l, p.wide, nb);                                         \
+    else                                                                                                      \
+        paged_join<DT, 1><<<nb + wb, 256, 0, st>>>(a, l, p.wide, nb);                                         \
     PAGED_W(DT, DP)
 #define PAGED(DT)               \
     if (padded(d->d) == 64) {   \
