@@ -93,16 +93,17 @@ template <int DT, int DP, int VEC>
 __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, const void *__restrict__ q,
                                                     const void *__restrict__ k, const void *__restrict__ v) {
     constexpr int TS = DP + 4, CPR = DP / VEC, DTN = DP / 32, HALF = DP / 2;
-    __shared__ PlanSmem<256> plan;
+    __shared__ PlanSmem<256, 1> plan;
     __shared__ __align__(16) float tiles[4][32 * TS];
     const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
     const int32_t worker = blockIdx.x * 4 + wave;
     PagedWalk walk;
-    int64_t p;
-    bool valid;
-    const PagedShare sh = plan_line<256>(
-        a, l, plan, [&](const PagedShare &s) { return worker < s.workers ? s.at(worker) : -1; }, &walk, &p, &valid);
-    fill_outside<DT>(a, valid);
+    const PagedLine lines[1] = {l};
+    PagedShare shares[1];
+    fill_outside<DT>(a, plan_lines(a, lines, plan, shares));
+    const PagedShare &sh = shares[0];
+    int64_t p = sh.total > 0 && worker < sh.workers ? sh.at(worker) : -1;
+    plan_find<0>(a, lines, plan, sh, p, &walk);
     if (lane == 0 && worker < l.workers) l.jobs[worker].rows = 0;
     if (p < 0) return;
     const int64_t end = sh.at(worker + 1);
@@ -800,18 +801,18 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void paged_narrow_kernel(P
                                                                               const void *__restrict__ k,
                                                                               const void *__restrict__ v) {
     __shared__ union {
-        PlanSmem<256> plan;
+        PlanSmem<256, 1> plan;
         NarrowTile<D> tiles[4];
     } sm;
     const int wave = uni(threadIdx.x >> 6);
     const int32_t worker = blockIdx.x * 4 + wave;
     PagedWalk walk;
-    int64_t p;
-    bool valid;
-    const PagedShare sh = plan_line<256>(
-        a, l, sm.plan, [&](const PagedShare &s) { return worker < s.workers ? s.at(worker) : -1; }, &walk, &p, &valid);
-    fill_outside<DT>(a, valid);
-    narrow_share<DT, D>(a, l, sh, worker, walk, p, q, k, v, sm.tiles[wave]);
+    const PagedLine lines[1] = {l};
+    PagedShare sh[1];
+    fill_outside<DT>(a, plan_lines(a, lines, sm.plan, sh));
+    const int64_t p = sh[0].total > 0 && worker < sh[0].workers ? sh[0].at(worker) : -1;
+    plan_find<0>(a, lines, sm.plan, sh[0], p, &walk);
+    narrow_share<DT, D>(a, l, sh[0], worker, walk, p, q, k, v, sm.tiles[wave]);
 }
 
 // Any call: the wide tiles' line, a workgroup a worker, and the narrow tiles', a wavefront a worker. Every other
@@ -822,36 +823,33 @@ __global__ __launch_bounds__((64 * paged_waves<D>()), (D == 256 ? 1 : 2)) void p
                                                                                    const void *__restrict__ k,
                                                                                    const void *__restrict__ v) {
     constexpr int NW = paged_waves<D>();
+    __shared__ PlanSmem<64 * NW, 2> plan;
     __shared__ union {
-        PlanSmem<64 * NW> plan;
         WideTiles<D> wide;
         NarrowTile<D> tiles[NW];
     } sm;
     const int wave = uni(threadIdx.x >> 6);
+    const PagedLine lines[2] = {wide, narrow};
+    PagedShare shares[2];
+    fill_outside<DT>(a, plan_lines(a, lines, plan, shares));
     for (int turn = 0; turn < 2; turn++) {
         PagedWalk walk;
-        int64_t p;
-        bool valid;
         if ((turn ^ (int)(blockIdx.x >> 3)) & 1) {
+            const PagedShare &sh = shares[1];
             const int32_t worker = blockIdx.x * NW + wave;
-            const PagedShare sh = plan_line<64 * NW>(
-                a, narrow, sm.plan, [&](const PagedShare &s) { return worker < s.workers ? s.at(worker) : -1; }, &walk, &p,
-                &valid);
+            const int64_t p = sh.total > 0 && worker < sh.workers ? sh.at(worker) : -1;
+            if (sh.total > 0) plan_find<1>(a, lines, plan, sh, p, &walk);
             narrow_share<DT, D>(a, narrow, sh, worker, walk, p, q, k, v, sm.tiles[wave]);
             __syncthreads();
             continue;
         }
         // workgroups go to the XCDs in turn: each XCD has a part of the line of its own
+        const PagedShare &sh = shares[0];
         int32_t worker = blockIdx.x;
-        const PagedShare sh = plan_line<64 * NW>(
-            a, wide, sm.plan,
-            [&](const PagedShare &s) {
-                if (s.workers == (int32_t)gridDim.x && s.workers % 8 == 0)
-                    worker = blockIdx.x % 8 * (s.workers / 8) + blockIdx.x / 8;
-                return worker < s.workers ? s.at(worker) : -1;
-            },
-            &walk, &p, &valid);
-        fill_outside<DT>(a, valid);
+        if (sh.workers == (int32_t)gridDim.x && sh.workers % 8 == 0)
+            worker = blockIdx.x % 8 * (sh.workers / 8) + blockIdx.x / 8;
+        int64_t p = sh.total > 0 && worker < sh.workers ? sh.at(worker) : -1;
+        if (sh.total > 0) plan_find<0>(a, lines, plan, sh, p, &walk);
         if (threadIdx.x == 0) wide.jobs[worker].rows = 0;
         if (p < 0) continue;
         const int64_t end = sh.at(worker + 1);
@@ -1031,7 +1029,7 @@ constexpr int key_tile() { return 8 * 32 * key_cols<D>(); }
 template <int D>
 union KeyTiles {
     static constexpr int KS = D + 8;
-    PlanSmem<512> plan;
+    PlanSmem<512, 1> plan;
     struct {
         alignas(16) uint16_t q[2][64 * KS];
         alignas(16) float ref[2][64];  // -lse in log2 units, -inf for a row that is none or sees no key
@@ -1050,10 +1048,12 @@ __global__ __launch_bounds__(512, 2) void paged_weights_kernel(PagedArgs a, KeyL
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), col = lane & 31, half = lane >> 5;
     const int32_t worker = blockIdx.x;
     PagedWalk walk;
-    int64_t p;
-    bool valid;
-    const PagedShare sh = plan_line<512>(
-        a, l, sm.plan, [&](const PagedShare &s) { return worker < s.workers ? s.at(worker) : -1; }, &walk, &p, &valid);
+    const KeyLine lines[1] = {l};
+    PagedShare shares[1];
+    plan_lines(a, lines, sm.plan, shares);
+    const PagedShare &sh = shares[0];
+    int64_t p = sh.total > 0 && worker < sh.workers ? sh.at(worker) : -1;
+    plan_find<0>(a, lines, sm.plan, sh, p, &walk);
     if (tid == 0) l.jobs[worker].rows = 0;
     if (p < 0) return;
     const int64_t end = sh.at(worker + 1);
@@ -1296,8 +1296,12 @@ static PagedPlan paged_plan(const dm_attention_desc *d, char *base, bool weights
     p.narrow = line_of(d, 32, 0, p.mixed ? kNarrowRows : INT32_MAX);
     p.narrow.workers = d->d > 128 ? 1024 : 2048;
     p.narrow.unit = 32;
-    p.narrow.start = 64;
-    p.narrow.least = 192;
+#ifndef NST
+#define NST 64
+#define NLE 96
+#endif
+    p.narrow.start = NST;
+    p.narrow.least = NLE;
     p.bytes = place_line(d, &p.narrow, base, p.bytes);
     p.lse = p.bytes;
     if (weights) {

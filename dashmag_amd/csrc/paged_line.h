@@ -35,7 +35,7 @@ struct PagedLine {
     int32_t rt, pitch;  // most rows of a tile, and of this call's tiles
     int32_t m, hc, per; // tokens of a tile; tiles of a token (above rt heads); row r: token r / per, head r % per
     int32_t over, upto; // the sequences of over < n rep <= upto rows
-    int32_t workers, unit;   // most workers; a piece's keys begin at multiples of unit from the tile's first
+    int32_t workers, unit;   // most workers; a piece's keys begin at multiples of unit (a power of 2) from the tile's first
     int32_t start, least;    // a tile's start in keys, and what a worker has at least
     float *o;           // [2 workers, pitch, D]: unnormalised outputs
     float2 *ml;         // [2 workers, pitch]: reference (log2 units) and sum
@@ -114,57 +114,64 @@ __device__ __forceinline__ bool on_line(const PagedArgs &a, const KeyLine &l, co
     return q.n > 0 && q.len > 0 && (int64_t)q.n * a.rep > l.over;
 }
 
-// The exclusive prefix sums of the workgroup's x, and its total.
-template <int NT>
+// The exclusive prefix sums of the workgroup's x on each of L lines, and their totals.
+template <int NT, int L>
 struct PlanSmem {
-    int64_t pre[NT], waves[NT / 64];
-    int64_t base;
+    int64_t pre[L][NT], waves[L][NT / 64];
 };
-template <int NT>
-__device__ __forceinline__ int64_t scan64(int64_t x, PlanSmem<NT> &sm) {
+template <int NT, int L, class Line>
+__device__ __forceinline__ void plan_chunk(const PagedArgs &a, const Line (&l)[L], int32_t s0, PlanSmem<NT, L> &sm, bool *ok,
+                                           int64_t (&all)[L]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t in = x;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t y = __shfl_up((long long)in, o, 64);
-        if (lane >= o) in += y;
-    }
-    __syncthreads();  // (the last chunk's sums have been read)
-    if (lane == 63) sm.waves[wave] = in;
-    __syncthreads();
-    int64_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 64; w++) {
-        before += w < wave ? sm.waves[w] : 0;
-        all += sm.waves[w];
-    }
-    sm.pre[threadIdx.x] = before + in - x;
-    __syncthreads();
-    return all;
-}
-template <int NT, class Line>
-__device__ __forceinline__ int64_t plan_chunk(const PagedArgs &a, const Line &l, int32_t s0, PlanSmem<NT> &sm,
-                                              bool *ok) {
     const int32_t s = s0 + (int32_t)threadIdx.x;
-    int64_t x = 0;
+    int64_t x[L], in[L];
+#pragma unroll
+    for (int i = 0; i < L; i++) x[i] = 0;
     if (s < a.S) {
         const PagedSeq q = paged_seq(a, s);
         *ok = *ok && q.ok;
-        if (on_line(a, l, q)) x = turns_of(a, l) * tiles_cost(a, l, q, tiles_of(a, l, q));
+#pragma unroll
+        for (int i = 0; i < L; i++)
+            if (on_line(a, l[i], q)) x[i] = turns_of(a, l[i]) * tiles_cost(a, l[i], q, tiles_of(a, l[i], q));
     }
-    return scan64<NT>(x, sm);
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+        in[i] = x[i];
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t y = __shfl_up((long long)in[i], o, 64);
+            if (lane >= o) in[i] += y;
+        }
+    }
+    __syncthreads();  // (the last chunk's sums have been read)
+#pragma unroll
+    for (int i = 0; i < L; i++)
+        if (lane == 63) sm.waves[i][wave] = in[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+        int64_t before = 0;
+        all[i] = 0;
+#pragma unroll
+        for (int w = 0; w < NT / 64; w++) {
+            before += w < wave ? sm.waves[i][w] : 0;
+            all[i] += sm.waves[i][w];
+        }
+        sm.pre[i][threadIdx.x] = before + in[i] - x[i];
+    }
+    __syncthreads();
 }
 
 // A worker's place on a line of length `total` with `workers` workers: worker w has [at(w), at(w + 1)).
 struct PagedShare {
-    int64_t total;
-    int32_t workers;
+    int64_t total, each;
+    int32_t workers, rest;  // total = each x workers + rest
     __device__ __forceinline__ int64_t at(int32_t w) const {
-        return total / workers * w + total % workers * w / workers;
+        return each * w + (int32_t)((uint32_t)(rest * w) / (uint32_t)workers);
     }
     // the last worker that begins in front of x > 0
     __device__ __forceinline__ int32_t last_before(int64_t x) const {
-        int32_t w = (int32_t)min((int64_t)workers - 1, (x - 1) / max(total / workers, (int64_t)1));
+        int32_t w = (int32_t)min((int64_t)workers - 1, (x - 1) / each);
         while (w > 0 && at(w) >= x) w--;
         return w;
     }
@@ -178,57 +185,68 @@ struct PagedWalk {
     int64_t base;
 };
 
-// The whole workgroup: the line's total, 0 where offsets do not go up; and the walk of the worker at `p`
-// (wavefront-uniform; each wavefront its own), if it has anything. `where` maps (total) to p, or -1 for none.
-template <int NT, class Line, class Where>
-__device__ __forceinline__ PagedShare plan_line(const PagedArgs &a, const Line &l, PlanSmem<NT> &sm, Where where,
-                                                PagedWalk *walk, int64_t *p, bool *valid) {
+// The whole workgroup: the lines' lengths and shares; every line is of length 0 where the offsets do not go up (false).
+template <int NT, int L, class Line>
+__device__ __forceinline__ bool plan_lines(const PagedArgs &a, const Line (&l)[L], PlanSmem<NT, L> &sm, PagedShare (&sh)[L]) {
     bool ok = true;
-    int64_t total = 0;
-    for (int32_t s0 = 0; s0 < a.S; s0 += NT) total += plan_chunk<NT>(a, l, s0, sm, &ok);
+#pragma unroll
+    for (int i = 0; i < L; i++) sh[i].total = 0;
+    for (int32_t s0 = 0; s0 < a.S; s0 += NT) {
+        int64_t all[L];
+        plan_chunk<NT, L>(a, l, s0, sm, &ok, all);
+#pragma unroll
+        for (int i = 0; i < L; i++) sh[i].total += all[i];
+    }
     ok = __syncthreads_and(ok);
-    *valid = ok;
-    PagedShare sh;
-    sh.total = ok ? total : 0;
-    sh.workers = (int32_t)max((int64_t)1, min((int64_t)l.workers, sh.total / l.least));
-    *p = sh.total > 0 ? where(sh) : -1;
-    int64_t base = 0;
-    int32_t found = -1;
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+        if (!ok) sh[i].total = 0;
+        sh[i].workers = (int32_t)max((int64_t)1, min((int64_t)l[i].workers, sh[i].total / l[i].least));
+        sh[i].each = sh[i].total / sh[i].workers;
+        sh[i].rest = (int32_t)(sh[i].total - sh[i].each * sh[i].workers);
+    }
+    return ok;
+}
+
+// The whole workgroup: the walk of the worker that begins at p of line I (wavefront-uniform, each wavefront its own; none:
+// a p below zero).
+template <int I, int NT, int L, class Line>
+__device__ __forceinline__ void plan_find(const PagedArgs &a, const Line (&l)[L], PlanSmem<NT, L> &sm, const PagedShare &sh,
+                                          int64_t p, PagedWalk *walk) {
     const int lane = threadIdx.x & 63;
+    int64_t base = 0;
     for (int32_t s0 = 0; s0 < a.S && sh.total > 0; s0 += NT) {
-        int64_t all = sh.total;
-        if (a.S > NT) all = plan_chunk<NT>(a, l, s0, sm, &ok);
-        if (*p >= base && *p < base + all) {
+        int64_t all[L];
+        all[I] = sh.total;
+        bool ok = true;
+        if (a.S > NT) plan_chunk<NT, L>(a, l, s0, sm, &ok, all);
+        if (p >= base && p < base + all[I]) {
             int n = 0;
 #pragma unroll 1
-            for (int i = 0; i < NT; i += 64) n += __popcll(__ballot(sm.pre[i + lane] <= *p - base));
-            found = s0 + n - 1;
-            walk->base = base + sm.pre[n - 1];
+            for (int i = 0; i < min(NT, a.S - s0); i += 64)
+                n += __popcll(__ballot(i + lane < a.S - s0 && sm.pre[I][i + lane] <= p - base));
+            walk->s = __builtin_amdgcn_readfirstlane(s0 + n - 1);
+            walk->base = base + sm.pre[I][n - 1];
         }
-        base += all;
+        base += all[I];
     }
     __syncthreads();  // (the sums have been read)
-    if (found < 0) {
-        *p = -1;
-        return sh;
-    }
-    walk->s = __builtin_amdgcn_readfirstlane(found);
+    if (p < 0) return;
     walk->q = paged_seq(a, walk->s);
-    walk->nt = tiles_of(a, l, walk->q);
-    int64_t rem = *p - walk->base;
-    const int64_t turn = tiles_cost(a, l, walk->q, walk->nt), u = rem / turn;
+    walk->nt = tiles_of(a, l[I], walk->q);
+    int64_t rem = p - walk->base;
+    const int64_t turn = tiles_cost(a, l[I], walk->q, walk->nt), u = rem / turn;
     rem -= u * turn;
     // the last tile that begins at rem or in front of it: 64 probes at a time
     int32_t lo = 0, hi = walk->nt;  // it lies in [lo, hi)
     while (hi - lo > 1) {
         const int32_t step = (hi - lo + 63) / 64, t = lo + lane * step;
-        const int n = __popcll(__ballot(t < hi && tiles_cost(a, l, walk->q, t) <= rem));
+        const int n = __popcll(__ballot(t < hi && tiles_cost(a, l[I], walk->q, t) <= rem));
         lo += (n - 1) * step;
         hi = min(hi, lo + step);
     }
     walk->u = (int32_t)u, walk->t = lo;
-    walk->base = *p - rem + tiles_cost(a, l, walk->q, lo);
-    return sh;
+    walk->base = p - rem + tiles_cost(a, l[I], walk->q, lo);
 }
 
 // A worker's next piece: rows of one tile, the keys [s0, s1) of those [lo, hi) that the tile sees.
@@ -256,7 +274,7 @@ __device__ __forceinline__ PagedPiece piece_of(const PagedArgs &a, const PagedLi
     const int32_t hi = max(0, w.q.len - w.q.n + i1);
     const int32_t lo = a.left >= 0 ? min(hi, max(0, x.pos - a.left)) : 0;
     auto key = [&](int64_t off) -> int32_t {  // the key at `off` of the tile's part of the line
-        const int64_t k = (off - l.start) / l.unit * l.unit;
+        const int64_t k = (off - l.start) & -(int64_t)l.unit;
         return off >= cost ? hi : (k <= 0 ? lo : (int32_t)min((int64_t)hi, lo + k));
     };
     const int64_t o0 = p - w.base, o1 = min(end - w.base, cost);
