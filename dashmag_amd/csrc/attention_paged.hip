@@ -542,12 +542,14 @@ struct WideTiles {
     static constexpr int KS = D + 8, VS = D + 32, NW = paged_waves<D>();
     alignas(16) uint16_t k[2][64 * KS], v[2][64 * VS];
     uint32_t places[1024];  // of 16 tiles' keys, see `fill`
-    int32_t lo[NW], hi[NW], bad;
+};
+struct WideFlags {
+    int32_t lo[8], hi[8], bad, missing;  // values that are not finite taken out; keys of no page
 };
 
 template <int DT, int D>
 __device__ __forceinline__ void paged_wide(const PagedArgs &a, const PagedLine &l, const PagedPiece &x, const PoolMap &map,
-                                           const void *q, WideTiles<D> &sm, NarrowTile<D> *area) {
+                                           const void *q, WideTiles<D> &sm, WideFlags &flags, NarrowTile<D> *area) {
     constexpr int NW = paged_waves<D>(), NT = NW * 64, KS = WideTiles<D>::KS, VS = WideTiles<D>::VS;
     constexpr int CPR = D / 8, RSTEP = NT / CPR, NCH = 64 / RSTEP;  // pieces a row, rows at a time, pieces a thread
     constexpr int KST = D / 16, DTN = D / 32, AHEAD = 2, PK = 512 / NT;
@@ -555,19 +557,22 @@ __device__ __forceinline__ void paged_wide(const PagedArgs &a, const PagedLine &
     const bool first = NW == 4 || wave < 4;  // products first in each step
     const int32_t s0 = x.s0, s1 = x.s1, nt = (s1 - s0 + 63) / 64;
     int32_t entry[PK], entry1[PK];
-    auto look_up = [&](int32_t key, int32_t (&entry)[PK]) __attribute__((always_inline)) {  // of 512 keys from `key` on
+    // the entries of 512 keys from `key` on, and the places that these say; behind the piece the last key's (masked, but
+    // loaded), and the pool's start for a key of no page
+    auto look_up = [&](int32_t key, int32_t (&entry)[PK]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < PK; u++) entry[u] = entry_of(map, s0 + key + u * NT + (int32_t)threadIdx.x, s1);
+        for (int u = 0; u < PK; u++) entry[u] = entry_of(map, min(s0 + key + u * NT + (int32_t)threadIdx.x, s1 - 1), s1);
     };
     auto fill = [&](int32_t key, const int32_t (&entry)[PK]) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < PK; u++) {
             const int32_t j = key + u * NT + (int32_t)threadIdx.x;
-            sm.places[j & 1023] = place_of(map, s0 + j, entry[u]);
+            const uint32_t at = place_of(map, min(s0 + j, s1 - 1), entry[u]);
+            if (at == kNoKey) flags.missing = 1;
+            sm.places[j & 1023] = at == kNoKey ? 0 : at;
         }
     };
-    look_up(0, entry);
-    look_up(512, entry1);
+    if (nt > 0) look_up(0, entry), look_up(512, entry1);
     const RowKeys rk = row_keys(a, x, wave * 32);
     QueryRows<D> qr;
     load_q<D>(a, rk, q, qr);
@@ -580,17 +585,17 @@ __device__ __forceinline__ void paged_wide(const PagedArgs &a, const PagedLine &
     }
     wlo = uni(wlo), whi = uni(whi);
     __syncthreads();  // (the last piece's results have left LDS)
+    if (lane == 0) flags.lo[wave] = rk.flo, flags.hi[wave] = rk.fhi;
+    if (threadIdx.x == 0) flags.bad = flags.missing = 0;
     settle_q<D>(a, (uint16_t *)&area[wave], false, qr);
     __syncthreads();  // (the queries' way through LDS is what the places and tiles lie in)
-    fill(0, entry);
-    fill(512, entry1);
-    if (lane == 0) sm.lo[wave] = rk.flo, sm.hi[wave] = rk.fhi;
-    if (threadIdx.x == 0) sm.bad = 0;
-    __syncthreads();
+    if (nt > 0) fill(0, entry), fill(512, entry1);
     int32_t tlo = INT32_MIN, thi = INT32_MAX;  // the keys that every row of the tile sees
 #pragma unroll
-    for (int w = 0; w < NW; w++) tlo = max(tlo, sm.lo[w]), thi = min(thi, sm.hi[w]);
+    for (int w = 0; w < NW; w++) tlo = max(tlo, flags.lo[w]), thi = min(thi, flags.hi[w]);
     tlo = uni(tlo), thi = uni(thi);
+    __syncthreads();
+    bool missing = uni(flags.missing);
     // (a scale of 0 as the smallest: a masked score stays -inf, the others' weights are alike)
     const float c2 = a.scale == 0.f ? 1.2e-38f : fabsf(a.scale) * kLog2e;
 
@@ -599,40 +604,43 @@ __device__ __forceinline__ void paged_wide(const PagedArgs &a, const PagedLine &
     const int row0 = threadIdx.x / CPR, lc = threadIdx.x % CPR;
     uint4 rk4[NCH], rv4[NCH];
     uint32_t ak[NCH], av[NCH];
-    bool okk[NCH], okv[NCH];
+    const char *kbase = map.k + lc * 16, *vbase = map.v + lc * 16;
     auto offsets = [&](int32_t j) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < NCH; u++) ak[u] = sm.places[(j * 64 + row0 + u * RSTEP) & 1023];
     };
-    auto load = [&](const char *base, const uint32_t (&at)[NCH], uint4 (&y)[NCH], bool (&ok)[NCH]) __attribute__((always_inline)) {
+    auto load_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < NCH; u++) {
-            ok[u] = at[u] != kNoKey;
-            y[u] = *(const uint4 *)(base + (uint64_t)(ok[u] ? at[u] : 0u) * 16 + lc * 16);
-        }
+        for (int u = 0; u < NCH; u++) rv4[u] = *(const uint4 *)(vbase + (uint64_t)av[u] * 16);
     };
-    auto load_v = [&]() __attribute__((always_inline)) { load(map.v, av, rv4, okv); };
     // the keys of tile j, then the places of the tile behind it
     auto load_k = [&](int32_t j) __attribute__((always_inline)) {
-        load(map.k, ak, rk4, okk);
+#pragma unroll
+        for (int u = 0; u < NCH; u++) rk4[u] = *(const uint4 *)(kbase + (uint64_t)ak[u] * 16);
 #pragma unroll
         for (int u = 0; u < NCH; u++) av[u] = ak[u];
         offsets(j + 1);
     };
-    auto store_k = [&](int32_t j) __attribute__((always_inline)) {
+    auto zeros = [&](int32_t j, uint4 (&y)[NCH]) __attribute__((always_inline)) {  // keys of no page
 #pragma unroll
-        for (int u = 0; u < NCH; u++)
-            *(uint4 *)(sm.k[j & 1] + (row0 + u * RSTEP) * KS + lc * 8) = only(okk[u], rk4[u]);
+        for (int u = 0; u < NCH; u++) {
+            const int32_t key = min(s0 + j * 64 + row0 + u * RSTEP, s1 - 1);
+            if (place_of(map, key, entry_of(map, key, s1)) == kNoKey) y[u] = zero4();
+        }
+    };
+    auto store_k = [&](int32_t j) __attribute__((always_inline)) {
+        if (missing) zeros(j, rk4);
+#pragma unroll
+        for (int u = 0; u < NCH; u++) *(uint4 *)(sm.k[j & 1] + (row0 + u * RSTEP) * KS + lc * 8) = rk4[u];
     };
     auto store_v = [&](int32_t j) __attribute__((always_inline)) {
         const int32_t t = s0 + j * 64;
-#pragma unroll
-        for (int u = 0; u < NCH; u++) rv4[u] = only(okv[u], rv4[u]);
+        if (missing) zeros(j, rv4);
         if (t < tlo || t + 64 > thi) {  // (a tile that some row does not see all of)
             uint32_t bad = 0;
 #pragma unroll
             for (int u = 0; u < NCH; u++) bad |= take_out<DT>(rv4[u]);
-            if (__any(bad) && lane == 0) sm.bad = 1;
+            if (__any(bad) && lane == 0) flags.bad = 1;
         }
 #pragma unroll
         for (int u = 0; u < NCH; u++) *(uint4 *)(sm.v[j & 1] + (row0 + u * RSTEP) * VS + lc * 8) = rv4[u];
@@ -742,6 +750,7 @@ __device__ __forceinline__ void paged_wide(const PagedArgs &a, const PagedLine &
         // now and written two steps later, three steps before any of them is read.
         if (j > 0 && (j & 7) == 0) look_up(64 * (j + 8), entry);
         if (j > 2 && (j & 7) == 2) fill(64 * (j + 6), entry);
+        if (j > 2 && (j & 7) == 4) missing = uni(flags.missing);
     };
     if (nt > 0) {
         offsets(0);
@@ -764,7 +773,7 @@ __device__ __forceinline__ void paged_wide(const PagedArgs &a, const PagedLine &
     }
     if (first) __syncthreads();
     const bool rows = wave * 32 < x.rows;
-    if (rows && sm.bad)
+    if (rows && flags.bad)
         for (int32_t j0 = s0; j0 < s1; j0 += 64)
             if (j0 < tlo || j0 + 64 > thi) add_back16<DT, D>(map, j0, min(j0 + 64, s1), rk, acc);
     __syncthreads();  // (every wavefront is past its last tile, and has read whether there was a bad one)
@@ -828,6 +837,7 @@ __global__ __launch_bounds__((64 * paged_waves<D>()), (D == 256 ? 1 : 2)) void p
         WideTiles<D> wide;
         NarrowTile<D> tiles[NW];
     } sm;
+    __shared__ WideFlags flags;
     const int wave = uni(threadIdx.x >> 6);
     const PagedLine lines[2] = {wide, narrow};
     PagedShare shares[2];
@@ -860,7 +870,7 @@ __global__ __launch_bounds__((64 * paged_waves<D>()), (D == 256 ? 1 : 2)) void p
             settle_piece(x);
             if (last >= 0 && threadIdx.x == 0)
                 wide.jobs[worker] = PagedJob{x.tok, x.head, x.per, x.rows, worker - 1, last};
-            paged_wide<DT, D>(a, wide, x, pool_of(a, x, k, v), q, sm.wide, sm.tiles);
+            paged_wide<DT, D>(a, wide, x, pool_of(a, x, k, v), q, sm.wide, flags, sm.tiles);
             p = next;
             if (p >= end || !walk_on(a, wide, walk, next)) break;
         }
