@@ -70,29 +70,25 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 // output layout is the operand that O^T += V^T P^T takes. Keys and values go through one LDS tile of f32, DP columns
 // wide (the head width and zeros behind it).
 
-// VEC elements of a row of `n` from element e on, zeros past it.
+// VEC elements from p on.
 template <int DT, int VEC>
-__device__ __forceinline__ float4 load_some(const void *p, int64_t row, int e, int n) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if constexpr (VEC == 4) {
-        if (e < n) {
-            if constexpr (DT == DM_F32) {
-                x = *(const float4 *)((const float *)p + row + e);
-            } else {
-                const uint2 w = *(const uint2 *)((const uint16_t *)p + row + e);
-                x = make_float4(unpack_lo<DT>(w.x), unpack_hi<DT>(w.x), unpack_lo<DT>(w.y), unpack_hi<DT>(w.y));
-            }
-        }
+__device__ __forceinline__ float4 load_some(const char *p) {
+    if constexpr (VEC == 1) {
+        return make_float4(ld<DT>(p, 0), 0.f, 0.f, 0.f);
+    } else if constexpr (DT == DM_F32) {
+        return *(const float4 *)p;
     } else {
-        if (e < n) x.x = ld<DT>(p, row + e);
+        const uint2 w = *(const uint2 *)p;
+        return make_float4(unpack_lo<DT>(w.x), unpack_hi<DT>(w.x), unpack_lo<DT>(w.y), unpack_hi<DT>(w.y));
     }
-    return x;
 }
 
 template <int DT, int DP, int VEC>
 __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, const void *__restrict__ q,
                                                     const void *__restrict__ k, const void *__restrict__ v) {
-    constexpr int TS = DP + 4, CPR = DP / VEC, DTN = DP / 32, HALF = DP / 2;
+    // (at DP = 256 the outputs and queries leave no registers for keys ahead)
+    constexpr int TS = DP + 4, CPR = DP / VEC, NLD = CPR / 2, DTN = DP / 32, HALF = DP / 2, SIZE = DT == DM_F32 ? 4 : 2;
+    constexpr bool AHEAD = DP <= 128;
     __shared__ PlanSmem<256, 1> plan;
     __shared__ __align__(16) float tiles[4][32 * TS];
     const int lane = threadIdx.x & 63, wave = uni(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
@@ -115,14 +111,15 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
         const PagedPiece x = piece_of(a, l, walk, sh, worker, p, end, &next, &last);
         if (last >= 0 && lane == 0) l.jobs[worker] = PagedJob{x.tok, x.head, x.per, x.rows, worker - 1, last};
         const RowKeys rk = row_keys(a, x, 0);
+        // (no load stands under a condition, which would have each waited for by itself: what is not there is read
+        // somewhere else and cleared)
         float qf[HALF];
         {
             const int64_t row = (int64_t)rk.tok * a.qt + rk.head * a.qh;
 #pragma unroll
-            for (int e = 0; e < HALF; e++) {
-                const int c = half * HALF + e;
-                qf[e] = rk.on && c < a.d ? ld<DT>(q, row + c) : 0.f;
-            }
+            for (int e = 0; e < HALF; e++) qf[e] = ld<DT>(q, row + min(half * HALF + e, a.d - 1));
+#pragma unroll
+            for (int e = 0; e < HALF; e++) qf[e] = rk.on && half * HALF + e < a.d ? qf[e] : 0.f;
         }
         f32x16_t acc[DTN];
 #pragma unroll
@@ -130,26 +127,43 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
         float m = -INFINITY, sum = 0.f;
         const int32_t *entries = a.table + x.s * a.max_pages;
         bool bad = false;
+        int64_t ko, vo;  // this lane's key's rows in the pools, -1 for none
+        auto places = [&](int32_t j0) __attribute__((always_inline)) {
+            const int32_t key = min(j0 + col, max(x.s1 - 1, 0));
+            const int64_t e = key / a.page_size, r = key - e * a.page_size, pg = entries[e];
+            const bool is = j0 + col < x.s1 && pg >= 0 && pg < a.num_pages;
+            ko = is ? pg * a.kb + r * a.kt + x.kh * a.kh : -1;
+            vo = is ? pg * a.vb + r * a.vt + x.kh * a.vh : -1;
+        };
+        float4 kreg[NLD], vreg[NLD];
+        auto load = [&](const void *pool, int64_t at, float4 (&y)[NLD]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < NLD; u++) {
+                const int i = u * 64 + lane, r = i / CPR, e = i % CPR * VEC;
+                const int64_t off = __shfl((long long)at, r, 64);
+                const bool is = off >= 0 && e < a.d;
+                y[u] = load_some<DT, VEC>(is ? (const char *)pool + (off + e) * SIZE : (const char *)q);
+                if (!is) y[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        };
+        auto put = [&](const float4 (&y)[NLD]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < NLD; u++) {
+                const int i = u * 64 + lane, r = i / CPR, e = i % CPR * VEC;
+                if constexpr (VEC == 4)
+                    *(float4 *)(tile + r * TS + e) = y[u];
+                else
+                    tile[r * TS + e] = y[u].x;
+            }
+        };
+        if (x.s0 < x.s1) {
+            places(x.s0);
+            load(k, ko, kreg);
+        }
         for (int32_t j0 = x.s0; j0 < x.s1; j0 += 32) {
             const bool cut = j0 < rk.flo || j0 + 32 > rk.fhi;
-            int64_t ko = -1, vo = -1;
-            if (j0 + col < x.s1) {
-                const int64_t e = (j0 + col) / a.page_size, r = j0 + col - e * a.page_size, pg = entries[e];
-                if (pg >= 0 && pg < a.num_pages) {
-                    ko = pg * a.kb + r * a.kt + x.kh * a.kh;
-                    vo = pg * a.vb + r * a.vt + x.kh * a.vh;
-                }
-            }
-#pragma unroll 8
-            for (int u = 0; u < CPR / 2; u++) {
-                const int i = u * 64 + lane, r = i / CPR, e = i % CPR * VEC;
-                const int64_t off = __shfl((long long)ko, r, 64);
-                const float4 y = off >= 0 ? load_some<DT, VEC>(k, off, e, a.d) : make_float4(0.f, 0.f, 0.f, 0.f);
-                if constexpr (VEC == 4)
-                    *(float4 *)(tile + r * TS + e) = y;
-                else
-                    tile[r * TS + e] = y.x;
-            }
+            put(kreg);
+            if constexpr (AHEAD) load(v, vo, vreg);
             __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS accesses complete in order)
             f32x16_t sc = zero16();
 #pragma unroll
@@ -161,21 +175,10 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
                 sc = mfma2(y.w, qf[e + 3], sc);
             }
             __builtin_amdgcn_wave_barrier();
-#pragma unroll 8
-            for (int u = 0; u < CPR / 2; u++) {
-                const int i = u * 64 + lane, r = i / CPR, e = i % CPR * VEC;
-                const int64_t off = __shfl((long long)vo, r, 64);
-                float4 y = off >= 0 ? load_some<DT, VEC>(v, off, e, a.d) : make_float4(0.f, 0.f, 0.f, 0.f);
-                if (cut) {  // (a hidden key's weight is 0, and 0 times what is not finite is NaN)
-                    float *c = (float *)&y;
-#pragma unroll
-                    for (int y = 0; y < VEC; y++)
-                        if (!(fabsf(c[y]) < INFINITY)) c[y] = 0.f, bad = true;
-                }
-                if constexpr (VEC == 4)
-                    *(float4 *)(tile + r * TS + e) = y;
-                else
-                    tile[r * TS + e] = y.x;
+            if constexpr (!AHEAD) load(v, vo, vreg);
+            if (AHEAD && j0 + 32 < x.s1) {
+                places(j0 + 32);
+                load(k, ko, kreg);
             }
             float mx = -INFINITY;
 #pragma unroll
@@ -203,6 +206,16 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
                 ps += sc[i];
             }
             sum += ps;
+            if (cut) {  // (a hidden key's weight is 0, and 0 times what is not finite is NaN)
+#pragma unroll
+                for (int u = 0; u < NLD; u++) {
+                    float *c = (float *)&vreg[u];
+#pragma unroll
+                    for (int y = 0; y < VEC; y++)
+                        if (!(fabsf(c[y]) < INFINITY)) c[y] = 0.f, bad = true;
+                }
+            }
+            put(vreg);
             __builtin_amdgcn_wave_barrier();
             // (a step's products first: with an addition a key to the sum so far, long sums of like terms lose bits)
 #pragma unroll
@@ -213,6 +226,10 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
                 acc[t] += step;
             }
             __builtin_amdgcn_wave_barrier();
+            if (!AHEAD && j0 + 32 < x.s1) {
+                places(j0 + 32);
+                load(k, ko, kreg);
+            }
         }
         if (__any(bad)) {  // what was taken out of V, for the rows that see it
             for (int32_t j = x.s0; j < x.s1; j++) {
@@ -302,10 +319,9 @@ __device__ __forceinline__ PoolMap pool_of(const PagedArgs &a, const PagedPiece 
     m.size = (uint32_t)a.page_size, m.pages = (uint32_t)a.num_pages;
     return m;
 }
-// Key j's entry in the table (-1 behind `end`), and its place from that.
-__device__ __forceinline__ int32_t entry_of(const PoolMap &m, int32_t j, int32_t end) {
-    return j < end ? m.table[(uint32_t)j / m.size] : -1;
-}
+// Key j's entry in the table, and its place from that. (Of keys behind a piece the last one's is read: a load under a
+// condition would be waited for at once.)
+__device__ __forceinline__ int32_t entry_of(const PoolMap &m, int32_t j) { return m.table[(uint32_t)j / m.size]; }
 __device__ __forceinline__ uint32_t place_of(const PoolMap &m, int32_t j, int32_t entry) {
     return (uint32_t)entry < m.pages ? (uint32_t)entry * m.page + ((uint32_t)j % m.size) * m.row : kNoKey;
 }
@@ -365,7 +381,7 @@ template <int DT, int D>
 __device__ __forceinline__ void add_back16(const PoolMap &m, int32_t j0, int32_t j1, const RowKeys &rk, f32x16_t (&acc)[D / 32]) {
     const int lane = threadIdx.x & 63;
     for (int32_t j = j0; j < j1; j++) {
-        const uint32_t at = place_of(m, j, entry_of(m, j, j1));
+        const uint32_t at = place_of(m, j, entry_of(m, j));
         if (at == kNoKey || j < rk.lo || j >= rk.hi) continue;
         const uint16_t *row = (const uint16_t *)(m.v + (uint64_t)at * 16);
 #pragma unroll
@@ -426,21 +442,28 @@ struct NarrowTile {
 static_assert(sizeof(NarrowTile<64>) >= 32 * 68 * 4 && sizeof(NarrowTile<256>) >= 32 * 260 * 4,
               "a tile's results go through its place");
 
-template <int DT, int D>
+// SCORES: the rows' scores are kept, for the weights of the keys.
+template <int DT, int D, bool SCORES>
 __device__ __forceinline__ void paged_narrow(const PagedArgs &a, const PagedLine &l, const PagedPiece &x, const PoolMap &map,
                                              const void *q, NarrowTile<D> &t) {
     constexpr int KS = NarrowTile<D>::KS, VS = NarrowTile<D>::VS, KST = D / 16, DTN = D / 32;
     constexpr int LPR = D / 8, RPL = 64 / LPR, NLD = 32 / RPL;  // lanes a row, rows a load, loads
-    const int lane = threadIdx.x & 63, col = lane & 31;
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
     const int32_t s0 = x.s0, s1 = x.s1;
     const float qscale = fabsf(a.scale) * kLog2e;
     // the entries and places of the 64 keys at hand, a lane each, and the entries of the 64 behind them
-    int32_t ahead = entry_of(map, s0 + lane, s1);
+    const int32_t end = max(s1 - 1, 0);
+    int32_t ahead = entry_of(map, min(s0 + lane, end));
     const RowKeys rk = row_keys(a, x, 0);
     QueryRows<D> qr;
     load_q<D>(a, rk, q, qr);
-    uint32_t at = place_of(map, s0 + lane, ahead);
-    ahead = entry_of(map, s0 + 64 + lane, s1);
+    auto place = [&](int32_t j) __attribute__((always_inline)) { return j < s1 ? place_of(map, j, ahead) : kNoKey; };
+    uint32_t at = place(s0 + lane);
+    ahead = entry_of(map, min(s0 + 64 + lane, end));
+    __amdgpu_buffer_rsrc_t keep;
+    if constexpr (SCORES)
+        keep = make_rsrc(a.scores + (((int64_t)x.s * a.hkv + x.kh) * a.score_rows + x.row0) * a.cap,
+                         (uint32_t)x.rows * (uint32_t)a.cap * 4);
     uint4 sk[NLD], sv[NLD];
     uint32_t have = 0;  // the loads of this lane that are keys'
     auto load = [&](int32_t n) __attribute__((always_inline)) {  // the n-th 32 keys
@@ -490,8 +513,8 @@ __device__ __forceinline__ void paged_narrow(const PagedArgs &a, const PagedLine
                 }
             }
             if (n & 1) {
-                at = place_of(map, j0 + 32 + lane, ahead);
-                ahead = entry_of(map, j0 + 96 + lane, s1);
+                at = place(j0 + 32 + lane);
+                ahead = entry_of(map, min(j0 + 96 + lane, end));
             }
             load(n + 1);  // (past the last: the pool's start, unused)
             f32x16_t sc = zero16();
@@ -503,6 +526,20 @@ __device__ __forceinline__ void paged_narrow(const PagedArgs &a, const PagedLine
                 const int32_t key = j0 + crow(i, lane);
                 sc[i] = !cut || (key >= rk.lo && key < rk.hi) ? sc[i] * qscale : -INFINITY;
                 mx = fmaxf(mx, sc[i]);
+            }
+            if constexpr (SCORES) {
+                // (a lane without a row, and a key behind the piece: past the buffer's end, so not stored)
+                const uint32_t to = rk.on ? (uint32_t)(col * a.cap + j0 + half * 4) * 4 : kNoKey;
+                if (j0 + 32 <= s1) {
+#pragma unroll
+                    for (int g = 0; g < 4; g++)
+                        buf_store16(keep, rk.on ? to + g * 32 : kNoKey, sc[g * 4], sc[g * 4 + 1], sc[g * 4 + 2], sc[g * 4 + 3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        __builtin_amdgcn_raw_buffer_store_b32(
+                            __float_as_uint(sc[i]), keep, rk.on && j0 + crow(i, lane) < s1 ? to + (i / 4 * 8 + i % 4) * 4 : kNoKey, 0, 0);
+                }
             }
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             const bool grow = mx > m + 8.f;
@@ -561,7 +598,7 @@ __device__ __forceinline__ void paged_wide(const PagedArgs &a, const PagedLine &
     // loaded), and the pool's start for a key of no page
     auto look_up = [&](int32_t key, int32_t (&entry)[PK]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < PK; u++) entry[u] = entry_of(map, min(s0 + key + u * NT + (int32_t)threadIdx.x, s1 - 1), s1);
+        for (int u = 0; u < PK; u++) entry[u] = entry_of(map, min(s0 + key + u * NT + (int32_t)threadIdx.x, s1 - 1));
     };
     auto fill = [&](int32_t key, const int32_t (&entry)[PK]) __attribute__((always_inline)) {
 #pragma unroll
@@ -625,7 +662,7 @@ __device__ __forceinline__ void paged_wide(const PagedArgs &a, const PagedLine &
 #pragma unroll
         for (int u = 0; u < NCH; u++) {
             const int32_t key = min(s0 + j * 64 + row0 + u * RSTEP, s1 - 1);
-            if (place_of(map, key, entry_of(map, key, s1)) == kNoKey) y[u] = zero4();
+            if (place_of(map, key, entry_of(map, key)) == kNoKey) y[u] = zero4();
         }
     };
     auto store_k = [&](int32_t j) __attribute__((always_inline)) {
@@ -783,11 +820,11 @@ __device__ __forceinline__ void paged_wide(const PagedArgs &a, const PagedLine &
 // Everything uniform in a wavefront that the loads' scalar bases come from.
 __device__ __forceinline__ void settle_piece(PagedPiece &x) {
     x.tok = uni(x.tok), x.head = uni(x.head), x.rows = uni(x.rows), x.pos = uni(x.pos), x.kh = uni(x.kh), x.s = uni(x.s);
-    x.s0 = uni(x.s0), x.s1 = uni(x.s1), x.slot = uni(x.slot), x.whole = uni(x.whole);
+    x.row0 = uni(x.row0), x.s0 = uni(x.s0), x.s1 = uni(x.s1), x.slot = uni(x.slot), x.whole = uni(x.whole);
 }
 
 // A call whose sequences all have few rows: every wavefront a worker.
-template <int DT, int D>
+template <int DT, int D, bool SCORES>
 __device__ __forceinline__ void narrow_share(const PagedArgs &a, const PagedLine &l, const PagedShare &sh, int32_t worker,
                                              PagedWalk &walk, int64_t p, const void *q, const void *k, const void *v,
                                              NarrowTile<D> &tile) {
@@ -800,12 +837,12 @@ __device__ __forceinline__ void narrow_share(const PagedArgs &a, const PagedLine
         PagedPiece x = piece_of(a, l, walk, sh, worker, p, end, &next, &last);
         settle_piece(x);
         if (last >= 0 && (threadIdx.x & 63) == 0) l.jobs[worker] = PagedJob{x.tok, x.head, x.per, x.rows, worker - 1, last};
-        paged_narrow<DT, D>(a, l, x, pool_of(a, x, k, v), q, tile);
+        paged_narrow<DT, D, SCORES>(a, l, x, pool_of(a, x, k, v), q, tile);
         p = next;
         if (p >= end || !walk_on(a, l, walk, next)) return;
     }
 }
-template <int DT, int D>
+template <int DT, int D, bool SCORES>
 __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void paged_narrow_kernel(PagedArgs a, PagedLine l, const void *__restrict__ q,
                                                                               const void *__restrict__ k,
                                                                               const void *__restrict__ v) {
@@ -821,12 +858,12 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void paged_narrow_kernel(P
     fill_outside<DT>(a, plan_lines(a, lines, sm.plan, sh));
     const int64_t p = sh[0].total > 0 && worker < sh[0].workers ? sh[0].at(worker) : -1;
     plan_find<0>(a, lines, sm.plan, sh[0], p, &walk);
-    narrow_share<DT, D>(a, l, sh[0], worker, walk, p, q, k, v, sm.tiles[wave]);
+    narrow_share<DT, D, SCORES>(a, l, sh[0], worker, walk, p, q, k, v, sm.tiles[wave]);
 }
 
 // Any call: the wide tiles' line, a workgroup a worker, and the narrow tiles', a wavefront a worker. Every other
 // workgroup begins with its narrow share, so that reading and multiplying go on side by side.
-template <int DT, int D>
+template <int DT, int D, bool SCORES>
 __global__ __launch_bounds__((64 * paged_waves<D>()), (D == 256 ? 1 : 2)) void paged_mixed_kernel(PagedArgs a, PagedLine wide, PagedLine narrow,
                                                                                    const void *__restrict__ q,
                                                                                    const void *__restrict__ k,
@@ -849,7 +886,7 @@ __global__ __launch_bounds__((64 * paged_waves<D>()), (D == 256 ? 1 : 2)) void p
             const int32_t worker = blockIdx.x * NW + wave;
             const int64_t p = sh.total > 0 && worker < sh.workers ? sh.at(worker) : -1;
             if (sh.total > 0) plan_find<1>(a, lines, plan, sh, p, &walk);
-            narrow_share<DT, D>(a, narrow, sh, worker, walk, p, q, k, v, sm.tiles[wave]);
+            narrow_share<DT, D, SCORES>(a, narrow, sh, worker, walk, p, q, k, v, sm.tiles[wave]);
             __syncthreads();
             continue;
         }
@@ -1238,6 +1275,34 @@ __global__ __launch_bounds__(256) void paged_weights_join(PagedArgs a, KeyLine l
     weights[job.tok * stride + key] += y;
 }
 
+// Narrow tiles: their sweep has left the scores, 4 bytes a (row, key) where the keys themselves are 2 D a head. A thread
+// a key, the rows of a head first, then the heads.
+__global__ __launch_bounds__(256) void paged_weights_narrow(PagedArgs a, float *__restrict__ weights, int64_t stride,
+                                                            int32_t blocks, int32_t upto) {
+    const int32_t s = blockIdx.x / blocks, key = (blockIdx.x - s * blocks) * 256 + threadIdx.x;
+    const PagedSeq q = paged_seq(a, s);
+    const int32_t rows = q.n * a.rep;
+    if (q.n == 0 || (int64_t)q.n * a.rep > upto || key >= q.len) return;
+    const int32_t p0 = q.len - q.n;
+    float total = 0.f;
+    for (int32_t kh = 0; kh < a.hkv; kh++) {
+        const float *at = a.scores + ((int64_t)s * a.hkv + kh) * a.score_rows * a.cap + key;
+        const float *ls = a.lse + (int64_t)q.first * a.hq + kh * a.rep;
+        float sub = 0.f;
+        int32_t i = 0, h = 0;
+#pragma unroll 8
+        for (int32_t r = 0; r < rows; r++) {
+            const float l = ls[(int64_t)i * a.hq + h];
+            const bool seen = key <= p0 + i && (a.left < 0 || key >= p0 + i - a.left) && l != -INFINITY;
+            const float x = at[(int64_t)r * a.cap];  // (of a key that the row does not see: whatever lies there)
+            sub += seen ? fast_exp2(fmaf(-l, kLog2e, x)) : 0.f;
+            if (++h == a.rep) h = 0, i++;
+        }
+        total += sub;
+    }
+    weights[s * stride + key] += total;
+}
+
 // ------------------------------------------------------------------------------------------
 // Host
 // ------------------------------------------------------------------------------------------
@@ -1273,11 +1338,15 @@ static bool paged_fast_pool(const PagedArgs &a) {
     return a.num_pages > 0 && a.kb < most / a.num_pages / 2 && a.kt < most / a.page_size / 2;
 }
 
+// Most bytes of scores kept (half a percent of the card's memory; calls that could need more go through the keys again).
+constexpr int64_t kScoreBytes = (int64_t)1 << 31;
 struct PagedPlan {
     bool fast, mixed;
     PagedLine wide, narrow;  // the simple kernel's: narrow
     size_t bytes;
     KeyLine keys;            // with weights
+    int64_t score_rows;      // of a sequence's head, with the narrow tiles' scores kept (0: not)
+    size_t scores;
     size_t lse;              // where their own log-sum-exps lie
 };
 static size_t place_line(const dm_attention_desc *d, PagedLine *l, char *base, size_t at) {
@@ -1326,6 +1395,16 @@ static PagedPlan paged_plan(const dm_attention_desc *d, char *base, bool weights
         p.bytes += align_up((size_t)2 * l.workers * l.keys * sizeof(float));
         l.jobs = (PagedJob *)(base + p.bytes);
         p.bytes += align_up((size_t)l.workers * sizeof(PagedJob));
+        // the narrow tiles' scores, where the longest that the call could have fit
+        const int64_t most = std::min<int64_t>(kNarrowRows, (d->cu_seqlens_q ? d->tq : 1) * rep);
+        const int64_t row = d->tk * (int64_t)sizeof(float);
+        if (fast && d->b * d->hkv * most <= kScoreBytes / std::max<int64_t>(row, 1) && d->b * ((d->tk + 255) / 256) < (1 << 23) &&
+            kNarrowRows * row < ((int64_t)1 << 32)) {
+            p.score_rows = most;
+            p.scores = p.bytes;
+            p.bytes += align_up((size_t)(d->b * d->hkv * most * row));
+            l.over = kNarrowRows;
+        }
     }
     return p;
 }
@@ -1404,6 +1483,7 @@ int dm_attention_paged(const dm_attention_desc *d, const void *q, const void *k_
     const PagedPlan p = paged_plan(d, (char *)workspace, weights != nullptr, fast);
     a.o = o;
     a.lse = lse ? lse : (weights ? (float *)((char *)workspace + p.lse) : nullptr);
+    if (p.score_rows) a.scores = (float *)((char *)workspace + p.scores), a.score_rows = (int32_t)p.score_rows;
     // (four elements at a time where rows and bases allow it)
     const int64_t eb = dtype_bytes(d->dtype);
     const bool vec = ((d->d | a.kb | a.kt | a.kh | a.vb | a.vt | a.vh) & 3) == 0 &&
@@ -1416,17 +1496,26 @@ int dm_attention_paged(const dm_attention_desc *d, const void *q, const void *k_
 #define PAGED_W(DT, DP)                                                                                       \
     if (weights && !fast)                                                                                     \
         paged_weights_simple<DT, DP><<<1024, 256, 0, st>>>(a, q, k_pages, weights, weights_stride);           \
-    else if (weights) {                                                                                       \
+    if (p.score_rows)                                                                                         \
+        paged_weights_narrow<<<(unsigned)(d->b * ((d->tk + 255) / 256)), 256, 0, st>>>(                       \
+            a, weights, weights_stride, (int32_t)((d->tk + 255) / 256), kNarrowRows);                         \
+    if (weights && fast && (p.mixed || !p.score_rows)) {                                                      \
         if constexpr (DT != DM_F32)                                                                           \
             paged_weights_kernel<DT, DP><<<p.keys.workers, 512, 0, st>>>(a, p.keys, q, k_pages, weights, weights_stride); \
         paged_weights_join<<<dim3(p.keys.workers, p.keys.keys / 256), 256, 0, st>>>(a, p.keys, weights, weights_stride); \
     }
+#define PAGED_FAST(DT, DP, SC)                                                                                \
+    if (p.mixed)                                                                                              \
+        paged_mixed_kernel<DT, DP, SC><<<256, 64 * paged_waves<DP>(), 0, st>>>(a, p.wide, l, q, k_pages, v_pages); \
+    else if (fast)                                                                                            \
+        paged_narrow_kernel<DT, DP, SC><<<g, 256, 0, st>>>(a, l, q, k_pages, v_pages)
 #define PAGED_V(DT, DP)                                                                                       \
     if constexpr (DT != DM_F32) {                                                                             \
-        if (p.mixed)                                                                                          \
-            paged_mixed_kernel<DT, DP><<<256, 64 * paged_waves<DP>(), 0, st>>>(a, p.wide, l, q, k_pages, v_pages); \
-        else if (fast)                                                                                        \
-            paged_narrow_kernel<DT, DP><<<g, 256, 0, st>>>(a, l, q, k_pages, v_pages);                        \
+        if (p.score_rows) {                                                                                   \
+            PAGED_FAST(DT, DP, true);                                                                         \
+        } else {                                                                                              \
+            PAGED_FAST(DT, DP, false);                                                                        \
+        }                                                                                                     \
     }                                                                                                         \
     if (!fast && vec)                                                                                         \
         paged_simple<DT, DP, 4><<<g, 256, 0, st>>>(a, l, q, k_pages, v_pages);                                \
@@ -1454,6 +1543,7 @@ int dm_attention_paged(const dm_attention_desc *d, const void *q, const void *k_
     }
 #undef PAGED
 #undef PAGED_V
+#undef PAGED_FAST
 #undef PAGED_W
     probe_add(DM_PROBE_ATTN_PAGED);
     if (weights) probe_add(DM_PROBE_ATTN_WEIGHTS);

@@ -203,6 +203,12 @@ __device__ __forceinline__ uint4 buf_load16_nt(__amdgpu_buffer_rsrc_t r, uint32_
     return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
+// 16 bytes to an offset of any multiple of 4; one that reaches past the resource's byte count stores nothing.
+__device__ __forceinline__ void buf_store16(__amdgpu_buffer_rsrc_t r, uint32_t off, float a, float b, float c, float d) {
+    const u32x4_t x = {__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d)};
+    __builtin_amdgcn_raw_buffer_store_b128(x, r, off, 0, 0);
+}
+
 // A product tile's output fragment as the B (or A) operand of a next product whose k is the
 // tile's rows: k step u takes elements 8 u .. 8 u + 7.
 template <int DT>

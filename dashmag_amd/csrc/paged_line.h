@@ -22,7 +22,9 @@ struct PagedArgs {
     int64_t page_size, max_pages, num_pages;
     int64_t qt, qh, kb, kt, kh, vb, vt, vh;  // strides in elements
     void *o;
-    float *lse;  // [N, Hq] or NULL
+    float *lse;     // [N, Hq] or NULL
+    float *scores;  // [S, Hkv, score_rows, cap]: the narrow tiles' scores (log2 units), or NULL
+    int32_t score_rows;
 };
 
 // A shared tile's join: its rows, and the workers that have pieces of it.
@@ -253,6 +255,7 @@ __device__ __forceinline__ void plan_find(const PagedArgs &a, const Line (&l)[L]
 struct PagedPiece {
     int32_t tok, head, per, rows;  // first token and query head; row r: token tok + r / per, head head + r % per
     int32_t pos, kh, s;            // the position of tok; key-value head, sequence
+    int32_t row0;                  // the sequence's row of this head that r = 0 is
     int32_t s0, s1;
     bool whole;
     int32_t slot;                  // not whole: its place
@@ -271,6 +274,7 @@ __device__ __forceinline__ PagedPiece piece_of(const PagedArgs &a, const PagedLi
     x.rows = l.hc > 1 ? min(l.rt, a.rep - c * l.rt) : (i1 - i0) * a.rep;
     x.pos = w.q.len - w.q.n + i0;
     x.s = w.s;
+    x.row0 = i0 * a.rep + c * l.rt;
     const int32_t hi = max(0, w.q.len - w.q.n + i1);
     const int32_t lo = a.left >= 0 ? min(hi, max(0, x.pos - a.left)) : 0;
     auto key = [&](int64_t off) -> int32_t {  // the key at `off` of the tile's part of the line
