@@ -156,14 +156,39 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
                     tile[r * TS + e] = y[u].x;
             }
         };
+        auto take = [&](float4 &y, bool cut) __attribute__((always_inline)) {
+            float *c = (float *)&y;
+#pragma unroll
+            for (int e = 0; e < VEC; e++)  // (a hidden key's weight is 0, and 0 times what is not finite is NaN)
+                if (cut && !(fabsf(c[e]) < INFINITY)) c[e] = 0.f, bad = true;
+        };
+        auto copy = [&](const void *pool, int64_t at, bool cut) __attribute__((always_inline)) {  // by way of few registers
+#pragma unroll 8
+            for (int u = 0; u < NLD; u++) {
+                const int i = u * 64 + lane, r = i / CPR, e = i % CPR * VEC;
+                const int64_t off = __shfl((long long)at, r, 64);
+                const bool is = off >= 0 && e < a.d;
+                float4 y = load_some<DT, VEC>(is ? (const char *)pool + (off + e) * SIZE : (const char *)q);
+                if (!is) y = make_float4(0.f, 0.f, 0.f, 0.f);
+                take(y, cut);
+                if constexpr (VEC == 4)
+                    *(float4 *)(tile + r * TS + e) = y;
+                else
+                    tile[r * TS + e] = y.x;
+            }
+        };
         if (x.s0 < x.s1) {
             places(x.s0);
-            load(k, ko, kreg);
+            if constexpr (AHEAD) load(k, ko, kreg);
         }
         for (int32_t j0 = x.s0; j0 < x.s1; j0 += 32) {
             const bool cut = j0 < rk.flo || j0 + 32 > rk.fhi;
-            put(kreg);
-            if constexpr (AHEAD) load(v, vo, vreg);
+            if constexpr (AHEAD) {
+                put(kreg);
+                load(v, vo, vreg);
+            } else {
+                copy(k, ko, false);
+            }
             __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS accesses complete in order)
             f32x16_t sc = zero16();
 #pragma unroll
@@ -175,7 +200,6 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
                 sc = mfma2(y.w, qf[e + 3], sc);
             }
             __builtin_amdgcn_wave_barrier();
-            if constexpr (!AHEAD) load(v, vo, vreg);
             if (AHEAD && j0 + 32 < x.s1) {
                 places(j0 + 32);
                 load(k, ko, kreg);
@@ -206,16 +230,13 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
                 ps += sc[i];
             }
             sum += ps;
-            if (cut) {  // (a hidden key's weight is 0, and 0 times what is not finite is NaN)
+            if constexpr (AHEAD) {
 #pragma unroll
-                for (int u = 0; u < NLD; u++) {
-                    float *c = (float *)&vreg[u];
-#pragma unroll
-                    for (int y = 0; y < VEC; y++)
-                        if (!(fabsf(c[y]) < INFINITY)) c[y] = 0.f, bad = true;
-                }
+                for (int u = 0; u < NLD; u++) take(vreg[u], cut);
+                put(vreg);
+            } else {
+                copy(v, vo, cut);
             }
-            put(vreg);
             __builtin_amdgcn_wave_barrier();
             // (a step's products first: with an addition a key to the sum so far, long sums of like terms lose bits)
 #pragma unroll
@@ -226,10 +247,7 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
                 acc[t] += step;
             }
             __builtin_amdgcn_wave_barrier();
-            if (!AHEAD && j0 + 32 < x.s1) {
-                places(j0 + 32);
-                load(k, ko, kreg);
-            }
+            if (!AHEAD && j0 + 32 < x.s1) places(j0 + 32);
         }
         if (__any(bad)) {  // what was taken out of V, for the rows that see it
             for (int32_t j = x.s0; j < x.s1; j++) {
@@ -265,14 +283,21 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
             else if (a.lse)
                 a.lse[(int64_t)rk.tok * a.hq + rk.head] = lse_of(m, total);
         }
-        for (int r = 0; r < x.rows; r++) {
-            const int64_t to = (int64_t)__shfl(rk.tok, r, 64) * a.hq + __shfl(rk.head, r, 64);
-            for (int e = lane; e < a.d; e += 64) {
-                const float y = tile[r * TS + e];
+        constexpr int LPR = DP / 4, RPL = 64 / LPR;  // lanes a row, rows at a time
+        const int64_t mine = (int64_t)rk.tok * a.hq + rk.head;
+        for (int r = 0; r < x.rows; r += RPL) {
+            const int y = r + lane / LPR, c = lane % LPR * 4;
+            const int64_t to = __shfl((long long)mine, min(y, 31), 64);
+            const float4 o = *(const float4 *)(tile + min(y, 31) * TS + c);
+            if (y >= x.rows) continue;
+            const float f4[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (c + e >= a.d) continue;
                 if (x.whole)
-                    st<DT>(a.o, to * a.d + e, y);
+                    st<DT>(a.o, to * a.d + c + e, f4[e]);
                 else
-                    l.o[(place + r) * a.d + e] = y;
+                    l.o[(place + y) * a.d + c + e] = f4[e];
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -1001,68 +1026,96 @@ __global__ __launch_bounds__(256) void paged_join(PagedArgs a, PagedLine narrow,
 // The weights that the cached keys get
 // ------------------------------------------------------------------------------------------
 //
-// weights[s, j] += sum over the tokens and heads that see key j of e^(scale q k_j - lse). A wavefront takes 32 keys
-// of a sequence and goes through every head's rows that see any of them, 32 at a time: S = q K^T, whose columns are
-// the keys, so that a key's sum stays in its lane and no other wavefront adds to it.
-template <int DT, int DP>
-__global__ __launch_bounds__(256) void paged_weights_simple(PagedArgs a, const void *__restrict__ q,
+// weights[s, j] += sum over the tokens and heads that see key j of e^(scale q k_j - lse). Keys lie in tiles, and a tile
+// goes through every head's rows that see any of its keys: S = q K^T, whose columns are the keys, so that a key's sum
+// stays in its lane. The tiles lie on a line as the attention's do, and a tile that workers share is summed by a
+// second launch, so that one value is added to a weight, in a fixed order.
+//
+// The simple form: a wavefront is a worker, a tile 32 keys in registers, rows 32 at a time straight from memory.
+
+// Half a row of DP elements (zeros past the row's d) for the f32 products, from `row` on; `is`: there is one.
+template <int DT, int VEC, int HALF>
+__device__ __forceinline__ void load_half(const void *pool, int64_t row, int d, bool is, const void *safe, float (&y)[HALF]) {
+    constexpr int SIZE = DT == DM_F32 ? 4 : 2;
+    const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int u = 0; u < HALF / VEC; u++) {
+        const int c = half * HALF + u * VEC;
+        const bool here = is && c < d;
+        const float4 v = load_some<DT, VEC>(here ? (const char *)pool + (row + c) * SIZE : (const char *)safe);
+        const float f4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < VEC; e++) y[u * VEC + e] = here ? f4[e] : 0.f;
+    }
+}
+
+template <int DT, int DP, int VEC>
+__global__ __launch_bounds__(256) void paged_weights_simple(PagedArgs a, KeyLine l, const void *__restrict__ q,
                                                             const void *__restrict__ k, float *__restrict__ weights,
                                                             int64_t stride) {
     constexpr int HALF = DP / 2;
+    __shared__ PlanSmem<256, 1> plan;
     const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    const int32_t nw = gridDim.x * 4, mine = uni(blockIdx.x * 4 + (threadIdx.x >> 6));
-    const float qscale = a.scale * kLog2e;
-    int32_t base = 0;  // (the 32-key blocks of the sequences in front, modulo nw)
-    for (int32_t s = 0; s < a.S; s++) {
-        const PagedSeq sq = paged_seq(a, s);
-        const int32_t blocks = sq.n > 0 ? (sq.len + 31) / 32 : 0;
-        const int32_t p0 = sq.len - sq.n;
-        for (int32_t b = (mine - base + nw) % nw; b < blocks; b += nw) {
-            const int32_t j0 = b * 32, key = j0 + col;
-            int64_t off = -1;
-            if (key < sq.len) {
-                const int64_t e = key / a.page_size, r = key - e * a.page_size, pg = a.table[s * a.max_pages + e];
-                if (pg >= 0 && pg < a.num_pages) off = pg * a.kb + r * a.kt;
-            }
-            // the tokens that see any of the keys
-            const int32_t t0 = max(0, j0 - p0);
-            const int32_t t1 = a.left >= 0 ? (int32_t)min((int64_t)sq.n, (int64_t)j0 + 32 + a.left - p0) : sq.n;
-            float total = 0.f;
-            for (int32_t kh = 0; kh < a.hkv && t0 < t1; kh++) {
-                float kf[HALF];
+    const int32_t worker = blockIdx.x * 4 + uni(threadIdx.x >> 6);
+    PagedWalk walk;
+    const KeyLine lines[1] = {l};
+    PagedShare shares[1];
+    plan_lines(a, lines, plan, shares);
+    const PagedShare &sh = shares[0];
+    int64_t p = sh.total > 0 && worker < sh.workers ? sh.at(worker) : -1;
+    plan_find<0>(a, lines, plan, sh, p, &walk);
+    if (lane == 0) l.jobs[worker].rows = 0;
+    if (p < 0) return;
+    const int64_t end = sh.at(worker + 1);
+    const float c2 = a.scale * kLog2e;
+    for (;;) {
+        int64_t next;
+        int32_t last;
+        const KeyPiece x = key_piece(a, l, walk, sh, worker, p, end, &next, &last);
+        if (last >= 0 && lane == 0) l.jobs[worker] = PagedJob{x.s, walk.t, 0, 1, worker - 1, last};
+        const int32_t len = walk.q.len, p0 = walk.q.len - walk.q.n, key = x.k0 + col;
+        const int64_t e = min(key, len - 1) / a.page_size, pg = a.table[x.s * a.max_pages + e];
+        const bool is = key < len && pg >= 0 && pg < a.num_pages;
+        const int64_t off = is ? pg * a.kb + (key - e * a.page_size) * a.kt : 0;
+        float total = 0.f;
+        for (int32_t r = x.r0; r < x.r1;) {
+            const int32_t kh = r / x.steps, n = min(x.r1, (kh + 1) * x.steps) - r;  // this head's steps
+            float kf[HALF], qf[HALF], sub = 0.f;
+            load_half<DT, VEC>(k, off + kh * a.kh, a.d, is, q, kf);
+            for (int32_t i = 0; i < n; i++) {
+                const int32_t row = x.from + (r - kh * x.steps + i) * 32 + col;
+                const bool on = row < x.to;
+                const int32_t t = on ? row / a.rep : 0, h = on ? row - t * a.rep : 0;
+                const int64_t tok = walk.q.first + t;
+                load_half<DT, VEC>(q, tok * a.qt + (int64_t)(kh * a.rep + h) * a.qh, a.d, on, q, qf);
+                const float ls = a.lse[tok * a.hq + kh * a.rep + h];
+                const float ref = on && ls != -INFINITY ? -ls * kLog2e : -INFINITY;
+                f32x16_t sc = zero16();
 #pragma unroll
-                for (int e = 0; e < HALF; e++) {
-                    const int c = half * HALF + e;
-                    kf[e] = off >= 0 && c < a.d ? ld<DT>(k, off + kh * a.kh + c) : 0.f;
+                for (int c = 0; c < HALF; c++) sc = mfma2(qf[c], kf[c], sc);
+                float part = 0.f;
+#pragma unroll
+                for (int u = 0; u < 16; u++) {
+                    const int y = crow(u, lane);
+                    const float rf = __shfl(ref, y, 64);
+                    const int32_t pos = p0 + __shfl(t, y, 64);
+                    const bool seen = rf != -INFINITY && key <= pos && (a.left < 0 || key >= pos - a.left);
+                    part += seen ? fast_exp2(fmaf(sc[u], c2, rf)) : 0.f;
                 }
-                const int64_t r1 = (int64_t)t1 * a.rep;
-                for (int64_t r0 = (int64_t)t0 * a.rep; r0 < r1; r0 += 32) {
-                    const int64_t r = r0 + col;
-                    const bool on = r < r1;
-                    const int32_t i = on ? (int32_t)(r / a.rep) : t0, h = on ? (int32_t)(r - (int64_t)i * a.rep) : 0;
-                    const int64_t tok = sq.first + i, row = tok * a.qt + (kh * a.rep + h) * a.qh;
-                    const float ls = on ? a.lse[tok * a.hq + kh * a.rep + h] : -INFINITY;
-                    const float ref = ls * kLog2e;
-                    f32x16_t sc = zero16();
-#pragma unroll
-                    for (int e = 0; e < HALF; e++) {
-                        const int c = half * HALF + e;
-                        sc = mfma2(on && c < a.d ? ld<DT>(q, row + c) : 0.f, kf[e], sc);
-                    }
-#pragma unroll
-                    for (int u = 0; u < 16; u++) {
-                        const int x = crow(u, lane);
-                        const float rf = __shfl(ref, x, 64);
-                        const int32_t pos = p0 + __shfl(i, x, 64);
-                        const bool seen = rf != -INFINITY && key <= pos && (a.left < 0 || key >= pos - a.left);
-                        total += seen ? fast_exp2(sc[u] * qscale - rf) : 0.f;
-                    }
-                }
+                sub += part;
             }
-            total += __shfl_xor(total, 32, 64);
-            if (half == 0 && key < sq.len && t0 < t1) weights[s * stride + key] += total;
+            total += sub;
+            r += n;
         }
-        base = (int32_t)(((int64_t)base + blocks) % nw);
+        total += __shfl_xor(total, 32, 64);
+        if (half == 0) {
+            if (!x.whole)
+                l.sums[(int64_t)x.slot * l.keys + col] = total;
+            else if (key < len && x.r1 > 0)
+                weights[x.s * stride + key] += total;
+        }
+        p = next;
+        if (p >= end || !walk_on(a, l, walk, next)) return;
     }
 }
 
@@ -1375,22 +1428,20 @@ static PagedPlan paged_plan(const dm_attention_desc *d, char *base, bool weights
     p.narrow = line_of(d, 32, 0, p.mixed ? kNarrowRows : INT32_MAX);
     p.narrow.workers = d->d > 128 ? 1024 : 2048;
     p.narrow.unit = 32;
-#ifndef NST
-#define NST 64
-#define NLE 96
-#endif
-    p.narrow.start = NST;
-    p.narrow.least = NLE;
+    // (a worker has 32 keys at least: four tokens against 500 to 1000 keys 29 us with 128, 24.5 so. The simple kernel
+    // takes longer for 32 keys than for a tile's start: 210 tokens of 4 heads of 64 in f32 39 us with the same, 35.5 so)
+    p.narrow.start = fast ? 64 : 32;
+    p.narrow.least = fast ? 96 : 32;
     p.bytes = place_line(d, &p.narrow, base, p.bytes);
     p.lse = p.bytes;
     if (weights) {
         p.bytes += align_up((size_t)(d->tq * d->hq) * sizeof(float));
         KeyLine &l = p.keys;
-        l.keys = d->d == 256 ? key_tile<256>() : key_tile<128>();
-        l.workers = 256;
-        l.unit = 64;
-        l.start = 256;
-        l.least = 1024;
+        l.keys = !fast ? 32 : (d->d == 256 ? key_tile<256>() : key_tile<128>());
+        l.workers = fast ? 256 : 4096;
+        l.unit = fast ? 64 : 32;
+        l.start = fast ? 256 : 64;
+        l.least = fast ? 1024 : 128;
         l.sums = (float *)(base + p.bytes);
         p.bytes += align_up((size_t)2 * l.workers * l.keys * sizeof(float));
         l.jobs = (PagedJob *)(base + p.bytes);
@@ -1488,21 +1539,26 @@ int dm_attention_paged(const dm_attention_desc *d, const void *q, const void *k_
     const int64_t eb = dtype_bytes(d->dtype);
     const bool vec = ((d->d | a.kb | a.kt | a.kh | a.vb | a.vt | a.vh) & 3) == 0 &&
                      (((uintptr_t)k_pages | (uintptr_t)v_pages) & (4 * eb - 1)) == 0;
+    const bool vecq = vec && ((a.qt | a.qh) & 3) == 0 && ((uintptr_t)q & (4 * eb - 1)) == 0;
     const PagedLine &l = p.narrow;
     const unsigned g = l.workers / 4;
     const int slots = 256 / (int)(d->d % 4 == 0 && aligned_16b(o) ? d->d / 4 : d->d);  // rows of a joining workgroup
     const int nb = l.workers * ((l.pitch + slots - 1) / slots);
     const int wb = p.mixed ? p.wide.workers * ((p.wide.pitch + slots - 1) / slots) : 0;
 #define PAGED_W(DT, DP)                                                                                       \
-    if (weights && !fast)                                                                                     \
-        paged_weights_simple<DT, DP><<<1024, 256, 0, st>>>(a, q, k_pages, weights, weights_stride);           \
+    if (weights && !fast && vecq)                                                                             \
+        paged_weights_simple<DT, DP, 4><<<p.keys.workers / 4, 256, 0, st>>>(a, p.keys, q, k_pages, weights, weights_stride); \
+    else if (weights && !fast)                                                                                \
+        paged_weights_simple<DT, DP, 1><<<p.keys.workers / 4, 256, 0, st>>>(a, p.keys, q, k_pages, weights, weights_stride); \
     if (p.score_rows)                                                                                         \
         paged_weights_narrow<<<(unsigned)(d->b * ((d->tk + 255) / 256)), 256, 0, st>>>(                       \
             a, weights, weights_stride, (int32_t)((d->tk + 255) / 256), kNarrowRows);                         \
-    if (weights && fast && (p.mixed || !p.score_rows)) {                                                      \
-        if constexpr (DT != DM_F32)                                                                           \
-            paged_weights_kernel<DT, DP><<<p.keys.workers, 512, 0, st>>>(a, p.keys, q, k_pages, weights, weights_stride); \
-        paged_weights_join<<<dim3(p.keys.workers, p.keys.keys / 256), 256, 0, st>>>(a, p.keys, weights, weights_stride); \
+    if (weights && (!fast || p.mixed || !p.score_rows)) {                                                     \
+        if constexpr (DT != DM_F32) {                                                                         \
+            if (fast)                                                                                         \
+                paged_weights_kernel<DT, DP><<<p.keys.workers, 512, 0, st>>>(a, p.keys, q, k_pages, weights, weights_stride); \
+        }                                                                                                     \
+        paged_weights_join<<<dim3(p.keys.workers, (p.keys.keys + 255) / 256), 256, 0, st>>>(a, p.keys, weights, weights_stride); \
     }
 #define PAGED_FAST(DT, DP, SC)                                                                                \
     if (p.mixed)                                                                                              \
