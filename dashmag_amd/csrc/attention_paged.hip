@@ -1159,6 +1159,7 @@ __global__ __launch_bounds__(512, 2) void paged_weights_kernel(PagedArgs a, KeyL
     const int64_t end = sh.at(worker + 1);
     const float c2 = a.scale * kLog2e;
     const int32_t rep = a.rep, more = 64 / rep, rest = 64 - more * rep;  // 64 rows on: tokens and heads
+    const int32_t left = a.left >= 0 ? a.left : 1 << 30;  // (without a window more than a row holds)
     for (;;) {
         int64_t next;
         int32_t last;
@@ -1253,29 +1254,35 @@ __global__ __launch_bounds__(512, 2) void paged_weights_kernel(PagedArgs a, KeyL
                 const int tiles = first + i * 64 + 32 < to ? 2 : 1;
                 const uint16_t *tq = sm.rows.q[b] + col * KS + half * 8;
                 for (int y = 0; y < tiles; y++) {
+                    // (each fragment is read ahead of the products in front of it)
+                    constexpr int READ = 3;
+                    Frag8 f[READ + 1];
+                    auto read = [&](int st) __attribute__((always_inline)) {
+                        f[st % (READ + 1)].u = *(const uint4 *)(tq + y * 32 * KS + st * 16);
+                    };
                     f32x16_t sc[COLS];
 #pragma unroll
                     for (int c = 0; c < COLS; c++) sc[c] = zero16();
 #pragma unroll
+                    for (int st = 0; st < READ; st++) read(st);
+#pragma unroll
                     for (int st = 0; st < KST; st++) {
-                        Frag8 f;
-                        f.u = *(const uint4 *)(tq + y * 32 * KS + st * 16);
+                        if (st + READ < KST) read(st + READ);
 #pragma unroll
-                        for (int c = 0; c < COLS; c++) sc[c] = mfma32<DT>(f, kf[c][st], sc[c]);
+                        for (int c = 0; c < COLS; c++) sc[c] = mfma32<DT>(f[st % (READ + 1)], kf[c][st], sc[c]);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    float part[COLS];
+                    float rf[16];
 #pragma unroll
-                    for (int c = 0; c < COLS; c++) part[c] = 0.f;
+                    for (int g = 0; g < 4; g++)
+                        *(float4 *)(rf + g * 4) = *(const float4 *)(sm.rows.ref[b] + y * 32 + g * 8 + half * 4);
 #pragma unroll
-                    for (int g = 0; g < 4; g++) {
-                        const float4 rf = *(const float4 *)(sm.rows.ref[b] + y * 32 + g * 8 + half * 4);
-                        const float f4[4] = {rf.x, rf.y, rf.z, rf.w};
-                        if (full) {
+                    for (int e = 0; e < 16; e++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
+                        for (int c = 0; c < COLS; c++) sc[c][e] = fmaf(sc[c][e], c2, rf[e]);
+                    if (!full) {
 #pragma unroll
-                                for (int c = 0; c < COLS; c++) part[c] += fast_exp2(fmaf(sc[c][g * 4 + e], c2, f4[e]));
-                        } else {
+                        for (int g = 0; g < 4; g++) {
                             const int4 ps = *(const int4 *)(sm.rows.pos[b] + y * 32 + g * 8 + half * 4);
                             const int32_t p4[4] = {ps.x, ps.y, ps.z, ps.w};
 #pragma unroll
@@ -1283,13 +1290,18 @@ __global__ __launch_bounds__(512, 2) void paged_weights_kernel(PagedArgs a, KeyL
 #pragma unroll
                                 for (int c = 0; c < COLS; c++) {
                                     const int32_t key = w0 + c * 32 + col;
-                                    const bool seen = key <= p4[e] && (a.left < 0 || key >= p4[e] - a.left) && f4[e] != -INFINITY;
-                                    part[c] += seen ? fast_exp2(fmaf(sc[c][g * 4 + e], c2, f4[e])) : 0.f;
+                                    const bool seen = (key <= p4[e]) & (key >= p4[e] - left) & (rf[g * 4 + e] != -INFINITY);
+                                    sc[c][g * 4 + e] = seen ? sc[c][g * 4 + e] : -INFINITY;
                                 }
                         }
                     }
 #pragma unroll
-                    for (int c = 0; c < COLS; c++) sub[c] += part[c];
+                    for (int c = 0; c < COLS; c++) {
+                        float part = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 16; e++) part += fast_exp2(sc[c][e]);
+                        sub[c] += part;
+                    }
                 }
                 ts += more, hs += rest;
                 if (hs >= rep) ts++, hs -= rep;
