@@ -1024,8 +1024,8 @@ def cache_evict(pools, weights, block_table, lengths, refcounts, budgets, recent
     first) until it holds its budget. So it ends with its budget of keys, or those that it has to keep where they are
     more. The keys that stay stay in order, so that later tokens and windows see them as before; they move
     down within the row's pages in every tensor of ``pools``, their weights with them (the weights behind become
-    0), and the pages behind them are given up, as in :func:`cache_free`. ``block_table``, ``lengths`` and
-    ``refcounts`` change in place, as in :func:`cache_reserve`.
+    0), and the pages behind them are given up, as in :func:`cache_free`. No two of the pools may overlap.
+    ``block_table``, ``lengths`` and ``refcounts`` change in place, as in :func:`cache_reserve`.
 
     Returns ``kept [R, max_pages * page_size]`` int32: where in its row the key now at ``j`` was, -1 from the
     row's length on. Keys that were rotated by their positions keep those: give :func:`qk_norm_rope_paged` the

@@ -456,7 +456,8 @@ int dm_cache_compact(const dm_cache_table *table, const dm_cache_pool *pools, in
  * 0 .. n - 1 in every pool, their weights with them, and the weights of n .. L - 1 become 0; the pages
  * behind ceil(n / page_size) are given up as by dm_cache_free. kept [rows, max_pages * page_size]: where each key
  * of a row, now at j, was before (j itself in a row that gives up none), -1 from its length on. A key on a page
- * outside the pools is not moved. Refused: rows that could hold 2^35 keys together. */
+ * outside the pools is not moved. Refused: rows that could hold 2^35 keys together, pools that overlap (one given
+ * twice). */
 size_t dm_cache_evict_workspace(const dm_cache_table *table);
 int dm_cache_evict(const dm_cache_table *table, const dm_cache_pool *pools, int64_t npools, float *weights,
                    int64_t weights_stride, const int32_t *budgets, int64_t recent, int32_t *kept,

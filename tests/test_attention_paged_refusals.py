@@ -102,7 +102,10 @@ def _evict(ws=1 << 40, pools=(), w=256, stride=64, b=256, kept=256, recent=0, **
     (dict(max_pages=(1 << 26) + 1), "at most 2^30"), (dict(rows=1 << 22, max_pages=1 << 13, page_size=1), "less than 2^35"),
     (dict(rows=1 << 22, pools=[_lib.CachePool(256, 32, 32)]), "more rows and bytes"),
     (dict(rows=1 << 20, pools=[_lib.CachePool(256, 1 << 16, 1 << 16)]), "more rows and bytes"),
-    (dict(pools=[_lib.CachePool(256, 24, 24)]), "a pool's pages"), (dict(pools=[_lib.CachePool(None, 32, 32)]), "missing")])
+    (dict(pools=[_lib.CachePool(256, 24, 24)]), "a pool's pages"), (dict(pools=[_lib.CachePool(256, 32, 32)] * 2), "two of them"),
+    (dict(pools=[_lib.CachePool(256, 64, 128), _lib.CachePool(4096, 64, 128), _lib.CachePool(304, 32, 128)]), "two of them"),
+    (dict(pools=[_lib.CachePool(256, 64, 128), _lib.CachePool(368, 32, 128)]), "two of them"),
+    (dict(pools=[_lib.CachePool(256, 32, 64), _lib.CachePool(320, 16, 128)]), "two of them"), (dict(pools=[_lib.CachePool(None, 32, 32)]), "missing")])
 def test_the_eviction_refuses(kw, what):
     rc, msg = _evict(**kw)
     assert rc == _lib.DM_ERR_REFUSED and msg.startswith("cache_evict: ") and what in msg

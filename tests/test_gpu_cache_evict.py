@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import dashmag_amd as dm
+from dashmag_amd import ops
 from evict_oracle import Evicting
 
 pytestmark = pytest.mark.gpu
@@ -142,6 +143,39 @@ def test_strided_weights_and_a_stream():
     with torch.cuda.stream(side):
         b.evict([40, 50], 6)
     assert (wide[:, :4] == -1).all() and (wide[:, 116:] == -1).all()
+
+
+def test_pools_past_32_bits():
+    """Pages 3 GB apart: the places of the third on lie past 2^32 bytes."""
+    b = Both([50, 40], 16, 6, ((2, 8),) * 2, seed=3, spare=0)
+    n, each = len(b.cache.counts), 16 * 2 * 8
+    buf = torch.empty((n - 1) * (3 << 29) + 2 * each, dtype=torch.int16, device="cuda")
+    for i, p in enumerate(b.pools):
+        b.pools[i] = buf.as_strided(p.shape, (3 << 29, 16, 8, 1), i * each).copy_(p)
+    b.evict([20, 33], 4)
+
+
+def test_what_the_workspace_holds(monkeypatch):
+    """Nothing of a call's workspace is read before the call has written it."""
+    for fill in (0, 255):
+        monkeypatch.setattr(ops, "_workspace", lambda n, dev: torch.full((max(int(n), 1),), fill, dtype=torch.uint8, device=dev))
+        Both([9000, 40, 4097, 700], 16, 570, ((2, 8),), seed=fill, shared=2).evict([1000, 20, 4096, 700], 9)
+
+
+def test_two_streams_at_once():
+    """Calls of two caches in flight together."""
+    two = [Both([6000, 900], 16, 380, ((8, 16),), seed=s) for s in (1, 2)]
+    streams = [torch.cuda.Stream() for _ in two]
+    budgets = [_i32([2000, 300]), _i32([100, 899])]
+    kept = []
+    torch.cuda.synchronize()
+    for s, b, n in zip(streams, two, budgets):
+        with torch.cuda.stream(s):
+            kept.append(dm.cache_evict(b.pools, b.weights, b.table, b.lengths, b.counts, n, 64))
+    torch.cuda.synchronize()
+    for b, n, k in zip(two, budgets, kept):
+        assert k.tolist() == b.cache.evict(n.tolist(), 64)
+        b.same()
 
 
 def test_graph():
