@@ -162,3 +162,21 @@ def test_the_same_sequence_twice():
         held("weights", (x + b.weights[0].cuda())[None], *want["weights"])
     same = dm.attention_paged(q, k, k, table, ln, cu)
     assert torch.equal(same, dm.attention_paged(q, k, k.clone(), table, ln, cu))
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (BF, 256), (F16, 64), (F32, 64), (BF, 40)])
+def test_the_weights_of_a_query_of_nan(dtype, d):
+    """NaN in a token's query reaches the weights of the keys that it sees and no other's."""
+    for seqs, tok, left in (([(80, 200), (1, 100)], 17, None), ([(5, 200), (1, 100)], 2, None), ([(5, 200), (70, 100)], 3, 40),
+                            ([(90, 200), (2, 100)], 60, 30), ([(1, 90), (1, 64)], 0, 20)):
+        b = Chunks(dtype, d, 2, 2, 16, seqs, seed=9, window=left)
+        q, *rest = b.cuda()
+        q[tok, 1] = float("nan")
+        w = b.weights.cuda()
+        _weigh(b, q, *rest, w)
+        pos = seqs[0][1] - seqs[0][0] + tok
+        seen = torch.zeros(b.weights.shape, dtype=torch.bool)
+        seen[0, 0 if left is None else max(0, pos - left):pos + 1] = True
+        assert torch.equal(torch.isnan(w).cpu(), seen)
+        want, bound = b.want()["weights"]
+        held("others", w[~seen.cuda()], want[~seen], bound[~seen])
