@@ -975,7 +975,7 @@ int dm_cache_evict(const dm_cache_table *t, const dm_cache_pool *pools, int64_t 
         int shift = 9;
         auto columns = [&](int n) { return (most + (grain << n) - 1) / (grain << n); };
         while (shift > 0 && (t->rows * pa.n * columns(shift) < kEvictGroups || (most <= grain << (shift - 1)))) shift--;
-        const int64_t items = t->rows * pa.n * columns(shift);
+        const int64_t items = t->num_pages > 0 ? t->rows * pa.n * columns(shift) : 0;  // (no page: nothing to load from)
         const int64_t finish = i == 0 ? t->rows : 0;
         if (finish + items == 0) continue;
 #define EVICT_MOVE(T)                                                                                             \

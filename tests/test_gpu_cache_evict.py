@@ -1,11 +1,13 @@
 """Eviction on the GPU against evict_oracle.py, to the bit: tables, lengths, counts, weights, the kept keys and
 every byte of the pools."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import dashmag_amd as dm
-from dashmag_amd import ops
+from dashmag_amd import _lib, ops
 from evict_oracle import Evicting
 
 pytestmark = pytest.mark.gpu
@@ -115,6 +117,23 @@ def test_pages_outside_are_passed_over():
         b.cache.table[r][c] = x
         b.table[r, c] = x
     b.evict([50, 30], 4)
+
+
+def test_a_pool_without_pages():
+    """Rows whose pages are all outside: nothing is read or moved, the rows get shorter all the same."""
+    table, lengths = _i32([[0, 3, -1, 1]]), _i32([60])
+    weights, kept = torch.arange(64.0, device="cuda")[None], torch.empty(1, 64, dtype=torch.int32, device="cuda")
+    counts, budget, ws = _i32([0]), _i32([20]), torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    t = _lib.CacheTable(rows=1, max_pages=4, num_pages=0, page_size=16, block_table=table.data_ptr(),
+                        lengths=lengths.data_ptr(), refcounts=counts.data_ptr())
+    pool = (_lib.CachePool * 1)(_lib.CachePool(None, 512, 512))
+    assert _lib.lib().dm_cache_evict_workspace(ctypes.byref(t)) <= ws.numel()
+    rc = _lib.lib().dm_cache_evict(ctypes.byref(t), pool, 1, weights.data_ptr(), 64, budget.data_ptr(), 5, kept.data_ptr(),
+                                   ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+    assert rc == _lib.DM_OK
+    torch.cuda.synchronize()
+    assert lengths.tolist() == [20] and kept[0, :21].tolist() == [*range(40, 60), -1]
+    assert weights[0, :21].tolist() == [float(x) for x in range(40, 60)] + [0.0] and table.tolist() == [[0, 3, -1, -1]]
 
 
 def test_lengths_past_the_table_and_below_zero():
