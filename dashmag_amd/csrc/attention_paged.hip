@@ -324,7 +324,15 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
 // ahead in registers; wide: 8 tiles ahead in an LDS ring), so any page size costs the same. A key of no
 // page, or behind the piece, is loaded from the pool's start and zeroed on its way into LDS.
 
-constexpr int kNarrowRows = 64;
+// Sequences of up to 48 rows lie in narrow tiles (32 sequences of 4096 keys, 32 heads of 128: 64 rows each 230 us so and
+// 163 in wide ones, whose keys are read once). Less would cost batches of a few drafts each both lines' starts: 32
+// sequences of 16 to 48 rows, 6000 keys, 49 us with 48 and 60 with 32 (48 rows each: 58 and 46).
+constexpr int kNarrowRows = 48;
+// Sequences whose narrow sweep leaves its scores for the keys' weights: a row's take 4 bytes a key to write and to read,
+// where the keys' second pass reads 2 D a head. With 32 heads of 128 and 4096 keys, kept and not, 64 sequences of
+// 4 rows a head 201 and 257 us; 32 of 8 rows 194 and 195, of 12 211 and 205, of 16 228 and 207, of 32 296 and 212.
+constexpr int kScoreRows = 8;
+static_assert(kScoreRows <= 16, "a larger sequence's first tile has more rows");
 template <int D>
 constexpr int paged_waves() { return D == 256 ? 4 : 8; }
 constexpr uint32_t kNoKey = 0xffffffffu;
@@ -486,6 +494,7 @@ __device__ __forceinline__ void paged_narrow(const PagedArgs &a, const PagedLine
     uint32_t at = place(s0 + lane);
     ahead = entry_of(map, min(s0 + 64 + lane, end));
     __amdgpu_buffer_rsrc_t keep;
+    const bool keeps = SCORES && uni(x.row0 == 0 && x.rows <= kScoreRows);
     if constexpr (SCORES)
         keep = make_rsrc(a.scores + (((int64_t)x.s * a.hkv + x.kh) * a.score_rows + x.row0) * a.cap,
                          (uint32_t)x.rows * (uint32_t)a.cap * 4);
@@ -552,7 +561,7 @@ __device__ __forceinline__ void paged_narrow(const PagedArgs &a, const PagedLine
                 sc[i] = !cut || (key >= rk.lo && key < rk.hi) ? sc[i] * qscale : -INFINITY;
                 mx = fmaxf(mx, sc[i]);
             }
-            if constexpr (SCORES) {
+            if (keeps) {
                 // (a lane without a row, and a key behind the piece: past the buffer's end, so not stored)
                 const uint32_t to = rk.on ? (uint32_t)(col * a.cap + j0 + half * 4) * 4 : kNoKey;
                 if (j0 + 32 <= s1) {
@@ -1433,8 +1442,11 @@ static PagedPlan paged_plan(const dm_attention_desc *d, char *base, bool weights
         p.wide = line_of(d, d->d == 256 ? 128 : 256, kNarrowRows, INT32_MAX);
         p.wide.workers = 256;
         p.wide.unit = 64;
+        // (a tile's start as long as 192 keys: three prompts of 300 tokens against 600 keys 61 us, with 64 69, with 384 63;
+        // the same prompts with 128, 256, 512 and 1024 keys a worker at least 59, 58, 61 and 75, two of 12 tokens of heads
+        // of 256 against 8000 keys 56, 46, 46 and more)
         p.wide.start = 192;
-        p.wide.least = 512;
+        p.wide.least = 256;
         p.bytes = place_line(d, &p.wide, base, p.bytes);
     }
     p.narrow = line_of(d, 32, 0, p.mixed ? kNarrowRows : INT32_MAX);
@@ -1452,21 +1464,23 @@ static PagedPlan paged_plan(const dm_attention_desc *d, char *base, bool weights
         l.keys = !fast ? 32 : (d->d == 256 ? key_tile<256>() : key_tile<128>());
         l.workers = fast ? 256 : 4096;
         l.unit = fast ? 64 : 32;
+        // (rows; three prompts of 300 tokens against 600 keys, with their weights, 127 us with 1024 rows a worker at least,
+        // 111 with 512, 105 with 256; 64 of 16 tokens of 8 heads against 1024 keys 79, 70, 68; a start of 64 136 and 97)
         l.start = fast ? 256 : 64;
-        l.least = fast ? 1024 : 128;
+        l.least = fast ? 256 : 128;
         l.sums = (float *)(base + p.bytes);
         p.bytes += align_up((size_t)2 * l.workers * l.keys * sizeof(float));
         l.jobs = (PagedJob *)(base + p.bytes);
         p.bytes += align_up((size_t)l.workers * sizeof(PagedJob));
         // the narrow tiles' scores, where the longest that the call could have fit
-        const int64_t most = std::min<int64_t>(kNarrowRows, (d->cu_seqlens_q ? d->tq : 1) * rep);
+        const int64_t most = std::min<int64_t>(kScoreRows, (d->cu_seqlens_q ? d->tq : 1) * rep);
         const int64_t row = d->tk * (int64_t)sizeof(float);
         if (fast && d->b * d->hkv * most <= kScoreBytes / std::max<int64_t>(row, 1) && d->b * ((d->tk + 255) / 256) < (1 << 23) &&
-            kNarrowRows * row < ((int64_t)1 << 32)) {
+            kScoreRows * row < ((int64_t)1 << 32)) {
             p.score_rows = most;
             p.scores = p.bytes;
             p.bytes += align_up((size_t)(d->b * d->hkv * most * row));
-            l.over = kNarrowRows;
+            l.over = kScoreRows;
         }
     }
     return p;
@@ -1564,8 +1578,8 @@ int dm_attention_paged(const dm_attention_desc *d, const void *q, const void *k_
         paged_weights_simple<DT, DP, 1><<<p.keys.workers / 4, 256, 0, st>>>(a, p.keys, q, k_pages, weights, weights_stride); \
     if (p.score_rows)                                                                                         \
         paged_weights_narrow<<<(unsigned)(d->b * ((d->tk + 255) / 256)), 256, 0, st>>>(                       \
-            a, weights, weights_stride, (int32_t)((d->tk + 255) / 256), kNarrowRows);                         \
-    if (weights && (!fast || p.mixed || !p.score_rows)) {                                                     \
+            a, weights, weights_stride, (int32_t)((d->tk + 255) / 256), kScoreRows);                         \
+    if (weights && (!p.score_rows || (d->cu_seqlens_q ? d->tq : 1) * a.rep > kScoreRows)) {                                                     \
         if constexpr (DT != DM_F32) {                                                                         \
             if (fast)                                                                                         \
                 paged_weights_kernel<DT, DP><<<p.keys.workers, 512, 0, st>>>(a, p.keys, q, k_pages, weights, weights_stride); \
