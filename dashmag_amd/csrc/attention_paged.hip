@@ -4,6 +4,11 @@
 // max(0, p - W) .. p: o = softmax(scale q K^T) V and lse = log sum e^(scale q k). The rows of a tile (tokens x
 // query heads of one key-value head) sweep their keys once with a running maximum and sum; paged_line.h says how
 // the tiles are shared out and cut.
+//
+// Chunks are bound by the products: 2048 tokens of 32 heads of 128 over 8 against 32768 keys take 1058-1118 us (960-1010
+// TFLOP/s), 24 of them the join; prompts of about 1400 tokens are at 640, since each piece of a tile costs 10 us to begin and
+// end. Single tokens are bound by memory: 64 of up to 8192 keys 282 us, 5.6 TB/s. Four short ones take 22-25 us, of which
+// the plan is 4, the way to the first keys 5, 2.5 a block of 32 keys and the join's launch 5.
 #include <algorithm>
 #include <string>
 
@@ -68,7 +73,8 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 //
 // A wavefront takes 32 rows and 32 keys at a time, both products on the f32 matrix cores: S^T = K q^T, whose
 // output layout is the operand that O^T += V^T P^T takes. Keys and values go through one LDS tile of f32, DP columns
-// wide (the head width and zeros behind it).
+// wide (the head width and zeros behind it). 210 tokens of 4 heads of 64 in f32 against 300 keys each: 27 us and 5 of
+// join, bound by latency.
 
 // VEC elements from p on.
 template <int DT, int VEC>
@@ -1130,7 +1136,9 @@ __global__ __launch_bounds__(256) void paged_weights_simple(PagedArgs a, KeyLine
 
 // The 16-bit kernel: a workgroup takes a tile of keys, 64 of them a wavefront (32 at D = 256) in registers as the second
 // operand, and sweeps the rows that see them, 64 at a time through LDS, head by head. A key's sum over a step's 32
-// rows is taken first, then over a head's, then over the heads (one at a time, a long sum would lose bits).
+// rows is taken first, then over a head's, then over the heads (one at a time, a long sum would lose bits). 1024 tokens
+// of 32 heads of 128 against 16384 keys take 250-280 us (490-530 TFLOP/s): the products and the exponentials follow one
+// another in a wavefront, and two wavefronts a SIMD are all that the keys' registers leave.
 template <int D>
 constexpr int key_cols() { return D == 256 ? 1 : 2; }  // 32-key columns of a wavefront
 template <int D>
