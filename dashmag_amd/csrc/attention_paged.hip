@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
         int64_t next;
         int32_t last;
         const PagedPiece x = piece_of(a, l, walk, sh, worker, p, end, &next, &last);
-        if (last >= 0 && lane == 0) l.jobs[worker] = PagedJob{x.tok, x.head, x.per, x.rows, worker - 1, last};
+        if (last >= 0 && lane == 0) l.jobs[worker] = PagedJob{x.tok, x.head, x.per, x.rows, x.first, last};
         const RowKeys rk = row_keys(a, x, 0);
         // (no load stands under a condition, which would have each waited for by itself: what is not there is read
         // somewhere else and cleared)
@@ -876,7 +876,7 @@ __device__ __forceinline__ void narrow_share(const PagedArgs &a, const PagedLine
         int32_t last;
         PagedPiece x = piece_of(a, l, walk, sh, worker, p, end, &next, &last);
         settle_piece(x);
-        if (last >= 0 && (threadIdx.x & 63) == 0) l.jobs[worker] = PagedJob{x.tok, x.head, x.per, x.rows, worker - 1, last};
+        if (last >= 0 && (threadIdx.x & 63) == 0) l.jobs[worker] = PagedJob{x.tok, x.head, x.per, x.rows, x.first, last};
         paged_narrow<DT, D, SCORES>(a, l, x, pool_of(a, x, k, v), q, tile);
         p = next;
         if (p >= end || !walk_on(a, l, walk, next)) return;
@@ -946,7 +946,7 @@ __global__ __launch_bounds__((64 * paged_waves<D>()), (D == 256 ? 1 : 2)) void p
             PagedPiece x = piece_of(a, wide, walk, sh, worker, p, end, &next, &last);
             settle_piece(x);
             if (last >= 0 && threadIdx.x == 0)
-                wide.jobs[worker] = PagedJob{x.tok, x.head, x.per, x.rows, worker - 1, last};
+                wide.jobs[worker] = PagedJob{x.tok, x.head, x.per, x.rows, x.first, last};
             paged_wide<DT, D>(a, wide, x, pool_of(a, x, k, v), q, sm.wide, flags, sm.tiles);
             p = next;
             if (p >= end || !walk_on(a, wide, walk, next)) break;
@@ -956,9 +956,9 @@ __global__ __launch_bounds__((64 * paged_waves<D>()), (D == 256 ? 1 : 2)) void p
 }
 
 // The pieces of shared tiles joined: D / V threads a row, V columns each, the workgroup's other threads take other rows,
-// or share out the pieces of one where they are more than kJoinMany (each every so-many-th of them, added in order). A
+// or where a row's pieces are more than kJoinMany share those out (each every so-many-th of them, added in order). A
 // thread needs nothing but its own loads: its reference moves as in the sweep.
-constexpr int kJoinMany = 48, kJoinFew = 4;  // and the pieces that a thread has in flight
+constexpr int kJoinFew = 4;  // the pieces that a thread has in flight
 template <int V>
 struct Joined {
     float m, sum, acc[V];
@@ -980,61 +980,60 @@ __global__ __launch_bounds__(256) void paged_join(PagedArgs a, PagedLine narrow,
     // (narrow tiles' workgroups first: y of them a job)
     const bool w = (int32_t)blockIdx.x >= nblocks;
     const PagedLine &l = w ? wide : narrow;
-    const int32_t y = (l.pitch + slots - 1) / slots, i = blockIdx.x - (w ? nblocks : 0), jb = i / y, r0 = (i - jb * y) * slots;
+    const int32_t y = (l.pitch + slots - 1) / slots, i = blockIdx.x - (w ? nblocks : 0), jb = i / y;
     const PagedJob job = l.jobs[jb];
-    if (r0 >= job.rows) return;
+    if (job.rows == 0) return;  // (of a worker without a job the rest is not written)
     const int32_t n = job.last - job.first + 1;
     const bool few = n <= kJoinMany;
-    const int32_t rows = min(slots, job.rows - r0);
-    for (int32_t x = 0; x < (few ? 1 : rows); x++) {
-        const int32_t r = r0 + (few ? slot : x), step = few ? 1 : slots;
-        const bool on = slot < slots && r < job.rows;
-        Joined<V> j{-INFINITY, 0.f, {}};
-        for (int32_t p0 = few ? 0 : slot; on && p0 < n; p0 += kJoinFew * step) {
-            float2 ml[kJoinFew];
-            float o[kJoinFew][V];
+    // (many: kJoinMany jobs or more of y workgroups each are more than a tile has rows, narrow or wide)
+    const int32_t r0 = few ? (i - jb * y) * slots : i - jb * y + (jb - job.first - 1) * y, r = few ? r0 + slot : r0;
+    if (r0 >= job.rows) return;
+    const int32_t step = few ? 1 : slots;
+    const bool on = slot < slots && r < job.rows;
+    Joined<V> j{-INFINITY, 0.f, {}};
+    for (int32_t p0 = few ? 0 : slot; on && p0 < n; p0 += kJoinFew * step) {
+        float2 ml[kJoinFew];
+        float o[kJoinFew][V];
 #pragma unroll
-            for (int u = 0; u < kJoinFew; u++) {
-                const int32_t p = min(p0 + u * step, n - 1);  // (past the last: read again, left out)
-                const int64_t at = (int64_t)(2 * (job.first + p) + (p == 0 ? 1 : 0)) * l.pitch + r;
-                ml[u] = l.ml[at];
-                if constexpr (V == 4)
-                    *(float4 *)o[u] = *(const float4 *)(l.o + at * a.d + c);
-                else
-                    o[u][0] = l.o[at * a.d + c];
-            }
+        for (int u = 0; u < kJoinFew; u++) {
+            const int32_t p = min(p0 + u * step, n - 1);  // (past the last: read again, left out)
+            const int64_t at = (int64_t)(2 * (job.first + p) + (p == 0 ? 1 : 0)) * l.pitch + r;
+            ml[u] = l.ml[at];
+            if constexpr (V == 4)
+                *(float4 *)o[u] = *(const float4 *)(l.o + at * a.d + c);
+            else
+                o[u][0] = l.o[at * a.d + c];
+        }
 #pragma unroll
-            for (int u = 0; u < kJoinFew; u++)
-                if (p0 + u * step < n) join_one<V>(j, ml[u].x, ml[u].y, o[u]);
-        }
-        if (!few) {
-            __syncthreads();
-            float *mine = red + tid * (V + 2);
-            mine[0] = j.m, mine[1] = j.sum;
-#pragma unroll
-            for (int u = 0; u < V; u++) mine[2 + u] = j.acc[u];
-            __syncthreads();
-            if (slot != 0) continue;
-            for (int k = 1; k < min(slots, n); k++) {
-                const float *other = red + (tid + k * per) * (V + 2);
-                join_one<V>(j, other[0], other[1], other + 2);
-            }
-        }
-        if (!on) continue;
-        const float inv = j.sum == 0.f ? 0.f : 1.f / j.sum;  // (NaN is not 0)
-        const int32_t t = r / job.per;
-        const int64_t row = (int64_t)(job.tok + t) * a.hq + job.head + (r - t * job.per);
-        if constexpr (V == 4 && DT != DM_F32) {
-            *(uint2 *)((uint16_t *)a.o + row * a.d + c) =
-                make_uint2(pack2<DT>(j.acc[0] * inv, j.acc[1] * inv), pack2<DT>(j.acc[2] * inv, j.acc[3] * inv));
-        } else if constexpr (V == 4) {
-            *(float4 *)((float *)a.o + row * a.d + c) =
-                make_float4(j.acc[0] * inv, j.acc[1] * inv, j.acc[2] * inv, j.acc[3] * inv);
-        } else {
-            st<DT>(a.o, row * a.d + c, j.acc[0] * inv);
-        }
-        if (c == 0 && a.lse) a.lse[row] = lse_of(j.m, j.sum);
+        for (int u = 0; u < kJoinFew; u++)
+            if (p0 + u * step < n) join_one<V>(j, ml[u].x, ml[u].y, o[u]);
     }
+    if (!few) {
+        float *mine = red + tid * (V + 2);
+        mine[0] = j.m, mine[1] = j.sum;
+#pragma unroll
+        for (int u = 0; u < V; u++) mine[2 + u] = j.acc[u];
+        __syncthreads();
+        if (slot != 0) return;
+        for (int k = 1; k < min(slots, n); k++) {
+            const float *other = red + (tid + k * per) * (V + 2);
+            join_one<V>(j, other[0], other[1], other + 2);
+        }
+    }
+    if (!on) return;
+    const float inv = j.sum == 0.f ? 0.f : 1.f / j.sum;  // (NaN is not 0)
+    const int32_t t = r / job.per;
+    const int64_t row = (int64_t)(job.tok + t) * a.hq + job.head + (r - t * job.per);
+    if constexpr (V == 4 && DT != DM_F32) {
+        *(uint2 *)((uint16_t *)a.o + row * a.d + c) =
+            make_uint2(pack2<DT>(j.acc[0] * inv, j.acc[1] * inv), pack2<DT>(j.acc[2] * inv, j.acc[3] * inv));
+    } else if constexpr (V == 4) {
+        *(float4 *)((float *)a.o + row * a.d + c) =
+            make_float4(j.acc[0] * inv, j.acc[1] * inv, j.acc[2] * inv, j.acc[3] * inv);
+    } else {
+        st<DT>(a.o, row * a.d + c, j.acc[0] * inv);
+    }
+    if (c == 0 && a.lse) a.lse[row] = lse_of(j.m, j.sum);
 }
 
 // ------------------------------------------------------------------------------------------

@@ -180,3 +180,12 @@ def test_the_weights_of_a_query_of_nan(dtype, d):
         assert torch.equal(torch.isnan(w).cpu(), seen)
         want, bound = b.want()["weights"]
         held("others", w[~seen.cuda()], want[~seen], bound[~seen])
+
+
+@pytest.mark.parametrize("dtype,d,rep,seqs,window", [
+    (BF, 128, 4, [(1, 20000)], None), (BF, 128, 4, [(8, 16000), (1, 50)], None), (F16, 64, 8, [(5, 30000)], 25000),
+    (BF, 256, 2, [(3, 9000)], None), (F32, 64, 4, [(6, 9000)], None), (BF, 36, 3, [(2, 9000)], None),
+    (BF, 128, 1, [(49, 31000)], None), (BF, 128, 40, [(2, 26000)], None), (BF, 33, 1, [(30, 5000)], None)])
+def test_tiles_of_many_pieces(dtype, d, rep, seqs, window):
+    """One sequence's keys over all workers: the pieces of its rows are joined by many."""
+    _held_all(Chunks(dtype, d, 1, rep, 16, seqs, seed=rep, window=window))
