@@ -6,7 +6,7 @@
 // the tiles are shared out and cut.
 //
 // Chunks are bound by the products: 2048 tokens of 32 heads of 128 over 8 against 32768 keys take 1058-1118 us (960-1010
-// TFLOP/s), 24 of them the join; prompts of about 1400 tokens are at 640, since each piece of a tile costs 10 us to begin and
+// TFLOP/s), 24 of them the join; prompts of about 1400 tokens are at 620-700, since each piece of a tile costs 10 us to begin and
 // end. Single tokens are bound by memory: 64 of up to 8192 keys 282 us, 5.6 TB/s. Four short ones take 22-25 us, of which
 // the plan is 4, the way to the first keys 5, 2.5 a block of 32 keys and the join's launch 5.
 #include <algorithm>
