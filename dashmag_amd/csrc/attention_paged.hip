@@ -1265,9 +1265,11 @@ __global__ __launch_bounds__(512, 2) void paged_weights_kernel(PagedArgs a, KeyL
             for (int32_t i = 0; i < n; i++) {
                 const int b = i & 1;
                 if (i + 1 < n) load(i + 1);
-                // all of the step's rows see all of the wavefront's keys (those of the last token may be fewer)
-                const bool full = p0 + ts >= w0 + 32 * COLS - 1 && (a.left < 0 || p0 + ts + more + 1 - a.left <= w0);
                 const int tiles = first + i * 64 + 32 < to ? 2 : 1;
+                // all of the step's rows see all of the wavefront's keys (those of the last token may be fewer), and none is
+                // absent: its zeros times an infinite key are NaN, which a reference of -inf does not take out
+                const bool full = p0 + ts >= w0 + 32 * COLS - 1 && (a.left < 0 || p0 + ts + more + 1 - a.left <= w0) &&
+                                  first + i * 64 + tiles * 32 <= to;
                 const uint16_t *tq = sm.rows.q[b] + col * KS + half * 8;
                 for (int y = 0; y < tiles; y++) {
                     // (each fragment is read ahead of the products in front of it)

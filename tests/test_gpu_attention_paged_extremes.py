@@ -1,0 +1,57 @@
+"""The attention of new tokens over a paged cache and its keys' weights where values, lengths and batches are
+extreme, against 64 bits (chunk_cases.py, which derives the bounds)."""
+import pytest
+import torch
+
+import dashmag_amd as dm
+from chunk_cases import Chunks, held_lse
+from rope_cases import held
+from shared_cases import U
+
+pytestmark = pytest.mark.gpu
+
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _without(b, gone):
+    """b.want() of one sequence without a window, whose key `gone` has a score of -inf in every row."""
+    (n, x), d = b.seqs[0], b.d
+    k, v = (y.double().transpose(0, 1) for y in b.keys[0])
+    k = k.clone()
+    k[:, gone] = 0.0
+    q = b.q.double().unflatten(1, (k.shape[0], b.rep)).permute(1, 2, 0, 3)  # [Hkv, rep, n, D]
+    seen = (torch.arange(x) <= torch.arange(x - n, x)[:, None]) & (torch.arange(x) != gone)
+    z = (q @ k.transpose(1, 2)[:, None] * d ** -0.5).masked_fill(~seen, -torch.inf)
+    total = torch.logsumexp(z, -1, keepdim=True)
+    p = torch.exp(z - total)
+    s = ((q.abs() @ k.abs().transpose(1, 2)[:, None]) * d ** -0.5).masked_fill(~seen, 0.0).amax(-1, keepdim=True)
+    e = (d + 16) * U * s
+    half = 0.0 if b.q.dtype == F32 else torch.finfo(b.q.dtype).eps / 2
+    bound = (half + 2 * e + 2 * (x / 16 + 64) * U) * (p @ v[:, None].abs())
+    if b.q.dtype == F16:
+        bound = bound + 2.0 ** -25 * seen.double() @ v[:, None].abs()
+    g = e + (x / 16 + 64) * U + 8 * U * (total.abs() + 1)
+    back = lambda y: y.permute(2, 0, 1, 3).flatten(1, 2)  # noqa: E731
+    w, woff = b.weights.double(), torch.zeros(b.weights.shape, dtype=torch.float64)
+    w[0, :x] += p.sum((0, 1, 2))
+    woff[0, :x] = (p * (e + g + (p.shape[0] * p.shape[1] * n + 40) * U)).sum((0, 1, 2))
+    return (back(p @ v[:, None]), back(bound)), (back(total)[..., 0], back(g)[..., 0]), (w, woff + U * w)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F16, 64), (BF, 256), (F32, 64), (BF, 40)])
+@pytest.mark.parametrize("rep,n", [(1, 5), (4, 3), (3, 15), (1, 33), (4, 24), (4, 25)])
+def test_a_key_of_infinity_that_no_token_gives_weight(dtype, d, rep, n):
+    """An infinite element of a key makes its scores -inf in every row: a weight of 0, whether or not the rows fill
+    the steps that the keys are swept in."""
+    x, gone = 300, 70
+    b = Chunks(dtype, d, 2, rep, 16, [(n, x)], seed=d + n)
+    b.q[..., 0] = b.q[..., 0].abs() + 0.5
+    q, k, v, table, ln, cu = b.cuda()
+    k[int(table[0, gone // 16]), gone % 16, :, 0] = -torch.inf
+    w = b.weights.cuda()
+    out, lse = dm.attention_paged_with_weights(q, k, v, table, ln, w, cu)
+    want, want_lse, want_w = _without(b, gone)
+    assert w[0, gone] == b.weights[0, gone]
+    held("out", out, *want)
+    held_lse("lse", lse, *want_lse)
+    held("weights", w, *want_w)
