@@ -330,10 +330,17 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
 // ahead in registers; wide: 8 tiles ahead in an LDS ring), so any page size costs the same. A key of no
 // page, or behind the piece, is loaded from the pool's start and zeroed on its way into LDS.
 
-// Sequences of up to 48 rows lie in narrow tiles (32 sequences of 4096 keys, 32 heads of 128: 64 rows each 230 us so and
-// 163 in wide ones, whose keys are read once). Less would cost batches of a few drafts each both lines' starts: 32
-// sequences of 16 to 48 rows, 6000 keys, 49 us with 48 and 60 with 32 (48 rows each: 58 and 46).
-constexpr int kNarrowRows = 48;
+// Sequences whose rows one narrow tile holds lie in narrow tiles, larger ones in wide tiles, whose keys are read once for all
+// of their rows. 32 sequences of 36 to 48 rows each, 4096 keys, in wide and in two narrow tiles: widths of 64 (2 key
+// heads) 45 and 58 us, 128 (8) 165 and 230, 128 (2) 62 and 95, 256 (2) 78 and 123; 8 of them of 4000 keys 35 and 39,
+// 62 and 95, 46 and 55, 50 and 59. Batches of both sizes (8 to 64 sequences of 8 to 52 rows) pay both lines' starts,
+// -20% to +35%: with 48 here the geometric mean of 56 of them is the same, with 64 3% less, and the equal ones' 9 and 17% more.
+constexpr int kNarrowRows = 32;
+// Calls that have no more rows a key head altogether get no wide line, only narrow tiles (two at most of a sequence): without a
+// line to plan and its workgroups a call of 33 to 64 rows takes 22-32 us where both lines take 28-40 (1 to 16
+// sequences of 1000 to 8000 keys, 2 key heads of 64 or 128); one sequence of 30000 keys 46 and 41. At 256, whose narrow
+// line has half as many workers: 39-45 and 40-44, of 30000 keys 65 and 48.
+static int64_t lone_rows(int64_t d) { return d == 256 ? kNarrowRows : 2 * kNarrowRows; }
 // Sequences whose narrow sweep leaves its scores for the keys' weights: a row's take 4 bytes a key to write and to read,
 // where the keys' second pass reads 2 D a head. With 32 heads of 128 and 4096 keys, kept and not, 64 sequences of
 // 4 rows a head 201 and 257 us; 32 of 8 rows 194 and 195, of 12 211 and 205, of 16 228 and 207, of 32 296 and 212.
@@ -1446,14 +1453,14 @@ static PagedPlan paged_plan(const dm_attention_desc *d, char *base, bool weights
     const int64_t rep = d->hq / d->hkv;
     p.fast = fast;
     // (whether a sequence has more rows than a narrow one's is known only on the device, but for calls that cannot)
-    p.mixed = fast && (d->cu_seqlens_q ? d->tq : 1) * rep > kNarrowRows;
+    p.mixed = fast && (d->cu_seqlens_q ? d->tq : 1) * rep > lone_rows(d->d);
     if (p.mixed) {
         p.wide = line_of(d, d->d == 256 ? 128 : 256, kNarrowRows, INT32_MAX);
         p.wide.workers = 256;
         p.wide.unit = 64;
-        // (a tile's start as long as 192 keys: three prompts of 300 tokens against 600 keys 61 us, with 64 69, with 384 63;
-        // the same prompts with 128, 256, 512 and 1024 keys a worker at least 59, 58, 61 and 75, two of 12 tokens of heads
-        // of 256 against 8000 keys 56, 46, 46 and more)
+        // (a tile's start as long as 192 keys: 48 calls of 1 to 16 sequences, 4 to 1200 rows a key head each, widths of 64
+        // to 256, in the mean 44.0 us, with 64 45.2, with 384 44.9; with 128, 256, 512 and 1024 keys a worker at least 43.3,
+        // 44.0, 46.9 and 55.2: 128 is ahead for one or two sequences, 3-20%, 256 for eight of 20 tokens, 4-12%)
         p.wide.start = 192;
         p.wide.least = 256;
         p.bytes = place_line(d, &p.wide, base, p.bytes);

@@ -55,3 +55,39 @@ def test_a_key_of_infinity_that_no_token_gives_weight(dtype, d, rep, n):
     held("out", out, *want)
     held_lse("lse", lse, *want_lse)
     held("weights", w, *want_w)
+
+
+def _held_all(b, scale=None):
+    q, k, v, table, ln, cu = b.cuda()
+    w = b.weights.cuda()
+    opts = dm.AttentionOptions(window=None if b.window is None else dm.Window(b.window, 0), scale=scale)
+    out, lse = dm.attention_paged_with_weights(q, k, v, table, ln, w, cu, opts)
+    want = b.want(scale)
+    held("out", out, *want["out"])
+    held_lse("lse", lse, *want["lse"])
+    held("weights", w, *want["weights"])
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F16, 64), (BF, 256), (F32, 64)])
+def test_rows_around_the_tiles_borders(dtype, d):
+    """Sequences of a row more and less than one narrow tile, two of them, and what leaves its scores; keys around a
+    narrow worker's least."""
+    for rep, news in ((1, (7, 8, 9, 31, 32, 33, 47, 48, 49, 63, 64, 65)), (4, (1, 2, 3, 7, 8, 9, 11, 12, 13, 15, 16, 17))):
+        for window in (None, 70):
+            print(f"rep={rep} window={window}", flush=True)
+            _held_all(Chunks(dtype, d, 1, rep, 16, [(n, x) for n in news for x in (n, n + 64, n + 130)], seed=rep, window=window))
+    _held_all(Chunks(dtype, d, 1, 4, 16, [(8, x) for x in (8, 31, 32, 33, 63, 64, 65, 95, 96, 97, 511, 513)], seed=3))
+    _held_all(Chunks(dtype, d, 1, 4, 16, [(9, x) for x in (9, 63, 64, 65, 191, 192, 193, 255, 256, 257)], seed=4))
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F16, 64), (BF, 256), (BF, 64)])
+def test_calls_of_few_rows(dtype, d):
+    """Calls of 31 to 65 rows a key head altogether: a sequence's, several sequences', tokens', in and out of a wide line."""
+    for rep, rows in ((1, (31, 32, 33, 47, 48, 49, 63, 64, 65)), (4, (32, 36, 48, 52, 64, 68)), (40, (40, 80)), (33, (33, 66))):
+        for n in (r // rep for r in rows):
+            print(f"rep={rep} tokens={n}", flush=True)
+            _held_all(Chunks(dtype, d, 2, rep, 16, [(n, n + 700)], seed=n))
+            _held_all(Chunks(dtype, d, 2, rep, 7, [(1, 40 * i) for i in range(n)], seed=n, window=300))
+            _held_all(Chunks(dtype, d, 2, rep, 16, [(1, 90 + i) for i in range(n)], seed=n, single=True))
+            if n > 3:
+                _held_all(Chunks(dtype, d, 2, rep, 16, [(2, 900), (0, 5), (n - 3, 400)], seed=n, gaps=(0, 1)))
