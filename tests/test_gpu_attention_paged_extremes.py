@@ -1,9 +1,12 @@
 """The attention of new tokens over a paged cache and its keys' weights where values, lengths and batches are
 extreme, against 64 bits (chunk_cases.py, which derives the bounds)."""
+import ctypes
+
 import pytest
 import torch
 
 import dashmag_amd as dm
+from dashmag_amd import _lib
 from chunk_cases import Chunks, held_lse
 from rope_cases import held
 from shared_cases import U
@@ -91,3 +94,34 @@ def test_calls_of_few_rows(dtype, d):
             _held_all(Chunks(dtype, d, 2, rep, 16, [(1, 90 + i) for i in range(n)], seed=n, single=True))
             if n > 3:
                 _held_all(Chunks(dtype, d, 2, rep, 16, [(2, 900), (0, 5), (n - 3, 400)], seed=n, gaps=(0, 1)))
+
+
+def _weighing_workspace(b, cols):
+    """Bytes of the call's workspace."""
+    d = _lib.AttentionDesc(b=len(b.seqs), tq=len(b.q), tk=cols * b.page, hq=b.q.shape[1], hkv=b.k.shape[2], d=b.d,
+                           dtype=_lib.DM_BF16 if b.q.dtype == BF else _lib.DM_F16, cu_seqlens_q=256)
+    return _lib.lib().dm_attention_paged_workspace(ctypes.byref(d), b.page, 1)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F16, 64), (BF, 256)])
+@pytest.mark.parametrize("window", [None, 50])
+def test_weights_of_few_rows_without_kept_scores(dtype, d, window):
+    """Batches of prompts, drafts and tokens on a table so wide that no scores are kept: those of few rows too get their
+    weights by another pass over the keys; the same on a narrow table, whose scores are kept."""
+    seqs = [(90, 400), (1, 700), (2, 130), (17, 130), (3, 9), (0, 12), (8, 2100)]
+    b = Chunks(dtype, d, 2, 4, 16, seqs, seed=d + 1, window=window)
+    q, k, v, table, ln, cu = b.cuda()
+    opts = dm.AttentionOptions(window=None if window is None else dm.Window(window, 0))
+    want = b.want()
+    scores = len(seqs) * 2 * 8 * table.shape[1] * 16 * 4  # (of 8 rows a sequence and key head: kept on the narrow table alone)
+    assert _weighing_workspace(b, table.shape[1]) - _weighing_workspace(b, 1 << 19) >= scores
+    for cols in (1 << 19, table.shape[1]):
+        wide = torch.full((len(seqs), cols), -1, dtype=torch.int32, device="cuda")
+        wide[:, :table.shape[1]] = table
+        w = torch.full((len(seqs), cols * 16), 0.25, device="cuda")
+        w[:, :b.weights.shape[1]] = b.weights.cuda()
+        out, lse = dm.attention_paged_with_weights(q, k, v, wide, ln, w, cu, opts)
+        held("out", out, *want["out"])
+        held_lse("lse", lse, *want["lse"])
+        held("weights", w[:, :b.weights.shape[1]], *want["weights"])
+        assert (w[:, b.weights.shape[1]:] == 0.25).all()
