@@ -914,6 +914,21 @@ static EvictWork evict_work(const dm_cache_table *t, char *at, size_t *bytes) {
 // Workgroups that a launch of the moves has at least, where the rows are wide enough: 16 rows cut to half 174, 131 and 135 us
 // with 128, 256 and 512, a document to an eighth 84, 93 and 116 (before its places were shared out).
 constexpr int64_t kEvictGroups = 256;
+// How the pools from `at` on that one launch takes are cut: into columns of grain << shift bytes of a key.
+struct EvictColumns {
+    int64_t n, most, grain;  // pools, bytes of their widest key, bytes that all of their keys are whole numbers of
+    int64_t of(int shift) const { return (most + (grain << shift) - 1) / (grain << shift); }
+};
+static EvictColumns evict_columns(const dm_cache_table *t, const dm_cache_pool *pools, int64_t npools, int64_t at) {
+    EvictColumns c{std::min<int64_t>(kPoolsPerLaunch, npools - at), 0, 16};
+    for (int64_t i = at; i < at + c.n; i++) {
+        const int64_t row = pools[i].page_bytes / t->page_size;
+        const uint64_t bits = (uint64_t)pools[i].pages | (uint64_t)pools[i].page_stride | (uint64_t)row;
+        while (bits % c.grain) c.grain /= 2;
+        c.most = std::max(c.most, row);
+    }
+    return c;
+}
 static bool evict_sizes(const dm_cache_table *t) {
     return table_sizes(t) && t->rows <= kMostRows && t->max_pages <= ((int64_t)1 << 30) / t->page_size &&
            t->rows * t->max_pages * t->page_size < kI31 * 16;
@@ -947,10 +962,12 @@ int dm_cache_evict(const dm_cache_table *t, const dm_cache_pool *pools, int64_t 
     if (t->rows == 0 || cap == 0) return DM_OK;
     if (!weights || !budgets || !kept) return refuse(op + ": the weights, the budgets or the results' place are missing");
     for (int64_t i = 0; i < npools; i += kPoolsPerLaunch) {  // (workgroups of a launch: a row each, and columns of 512 bytes or more)
+        const EvictColumns c = evict_columns(t, pools, npools, i);
         int64_t groups = t->rows;
-        for (int64_t x = i; x < std::min(npools, i + kPoolsPerLaunch); x++)
-            groups += t->rows * (pools[x].page_bytes / t->page_size / 512 + 1);
-        if (groups >= ((int64_t)1 << 23)) return refuse(op + ": more rows and bytes than one launch takes");
+        for (int64_t x = i; x < i + c.n; x++) groups += t->rows * (pools[x].page_bytes / t->page_size / 512 + 1);
+        // (each pool has as many columns as the launch's widest one)
+        if (std::max(groups, t->rows + t->rows * c.n * c.of(9)) >= ((int64_t)1 << 23))
+            return refuse(op + ": more rows and bytes than one launch takes");
     }
     hipStream_t st = (hipStream_t)stream;
     size_t bytes;
@@ -968,24 +985,19 @@ int dm_cache_evict(const dm_cache_table *t, const dm_cache_pool *pools, int64_t 
     }
     for (int64_t i = 0; i == 0 || i < npools; i += kPoolsPerLaunch) {
         bool wide;
-        int64_t pieces, most = 0, grain = 16;
+        int64_t pieces;
         const PoolArgs pa = pools_of(pools, npools, i, &wide, &pieces);
-        for (int x = 0; x < pa.n; x++) {
-            const int64_t row = pa.at[x].bytes / t->page_size;
-            const uint64_t bits = (uint64_t)pa.at[x].pages | (uint64_t)pa.at[x].stride | (uint64_t)row;
-            while (bits % grain) grain /= 2;
-            most = std::max(most, row);
-        }
+        const EvictColumns c = evict_columns(t, pools, npools, i);
+        const int64_t grain = c.grain;
         // the widest columns that make kEvictGroups workgroups
         int shift = 9;
-        auto columns = [&](int n) { return (most + (grain << n) - 1) / (grain << n); };
-        while (shift > 0 && (t->rows * pa.n * columns(shift) < kEvictGroups || (most <= grain << (shift - 1)))) shift--;
-        const int64_t items = t->num_pages > 0 ? t->rows * pa.n * columns(shift) : 0;  // (no page: nothing to load from)
+        while (shift > 0 && (t->rows * pa.n * c.of(shift) < kEvictGroups || (c.most <= grain << (shift - 1)))) shift--;
+        const int64_t items = t->num_pages > 0 ? t->rows * pa.n * c.of(shift) : 0;  // (no page: nothing to load from)
         const int64_t finish = i == 0 ? t->rows : 0;
         if (finish + items == 0) continue;
 #define EVICT_MOVE(T)                                                                                             \
     cache_evict_move<T><<<(unsigned)(finish + items), kEvictThreads, 0, st>>>(ca, w, weights, weights_stride,     \
-                                                                              (int32_t)finish, pa, (int32_t)columns(shift), shift)
+                                                                              (int32_t)finish, pa, (int32_t)c.of(shift), shift)
         if (grain == 16)
             EVICT_MOVE(u32x4_vec);
         else if (grain == 8)
