@@ -973,15 +973,16 @@ int dm_cache_evict(const dm_cache_table *t, const dm_cache_pool *pools, int64_t 
     size_t bytes;
     const EvictWork w = evict_work(t, (char *)workspace, &bytes);
     const CacheArgs ca = cache_args(t);
-    cache_evict_select<<<(unsigned)t->rows, kPlan, 0, st>>>(ca, weights, weights_stride, budgets, recent, w);
     const unsigned shares = (unsigned)std::min<int64_t>(kEvictShares, (cap + 4 * kPlan - 1) / (4 * kPlan));
-    for (int64_t r = 0; r < t->rows; r += 65535) {  // (rows of a launch)
+    for (int64_t r = 0; r < t->rows; r += 65535) {  // (rows of a launch: 2^22 of them together would be 2^32 threads)
+        const unsigned n = (unsigned)std::min<int64_t>(65535, t->rows - r);
         EvictWork part = w;
         part.rows += r, part.from += r * cap, part.to += r * cap, part.weight += r * cap;
         CacheArgs pa = ca;
-        pa.table += r * t->max_pages;
-        cache_evict_place<<<dim3(shares, (unsigned)std::min<int64_t>(65535, t->rows - r)), kPlan, 0, st>>>(
-            pa, weights + r * weights_stride, weights_stride, kept + r * cap, part);
+        pa.table += r * t->max_pages, pa.lengths += r;
+        float *at = weights + r * weights_stride;
+        cache_evict_select<<<n, kPlan, 0, st>>>(pa, at, weights_stride, budgets + r, recent, part);
+        cache_evict_place<<<dim3(shares, n), kPlan, 0, st>>>(pa, at, weights_stride, kept + r * cap, part);
     }
     for (int64_t i = 0; i == 0 || i < npools; i += kPoolsPerLaunch) {
         bool wide;
