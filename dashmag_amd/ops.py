@@ -775,6 +775,7 @@ def attention_paged_with_weights(query, key_pages, value_pages, block_table, len
     [S, max_pages * page_size]`` f32 in place: to key ``j`` of sequence ``s`` the sum of its softmax weights
     over the tokens and query heads that see it, in a fixed order. What :func:`cache_evict` goes by; the layers
     of a model, whose pools share a table, add to one such array."""
+    _weights_given("attention_paged_with_weights", weights)
     return _attention_paged("attention_paged_with_weights", query, key_pages, value_pages, block_table, lengths, weights,
                             cu_seqlens, options, True)
 
@@ -838,6 +839,11 @@ def _paged_arrays(op, block_table, lengths, cu_seqlens, n, device):
         if min(at) < 0 or max(at) > n or any(x > y for x, y in zip(at, at[1:])):
             raise Unsupported(f"{op}: cu_seqlens must go from 0 or more to at most N = {n} without decreasing, got {at}")
     return bt, ln, cu
+
+
+def _weights_given(op, weights):
+    if weights is None:
+        raise Unsupported(f"{op}: the weights are missing")
 
 
 def _paged_weights(op, weights, rows, cap):
@@ -1031,6 +1037,7 @@ def cache_evict(pools, weights, block_table, lengths, refcounts, budgets, recent
     row's length on. Keys that were rotated by their positions keep those: give :func:`qk_norm_rope_paged` the
     ``positions`` of what follows."""
     op = "cache_evict"
+    _weights_given(op, weights)
     _one_device(op, block_table, weights)
     dev = block_table.device
     arr, page_size = _cache_pools(op, pools, refcounts.shape[0], dev)
