@@ -183,6 +183,7 @@ SIGNATURES = {
     "dm_qk_norm_rope_bwd_workspace": (_SZ, [_QD]),
     "dm_qk_norm_rope_bwd": (ctypes.c_int, [_QD] + [_VP] * 12 + [_SZ, _VP]),
     "dm_qk_norm_rope_paged": (ctypes.c_int, [_QD, _PD] + [_VP] * 10),
+    "dm_qk_norm_rope_paged_at": (ctypes.c_int, [_QD, _PD] + [_VP] * 10),
 }
 
 _lib = None

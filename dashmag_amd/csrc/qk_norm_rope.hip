@@ -846,9 +846,10 @@ int dm_qk_norm_rope_bwd(const dm_qk_norm_rope_desc *d, const void *q, const void
     return DM_OK;
 }
 
-int dm_qk_norm_rope_paged(const dm_qk_norm_rope_desc *d, const dm_kv_pages *pages, const void *q,
-                          const void *k, const void *v, const void *q_weight, const void *k_weight,
-                          const float *inv_freq, void *q_out, void *k_pages, void *v_pages, void *stream) {
+// turned: by the descriptor's positions, where it has some.
+static int rope_paged(const dm_qk_norm_rope_desc *d, bool turned, const dm_kv_pages *pages, const void *q,
+                      const void *k, const void *v, const void *q_weight, const void *k_weight,
+                      const float *inv_freq, void *q_out, void *k_pages, void *v_pages, void *stream) {
     const std::string op("qk_norm_rope_paged");
     if (int rc = check_rope(op, d)) return rc;
     if (!pages) return refuse(op + ": null pages");
@@ -869,8 +870,21 @@ int dm_qk_norm_rope_paged(const dm_qk_norm_rope_desc *d, const dm_kv_pages *page
     pg.nseq = (int32_t)pages->nseq;
     pg.block_table = pages->block_table, pg.lengths = pages->lengths, pg.cu = pages->cu_seqlens;
     pg.k = strd(pages->sk), pg.v = strd(pages->sv);
-    return run_rope<kRopePaged>(op.c_str(), d, rope_args(d, q_weight, k_weight, inv_freq), pg, q, k, v, q_out,
-                                k_pages, v_pages, (hipStream_t)stream);
+    RopeArgs a = rope_args(d, q_weight, k_weight, inv_freq);
+    if (!turned) a.positions = nullptr;
+    return run_rope<kRopePaged>(op.c_str(), d, a, pg, q, k, v, q_out, k_pages, v_pages, (hipStream_t)stream);
+}
+
+int dm_qk_norm_rope_paged(const dm_qk_norm_rope_desc *d, const dm_kv_pages *pages, const void *q,
+                          const void *k, const void *v, const void *q_weight, const void *k_weight,
+                          const float *inv_freq, void *q_out, void *k_pages, void *v_pages, void *stream) {
+    return rope_paged(d, false, pages, q, k, v, q_weight, k_weight, inv_freq, q_out, k_pages, v_pages, stream);
+}
+
+int dm_qk_norm_rope_paged_at(const dm_qk_norm_rope_desc *d, const dm_kv_pages *pages, const void *q,
+                             const void *k, const void *v, const void *q_weight, const void *k_weight,
+                             const float *inv_freq, void *q_out, void *k_pages, void *v_pages, void *stream) {
+    return rope_paged(d, true, pages, q, k, v, q_weight, k_weight, inv_freq, q_out, k_pages, v_pages, stream);
 }
 
 }  // extern "C"

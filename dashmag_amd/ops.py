@@ -690,7 +690,8 @@ def qk_norm_rope_paged(query, key, value, q_weight, k_weight, inv_freq, key_page
     pages = _lib.KvPages(ps[0], ps[1], bt.shape[1], nseq, bt.data_ptr(), ln.data_ptr(), _at(cu))
     _put_strides(pages, _PAGES_SK, *key_pages.stride()[:3], *value_pages.stride()[:3])
     qo = _contiguous_like(q)
-    _run(op, dev, _lib.lib().dm_qk_norm_rope_paged, ctypes.byref(desc), ctypes.byref(pages), q.data_ptr(),
+    run = _lib.lib().dm_qk_norm_rope_paged if at is None else _lib.lib().dm_qk_norm_rope_paged_at
+    _run(op, dev, run, ctypes.byref(desc), ctypes.byref(pages), q.data_ptr(),
          k.data_ptr(), v.data_ptr(), _at(wq), _at(wk), freq.data_ptr(), qo.data_ptr(), key_pages.data_ptr(),
          value_pages.data_ptr())
     return qo

@@ -12,7 +12,7 @@
  *   dm_attention_paged   (none: the attention of new tokens over a paged cache, and the weights that
  *                        its keys get)
  *   dm_cache_reserve, _fork, _free, _compact, _evict  (none: the pages of a paged cache)
- *   dm_qk_norm_rope{,_bwd,_paged}  (none: the norms and the rotation of queries and keys that
+ *   dm_qk_norm_rope{,_bwd,_paged,_paged_at}  (none: the norms and the rotation of queries and keys that
  *                        precede the attention; the reference's callers bring them rotated)
  *   dm_gdr_chunk_fwd     ChunkGatedDeltaBackend::chunk_gated_delta_forward
  *                                                               crates/dash-ops/src/gated_delta/chunk.rs:340-425, :856
@@ -189,7 +189,8 @@ typedef struct {
     int32_t weight_dtype; /* the weights and their gradients: DM_F32 or dtype */
     int32_t interleaved, unit_offset;
     float eps;
-    const void *positions;   /* [B, T] int32 or int64 on the device; NULL: 0 .. T - 1 in each row */
+    const void *positions;   /* [B, T] int32 or int64 on the device; NULL: 0 .. T - 1 in each row
+                              * (of the paged forms dm_qk_norm_rope_paged_at reads it) */
     int32_t positions_i64;   /* 1: int64 */
     int64_t positions_b;     /* the elements between two batch rows' positions (0: one row for all) */
     int32_t strided;         /* 1: the strides below (each >= 0); sv is the paged form's v, sgq and
@@ -480,13 +481,18 @@ int dm_qk_norm_rope_bwd(const dm_qk_norm_rope_desc *desc, const void *q, const v
 /* The same into a paged cache: q_out [N, Hq, D] contiguous; the keys, normalised and rotated (there
  * is no form without the norm), and the values as they are go to their rows of k_pages and
  * v_pages. No two tokens of a call may have one page row (sequences that share the page that they
- * append to, a page twice in a row's table): which of them it then holds is not said. With
- * desc->positions [N] the tokens turn by those and not by their places in the sequences (a cache whose
- * rows have given up keys: dm_cache_evict). */
+ * append to, a page twice in a row's table): which of them it then holds is not said. The tokens turn by
+ * their places in the sequences, whatever desc->positions is. */
 int dm_qk_norm_rope_paged(const dm_qk_norm_rope_desc *desc, const dm_kv_pages *pages, const void *q,
                           const void *k, const void *v, const void *q_weight, const void *k_weight,
                           const float *inv_freq, void *q_out, void *k_pages, void *v_pages,
                           void *stream);
+/* The same with the tokens turned by desc->positions [N] (NULL: by their places): the tokens of a cache whose
+ * rows have given up keys (dm_cache_evict). */
+int dm_qk_norm_rope_paged_at(const dm_qk_norm_rope_desc *desc, const dm_kv_pages *pages, const void *q,
+                             const void *k, const void *v, const void *q_weight, const void *k_weight,
+                             const float *inv_freq, void *q_out, void *k_pages, void *v_pages,
+                             void *stream);
 
 /* The chunked gated delta rule forward: out [B, T, H, Dv] in dtype and, if final_state is not
  * NULL, each sequence's final state [S, H, Dk, Dv] f32; h0 [S, H, Dk, Dv] f32 or NULL (zeros).
