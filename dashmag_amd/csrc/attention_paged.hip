@@ -346,6 +346,14 @@ static int64_t lone_rows(int64_t d) { return d == 256 ? kNarrowRows : 2 * kNarro
 // 4 rows a head 201 and 257 us; 32 of 8 rows 194 and 195, of 12 211 and 205, of 16 228 and 207, of 32 296 and 212.
 constexpr int kScoreRows = 8;
 static_assert(kScoreRows <= 16, "a larger sequence's first tile has more rows");
+// The reference that weights are taken against lies kLift (log2 units) below the row's maximum when it moves, and moves
+// when the maximum is kTop or more above it. f16 has no weight below 2^-25, and 131072 keys of such weights beside one of 1
+// are 0.3% of their sum: its weights reach up to 2^11, so that what is lost is below 2^-32 of the row's largest (the 2^5 from
+// there to its largest number are left to the scores' own rounding, half a step of 4 at 2^26).
+template <int DT>
+constexpr float kLift = DT == DM_F16 ? 7.f : 0.f;
+template <int DT>
+constexpr float kTop = DT == DM_F16 ? 11.f : 8.f;
 template <int D>
 constexpr int paged_waves() { return D == 256 ? 4 : 8; }
 constexpr uint32_t kNoKey = 0xffffffffu;
@@ -589,9 +597,9 @@ __device__ __forceinline__ void paged_narrow(const PagedArgs &a, const PagedLine
                 }
             }
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const bool grow = mx > m + 8.f;
+            const bool grow = mx - m > kTop<DT>;  // false while both are -inf
             if (__any(grow)) {
-                const float mn = grow ? mx : m, alpha = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
+                const float mn = grow ? mx - kLift<DT> : m, alpha = mn == -INFINITY ? 1.f : fast_exp2(m - mn);
                 m = mn;
                 sum *= alpha;
 #pragma unroll
@@ -795,9 +803,9 @@ __device__ __forceinline__ void paged_wide(const PagedArgs &a, const PagedLine &
             for (int i = 0; i < 16; i++) tmax = fmaxf(tmax, s[t][i]);
         tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
         const float tmc = tmax * c2;
-        const bool grow = tmc - m > 8.f;  // false while both are -inf
+        const bool grow = tmc - m > kTop<DT>;  // false while both are -inf
         if (__any(grow)) {
-            const float mnew = grow ? tmc : m, alpha = grow ? fast_exp2(m - mnew) : 1.f;  // 0 from -inf
+            const float mnew = grow ? tmc - kLift<DT> : m, alpha = grow ? fast_exp2(m - mnew) : 1.f;  // 0 from -inf
             m = mnew;
             sum *= alpha;
 #pragma unroll

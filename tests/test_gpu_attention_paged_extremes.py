@@ -125,3 +125,34 @@ def test_weights_of_few_rows_without_kept_scores(dtype, d, window):
         held_lse("lse", lse, *want["lse"])
         held("weights", w[:, :b.weights.shape[1]], *want["weights"])
         assert (w[:, b.weights.shape[1]:] == 0.25).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF])
+@pytest.mark.parametrize("d,seqs,new", [(64, 2048, 1), (128, 2048, 1), (256, 1024, 1), (64, 256, 70), (128, 256, 70), (256, 256, 70)])
+def test_many_small_weights_beside_a_large_one(dtype, d, seqs, new):
+    """131072 keys of a weight of 2^-25.5 each beside a first of 1, as many sequences as workers: together they are 0.0028 of
+    the sum. With values of 1 an output is 1 but for its rounding and its weights' (half a step each), f16 weights lost
+    below 2^-32, and the f32 sums of its weights and products: chains of keys / 16 + 64 additions to sums near their last
+    value, each off by u = 2^-24 of it, 2^13 u = 2^-11 a sum; E = 17 u S for scores of one product up to S = 17.7."""
+    keys, page = 131073, 16
+    pages = -(-keys // page)
+    q = torch.zeros(seqs * new, 1, d, dtype=dtype, device="cuda")
+    k = torch.zeros(pages, page, 1, d, dtype=dtype, device="cuda")
+    v = torch.ones_like(k)
+    q[..., 0] = 16.0
+    k[0, 0, 0, 0] = 1.0
+    scale = 25.5 * 0.6931471805599453 / 16
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(seqs, pages).contiguous()
+    ln = torch.full((seqs,), keys, dtype=torch.int32, device="cuda")
+    cu = torch.arange(0, seqs * new + 1, new, dtype=torch.int32, device="cuda")
+    print(f"{dtype} D={d} {seqs} sequences of {new}", flush=True)
+    out, lse = dm.attention_paged_with_lse(q, k, v, table, ln, cu, dm.AttentionOptions(scale=scale))
+    half = torch.finfo(dtype).eps / 2
+    off = (out.double() - 1).abs().max().item()
+    seen = keys - new + 1 + (torch.arange(new, dtype=torch.float64) if new > 1 else torch.zeros(1, dtype=torch.float64))
+    want = 25.5 * 0.6931471805599453 + torch.log1p((seen - 1) * 2.0 ** -25.5)
+    loff = (lse.cpu().double().view(seqs, new) - want).abs().max().item()
+    print(f"out {off:.2e}, lse {loff:.2e}", flush=True)
+    chain, e = (keys / 16 + 64) * U, 17 * U * 17.7
+    assert off <= 2 * half + keys * 2.0 ** -32 * (dtype == F16) + 2 * chain + 2 * e
+    assert loff <= chain + e + 8 * U * (17.7 + 1)
