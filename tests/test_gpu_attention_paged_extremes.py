@@ -156,3 +156,14 @@ def test_many_small_weights_beside_a_large_one(dtype, d, seqs, new):
     chain, e = (keys / 16 + 64) * U, 17 * U * 17.7
     assert off <= 2 * half + keys * 2.0 ** -32 * (dtype == F16) + 2 * chain + 2 * e
     assert loff <= chain + e + 8 * U * (17.7 + 1)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F16, 64), (BF, 256), (F32, 64)])
+@pytest.mark.parametrize("between", [1, 63, 64, 65, 127, 200, 1100])
+def test_sequences_between_those_of_a_line(dtype, d, between):
+    """Prompts with many sequences of few or no tokens between them and behind the last: a worker goes from one to the
+    next past all of them, among the wide tiles, the narrow ones and the keys'."""
+    few = [(0, 7), (1, 5), (0, 0), (2, 3)]
+    gap = [few[i % 4] for i in range(between)]
+    _held_all(Chunks(dtype, d, 1, 4, 16, [(90, 400), *gap, (41, 333), *gap[:between // 2], (130, 131), (0, 3)], seed=between))
+    _held_all(Chunks(dtype, d, 1, 4, 16, [(3, 90), *[(0, 9)] * between, (5, 400), *[(0, 0)] * between, (12, 30)], seed=between))
