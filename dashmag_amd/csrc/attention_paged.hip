@@ -5,10 +5,11 @@
 // query heads of one key-value head) sweep their keys once with a running maximum and sum; paged_line.h says how
 // the tiles are shared out and cut.
 //
-// Chunks are bound by the products: 2048 tokens of 32 heads of 128 over 8 against 32768 keys take 1058-1118 us (960-1010
-// TFLOP/s), 24 of them the join; prompts of about 1400 tokens are at 620-700, since each piece of a tile costs 10 us to begin and
-// end. Single tokens are bound by memory: 64 of up to 8192 keys 282 us, 5.6 TB/s. Four short ones take 22-25 us, of which
-// the plan is 4, the way to the first keys 5, 2.5 a block of 32 keys and the join's launch 5.
+// Times are a call's among others; a kernel trace of thirteen at once, whose clock has fallen, is in brackets. Chunks are bound
+// by the products: 2048 tokens of 32 heads of 128 over 8 against 32768 keys take 1071-1081 us (1195 and the join's 22), 985-991
+// TFLOP/s; nine prompts of up to 1400 tokens 295 us (352 and 24), 690, since each piece of a tile costs 10 us to begin
+// and end. Single tokens are bound by memory: 64 of up to 8192 keys 287 us (280 and 6), 5.5 TB/s. Four short ones take 23 us
+// (18.4 and 4.5), of which the plan is 4, the way to the first keys 5, 2.5 a block of 32 keys.
 #include <algorithm>
 #include <string>
 
@@ -73,8 +74,9 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 //
 // A wavefront takes 32 rows and 32 keys at a time, both products on the f32 matrix cores: S^T = K q^T, whose
 // output layout is the operand that O^T += V^T P^T takes. Keys and values go through one LDS tile of f32, DP columns
-// wide (the head width and zeros behind it). 210 tokens of 4 heads of 64 in f32 against 300 keys each: 27 us and 5 of
-// join, bound by latency.
+// wide (the head width and zeros behind it). 210 tokens of 4 heads of 64 in f32 against 300 keys each: 28 us and 5 of
+// join, bound by latency. 1024 tokens of 32 heads over 8 against 5120 keys: f32 of 128 1218 us (63 TFLOP/s), 16-bit
+// widths between the fast ones 2340 to 2410; 64 single tokens of 4352 keys f32 603 us, 96 wide in bf16 1468.
 
 // VEC elements from p on.
 template <int DT, int VEC>
@@ -1151,7 +1153,7 @@ __global__ __launch_bounds__(256) void paged_weights_simple(PagedArgs a, KeyLine
 // The 16-bit kernel: a workgroup takes a tile of keys, 64 of them a wavefront (32 at D = 256) in registers as the second
 // operand, and sweeps the rows that see them, 64 at a time through LDS, head by head. A key's sum over a step's 32
 // rows is taken first, then over a head's, then over the heads (one at a time, a long sum would lose bits). 1024 tokens
-// of 32 heads of 128 against 16384 keys take 250-280 us (490-530 TFLOP/s): the products and the exponentials follow one
+// of 32 heads of 128 against 16384 keys take 236-250 us (530-560 TFLOP/s): the products and the exponentials follow one
 // another in a wavefront, and two wavefronts a SIMD are all that the keys' registers leave.
 template <int D>
 constexpr int key_cols() { return D == 256 ? 1 : 2; }  // 32-key columns of a wavefront
@@ -1436,7 +1438,8 @@ static bool paged_fast_pool(const PagedArgs &a) {
     return a.num_pages > 0 && a.kb < most / a.num_pages / 2 && a.kt < most / a.page_size / 2;
 }
 
-// Most bytes of scores kept (half a percent of the card's memory; calls that could need more go through the keys again).
+// Most bytes of scores kept (0.7% of the card's memory; calls whose table is so wide that they could need more go through
+// the keys again: 64 tokens of 4 rows a head against 4096 keys 257 us for 201).
 constexpr int64_t kScoreBytes = (int64_t)1 << 31;
 struct PagedPlan {
     bool fast, mixed;

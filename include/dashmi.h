@@ -412,6 +412,11 @@ int dm_attention_decode_shared(const dm_attention_desc *desc, const void *q, con
  * weights [S, tk] f32 with rows weights_stride elements apart, or NULL: key j of sequence s is given, on top of
  * what is there, the sum over the tokens and the query heads that see it of e^(scale q k - lse), in a fixed
  * order.
+ * Scores, sums, lse and the keys' weights are f32. For the product with V a 16-bit call of D = 64, 128 or 256 (whose
+ * rows are whole 16-byte pieces) rounds the softmax weights to dtype, half a step each; every other call keeps them
+ * in f32. With weights such a call keeps the scores of sequences of up to 8 rows (tokens x query heads of a key-value
+ * head), b hkv 8 tk floats of its workspace, unless those are more than 2 GiB: on a wider table the same rows take another
+ * pass over their keys, whose sums are not the others' to the bit.
  * All int32 arrays are read on the device only: a length counts as between 0 and tk, offsets that do not go up
  * between 0 and N leave every token without a sequence, a page outside [0, num_pages) reads as zeros.
  * Refused: N * Hq of 2^26 or more, tk above 2^30. */
@@ -456,7 +461,9 @@ int dm_cache_compact(const dm_cache_table *table, const dm_cache_pool *pools, in
  * (rows weights_stride elements apart; NaN above all, of equal ones the first). They stay in order and move down to
  * 0 .. n - 1 in every pool, their weights with them, and the weights of n .. L - 1 become 0; the pages
  * behind ceil(n / page_size) are given up as by dm_cache_free. kept [rows, max_pages * page_size]: where each key
- * of a row, now at j, was before (j itself in a row that gives up none), -1 from its length on. A key on a page
+ * of a row, now at j, was before (j itself in a row that gives up none), -1 from its length on. Places change: a
+ * window counts those, and so reaches further back in a row that has given up keys. The weights of a row that is freed
+ * or forked are the caller's to clear or copy. A key on a page
  * outside the pools is not moved. Refused: rows that could hold 2^35 keys together, pools that overlap (one given
  * twice). */
 size_t dm_cache_evict_workspace(const dm_cache_table *table);
