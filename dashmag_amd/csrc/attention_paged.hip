@@ -6,7 +6,8 @@
 // the tiles are shared out and cut.
 //
 // Times are a call's among others; the kernels' medians in a trace of a process's first thirteen are in brackets (the products
-// run slower then: the document's kernel goes from 1340 us down to 1030 over thirty passes). Chunks are bound by the products: 2048 tokens of 32 heads of 128 over 8 against 32768 keys take 1071-1081 us (1195 and the join's 22), 985-991
+// run slower then: the document's kernel goes from 1340 us down to 1030 over thirty passes). Chunks are bound by the
+// products: 2048 tokens of 32 heads of 128 over 8 against 32768 keys take 1071-1081 us (1195 and the join's 22), 985-991
 // TFLOP/s; nine prompts of up to 1400 tokens 295 us (352 and 24), 690, since each piece of a tile costs 10 us to begin
 // and end. Single tokens are bound by memory: 64 of up to 8192 keys 287 us (280 and 6), 5.5 TB/s. Four short ones take 23 us
 // (18.4 and 4.5), of which the plan is 4, the way to the first keys 5, 2.5 a block of 32 keys.
