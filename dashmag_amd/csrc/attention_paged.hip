@@ -339,8 +339,8 @@ __global__ __launch_bounds__(256) void paged_simple(PagedArgs a, PagedLine l, co
 // 62 and 95, 46 and 55, 50 and 59. Batches of both sizes (8 to 64 sequences of 8 to 52 rows) pay both lines' starts,
 // -20% to +35%: with 48 here the geometric mean of 56 of them is the same, with 64 3% less, and the equal ones' 9 and 17% more.
 constexpr int kNarrowRows = 32;
-// Calls that have no more rows a key head altogether get no wide line, only narrow tiles (two at most of a sequence): without a
-// line to plan and its workgroups a call of 33 to 64 rows takes 22-32 us where both lines take 28-40 (1 to 16
+// Calls of at most so many rows a key head altogether get no wide line, only narrow tiles (two at most of a sequence): without
+// a line to plan and its workgroups a call of 33 to 64 rows takes 22-32 us where both lines take 28-40 (1 to 16
 // sequences of 1000 to 8000 keys, 2 key heads of 64 or 128); one sequence of 30000 keys 46 and 41. At 256, whose narrow
 // line has half as many workers: 39-45 and 40-44, of 30000 keys 65 and 48.
 static int64_t lone_rows(int64_t d) { return d == 256 ? kNarrowRows : 2 * kNarrowRows; }
